@@ -1,0 +1,127 @@
+// What the two kernels of attention over rows (attention_rows.cu, attention_rows_tc.cu) share.
+//
+// A work item is a stretch of a request's tokens; its query rows are (token, head of the KV head's group) pairs, token by
+// token, row r = token * G + head: a tile of rows packs a few tokens' heads, so that one read of a key serves all of them.
+//
+//   causal: a token at position p sees the cached keys up to its own place p;
+//   tree:   the request's tokens of this step are drafted ones, stored behind the `base` cached keys in the order of the step;
+//           token i sees the cached keys and the drafted tokens j whose bit masks[i] holds.  A drafted key's position is its
+//           token's, a cached key's is its place.
+//   Both: and of these the keys at positions from start(p) = max(chunk ? p - p % chunk : 0, window ? p - window + 1 : 0) on.
+//
+//   s = scale temp(p) q.k (soft-capped: cap tanh(s / cap)) - slope (p - key position);   out = sum w v / (sum w + exp(sink)),
+//   w = exp(s - max).  A row that sees nothing gives 0.
+#pragma once
+#include "common.cuh"
+#include "fp8_rows.cuh"
+#include "softcap.cuh"
+
+#define ROWS_NEG_BIG (-1.0e30f)
+#define LOG2E 1.4426950408889634f
+
+struct RowsParams {
+  const bf16* q;           // [N, Hq, DH]
+  const void* pages;       // [P, 2, Hkv, page, DH] bfloat16, or e4m3 codes
+  const uint8_t* scales;   // [P, 2, Hkv, page] with codes
+  const int* block_table;
+  int bt_stride, n_requests;
+  const int* req_of_token;
+  const int* positions;
+  bf16* out;               // [N, Hq, DH]
+  const int* items;        // [n_items][2] = (first token row, count), one request each; null: single tokens
+  const int* rows;         // single tokens: their token rows (null: 0 .. n_items - 1)
+  int n_items;
+  const int* cu_q;         // tree: [R + 1] the requests' first token rows (null: causal)
+  const int* q_start;      // tree: [R] keys a request has cached before its drafted tokens
+  const int* masks;        // tree: [N, words]
+  int words;
+  int N, Hq, Hkv, page_size, num_pages;
+  float scale_log2;        // the score scale * log2(e); with a cap: the score scale / cap
+  float cap_log2;          // cap * log2(e), 0: none
+  int chunk, window;
+  float attn_scale, floor_scale;
+  const float* sink;       // [Hq] or null
+  const float* slopes;     // [Hq] or null
+  int splits, split_keys;  // ranges of keys an item's rows are cut into, and keys of a range (the last one takes the rest)
+  float* part_o;           // [N, Hq, splits, DH]: sums of weighted values against the maximum
+  float2* part_ml;         // [N, Hq, splits]: (maximum, sum of weights)
+  int* status;
+};
+
+struct RowsItem {
+  int n0, cnt, r, base, drafted;  // base: keys before the drafted tokens (causal: INT_MAX), drafted: their count
+};
+
+// The item's description; false: nothing to do (a description that points outside the step raises the status).
+__device__ __forceinline__ bool rows_item(const RowsParams& P, int i, RowsItem& it) {
+  it.n0 = P.items ? P.items[2 * i] : (P.rows ? P.rows[i] : i);
+  it.cnt = P.items ? P.items[2 * i + 1] : 1;
+  if (it.cnt <= 0) return false;
+  if (it.n0 < 0 || it.n0 > P.N - it.cnt) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
+  it.r = P.req_of_token[it.n0];
+  if (it.r < 0 || it.r >= P.n_requests) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
+  it.base = P.cu_q ? P.q_start[it.r] : 0x7fffffff;
+  it.drafted = 0;
+  if (P.cu_q) {
+    const int first = P.cu_q[it.r], end = P.cu_q[it.r + 1];
+    if (first < 0 || end > P.N || it.n0 < first || it.n0 + it.cnt > end || it.base < 0) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
+    it.drafted = end - first;
+  }
+  return true;
+}
+
+__device__ __forceinline__ int rows_first_key(const RowsParams& P, int p) {
+  int s = 0;
+  if (P.chunk > 0) s = p - p % P.chunk;
+  if (P.window > 0) s = max(s, p - P.window + 1);
+  return s;
+}
+
+// What a query row needs to know of its token.
+struct RowsToken {
+  int n, p, lo, head;
+  float sc, slope;  // score factor and slope in base-2 units (with a cap: the factor of the cap's argument)
+};
+__device__ __forceinline__ RowsToken rows_token(const RowsParams& P, const RowsItem& it, int row, int hk) {
+  const int G = P.Hq / P.Hkv, t = row / G;
+  RowsToken k;
+  k.n = it.n0 + t;
+  k.head = hk * G + (row - t * G);
+  k.p = P.positions[k.n];
+  k.lo = rows_first_key(P, k.p);
+  k.sc = P.scale_log2;
+  if (P.attn_scale != 0.f) k.sc *= 1.f + P.attn_scale * log1pf(floorf(((float)k.p + 1.f) / P.floor_scale));
+  k.slope = P.slopes ? P.slopes[k.head] * LOG2E : 0.f;
+  return k;
+}
+
+// Whether the row's token sees the key at `place`, and the key's position.
+__device__ __forceinline__ bool rows_sees(const RowsParams& P, const RowsItem& it, int n, int p, int lo, int place, int& key_pos) {
+  key_pos = place;
+  if (!P.cu_q) return place >= lo && place <= p;
+  if (place < it.base) return place >= lo;
+  const int j = place - it.base;
+  if (j >= it.drafted || j >= 32 * P.words) return false;
+  key_pos = P.positions[P.cu_q[it.r] + j];
+  return ((P.masks[(size_t)n * P.words + (j >> 5)] >> (j & 31)) & 1) && key_pos >= lo;
+}
+
+// The flat row of the key at `place` in the cache (values: Hkv * page_size further), or -1.
+__device__ __forceinline__ int rows_cache_row(const RowsParams& P, const int* table, int hk, int place) {
+  const int pi = place / P.page_size;
+  const int page = pi < P.bt_stride ? table[pi] : -1;
+  if (page < 0 || page >= P.num_pages) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return -1; }
+  return (page * 2 * P.Hkv + hk) * P.page_size + (place - pi * P.page_size);
+}
+
+__device__ __forceinline__ float rows_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What a row's weighted sum is divided by, inverted: l against the maximum m, the sink's term with them.
+__device__ __forceinline__ float rows_inverse(const RowsParams& P, float m, float l, int head) {
+  if (P.sink) l += exp2f(P.sink[head] * LOG2E - m);  // (a row that sees nothing has m = NEG_BIG: the term is infinite, the row 0)
+  return l == 0.f ? 0.f : 1.f / l;
+}

@@ -1104,6 +1104,196 @@ def attention_prefill_tc(q: torch.Tensor, pages: torch.Tensor, block_table: torc
          c_float(floor_scale), _ptr(sink), _ptr(slopes), c_float(softcap), c_int(keep), _diff(diff), _ptr(status), _stream())
 
 
+# ------------------------------------------------------- the cache in 8 bits, drafted trees
+FP8 = torch.float8_e4m3fn  # pages in 8 bits: e4m3 codes, and a byte of scale per row (csrc/fp8_rows.cuh)
+
+
+def _ints(what: str, **tensors: "tuple[torch.Tensor | None, int]") -> None:
+    """Index arrays: contiguous int32 with at least so many entries."""
+    for name, (t, n) in tensors.items():
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n):
+            raise KernelError(f"{what}: {name} must be contiguous int32 with at least {n} entries")
+
+
+def _on_device(what: str, *tensors: torch.Tensor | None) -> None:
+    """A launch goes to the current device's stream: tensors of another device have no place in it."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.is_cuda and t.device.index != dev:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
+
+
+def _cache8(what: str, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, Hkv: int, dh: int) -> None:
+    if pages.dtype != FP8 or pages.dim() != 5 or pages.shape[1] != 2 or pages.shape[2] != Hkv or pages.shape[4] != dh:
+        raise KernelError(f"{what}: pages must be float8_e4m3fn [pages, 2, {Hkv}, page size, {dh}], not {pages.dtype} {tuple(pages.shape)}")
+    if scales.dtype != torch.uint8 or scales.shape != pages.shape[:4]:
+        raise KernelError(f"{what}: scales must be uint8 {tuple(pages.shape[:4])}, a byte per row of the pages")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise KernelError(f"{what}: the block table must be int32 [requests, pages of one]")
+    _contig(pages, scales, block_table)
+
+
+def _cache8_args(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor) -> tuple:
+    return (_ptr(pages), _ptr(scales), _ptr(block_table), c_int(block_table.shape[1]), c_int(block_table.shape[0]))
+
+
+def kv_store_fp8(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+                 req_of_token: torch.Tensor, places: torch.Tensor, status: torch.Tensor) -> None:
+    """Rows of keys and values into a cache in 8 bits.  k, v: [N, Hkv, dh] (float32 or bfloat16; dh a multiple of 8 up to 256);
+    pages: float8_e4m3fn [pages, 2, Hkv, page size, dh]; scales: uint8 [pages, 2, Hkv, page size].  Token n of request
+    ``req_of_token[n]`` is kept at its place ``places[n]`` (page ``block_table[request, place // page size]``); the places of
+    one call are distinct.  A row's entries are kept as x * 2^-e rounded to e4m3, its byte as e + 127, e the smallest whole
+    number (at least -60) with max |x| <= 448 * 2^e.  A row with an infinity or a NaN, or above 448 * 2^60, gets byte 255 and
+    reads back as NaN.  A place without a page is left out and raises the status."""
+    _contig(k, v)
+    N, Hkv, dh = k.shape
+    _cache8("kv_store_fp8", pages, scales, block_table, Hkv, dh)
+    _ints("kv_store_fp8", req_of_token=(req_of_token, N), places=(places, N), status=(status, 1))
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise KernelError("kv_store_fp8: keys and values must have one shape and type")
+    _on_device("kv_store_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
+    _run("kv_fp8", "jlx_kv_store_fp8", _ptr(k), _ptr(v), c_int(code(k.dtype)), *_cache8_args(pages, scales, block_table), _ptr(req_of_token),
+         _ptr(places), c_int(N), c_int(Hkv), c_int(dh), c_int(pages.shape[3]), c_int(pages.shape[0]), _ptr(status), _stream())
+
+
+def rope_kv_store_fp8(qkv: torch.Tensor, q_out: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+                      req_of_token: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor | None, l2norm: bool, eps: float,
+                      Hq: int, Hkv: int, dh: int, status: torch.Tensor, splits: int = 1, places: torch.Tensor | None = None) -> None:
+    """:func:`rope_kv_store` into a cache in 8 bits (:func:`kv_store_fp8`), quantised from the 32-bit keys and values.  qkv:
+    [N, (Hq + 2 Hkv) * dh] projected rows (float32 or bfloat16), or ``splits`` float32 partials of them; q_out: bfloat16
+    [N, Hq, dh].  ``places`` (None: the positions): where the rows are kept, for drafted tokens whose position is not their place."""
+    _contig(qkv, q_out, inv_freq)
+    N = q_out.shape[0]
+    places = positions if places is None else places
+    _cache8("rope_kv_store_fp8", pages, scales, block_table, Hkv, dh)
+    _ints("rope_kv_store_fp8", req_of_token=(req_of_token, N), positions=(positions, N), places=(places, N), status=(status, 1))
+    if q_out.dtype != torch.bfloat16 or tuple(q_out.shape) != (N, Hq, dh) or splits < 1 or qkv.numel() != splits * N * (Hq + 2 * Hkv) * dh:
+        raise KernelError(f"rope_kv_store_fp8: {splits} x {N} projected rows of {Hq} + 2 * {Hkv} heads of {dh} and bfloat16 queries do not "
+                          f"fit qkv {tuple(qkv.shape)}, q_out {q_out.dtype} {tuple(q_out.shape)}")
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != dh // 2):
+        raise KernelError(f"rope_kv_store_fp8: {dh // 2} float32 frequencies are needed")
+    _on_device("rope_kv_store_fp8", qkv, q_out, pages, scales, block_table, req_of_token, positions, places, inv_freq, status)
+    sp, stride = _splits(qkv, splits)
+    _run("kv_fp8", "jlx_rope_kv_store_fp8", _ptr(qkv), c_int(code(qkv.dtype)), c_int(sp), c_longlong(stride), _ptr(q_out),
+         *_cache8_args(pages, scales, block_table), _ptr(req_of_token), _ptr(positions), _ptr(places), _ptr(inv_freq), c_int(int(l2norm)),
+         c_float(eps), c_int(N), c_int(Hq), c_int(Hkv), c_int(dh), c_int(pages.shape[3]), c_int(pages.shape[0]), _ptr(status), _stream())
+
+
+def kv_load_fp8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, req_of_token: torch.Tensor, places: torch.Tensor,
+                k: torch.Tensor, v: torch.Tensor, status: torch.Tensor) -> None:
+    """The rows that a cache in 8 bits keeps at the listed places, as numbers: k, v [N, Hkv, dh] (float32 or bfloat16, exact in
+    both).  A place without a page gives zeros and raises the status."""
+    _contig(k, v)
+    N, Hkv, dh = k.shape
+    _cache8("kv_load_fp8", pages, scales, block_table, Hkv, dh)
+    _ints("kv_load_fp8", req_of_token=(req_of_token, N), places=(places, N), status=(status, 1))
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise KernelError("kv_load_fp8: keys and values must have one shape and type")
+    _on_device("kv_load_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
+    _run("kv_fp8", "jlx_kv_load_fp8", *_cache8_args(pages, scales, block_table), _ptr(req_of_token), _ptr(places), _ptr(k), _ptr(v),
+         c_int(code(k.dtype)), c_int(N), c_int(Hkv), c_int(dh), c_int(pages.shape[3]), c_int(pages.shape[0]), _ptr(status), _stream())
+
+
+def attention_rows_supported(q_dtype: torch.dtype, Hq: int, Hkv: int, dh: int) -> bool:
+    """Whether :func:`attention_fp8` and :func:`attention_tree` take these queries (bfloat16, head size 64 or 128)."""
+    return q_dtype == torch.bfloat16 and bool(library("attention_rows").jlx_attention_rows_supported(c_int(Hq), c_int(Hkv), c_int(dh)))
+
+
+def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, positions, out, scale, chunk, window, attn_scale, floor_scale, status,
+                    max_kv_len, items, rows, n_items, max_count, tree, sink, slopes, softcap) -> None:
+    _contig(q, pages, scales, block_table, out)
+    N, Hq, dh = q.shape
+    P, two, Hkv, page_size, dh2 = pages.shape
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != q.shape or out.data_ptr() == q.data_ptr():
+        raise KernelError(f"{what}: queries and output must be bfloat16 [N, Hq, dh], and not the same rows")
+    if dh2 != dh or two != 2:
+        raise KernelError(f"{what}: cache pages {tuple(pages.shape)} and queries {tuple(q.shape)} disagree")
+    if scales is not None:
+        _cache8(what, pages, scales, block_table, Hkv, dh)
+    elif pages.dtype != torch.bfloat16:
+        raise KernelError(f"{what}: pages must be bfloat16, or float8_e4m3fn with scales")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise KernelError(f"{what}: the block table must be int32 [requests, pages of one]")
+    R = block_table.shape[0]
+    cu_q, q_start, masks = tree
+    _ints(what, req_of_token=(req_of_token, N), positions=(positions, N), items=(items, 2 * n_items), rows=(rows, n_items), status=(status, 1),
+          cu_q=(cu_q, R + 1), q_start=(q_start, R), masks=(masks, N))
+    if masks is not None and (masks.dim() != 2 or masks.shape[0] != N):
+        raise KernelError(f"{what}: masks must be int32 [{N}, words], a bit per drafted token of the request")
+    if max_kv_len < 1 or max_count < 1 or n_items < 0 or (items is None and rows is None and n_items > N):
+        raise KernelError(f"{what}: {n_items} items of up to {max_count} tokens over {max_kv_len} keys")
+    _check_sink(sink, Hq)
+    _check_sink(slopes, Hq, "slopes")
+    _on_device(what, q, pages, scales, block_table, req_of_token, positions, out, items, rows, cu_q, q_start, masks, sink, slopes, status)
+    if N == 0 or n_items == 0:
+        return
+    splits, split_keys = c_int(1), c_int(1)
+    library("attention_rows").jlx_attention_rows_plan(c_int(max_kv_len), c_int(chunk), c_int(window), c_int(n_items), c_int(max_count), c_int(Hq), c_int(Hkv),
+                                                      c_int(sm_count()), ctypes.byref(splits), ctypes.byref(split_keys))
+    part_o = part_ml = None
+    if splits.value > 1:
+        # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
+        part_o = torch.empty(N * Hq * splits.value * dh, dtype=torch.float32, device=q.device)
+        part_ml = torch.empty(N * Hq * splits.value * 2, dtype=torch.float32, device=q.device)
+    _run("attention_rows", "jlx_attention_rows", _ptr(q), _ptr(pages), _ptr(scales), _ptr(block_table), c_int(block_table.shape[1]), c_int(R),
+         _ptr(req_of_token), _ptr(positions), _ptr(out), _ptr(items), _ptr(rows), c_int(n_items), c_int(max_count), _ptr(cu_q), _ptr(q_start),
+         _ptr(masks), c_int(masks.shape[1] if masks is not None else 0), c_int(N), c_int(Hq), c_int(Hkv), c_int(dh), c_int(page_size), c_int(P),
+         c_float(scale), c_float(softcap), c_int(chunk), c_int(window), c_float(attn_scale), c_float(floor_scale), _ptr(sink), _ptr(slopes),
+         splits, split_keys, _ptr(part_o), _ptr(part_ml), _ptr(status), _stream())
+    global _launches
+    _launches += int(splits.value > 1)  # the joining kernel
+
+
+def attention_fp8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, req_of_token: torch.Tensor,
+                  positions: torch.Tensor, out: torch.Tensor, scale: float, chunk: int, window: int, attn_scale: float, floor_scale: float,
+                  status: torch.Tensor, max_kv_len: int, items: torch.Tensor | None = None, n_items: int = 0, max_count: int = 1,
+                  rows: torch.Tensor | None = None, n_rows: int = 0, sink: torch.Tensor | None = None, slopes: torch.Tensor | None = None,
+                  softcap: float = 0.0) -> None:
+    """:func:`attention_generic` over a cache in 8 bits (:func:`kv_store_fp8`), on the tensor cores: q, out bfloat16 [N, Hq, dh],
+    dh 64 or 128.  ``items``: int32 [n_items, 2] = (first token row, count <= max_count), consecutive tokens of one request each:
+    portions of prompts, of any length.  Without items: single tokens, the first n_rows of the listed ``rows``, or all.  Only the
+    served rows of ``out`` are written.  ``max_kv_len``: keys of the longest request (it sizes the work, and bounds nothing)."""
+    n = n_items if items is not None else (n_rows if rows is not None else q.shape[0])
+    if scales is None:
+        raise KernelError("attention_fp8: a cache in 8 bits has scales")
+    _attention_rows("attention_fp8", q, pages, scales, block_table, req_of_token, positions, out, scale, chunk, window, attn_scale, floor_scale,
+                    status, max_kv_len, items, None if items is not None else rows, n, max_count if items is not None else 1, (None, None, None),
+                    sink, slopes, softcap)
+
+
+def attention_tree(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, req_of_token: torch.Tensor, positions: torch.Tensor,
+                   cu_q: torch.Tensor, q_start: torch.Tensor, masks: torch.Tensor, out: torch.Tensor, scale: float, chunk: int, window: int,
+                   attn_scale: float, floor_scale: float, status: torch.Tensor, max_kv_len: int, items: torch.Tensor, n_items: int,
+                   max_count: int, scales: torch.Tensor | None = None, sink: torch.Tensor | None = None, slopes: torch.Tensor | None = None,
+                   softcap: float = 0.0) -> None:
+    """Attention of drafted tokens over the paged cache (bfloat16 pages, or 8 bits with their scales).  Request r's tokens of
+    this step are the rows cu_q[r] .. cu_q[r + 1], drafted behind ``q_start[r]`` cached ones: their keys and values lie at the
+    places q_start[r], q_start[r] + 1, ... in the rows' order (written before this call), whatever their ``positions``.  A token
+    sees the cached keys and the drafted tokens whose bit its row of ``masks`` holds (int32 [N, words]: bit j % 32 of word j // 32
+    for the request's j-th token; itself and its ancestors, see :func:`tree_masks`), within the chunk and the window of its
+    position.  items: int32 [n_items, 2] = (first token row, count <= max_count) within one request each, as a rule a request's
+    whole tree.  ``max_kv_len``: the longest request's keys, drafted ones included.  A row that sees nothing is 0."""
+    if cu_q is None or q_start is None or masks is None or items is None:
+        raise KernelError("attention_tree: offsets, cached lengths, masks and items are needed")
+    _attention_rows("attention_tree", q, pages, scales, block_table, req_of_token, positions, out, scale, chunk, window, attn_scale, floor_scale,
+                    status, max_kv_len, items, None, n_items, max_count, (cu_q, q_start, masks), sink, slopes, softcap)
+
+
+def tree_masks(parents) -> "tuple[list[int], list[list[int]]]":
+    """What :func:`attention_tree` needs of one request's drafted tokens, made on the host: ``parents[j]`` is the index of token
+    j's parent among them, or -1 for a token that follows the last cached one; parents come before their children.  Returns
+    (depth of every token: its position is q_start + depth, mask words of every token as int32 numbers)."""
+    words = max(1, -(-len(parents) // 32))
+    depth, bits = [], []
+    for j, p in enumerate(parents):
+        if not -1 <= p < j:
+            raise KernelError(f"tree_masks: token {j} has parent {p}; a parent is -1 or an earlier token")
+        depth.append(0 if p < 0 else depth[p] + 1)
+        bits.append((0 if p < 0 else bits[p]) | 1 << j)
+    signed = lambda w: w - (1 << 32) if w >> 31 else w  # noqa: E731
+    return depth, [[signed(b >> (32 * w) & 0xFFFFFFFF) for w in range(words)] for b in bits]
+
+
 # ------------------------------------------------------------------------------------- GEMMs
 GEMM_FORMS = {"rule": 0, "general": 1, "tile": 2, "rows": 3}  # csrc/gemm_simt.cu
 
