@@ -1,10 +1,11 @@
-// Grouped-query attention of few query rows over the paged cache, held in bfloat16 or in 8 bits (fp8_rows.cuh): single decoded
-// tokens, short portions and drafted trees (attention_rows.cuh has the mask and the formula), head sizes 64 and 128.
+// Grouped-query attention over the paged cache, held in bfloat16 or in 8 bits (fp8_rows.cuh), of more query rows than
+// attention_few.cu takes: short portions and drafted trees (attention_rows.cuh has the mask and the formula), head sizes 64
+// and 128.
 //
-// A block of four warps takes up to 16, 32 or 64 query rows of one item and KV head, and one range of its keys; keys come in
-// tiles of 64 by cp.async, row by row through the block table (any page size), STAGES tiles in flight.  With 16 rows every
-// warp takes 16 of a tile's keys, with 32 two warps share the rows' keys, with 64 each warp has 16 rows to itself; warps that
-// share rows keep maxima, sums and outputs of their own and meet once, at the end.  Ranges of one row (split over the key axis
+// A block of four warps takes up to 32 or 64 query rows of one item and KV head, and one range of its keys; keys come in
+// tiles of 64 by cp.async, row by row through the block table (any page size), STAGES tiles in flight.  With 32 rows
+// two warps share 16 rows' keys, with 64 each warp has 16 rows to itself; warps that share rows keep maxima, sums and outputs
+// of their own and meet once, at the end.  Ranges of one row (split over the key axis
 // when there are few rows) are joined by a second kernel.
 //
 // 8 bits: codes go to the tensor cores as float16, which holds every one of them; no number of the cache is rounded.  A key's
@@ -62,7 +63,7 @@ template <int DH, bool F8> struct RowsTile {
   static constexpr int SMEM = RING > MERGE ? RING : MERGE;
 };
 
-// WM: groups of 16 rows per block (1, 2, 4); the 4 / WM warps of a group share its keys.
+// WM: groups of 16 rows per block (2, 4); the 4 / WM warps of a group share its keys.
 template <int DH, bool F8, int WM>
 __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P) {
   JLX_TL(TL_ATTN_DECODE);
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
   int byte_of_last = 0;                       // scale byte of the tile fetched last round
 
   // queries, in the order of the scores' contraction
-  const int wm = WM == 1 ? 0 : warp / WK, wk = warp % WK;
+  const int wm = warp / WK, wk = warp % WK;
   const int r0 = wm * 16 + g, r1 = r0 + 8;
   const int4 tok0 = row_tok[r0], tok1 = row_tok[r1];
   float sc0 = __int_as_float(row_sc[r0].x), sc1 = __int_as_float(row_sc[r1].x);
@@ -457,62 +458,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
   }
 }
 
-// Joins the ranges of a row: a warp per row, DH / 32 entries a lane.
-template <int DH>
-__global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowsParams P) {
-  JLX_TL(TL_ATTN_COMBINE);
-  pdl_launch_dependents_if_small();
-  pdl_wait();
-  RowsItem it;
-  if (!rows_item(P, blockIdx.x, it)) return;
-  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
-  if (row >= it.cnt * P.Hq) return;
-  const int head = row % P.Hq;
-  const size_t at = (size_t)it.n0 * P.Hq + row;
-  const float2* ml = P.part_ml + at * P.splits;
-  float m = ROWS_NEG_BIG;
-  for (int s = lane; s < P.splits; s += 32) m = fmaxf(m, ml[s].x);
-  m = warp_max(m);
-  constexpr int E = DH / 32;
-  float acc[E], l = 0.f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) acc[i] = 0.f;
-  const float* po = P.part_o + at * P.splits * DH + lane * E;
-#pragma unroll 4
-  for (int s = 0; s < P.splits; ++s) {
-    const float2 x = ml[s];
-    const float f = x.x == m ? 1.f : rows_exp2(x.x - m);
-    l = fmaf(x.y, f, l);
-#pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = fmaf(po[(size_t)s * DH + i], f, acc[i]);
-  }
-  const float inv = rows_inverse(P, m, l, head);
-#pragma unroll
-  for (int i = 0; i < E; i += 2)
-    *reinterpret_cast<__nv_bfloat162*>(P.out + at * DH + lane * E + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
-}
-
 // -------------------------------------------------------------------------------------------- host
-JLX_API int jlx_attention_rows_supported(int Hq, int Hkv, int dh) { return Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && (dh == 64 || dh == 128); }
-
-// Into how many ranges of how many keys an item's rows are cut: blocks for about three per multiprocessor, no range below
-// 256 keys (a range's set-up and its share of the join cost as much as a few tiles).
-JLX_API void jlx_attention_rows_plan(int max_kv_len, int chunk, int window, int n_items, int max_count, int Hq, int Hkv, int sms, int* splits,
-                                     int* split_keys) {
-  long long seen = max_kv_len;
-  if (window > 0 && window + max_count < seen) seen = window + max_count;
-  if (chunk > 0 && (long long)chunk + max_count < seen) seen = chunk + max_count;
-  seen += KT;  // ranges start at a tile's first key
-  const int rows = max_count * (Hq / Hkv), per_block = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  const long long blocks = (long long)n_items * Hkv * ((rows + per_block - 1) / per_block);
-  long long s = 3ll * sms / (blocks > 0 ? blocks : 1);
-  if (s > seen / 256) s = seen / 256;
-  if (s < 1) s = 1;
-  const long long keys = ((seen + s - 1) / s + KT - 1) / KT * KT;
-  *split_keys = (int)keys;
-  *splits = (int)((seen + keys - 1) / keys);
-}
-
 template <int DH, bool F8, int WM>
 static int launch_rows(const RowsParams& P, dim3 grid, cudaStream_t stream) {
   constexpr int smem = RowsTile<DH, F8>::SMEM;
@@ -528,44 +474,19 @@ static int launch_rows(const RowsParams& P, dim3 grid, cudaStream_t stream) {
 }
 template <int DH, bool F8>
 static int launch_rows_of(const RowsParams& P, int max_count, cudaStream_t stream) {
-  const int rows = max_count * (P.Hq / P.Hkv), per_block = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  const int rows = max_count * (P.Hq / P.Hkv), per_block = rows <= 32 ? 32 : 64;
   const long long gx = (long long)P.n_items * P.splits, gy = (long long)P.Hkv * ((rows + per_block - 1) / per_block);
   JLX_REQUIRE(gx < (1ll << 31) && gy <= 65535, "attention over rows: too many items or rows");
+  JLX_REQUIRE(P.splits == 1 || (P.part_o && P.part_ml), "attention over rows: scratch for the ranges is missing");
   const dim3 grid((unsigned)gx, (unsigned)gy);
-  if (int rc = per_block == 16 ? launch_rows<DH, F8, 1>(P, grid, stream) : per_block == 32 ? launch_rows<DH, F8, 2>(P, grid, stream) : launch_rows<DH, F8, 4>(P, grid, stream)) return rc;
-  if (P.splits > 1) {
-    const long long jy = ((long long)max_count * P.Hq + 7) / 8;
-    JLX_REQUIRE(jy <= 65535, "attention over rows: an item has too many rows to join");
-    JLX_CUDA(jlx_launch_pdl(attention_rows_join_kernel<DH>, dim3(P.n_items, (unsigned)jy), dim3(256), 0, stream, P));
-  }
-  return 0;
+  if (int rc = per_block == 32 ? launch_rows<DH, F8, 2>(P, grid, stream) : launch_rows<DH, F8, 4>(P, grid, stream)) return rc;
+  return P.splits > 1 ? launch_rows_join<DH>(P, max_count, stream) : 0;
 }
 
-JLX_API int jlx_attention_rows(const void* q, const void* pages, const void* scales, const int* block_table, int bt_stride, int n_requests,
-                               const int* req_of_token, const int* positions, void* out, const int* items, const int* rows, int n_items,
-                               int max_count, const int* cu_q, const int* q_start, const int* masks, int words, int N, int Hq, int Hkv,
-                               int dh, int page_size, int num_pages, float scale, float softcap, int chunk, int window, float attn_scale,
-                               float floor_scale, const float* sink, const float* slopes, int splits, int split_keys, float* part_o,
-                               float* part_ml, int* status, cudaStream_t stream) {
-  JLX_REQUIRE(jlx_attention_rows_supported(Hq, Hkv, dh), "attention over rows: %d query heads on %d of %d entries (64 or 128) are not supported", Hq, Hkv, dh);
-  JLX_REQUIRE(N > 0 && n_items >= 0 && max_count > 0 && page_size > 0 && num_pages > 0 && bt_stride > 0 && n_requests > 0, "attention over rows: bad sizes");
-  JLX_REQUIRE((long long)num_pages * 2 * Hkv * page_size < (1ll << 31), "attention over rows: cache too large for 32-bit rows");
-  JLX_REQUIRE((((uintptr_t)q | (uintptr_t)pages | (uintptr_t)out) & 15) == 0, "attention over rows: q, pages and out must be 16-byte aligned");
-  JLX_REQUIRE(attn_scale == 0.f || floor_scale > 0.f, "attention: floor_scale must be positive");
-  JLX_REQUIRE(softcap >= 0.f && chunk >= 0 && window >= 0, "attention: the score cap, chunk and window must not be negative (0: none)");
-  JLX_REQUIRE(splits >= 1 && split_keys > 0 && split_keys % KT == 0 && (long long)splits * split_keys < (1ll << 30), "attention over rows: bad ranges");
-  JLX_REQUIRE(splits == 1 || (part_o && part_ml && ((uintptr_t)part_o & 15) == 0 && ((uintptr_t)part_ml & 7) == 0), "attention over rows: scratch for the ranges is missing");
-  JLX_REQUIRE(!cu_q == !masks && !cu_q == !q_start && (!cu_q || (items && words > 0)), "attention over rows: a tree needs its offsets, cached lengths, masks and items");
-  if (n_items == 0) return 0;
-  RowsParams P = {};
-  P.q = (const bf16*)q; P.pages = pages; P.scales = (const uint8_t*)scales; P.block_table = block_table; P.bt_stride = bt_stride;
-  P.n_requests = n_requests; P.req_of_token = req_of_token; P.positions = positions; P.out = (bf16*)out; P.items = items; P.rows = rows;
-  P.n_items = n_items; P.cu_q = cu_q; P.q_start = q_start; P.masks = masks; P.words = words; P.N = N; P.Hq = Hq; P.Hkv = Hkv;
-  P.page_size = page_size; P.num_pages = num_pages;
-  P.scale_log2 = softcap > 0.f ? scale / softcap : scale * LOG2E;
-  P.cap_log2 = softcap > 0.f ? softcap * LOG2E : 0.f;
-  P.chunk = chunk; P.window = window; P.attn_scale = attn_scale; P.floor_scale = floor_scale; P.sink = sink; P.slopes = slopes;
-  P.splits = splits; P.split_keys = split_keys; P.part_o = part_o; P.part_ml = (float2*)part_ml; P.status = status;
-  if (dh == 128) return scales ? launch_rows_of<128, true>(P, max_count, stream) : launch_rows_of<128, false>(P, max_count, stream);
-  return scales ? launch_rows_of<64, true>(P, max_count, stream) : launch_rows_of<64, false>(P, max_count, stream);
+JLX_API int jlx_attention_rows(const RowsArgs* a, cudaStream_t stream) {
+  RowsParams P;
+  if (rows_params(*a, P)) return 1;
+  if (P.n_items == 0) return 0;
+  if (a->dh == 128) return a->scales ? launch_rows_of<128, true>(P, a->max_count, stream) : launch_rows_of<128, false>(P, a->max_count, stream);
+  return a->scales ? launch_rows_of<64, true>(P, a->max_count, stream) : launch_rows_of<64, false>(P, a->max_count, stream);
 }

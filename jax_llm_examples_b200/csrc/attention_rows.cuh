@@ -125,3 +125,77 @@ __device__ __forceinline__ float rows_inverse(const RowsParams& P, float m, floa
   if (P.sink) l += exp2f(P.sink[head] * LOG2E - m);  // (a row that sees nothing has m = NEG_BIG: the term is infinite, the row 0)
   return l == 0.f ? 0.f : 1.f / l;
 }
+
+// Joins the ranges of a row from scratch: a warp per row, DH / 32 entries a lane.
+template <int DH>
+__global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowsParams P) {
+  JLX_TL(TL_ATTN_COMBINE);
+  pdl_launch_dependents_if_small();
+  pdl_wait();
+  RowsItem it;
+  if (!rows_item(P, blockIdx.x, it)) return;
+  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (row >= it.cnt * P.Hq) return;
+  const int head = row % P.Hq;
+  const size_t at = (size_t)it.n0 * P.Hq + row;
+  const float2* ml = P.part_ml + at * P.splits;
+  float m = ROWS_NEG_BIG;
+  for (int s = lane; s < P.splits; s += 32) m = fmaxf(m, ml[s].x);
+  m = warp_max(m);
+  constexpr int E = DH / 32;
+  float acc[E], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) acc[i] = 0.f;
+  const float* po = P.part_o + at * P.splits * DH + lane * E;
+#pragma unroll 4
+  for (int s = 0; s < P.splits; ++s) {
+    const float2 x = ml[s];
+    const float f = x.x == m ? 1.f : rows_exp2(x.x - m);
+    l = fmaf(x.y, f, l);
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] = fmaf(po[(size_t)s * DH + i], f, acc[i]);
+  }
+  const float inv = rows_inverse(P, m, l, head);
+#pragma unroll
+  for (int i = 0; i < E; i += 2)
+    *reinterpret_cast<__nv_bfloat162*>(P.out + at * DH + lane * E + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
+}
+
+// -------------------------------------------------------------------------------------------- host
+// What the callers hand over (_RowsArgs in kernels/api.py).
+struct RowsArgs {
+  const void *q, *pages, *scales, *block_table, *req_of_token, *positions, *out, *items, *rows, *cu_q, *q_start, *masks, *sink, *slopes, *part_o, *part_ml, *status;
+  int bt_stride, n_requests, n_items, max_count, words, N, Hq, Hkv, dh, page_size, num_pages, chunk, window, splits, split_keys;
+  float scale, softcap, attn_scale, floor_scale;
+};
+
+static int rows_params(const RowsArgs& a, RowsParams& P) {
+  JLX_REQUIRE(a.Hkv > 0 && a.Hq > 0 && a.Hq % a.Hkv == 0 && (a.dh == 64 || a.dh == 128), "attention over rows: %d query heads on %d of %d entries (64 or 128) are not supported", a.Hq, a.Hkv, a.dh);
+  JLX_REQUIRE(a.N > 0 && a.n_items >= 0 && a.max_count > 0 && a.page_size > 0 && a.num_pages > 0 && a.bt_stride > 0 && a.n_requests > 0, "attention over rows: bad sizes");
+  JLX_REQUIRE((long long)a.num_pages * 2 * a.Hkv * a.page_size < (1ll << 31), "attention over rows: cache too large for 32-bit rows");
+  JLX_REQUIRE((((uintptr_t)a.q | (uintptr_t)a.pages | (uintptr_t)a.out) & 15) == 0, "attention over rows: q, pages and out must be 16-byte aligned");
+  JLX_REQUIRE(a.attn_scale == 0.f || a.floor_scale > 0.f, "attention: floor_scale must be positive");
+  JLX_REQUIRE(a.softcap >= 0.f && a.chunk >= 0 && a.window >= 0, "attention: the score cap, chunk and window must not be negative (0: none)");
+  JLX_REQUIRE(a.splits >= 1 && a.split_keys > 0 && a.split_keys % 64 == 0 && (long long)a.splits * a.split_keys < (1ll << 30), "attention over rows: bad ranges");
+  JLX_REQUIRE((((uintptr_t)a.part_o & 15) | ((uintptr_t)a.part_ml & 7)) == 0, "attention over rows: scratch for the ranges is not aligned");
+  JLX_REQUIRE(!a.cu_q == !a.masks && !a.cu_q == !a.q_start && (!a.cu_q || (a.items && a.words > 0)), "attention over rows: a tree needs its offsets, cached lengths, masks and items");
+  JLX_REQUIRE((long long)a.max_count * a.Hq < (1ll << 30), "attention over rows: an item has too many rows");
+  P.q = (const bf16*)a.q; P.pages = a.pages; P.scales = (const uint8_t*)a.scales; P.block_table = (const int*)a.block_table; P.bt_stride = a.bt_stride;
+  P.n_requests = a.n_requests; P.req_of_token = (const int*)a.req_of_token; P.positions = (const int*)a.positions; P.out = (bf16*)a.out;
+  P.items = (const int*)a.items; P.rows = (const int*)a.rows; P.n_items = a.n_items; P.cu_q = (const int*)a.cu_q; P.q_start = (const int*)a.q_start;
+  P.masks = (const int*)a.masks; P.words = a.words; P.N = a.N; P.Hq = a.Hq; P.Hkv = a.Hkv; P.page_size = a.page_size; P.num_pages = a.num_pages;
+  P.scale_log2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E;
+  P.cap_log2 = a.softcap > 0.f ? a.softcap * LOG2E : 0.f;
+  P.chunk = a.chunk; P.window = a.window; P.attn_scale = a.attn_scale; P.floor_scale = a.floor_scale;
+  P.sink = (const float*)a.sink; P.slopes = (const float*)a.slopes; P.splits = a.splits; P.split_keys = a.split_keys;
+  P.part_o = (float*)a.part_o; P.part_ml = (float2*)a.part_ml; P.status = (int*)a.status;
+  return 0;
+}
+
+template <int DH>
+static int launch_rows_join(const RowsParams& P, int max_count, cudaStream_t stream) {
+  const long long jy = ((long long)max_count * P.Hq + 7) / 8;
+  JLX_REQUIRE(jy <= 65535, "attention over rows: an item has too many rows to join");
+  JLX_CUDA(jlx_launch_pdl(attention_rows_join_kernel<DH>, dim3(P.n_items, (unsigned)jy), dim3(256), 0, stream, P));
+  return 0;
+}

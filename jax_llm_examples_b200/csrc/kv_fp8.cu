@@ -251,46 +251,53 @@ static int lanes_of(int dh) {
   return l;
 }
 
-JLX_API int jlx_kv_store_fp8(const void* k, const void* v, int dtype, void* pages, void* scales, const int* block_table, int bt_stride,
-                             int n_requests, const int* req_of_token, const int* places, int N, int Hkv, int dh, int page_size,
-                             int num_pages, int* status, cudaStream_t stream) {
-  const KvFp8Params P = {(uint8_t*)pages, (uint8_t*)scales, block_table, bt_stride, n_requests, req_of_token, places, N, Hkv, dh, page_size, num_pages, lanes_of(dh), status};
+// `cache`: what kernels/api.py fills in, but for the lanes.
+JLX_API int jlx_kv_store_fp8(const KvFp8Params* cache, const void* k, const void* v, int dtype, cudaStream_t stream) {
+  KvFp8Params P = *cache;
   if (kv_fp8_check("kv_store_fp8", P)) return 1;
-  if (N == 0) return 0;
+  if (P.N == 0) return 0;
+  P.lanes = lanes_of(P.dh);
   const int wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
   JLX_DISPATCH_DTYPE(dtype, T, {
-    JLX_CUDA(jlx_launch_pdl(kv_store_fp8_kernel<T>, dim3(N, kv_fp8_grid_y(N, 2 * Hkv, P.lanes)), dim3(256), 0, stream, (const T*)k, (const T*)v, P, wide));
+    JLX_CUDA(jlx_launch_pdl(kv_store_fp8_kernel<T>, dim3(P.N, kv_fp8_grid_y(P.N, 2 * P.Hkv, P.lanes)), dim3(256), 0, stream, (const T*)k, (const T*)v, P, wide));
   });
   return 0;
 }
 
-JLX_API int jlx_rope_kv_store_fp8(const void* qkv, int in_dtype, int splits, long long split_stride, void* q_out, void* pages, void* scales,
-                                  const int* block_table, int bt_stride, int n_requests, const int* req_of_token, const int* positions,
-                                  const int* places, const float* inv_freq, int l2norm, float eps, int N, int Hq, int Hkv, int dh,
-                                  int page_size, int num_pages, int* status, cudaStream_t stream) {
-  const KvFp8Params P = {(uint8_t*)pages, (uint8_t*)scales, block_table, bt_stride, n_requests, req_of_token, places, N, Hkv, dh, page_size, num_pages, lanes_of(dh), status};
+struct RopeFp8Args {
+  const void* qkv;
+  void* q_out;
+  const int* positions;
+  const float* inv_freq;
+  long long split_stride;
+  int in_dtype, splits, Hq, l2norm;
+  float eps;
+};
+
+JLX_API int jlx_rope_kv_store_fp8(const KvFp8Params* cache, const RopeFp8Args* a, cudaStream_t stream) {
+  KvFp8Params P = *cache;
   if (kv_fp8_check("rope_kv_store_fp8", P)) return 1;
-  JLX_REQUIRE(Hq > 0 && Hq <= 65535, "rope_kv_store_fp8: bad head count %d", Hq);
-  JLX_REQUIRE(splits >= 1 && (splits == 1 || in_dtype == JLX_F32), "rope_kv_store_fp8: split-K partials are float32");
-  if (N == 0) return 0;
-  const int wide = (((uintptr_t)qkv | (uintptr_t)q_out) & 15) == 0 && split_stride % 4 == 0;
-  const size_t smem = (size_t)dh / 2 * sizeof(float2);
-  JLX_DISPATCH_DTYPE(in_dtype, TI, {
-    JLX_CUDA(jlx_launch_pdl(rope_kv_store_fp8_kernel<TI>, dim3(N, kv_fp8_grid_y(N, Hq + 2 * Hkv, P.lanes)), dim3(256), smem, stream, (const TI*)qkv,
-                            splits, split_stride, (bf16*)q_out, P, positions, inv_freq, l2norm, eps, Hq, wide));
+  JLX_REQUIRE(a->Hq > 0 && a->Hq <= 65535, "rope_kv_store_fp8: bad head count %d", a->Hq);
+  JLX_REQUIRE(a->splits >= 1 && (a->splits == 1 || a->in_dtype == JLX_F32), "rope_kv_store_fp8: split-K partials are float32");
+  if (P.N == 0) return 0;
+  P.lanes = lanes_of(P.dh);
+  const int wide = (((uintptr_t)a->qkv | (uintptr_t)a->q_out) & 15) == 0 && a->split_stride % 4 == 0;
+  const size_t smem = (size_t)P.dh / 2 * sizeof(float2);
+  JLX_DISPATCH_DTYPE(a->in_dtype, TI, {
+    JLX_CUDA(jlx_launch_pdl(rope_kv_store_fp8_kernel<TI>, dim3(P.N, kv_fp8_grid_y(P.N, a->Hq + 2 * P.Hkv, P.lanes)), dim3(256), smem, stream, (const TI*)a->qkv,
+                            a->splits, a->split_stride, (bf16*)a->q_out, P, a->positions, a->inv_freq, a->l2norm, a->eps, a->Hq, wide));
   });
   return 0;
 }
 
-JLX_API int jlx_kv_load_fp8(const void* pages, const void* scales, const int* block_table, int bt_stride, int n_requests, const int* req_of_token,
-                            const int* places, void* k, void* v, int dtype, int N, int Hkv, int dh, int page_size, int num_pages, int* status,
-                            cudaStream_t stream) {
-  const KvFp8Params P = {(uint8_t*)pages, (uint8_t*)scales, block_table, bt_stride, n_requests, req_of_token, places, N, Hkv, dh, page_size, num_pages, lanes_of(dh), status};
+JLX_API int jlx_kv_load_fp8(const KvFp8Params* cache, void* k, void* v, int dtype, cudaStream_t stream) {
+  KvFp8Params P = *cache;
   if (kv_fp8_check("kv_load_fp8", P)) return 1;
-  if (N == 0) return 0;
+  if (P.N == 0) return 0;
+  P.lanes = lanes_of(P.dh);
   const int wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
   JLX_DISPATCH_DTYPE(dtype, T, {
-    JLX_CUDA(jlx_launch_pdl(kv_load_fp8_kernel<T>, dim3(N, kv_fp8_grid_y(N, 2 * Hkv, P.lanes)), dim3(256), 0, stream, P, (T*)k, (T*)v, wide));
+    JLX_CUDA(jlx_launch_pdl(kv_load_fp8_kernel<T>, dim3(P.N, kv_fp8_grid_y(P.N, 2 * P.Hkv, P.lanes)), dim3(256), 0, stream, P, (T*)k, (T*)v, wide));
   });
   return 0;
 }

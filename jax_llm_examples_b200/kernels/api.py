@@ -1111,16 +1111,23 @@ FP8 = torch.float8_e4m3fn  # pages in 8 bits: e4m3 codes, and a byte of scale pe
 def _ints(what: str, **tensors: "tuple[torch.Tensor | None, int]") -> None:
     """Index arrays: contiguous int32 with at least so many entries."""
     for name, (t, n) in tensors.items():
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n):
+        if t is not None and (t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous()):
             raise KernelError(f"{what}: {name} must be contiguous int32 with at least {n} entries")
 
 
-def _on_device(what: str, *tensors: torch.Tensor | None) -> None:
-    """A launch goes to the current device's stream: tensors of another device have no place in it."""
+def _same_device(what: str, *tensors: torch.Tensor | None) -> int:
+    """The current device, to whose stream a launch goes: tensors of another device, or of none, have no place in it."""
     dev = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.is_cuda and t.device.index != dev:
+        if t is not None and t.get_device() != dev:
+            if not t.is_cuda:
+                raise KernelError(f"{what}: a kernel was given a tensor that is not on the GPU; there is no CPU path")
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
+    return dev
+
+
+def _raw_stream(dev: int):
+    return c_void_p(torch._C._cuda_getCurrentRawStream(dev))
 
 
 def _cache8(what: str, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, Hkv: int, dh: int) -> None:
@@ -1133,8 +1140,22 @@ def _cache8(what: str, pages: torch.Tensor, scales: torch.Tensor, block_table: t
     _contig(pages, scales, block_table)
 
 
-def _cache8_args(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor) -> tuple:
-    return (_ptr(pages), _ptr(scales), _ptr(block_table), c_int(block_table.shape[1]), c_int(block_table.shape[0]))
+class _KvFp8Args(ctypes.Structure):  # KvFp8Params in csrc/kv_fp8.cu
+    _fields_ = [("pages", c_void_p), ("scales", c_void_p), ("block_table", c_void_p), ("bt_stride", c_int), ("n_requests", c_int),
+                ("req_of_token", c_void_p), ("places", c_void_p), ("N", c_int), ("Hkv", c_int), ("dh", c_int), ("page_size", c_int),
+                ("num_pages", c_int), ("lanes", c_int), ("status", c_void_p)]
+
+
+class _RopeFp8Args(ctypes.Structure):  # RopeFp8Args in csrc/kv_fp8.cu
+    _fields_ = [("qkv", c_void_p), ("q_out", c_void_p), ("positions", c_void_p), ("inv_freq", c_void_p), ("split_stride", c_longlong), ("in_dtype", c_int),
+                ("splits", c_int), ("Hq", c_int), ("l2norm", c_int), ("eps", c_float)]
+
+
+def _kv_fp8_args(pages, scales, block_table, req_of_token, places, N: int, status) -> _KvFp8Args:
+    P, _, Hkv, page_size, dh = pages.shape
+    R, width = block_table.shape
+    return _KvFp8Args(pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), width, R, req_of_token.data_ptr(), places.data_ptr(), N, Hkv, dh,
+                      page_size, P, 0, status.data_ptr())
 
 
 def kv_store_fp8(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
@@ -1151,9 +1172,9 @@ def kv_store_fp8(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: 
     _ints("kv_store_fp8", req_of_token=(req_of_token, N), places=(places, N), status=(status, 1))
     if v.shape != k.shape or v.dtype != k.dtype:
         raise KernelError("kv_store_fp8: keys and values must have one shape and type")
-    _on_device("kv_store_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
-    _run("kv_fp8", "jlx_kv_store_fp8", _ptr(k), _ptr(v), c_int(code(k.dtype)), *_cache8_args(pages, scales, block_table), _ptr(req_of_token),
-         _ptr(places), c_int(N), c_int(Hkv), c_int(dh), c_int(pages.shape[3]), c_int(pages.shape[0]), _ptr(status), _stream())
+    dev = _same_device("kv_store_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
+    args = _kv_fp8_args(pages, scales, block_table, req_of_token, places, N, status)
+    _run("kv_fp8", "jlx_kv_store_fp8", ctypes.byref(args), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
 
 
 def rope_kv_store_fp8(qkv: torch.Tensor, q_out: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
@@ -1172,11 +1193,11 @@ def rope_kv_store_fp8(qkv: torch.Tensor, q_out: torch.Tensor, pages: torch.Tenso
                           f"fit qkv {tuple(qkv.shape)}, q_out {q_out.dtype} {tuple(q_out.shape)}")
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != dh // 2):
         raise KernelError(f"rope_kv_store_fp8: {dh // 2} float32 frequencies are needed")
-    _on_device("rope_kv_store_fp8", qkv, q_out, pages, scales, block_table, req_of_token, positions, places, inv_freq, status)
-    sp, stride = _splits(qkv, splits)
-    _run("kv_fp8", "jlx_rope_kv_store_fp8", _ptr(qkv), c_int(code(qkv.dtype)), c_int(sp), c_longlong(stride), _ptr(q_out),
-         *_cache8_args(pages, scales, block_table), _ptr(req_of_token), _ptr(positions), _ptr(places), _ptr(inv_freq), c_int(int(l2norm)),
-         c_float(eps), c_int(N), c_int(Hq), c_int(Hkv), c_int(dh), c_int(pages.shape[3]), c_int(pages.shape[0]), _ptr(status), _stream())
+    dev = _same_device("rope_kv_store_fp8", qkv, q_out, pages, scales, block_table, req_of_token, positions, places, inv_freq, status)
+    args = _kv_fp8_args(pages, scales, block_table, req_of_token, places, N, status)
+    rope = _RopeFp8Args(qkv.data_ptr(), q_out.data_ptr(), positions.data_ptr(), None if inv_freq is None else inv_freq.data_ptr(),
+                        0 if splits == 1 else qkv.numel() // splits, code(qkv.dtype), splits, Hq, int(l2norm), eps)
+    _run("kv_fp8", "jlx_rope_kv_store_fp8", ctypes.byref(args), ctypes.byref(rope), _raw_stream(dev))
 
 
 def kv_load_fp8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, req_of_token: torch.Tensor, places: torch.Tensor,
@@ -1189,22 +1210,55 @@ def kv_load_fp8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Te
     _ints("kv_load_fp8", req_of_token=(req_of_token, N), places=(places, N), status=(status, 1))
     if v.shape != k.shape or v.dtype != k.dtype:
         raise KernelError("kv_load_fp8: keys and values must have one shape and type")
-    _on_device("kv_load_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
-    _run("kv_fp8", "jlx_kv_load_fp8", *_cache8_args(pages, scales, block_table), _ptr(req_of_token), _ptr(places), _ptr(k), _ptr(v),
-         c_int(code(k.dtype)), c_int(N), c_int(Hkv), c_int(dh), c_int(pages.shape[3]), c_int(pages.shape[0]), _ptr(status), _stream())
+    dev = _same_device("kv_load_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
+    args = _kv_fp8_args(pages, scales, block_table, req_of_token, places, N, status)
+    _run("kv_fp8", "jlx_kv_load_fp8", ctypes.byref(args), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
+
+
+class _RowsArgs(ctypes.Structure):  # RowsArgs in csrc/attention_rows.cuh
+    _fields_ = [(n, c_void_p) for n in ("q", "pages", "scales", "block_table", "req_of_token", "positions", "out", "items", "rows", "cu_q", "q_start",
+                                        "masks", "sink", "slopes", "part_o", "part_ml", "status")] + \
+               [(n, c_int) for n in ("bt_stride", "n_requests", "n_items", "max_count", "words", "N", "Hq", "Hkv", "dh", "page_size", "num_pages", "chunk",
+                                     "window", "splits", "split_keys")] + \
+               [(n, c_float) for n in ("scale", "softcap", "attn_scale", "floor_scale")]
+
+
+ROWS_TILE = 64  # keys of a tile, csrc/attention_rows.cu and attention_few.cu
+ROWS_FEW = 16  # query rows of an item and KV head that attention_few.cu takes
+ROWS_CLUSTER = 8  # ranges that it joins without scratch
 
 
 def attention_rows_supported(q_dtype: torch.dtype, Hq: int, Hkv: int, dh: int) -> bool:
     """Whether :func:`attention_fp8` and :func:`attention_tree` take these queries (bfloat16, head size 64 or 128)."""
-    return q_dtype == torch.bfloat16 and bool(library("attention_rows").jlx_attention_rows_supported(c_int(Hq), c_int(Hkv), c_int(dh)))
+    return q_dtype == torch.bfloat16 and dh in (64, 128) and Hkv > 0 and Hq % Hkv == 0
+
+
+def attention_rows_plan(max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int) -> tuple[int, int]:
+    """(ranges that an item's keys are cut into, keys of a range)."""
+    seen = min(max_kv_len, window + max_count if window else max_kv_len, chunk + max_count if chunk else max_kv_len) + ROWS_TILE  # ranges start at a tile's first key
+    rows = max_count * (Hq // Hkv)
+    if rows <= ROWS_FEW:
+        # Three blocks share a multiprocessor.  Fewer blocks than places: ranges fill them, down to two tiles each (a range's
+        # set-up and join cost as much).  More: ranges that make four rounds or so, of at least 16 tiles, so that the last round's
+        # idle places are few.
+        blocks, places = n_items * Hkv, 3 * sms
+        splits = places // blocks if blocks < places else -(-4 * places // blocks)
+        splits = max(1, min(splits, seen // (2 * ROWS_TILE if blocks < places else 16 * ROWS_TILE)))
+        if splits > ROWS_CLUSTER and splits < 2 * ROWS_CLUSTER:
+            splits = ROWS_CLUSTER  # (joining through scratch costs a launch)
+    else:
+        blocks = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64))
+        splits = max(1, min(3 * sms // blocks, seen // 256))
+    keys = -(-(-(-seen // splits)) // ROWS_TILE) * ROWS_TILE
+    return -(-seen // keys), keys
 
 
 def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, positions, out, scale, chunk, window, attn_scale, floor_scale, status,
-                    max_kv_len, items, rows, n_items, max_count, tree, sink, slopes, softcap) -> None:
-    _contig(q, pages, scales, block_table, out)
+                    max_kv_len, items, rows, n_items, max_count, cu_q, q_start, masks, sink, slopes, softcap) -> None:
     N, Hq, dh = q.shape
     P, two, Hkv, page_size, dh2 = pages.shape
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != q.shape or out.data_ptr() == q.data_ptr():
+    out_p, q_p = out.data_ptr(), q.data_ptr()
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != q.shape or out_p == q_p:
         raise KernelError(f"{what}: queries and output must be bfloat16 [N, Hq, dh], and not the same rows")
     if dh2 != dh or two != 2:
         raise KernelError(f"{what}: cache pages {tuple(pages.shape)} and queries {tuple(q.shape)} disagree")
@@ -1214,34 +1268,40 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
         raise KernelError(f"{what}: pages must be bfloat16, or float8_e4m3fn with scales")
     if block_table.dtype != torch.int32 or block_table.dim() != 2:
         raise KernelError(f"{what}: the block table must be int32 [requests, pages of one]")
-    R = block_table.shape[0]
-    cu_q, q_start, masks = tree
+    R, width = block_table.shape
     _ints(what, req_of_token=(req_of_token, N), positions=(positions, N), items=(items, 2 * n_items), rows=(rows, n_items), status=(status, 1),
           cu_q=(cu_q, R + 1), q_start=(q_start, R), masks=(masks, N))
-    if masks is not None and (masks.dim() != 2 or masks.shape[0] != N):
-        raise KernelError(f"{what}: masks must be int32 [{N}, words], a bit per drafted token of the request")
+    words = 0
+    if masks is not None:
+        if masks.dim() != 2 or masks.shape[0] != N:
+            raise KernelError(f"{what}: masks must be int32 [{N}, words], a bit per drafted token of the request")
+        words = masks.shape[1]
     if max_kv_len < 1 or max_count < 1 or n_items < 0 or (items is None and rows is None and n_items > N):
         raise KernelError(f"{what}: {n_items} items of up to {max_count} tokens over {max_kv_len} keys")
     _check_sink(sink, Hq)
     _check_sink(slopes, Hq, "slopes")
-    _on_device(what, q, pages, scales, block_table, req_of_token, positions, out, items, rows, cu_q, q_start, masks, sink, slopes, status)
+    _contig(q, pages, block_table, out)
+    dev = _same_device(what, q, pages, scales, block_table, req_of_token, positions, out, items, rows, cu_q, q_start, masks, sink, slopes, status)
     if N == 0 or n_items == 0:
         return
-    splits, split_keys = c_int(1), c_int(1)
-    library("attention_rows").jlx_attention_rows_plan(c_int(max_kv_len), c_int(chunk), c_int(window), c_int(n_items), c_int(max_count), c_int(Hq), c_int(Hkv),
-                                                      c_int(sm_count()), ctypes.byref(splits), ctypes.byref(split_keys))
-    part_o = part_ml = None
-    if splits.value > 1:
+    if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
+        raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
+    splits, split_keys = attention_rows_plan(max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
+    few = max_count * (Hq // Hkv) <= ROWS_FEW
+    part_o = part_ml = joined = 0
+    if splits > (ROWS_CLUSTER if few else 1):
         # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
-        part_o = torch.empty(N * Hq * splits.value * dh, dtype=torch.float32, device=q.device)
-        part_ml = torch.empty(N * Hq * splits.value * 2, dtype=torch.float32, device=q.device)
-    _run("attention_rows", "jlx_attention_rows", _ptr(q), _ptr(pages), _ptr(scales), _ptr(block_table), c_int(block_table.shape[1]), c_int(R),
-         _ptr(req_of_token), _ptr(positions), _ptr(out), _ptr(items), _ptr(rows), c_int(n_items), c_int(max_count), _ptr(cu_q), _ptr(q_start),
-         _ptr(masks), c_int(masks.shape[1] if masks is not None else 0), c_int(N), c_int(Hq), c_int(Hkv), c_int(dh), c_int(page_size), c_int(P),
-         c_float(scale), c_float(softcap), c_int(chunk), c_int(window), c_float(attn_scale), c_float(floor_scale), _ptr(sink), _ptr(slopes),
-         splits, split_keys, _ptr(part_o), _ptr(part_ml), _ptr(status), _stream())
+        scratch = torch.empty(N * Hq * splits * (dh + 2), dtype=torch.float32, device=q.device)
+        part_o = scratch.data_ptr()
+        part_ml, joined = part_o + 4 * N * Hq * splits * dh, 1
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    args = _RowsArgs(q_p, pages.data_ptr(), p(scales), block_table.data_ptr(), req_of_token.data_ptr(), positions.data_ptr(), out_p, p(items), p(rows),
+                     p(cu_q), p(q_start), p(masks), p(sink), p(slopes), part_o, part_ml, status.data_ptr(), width, R, n_items, max_count, words, N, Hq,
+                     Hkv, dh, page_size, P, chunk, window, splits, split_keys, scale, softcap, attn_scale, floor_scale)
+    name = "attention_few" if few else "attention_rows"
+    _run(name, "jlx_" + name, ctypes.byref(args), _raw_stream(dev))
     global _launches
-    _launches += int(splits.value > 1)  # the joining kernel
+    _launches += joined  # the joining kernel
 
 
 def attention_fp8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, req_of_token: torch.Tensor,
@@ -1257,7 +1317,7 @@ def attention_fp8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, bl
     if scales is None:
         raise KernelError("attention_fp8: a cache in 8 bits has scales")
     _attention_rows("attention_fp8", q, pages, scales, block_table, req_of_token, positions, out, scale, chunk, window, attn_scale, floor_scale,
-                    status, max_kv_len, items, None if items is not None else rows, n, max_count if items is not None else 1, (None, None, None),
+                    status, max_kv_len, items, None if items is not None else rows, n, max_count if items is not None else 1, None, None, None,
                     sink, slopes, softcap)
 
 
@@ -1276,7 +1336,7 @@ def attention_tree(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tens
     if cu_q is None or q_start is None or masks is None or items is None:
         raise KernelError("attention_tree: offsets, cached lengths, masks and items are needed")
     _attention_rows("attention_tree", q, pages, scales, block_table, req_of_token, positions, out, scale, chunk, window, attn_scale, floor_scale,
-                    status, max_kv_len, items, None, n_items, max_count, (cu_q, q_start, masks), sink, slopes, softcap)
+                    status, max_kv_len, items, None, n_items, max_count, cu_q, q_start, masks, sink, slopes, softcap)
 
 
 def tree_masks(parents) -> "tuple[list[int], list[list[int]]]":
