@@ -2,8 +2,10 @@
 // single decoded tokens and small drafted trees (attention_rows.cuh has mask and formula), head sizes 64 and 128.  It reads
 // every key once and computes little with it: bytes bound it, and the instructions that stand between a byte and a product.
 //
-// A block takes one range of an item's keys, in tiles of 64: a warp of its own fetches them by cp.async, row by row through the
-// block table (any page size), up to STAGES tiles ahead; four warps take 16 keys of every tile each and meet only at the end.
+// A block takes one range of an item's keys, in tiles of 64: a warp of its own fetches them up to STAGES tiles ahead, by TMA
+// where pages hold whole boxes of 16, 32 or 64 rows (a lane per box: its entry of the block table, a tile ahead, and a few
+// copies), else by cp.async, row by row (any page size; that warp then sets the pace).  Four warps take 16 keys of every tile
+// each and meet only at the end.
 //
 // The products are transposed, S^T = K Q^T and O^T = V^T P^T: keys and entries fill the 16 rows of a tensor-core tile and the
 // query rows its 8 columns, of which a group of 5 heads wastes 3, not 11 of 16.  That halves products, scores, exponentials and
@@ -31,6 +33,7 @@
 // Ranges of one item (few items, long contexts) are a thread-block cluster of up to 8: they leave their sums in shared memory
 // and each reads its share of the others' there, no second kernel and no scratch.  More ranges than that go through scratch.
 #include <cooperative_groups.h>
+#include <cuda.h>
 
 #include "attention_rows.cuh"
 #include "mbarrier.cuh"
@@ -55,32 +58,45 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 
-// Where 16-byte chunk c of row `row` lies in a tile whose rows have CH chunks: rows that are read together (eight of one chunk,
-// or two of four neighbouring chunks) fall on different banks.
-template <int CH> __device__ __forceinline__ int chunk_at(int row, int c) {
-  if (CH == 4) return row * CH + (c ^ ((row >> 1) & 3));
-  return row * CH + (c ^ (((row & 1) << 2) | ((row >> 1) & 3)));
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// Where 16-byte chunk c of row `row` lies in a tile of KT rows of CH chunks: as TMA's swizzle of rows of 64 or 128 bytes puts
+// it; rows of 256 bytes are two halves of 128.
+template <int CH> __device__ __forceinline__ int chunk_at(int row, int c) {
+  if (CH == 4) return row * 4 + (c ^ ((row >> 1) & 3));
+  return (c >> 3) * KT * 8 + row * 8 + ((c & 7) ^ (row & 7));
+}
+// The key at position i of eight in the products: two keys whose four chunks a quarter of a warp reads at once (positions 2i
+// and 2i + 1) then differ in bit 2 of the swizzle, and fall on different banks.
+__device__ __forceinline__ int key_at(int i) { return (i >> 1) | ((i & 1) << 2); }
 
 template <int DH, bool F8, int NG> struct FewTile {
   static constexpr int ELEM = F8 ? 1 : 2;
   static constexpr int CH = DH * ELEM / 16;     // 16-byte chunks per row
   static constexpr int BYTES = KT * DH * ELEM;  // keys or values of a tile
   static constexpr int STAGES = DH * ELEM >= 256 ? 3 : 4;
-  static constexpr int SCALE_BYTES = F8 ? 3 * KT * 4 : 0;  // per stage: the keys' scales; the values' (exponent, 2^-exponent)
+  static constexpr int SCALE_BYTES = F8 ? 2 * KT : 0;  // per stage: the keys' scale bytes, the values'
   static constexpr int LD = DH + 4;             // floats between rows of the outputs as the warps leave them
   static constexpr int RING = STAGES * (2 * BYTES + SCALE_BYTES);
   static constexpr int MERGE = (CONSUMERS + 1) * 8 * NG * (LD * 4 + 8);
-  static constexpr int SMEM = RING > MERGE ? RING : MERGE;
+  static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + 1024;  // (up to 1 KB for the alignment)
 };
 
 // NG: groups of 8 query rows (1, 2).
 template <int DH, bool F8, int NG>
-__global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(const RowsParams P, int clustered) {
+__global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(const __grid_constant__ CUtensorMap map, const RowsParams P, int clustered, int box_rows) {
   JLX_TL(TL_ATTN_DECODE);
   using T = FewTile<DH, F8, NG>;
   constexpr int CH = T::CH, STAGES = T::STAGES, ROWS = 8 * NG;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // where the swizzle's pattern starts
   __shared__ __align__(8) uint64_t bars[2 * STAGES];
   __shared__ int4 row_tok[ROWS];   // (token, head, position, first key) of the block's rows
   __shared__ float2 row_sc[ROWS];  // (score factor, slope)
@@ -99,7 +115,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
   auto EMPTY = [&](int s) { return bar0 + 8u * (STAGES + s); };
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(FULL(s), F8 ? 33 : 32);  // every lane's copies, and the scales' store
+      mbar_init(FULL(s), box_rows ? 1 : F8 ? 33 : 32);  // TMA's bytes; else every lane's copies, and the scales' store
       mbar_init(EMPTY(s), CONSUMERS);
     }
     any_bad = failed = 0;
@@ -121,30 +137,62 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
   const int* table = P.block_table + (size_t)it.r * P.bt_stride;
   const int v_off = P.Hkv * P.page_size;  // rows between a key and its value
   auto k_tile = [&](int s) { return smem + s * 2 * T::BYTES; };
-  auto scales_of = [&](int s) { return reinterpret_cast<float*>(smem + STAGES * 2 * T::BYTES + s * T::SCALE_BYTES); };
+  auto scales_of = [&](int s) { return smem + STAGES * 2 * T::BYTES + s * T::SCALE_BYTES; };
   __syncthreads();
 
   float m[NG][2], l[NG][2];
   float o[NG][DH / 16][4];
   if (warp == CONSUMERS) {
     // ------------------------------------------------------------------------------ the fetching warp
+    bool ok = true;
+    if (box_rows) {
+      // lane i has box i of every tile
+      const int boxes = KT / box_rows;
+      auto find_page = [&](int t) {
+        const int pi = (range0 + t * KT + lane * box_rows) / P.page_size;
+        return lane < boxes && t < n_tiles && pi < P.bt_stride ? table[pi] : -1;
+      };
+      int page = find_page(0);
+      int t = 0;
+#pragma unroll 1
+      for (; t < n_tiles; ++t) {
+        const int s = t % STAGES;
+        if (t >= STAGES) ok = mbar_wait(EMPTY(s), (t / STAGES - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(FULL(s), 2 * T::BYTES + T::SCALE_BYTES);
+        __syncwarp();
+        if (lane < boxes) {
+          const int place = range0 + t * KT + lane * box_rows;
+          if (page < 0 || page >= P.num_pages) {
+            if (place < end && place + box_rows > begin) atomicOr(P.status, JLX_STATUS_BAD_PAGE);
+            page = 0;  // no page there: every key of the box is masked
+          }
+          const int row = (page * 2 * P.Hkv + hk) * P.page_size + place % P.page_size;
+          const uint32_t dst = smem_u32(k_tile(s)) + lane * box_rows * (CH == 4 ? 64 : 128);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+#pragma unroll
+            for (int h = 0; h < (CH + 7) / 8; ++h) tma_load_2d(dst + w * T::BYTES + h * KT * 128, &map, h * 128 / T::ELEM, row + w * v_off, FULL(s));
+            if (F8) bulk_load(smem_u32(scales_of(s)) + w * KT + lane * box_rows, P.scales + row + w * v_off, box_rows, FULL(s));
+          }
+        }
+        page = find_page(t + 1);
+      }
+      if (!ok)  // let the copies in flight land before the block's shared memory is given up
+        for (int u = max(0, t - STAGES); u < t; ++u) mbar_wait(FULL(u % STAGES), (u / STAGES) & 1);
+    } else {
     // Lane i knows the rows of keys 2i and 2i + 1 of the tile; each copy instruction takes 32 / CH rows.  The scales of a tile
     // are loaded before its copies are issued and stored a tile later, when they have come.
-    bool ok = true;
     auto find_rows = [&](int t) {
       const int place = range0 + t * KT + 2 * lane;
       return make_int2(t < n_tiles && place >= begin && place < end ? rows_cache_row(P, table, hk, place) : -1,
                        t < n_tiles && place + 1 >= begin && place + 1 < end ? rows_cache_row(P, table, hk, place + 1) : -1);
     };
     auto put_scales = [&](int t, const int4& bytes) {
-      float* sc = scales_of(t % STAGES);
-      auto value = [](int b) {
-        return b == FP8_BAD ? make_float2(__int_as_float(0x7fc00000), 1.f)
-                            : (b == 0 ? make_float2(0.f, 1.f) : make_float2((float)(b - 127), fp8_pow2(max(-60, min(60, 127 - b)))));
-      };
-      *reinterpret_cast<float2*>(sc + 2 * lane) = make_float2(fp8_scale(bytes.x), fp8_scale(bytes.y));
-      const float2 v0 = value(bytes.z), v1 = value(bytes.w);
-      *reinterpret_cast<float4*>(sc + KT + 4 * lane) = make_float4(v0.x, v0.y, v1.x, v1.y);
+      uint8_t* sc = scales_of(t % STAGES);
+      *reinterpret_cast<uint16_t*>(sc + 2 * lane) = (uint16_t)(bytes.x | bytes.y << 8);
+      *reinterpret_cast<uint16_t*>(sc + KT + 2 * lane) = (uint16_t)(bytes.z | bytes.w << 8);
       __syncwarp();
       if (lane == 0) mbar_arrive(FULL(t % STAGES));
     };
@@ -185,6 +233,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
     if (F8 && ok && n_tiles > 0) put_scales(n_tiles - 1, bytes_before);
     cp_async_commit();
     cp_async_wait<0>();  // nothing is in flight when the ring is used for something else
+    }
     if (!ok && lane == 0) {
       atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
       failed = 1;
@@ -253,7 +302,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
     }
     const bool capped = P.cap_log2 > 0.f, sloped = P.slopes != nullptr;
     const int key0 = warp * 16;
-    const int kg = key0 + g, kl = key0 + (lane & 7);
+    const int kg = key0 + key_at(g), kl = key0 + key_at(lane & 7);
     bool ok = true;
 
 #pragma unroll 1
@@ -265,21 +314,28 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
       if (!ok) break;
       const uint8_t* kt = k_tile(st);
       uint8_t* vt = k_tile(st) + T::BYTES;
-      if (!F8 && masked) {  // a value that is not finite leaves the tile before the product (a warp reads its own keys' values only)
+      if (masked) {
+        // A value that is not finite leaves the tile before the product (a warp reads its own keys' values only).  Codes of rows
+        // outside the range may be anything, those of rows inside are numbers.
         bool any = false;
 #pragma unroll 1
         for (int i = lane; i < 16 * CH; i += 32) {
+          const int place = place0 + key0 + i / CH;
           uint4* at = reinterpret_cast<uint4*>(vt + chunk_at<CH>(key0 + i / CH, i % CH) * 16);
-          uint32_t w[4] = {at->x, at->y, at->z, at->w};
-          bool bad = false;
+          if (place < begin || place >= end) {
+            *at = make_uint4(0u, 0u, 0u, 0u);
+          } else if (!F8) {
+            uint32_t w[4] = {at->x, at->y, at->z, at->w};
+            bool bad = false;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if ((w[u] & 0x7f80u) == 0x7f80u) { w[u] &= 0xffff0000u; bad = true; }
-            if ((w[u] & 0x7f800000u) == 0x7f800000u) { w[u] &= 0xffffu; bad = true; }
-          }
-          if (bad) {
-            *at = make_uint4(w[0], w[1], w[2], w[3]);
-            any = true;
+            for (int u = 0; u < 4; ++u) {
+              if ((w[u] & 0x7f80u) == 0x7f80u) { w[u] &= 0xffff0000u; bad = true; }
+              if ((w[u] & 0x7f800000u) == 0x7f800000u) { w[u] &= 0xffffu; bad = true; }
+            }
+            if (bad) {
+              *at = make_uint4(w[0], w[1], w[2], w[3]);
+              any = true;
+            }
           }
         }
         if (any) any_bad = 1;
@@ -316,10 +372,17 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
         }
       }
       // ---- base-2 exponents of the weights, and which of them count
-      const float* sp = scales_of(st);
-      const float ks0 = F8 ? sp[kg] : 1.f, ks1 = F8 ? sp[kg + 8] : 1.f;
-      const float2 ve0 = F8 ? *reinterpret_cast<const float2*>(sp + KT + 2 * kg) : make_float2(0.f, 1.f);
-      const float2 ve1 = F8 ? *reinterpret_cast<const float2*>(sp + KT + 2 * (kg + 8)) : make_float2(0.f, 1.f);
+      float ks0 = 1.f, ks1 = 1.f, ve0 = 0.f, ve1 = 0.f, vi0 = 1.f, vi1 = 1.f;  // keys' scales; values' exponents and 2^-exponent
+      if (F8) {
+        const uint8_t* sp = scales_of(st) + kg;
+        const int bk0 = sp[0], bk1 = sp[8], bv0 = sp[KT], bv1 = sp[KT + 8];
+        ks0 = fp8_scale(bk0);
+        ks1 = fp8_scale(bk1);
+        ve0 = bv0 == FP8_BAD ? __int_as_float(0x7fc00000) : (float)(bv0 - 127);
+        ve1 = bv1 == FP8_BAD ? __int_as_float(0x7fc00000) : (float)(bv1 - 127);
+        vi0 = __int_as_float((254 - min(bv0, 254)) << 23);  // (finite for any byte: a masked key's weight is 0 and stays 0)
+        vi1 = __int_as_float((254 - min(bv1, 254)) << 23);
+      }
       float x[NG][4];
       bool grown = false;
 #pragma unroll
@@ -334,9 +397,9 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
             const int4 k = tk[ng][e & 1];
             const int place = place0 + kg + (e < 2 ? 0 : 8);
             const bool sees = place >= begin && place < end && rows_sees(P, it, k.x, k.z, k.w, place, key_pos);
-            v = sees ? fmaf(-slope[ng][e & 1], (float)(k.z - key_pos), v) + (F8 ? (e < 2 ? ve0.x : ve1.x) : 0.f) : -INFINITY;
+            v = sees ? fmaf(-slope[ng][e & 1], (float)(k.z - key_pos), v) + (F8 ? (e < 2 ? ve0 : ve1) : 0.f) : -INFINITY;
           } else if (F8) {
-            v += e < 2 ? ve0.x : ve1.x;
+            v += e < 2 ? ve0 : ve1;
           }
           x[ng][e] = v;
           grown |= v > m[ng][e & 1] + GROWTH;
@@ -367,7 +430,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           w[e] = rows_exp2(x[ng][e] - m[ng][e & 1]);  // (a masked key's exponent is -infinity: exactly 0)
-          l[ng][e & 1] = F8 ? fmaf(w[e], e < 2 ? ve0.y : ve1.y, l[ng][e & 1]) : l[ng][e & 1] + w[e];
+          l[ng][e & 1] = F8 ? fmaf(w[e], e < 2 ? vi0 : vi1, l[ng][e & 1]) : l[ng][e & 1] + w[e];
         }
         if (F8) {
           const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
@@ -520,6 +583,13 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
 template <int DH, bool F8, int NG>
 static int launch_few(const RowsParams& P, dim3 grid, cudaStream_t stream) {
   using T = FewTile<DH, F8, NG>;
+  // boxes of whole rows within a page (and its scales, 16 bytes at a time); 0: pages too small or ragged for TMA
+  int box_rows = P.page_size % 64 == 0 ? 64 : P.page_size % 32 == 0 ? 32 : P.page_size % 16 == 0 ? 16 : 0;
+  if (F8 && ((uintptr_t)P.scales & 15) != 0) box_rows = 0;
+  CUtensorMap map = {};
+  if (box_rows) {
+    if (int rc = rows_map(P, DH, F8, box_rows, &map)) return rc;
+  }
   static unsigned long long allowed = 0;  // a bit per device: the attribute belongs to the device's context
   int dev = 0;
   JLX_CUDA(cudaGetDevice(&dev));
@@ -541,7 +611,7 @@ static int launch_few(const RowsParams& P, dim3 grid, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = clustered ? 2 : 1;
-  JLX_CUDA(cudaLaunchKernelEx(&cfg, attention_few_kernel<DH, F8, NG>, P, clustered));
+  JLX_CUDA(cudaLaunchKernelEx(&cfg, attention_few_kernel<DH, F8, NG>, map, P, clustered, box_rows));
   return 0;
 }
 

@@ -12,6 +12,8 @@
 //   s = scale temp(p) q.k (soft-capped: cap tanh(s / cap)) - slope (p - key position);   out = sum w v / (sum w + exp(sink)),
 //   w = exp(s - max).  A row that sees nothing gives 0.
 #pragma once
+#include <cuda.h>
+
 #include "common.cuh"
 #include "fp8_rows.cuh"
 #include "softcap.cuh"
@@ -189,6 +191,28 @@ static int rows_params(const RowsArgs& a, RowsParams& P) {
   P.chunk = a.chunk; P.window = a.window; P.attn_scale = a.attn_scale; P.floor_scale = a.floor_scale;
   P.sink = (const float*)a.sink; P.slopes = (const float*)a.slopes; P.splits = a.splits; P.split_keys = a.split_keys;
   P.part_o = (float*)a.part_o; P.part_ml = (float2*)a.part_ml; P.status = (int*)a.status;
+  return 0;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The cache as rows of keys and values, in boxes of box_rows rows of up to 128 bytes, swizzled.
+static int rows_map(const RowsParams& P, int dh, bool f8, int box_rows, CUtensorMap* map) {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (EncodeTiledFn)p;
+  }
+  JLX_REQUIRE(fn != nullptr, "attention over rows: the driver does not offer cuTensorMapEncodeTiled");
+  const int elem = f8 ? 1 : 2, inner = dh * elem < 128 ? dh : 128 / elem;
+  const cuuint64_t dims[2] = {(cuuint64_t)dh, (cuuint64_t)P.num_pages * 2 * P.Hkv * P.page_size}, strides[1] = {(cuuint64_t)dh * elem};
+  const cuuint32_t box[2] = {(cuuint32_t)inner, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+  const CUresult r = fn(map, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(P.pages), dims, strides, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, inner * elem == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  JLX_REQUIRE(r == CUDA_SUCCESS, "attention over rows: the cache's tensor map failed (%d)", (int)r);
   return 0;
 }
 

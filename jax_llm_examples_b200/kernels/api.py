@@ -1238,14 +1238,15 @@ def attention_rows_plan(max_kv_len: int, chunk: int, window: int, n_items: int, 
     seen = min(max_kv_len, window + max_count if window else max_kv_len, chunk + max_count if chunk else max_kv_len) + ROWS_TILE  # ranges start at a tile's first key
     rows = max_count * (Hq // Hkv)
     if rows <= ROWS_FEW:
-        # Three blocks share a multiprocessor.  Fewer blocks than places: ranges fill them, down to two tiles each (a range's
-        # set-up and join cost as much).  More: ranges that make four rounds or so, of at least 16 tiles, so that the last round's
-        # idle places are few.
+        # Three blocks share a multiprocessor.  A round of them takes as long as a range and what a block costs besides (about
+        # 3 tiles: set-up, the first tile's way, the join), a join through scratch 4 tiles more: the number of ranges with the
+        # least of it.
         blocks, places = n_items * Hkv, 3 * sms
-        splits = places // blocks if blocks < places else -(-4 * places // blocks)
-        splits = max(1, min(splits, seen // (2 * ROWS_TILE if blocks < places else 16 * ROWS_TILE)))
-        if splits > ROWS_CLUSTER and splits < 2 * ROWS_CLUSTER:
-            splits = ROWS_CLUSTER  # (joining through scratch costs a launch)
+        tiles, splits, least = -(-seen // ROWS_TILE), 1, 1 << 60
+        for s in (*range(1, ROWS_CLUSTER + 1), places // blocks):
+            cost = -(-blocks * s // places) * (-(-tiles // s) + 3) + (4 if s > ROWS_CLUSTER else 0) if 0 < s <= tiles else least
+            if cost < least:
+                splits, least = s, cost
     else:
         blocks = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64))
         splits = max(1, min(3 * sms // blocks, seen // 256))
