@@ -131,8 +131,9 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
   const int p_min = __reduce_min_sync(0xffffffffu, tok.p), p_max = __reduce_max_sync(0xffffffffu, tok.p);
   const int first = P.cu_q ? min(lo_min, it.base) : lo_min, end_all = P.cu_q ? it.base + it.drafted : p_max + 1;
   const int full_lo = lo_max, full_hi = P.cu_q ? it.base : p_min + 1;  // keys in between are seen by every row
-  const int range0 = first / KT * KT + split * P.split_keys;
-  const int begin = max(first, range0), end = split == P.splits - 1 ? end_all : min(end_all, range0 + P.split_keys);
+  // equal ranges of whole tiles (an item's own: a short request's blocks are as short as each other)
+  const int start = first / KT * KT, per = max((end_all - start + KT * P.splits - 1) / (KT * P.splits), 0) * KT, range0 = start + split * per;
+  const int begin = max(first, range0), end = min(end_all, range0 + per);
   const int n_tiles = end > begin ? (end - range0 + KT - 1) / KT : 0;
   const int* table = P.block_table + (size_t)it.r * P.bt_stride;
   const int v_off = P.Hkv * P.page_size;  // rows between a key and its value

@@ -44,7 +44,7 @@ struct RowsParams {
   float attn_scale, floor_scale;
   const float* sink;       // [Hq] or null
   const float* slopes;     // [Hq] or null
-  int splits, split_keys;  // ranges of keys an item's rows are cut into, and keys of a range (the last one takes the rest)
+  int splits;              // ranges that an item's keys are cut into
   float* part_o;           // [N, Hq, splits, DH]: sums of weighted values against the maximum
   float2* part_ml;         // [N, Hq, splits]: (maximum, sum of weights)
   int* status;
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowsPara
 // What the callers hand over (_RowsArgs in kernels/api.py).
 struct RowsArgs {
   const void *q, *pages, *scales, *block_table, *req_of_token, *positions, *out, *items, *rows, *cu_q, *q_start, *masks, *sink, *slopes, *part_o, *part_ml, *status;
-  int bt_stride, n_requests, n_items, max_count, words, N, Hq, Hkv, dh, page_size, num_pages, chunk, window, splits, split_keys;
+  int bt_stride, n_requests, n_items, max_count, words, N, Hq, Hkv, dh, page_size, num_pages, chunk, window, splits;
   float scale, softcap, attn_scale, floor_scale;
 };
 
@@ -178,7 +178,7 @@ static int rows_params(const RowsArgs& a, RowsParams& P) {
   JLX_REQUIRE((((uintptr_t)a.q | (uintptr_t)a.pages | (uintptr_t)a.out) & 15) == 0, "attention over rows: q, pages and out must be 16-byte aligned");
   JLX_REQUIRE(a.attn_scale == 0.f || a.floor_scale > 0.f, "attention: floor_scale must be positive");
   JLX_REQUIRE(a.softcap >= 0.f && a.chunk >= 0 && a.window >= 0, "attention: the score cap, chunk and window must not be negative (0: none)");
-  JLX_REQUIRE(a.splits >= 1 && a.split_keys > 0 && a.split_keys % 64 == 0 && (long long)a.splits * a.split_keys < (1ll << 30), "attention over rows: bad ranges");
+  JLX_REQUIRE(a.splits >= 1 && a.splits <= 4096, "attention over rows: %d ranges", a.splits);
   JLX_REQUIRE((((uintptr_t)a.part_o & 15) | ((uintptr_t)a.part_ml & 7)) == 0, "attention over rows: scratch for the ranges is not aligned");
   JLX_REQUIRE(!a.cu_q == !a.masks && !a.cu_q == !a.q_start && (!a.cu_q || (a.items && a.words > 0)), "attention over rows: a tree needs its offsets, cached lengths, masks and items");
   JLX_REQUIRE((long long)a.max_count * a.Hq < (1ll << 30), "attention over rows: an item has too many rows");
@@ -189,7 +189,7 @@ static int rows_params(const RowsArgs& a, RowsParams& P) {
   P.scale_log2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E;
   P.cap_log2 = a.softcap > 0.f ? a.softcap * LOG2E : 0.f;
   P.chunk = a.chunk; P.window = a.window; P.attn_scale = a.attn_scale; P.floor_scale = a.floor_scale;
-  P.sink = (const float*)a.sink; P.slopes = (const float*)a.slopes; P.splits = a.splits; P.split_keys = a.split_keys;
+  P.sink = (const float*)a.sink; P.slopes = (const float*)a.slopes; P.splits = a.splits;
   P.part_o = (float*)a.part_o; P.part_ml = (float2*)a.part_ml; P.status = (int*)a.status;
   return 0;
 }

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import functools
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
 
 import torch
@@ -1219,7 +1220,7 @@ class _RowsArgs(ctypes.Structure):  # RowsArgs in csrc/attention_rows.cuh
     _fields_ = [(n, c_void_p) for n in ("q", "pages", "scales", "block_table", "req_of_token", "positions", "out", "items", "rows", "cu_q", "q_start",
                                         "masks", "sink", "slopes", "part_o", "part_ml", "status")] + \
                [(n, c_int) for n in ("bt_stride", "n_requests", "n_items", "max_count", "words", "N", "Hq", "Hkv", "dh", "page_size", "num_pages", "chunk",
-                                     "window", "splits", "split_keys")] + \
+                                     "window", "splits")] + \
                [(n, c_float) for n in ("scale", "softcap", "attn_scale", "floor_scale")]
 
 
@@ -1233,8 +1234,9 @@ def attention_rows_supported(q_dtype: torch.dtype, Hq: int, Hkv: int, dh: int) -
     return q_dtype == torch.bfloat16 and dh in (64, 128) and Hkv > 0 and Hq % Hkv == 0
 
 
-def attention_rows_plan(max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int) -> tuple[int, int]:
-    """(ranges that an item's keys are cut into, keys of a range)."""
+@functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
+def attention_rows_plan(max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int) -> int:
+    """Ranges that an item's keys are cut into (equal ones, of the item's own keys)."""
     seen = min(max_kv_len, window + max_count if window else max_kv_len, chunk + max_count if chunk else max_kv_len) + ROWS_TILE  # ranges start at a tile's first key
     rows = max_count * (Hq // Hkv)
     if rows <= ROWS_FEW:
@@ -1250,8 +1252,7 @@ def attention_rows_plan(max_kv_len: int, chunk: int, window: int, n_items: int, 
     else:
         blocks = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64))
         splits = max(1, min(3 * sms // blocks, seen // 256))
-    keys = -(-(-(-seen // splits)) // ROWS_TILE) * ROWS_TILE
-    return -(-seen // keys), keys
+    return splits
 
 
 def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, positions, out, scale, chunk, window, attn_scale, floor_scale, status,
@@ -1287,7 +1288,7 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
         return
     if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
         raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
-    splits, split_keys = attention_rows_plan(max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
+    splits = attention_rows_plan(max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
     few = max_count * (Hq // Hkv) <= ROWS_FEW
     part_o = part_ml = joined = 0
     if splits > (ROWS_CLUSTER if few else 1):
@@ -1298,7 +1299,7 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     args = _RowsArgs(q_p, pages.data_ptr(), p(scales), block_table.data_ptr(), req_of_token.data_ptr(), positions.data_ptr(), out_p, p(items), p(rows),
                      p(cu_q), p(q_start), p(masks), p(sink), p(slopes), part_o, part_ml, status.data_ptr(), width, R, n_items, max_count, words, N, Hq,
-                     Hkv, dh, page_size, P, chunk, window, splits, split_keys, scale, softcap, attn_scale, floor_scale)
+                     Hkv, dh, page_size, P, chunk, window, splits, scale, softcap, attn_scale, floor_scale)
     name = "attention_few" if few else "attention_rows"
     _run(name, "jlx_" + name, ctypes.byref(args), _raw_stream(dev))
     global _launches
