@@ -301,7 +301,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
 #pragma unroll
       for (int i = 0; i < DH / 16; ++i) o[ng][i][0] = o[ng][i][1] = o[ng][i][2] = o[ng][i][3] = 0.f;
     }
-    const bool capped = P.cap_log2 > 0.f, sloped = P.slopes != nullptr;
+    const bool capped = P.cap_log2 > 0.f, bent = capped || P.slopes;
     const int key0 = warp * 16;
     const int kg = key0 + key_at(g), kl = key0 + key_at(lane & 7);
     bool ok = true;
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
       if (!ok) break;
       const uint8_t* kt = k_tile(st);
       uint8_t* vt = k_tile(st) + T::BYTES;
-      if (masked) {
+      if (__builtin_expect(masked, 0)) {
         // A value that is not finite leaves the tile before the product (a warp reads its own keys' values only).  Codes of rows
         // outside the range may be anything, those of rows inside are numbers.
         bool any = false;
@@ -385,27 +385,37 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
         vi1 = __int_as_float((254 - min(bv1, 254)) << 23);
       }
       float x[NG][4];
-      bool grown = false;
 #pragma unroll
       for (int ng = 0; ng < NG; ++ng)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float raw = s[ng][0][e] + s[ng][1][e];
-          float v = F8 ? raw * (sc[ng][e & 1] * (e < 2 ? ks0 : ks1)) : raw * sc[ng][e & 1];
-          if (capped) v = v == v ? P.cap_log2 * cap_tanh(v) : v;
-          if (masked || sloped) {
+          x[ng][e] = F8 ? raw * (sc[ng][e & 1] * (e < 2 ? ks0 : ks1)) : raw * sc[ng][e & 1];
+        }
+      // (one branch around all that most tiles do without: a jump over each element's part of it costs an instruction fetch)
+      if (__builtin_expect(masked || bent, 0)) {
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = x[ng][e];
+            if (capped) v = v == v ? P.cap_log2 * cap_tanh(v) : v;
             int key_pos;
             const int4 k = tk[ng][e & 1];
             const int place = place0 + kg + (e < 2 ? 0 : 8);
             const bool sees = place >= begin && place < end && rows_sees(P, it, k.x, k.z, k.w, place, key_pos);
-            v = sees ? fmaf(-slope[ng][e & 1], (float)(k.z - key_pos), v) + (F8 ? (e < 2 ? ve0 : ve1) : 0.f) : -INFINITY;
-          } else if (F8) {
-            v += e < 2 ? ve0 : ve1;
+            x[ng][e] = sees ? fmaf(-slope[ng][e & 1], (float)(k.z - key_pos), v) : -INFINITY;
           }
-          x[ng][e] = v;
-          grown |= v > m[ng][e & 1] + GROWTH;
+      }
+      bool grown = false;
+#pragma unroll
+      for (int ng = 0; ng < NG; ++ng)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (F8) x[ng][e] = x[ng][e] == -INFINITY ? x[ng][e] : x[ng][e] + (e < 2 ? ve0 : ve1);  // (a masked key's scale may be anything)
+          grown |= x[ng][e] > m[ng][e & 1] + GROWTH;
         }
-      if (__any_sync(0xffffffffu, grown)) {
+      if (__builtin_expect(__any_sync(0xffffffffu, grown), 0)) {
 #pragma unroll
         for (int ng = 0; ng < NG; ++ng) {
           float corr[2];

@@ -1240,14 +1240,14 @@ def attention_rows_plan(max_kv_len: int, chunk: int, window: int, n_items: int, 
     seen = min(max_kv_len, window + max_count if window else max_kv_len, chunk + max_count if chunk else max_kv_len) + ROWS_TILE  # ranges start at a tile's first key
     rows = max_count * (Hq // Hkv)
     if rows <= ROWS_FEW:
-        # Three blocks share a multiprocessor.  A round of them takes as long as a range and what a block costs besides (about
-        # 3 tiles: set-up, the first tile's way, the join), a join through scratch 4 tiles more: the number of ranges with the
-        # least of it.
-        blocks, places = n_items * Hkv, 3 * sms
-        tiles, splits, least = -(-seen // ROWS_TILE), 1, 1 << 60
-        for s in (*range(1, ROWS_CLUSTER + 1), places // blocks):
-            cost = -(-blocks * s // places) * (-(-tiles // s) + 3) + (4 if s > ROWS_CLUSTER else 0) if 0 < s <= tiles else least
-            if cost < least:
+        # Three blocks share a multiprocessor.  A round of them takes as long as a range and what a block costs besides, as much
+        # as 10 tiles (the way to the first tile, the join), a join through scratch 6 tiles more and one for 8 ranges: the
+        # number of ranges with the least of it.  (64 requests of 8,000 keys: 225 us with 1 range, 188 with 3, 205 with 6;
+        # one of 8,000: 90 with 1, 18.5 with 8, 16.7 with 24, 23.7 with 55.)
+        blocks, places, tiles, splits, least = n_items * Hkv, 3 * sms, -(-seen // ROWS_TILE), 1, 1 << 60
+        for s in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48):
+            cost = -(-blocks * s // places) * (-(-tiles // s) + 10) + (6 + s // 8 if s > ROWS_CLUSTER else 0)
+            if s <= tiles and cost < least:
                 splits, least = s, cost
     else:
         blocks = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64))
