@@ -1,0 +1,704 @@
+// Grouped-query attention of many query rows of an item over the paged cache on the 5th-generation tensor cores (tcgen05), head
+// size 128: drafted trees and prompt portions, over a cache in bfloat16 or in 8 bits (attention_rows.cuh has mask and formula).
+//
+// A block takes 128 query rows of one item and KV head, (token, head of the group) pairs token by token, so that every key is
+// read once for 128 / G tokens' heads together, and one range of their keys in tiles of 128.  Per tile:
+//   S = Q K^T    tcgen05.mma from shared memory into tensor memory
+//   P            PARTS threads per query row read their parts of its scores, keep the reference of the exponents and the sum
+//                in 32-bit, and write the weights as 16-bit numbers over the first half of the same S buffer
+//   O += P V     tcgen05.mma with P in tensor memory and V from shared memory as an MN-major operand
+// S is double-buffered, so the next tile's score product runs while this tile's softmax does; products run in the order of
+// their issue: the score product of tile g + 2, which overwrites the buffer of S_g and P_g, is issued after O += P_g V_g.
+// Warp 0 issues the copies, warp 1 the products, warps 2 and 3 prepare values (below), sixteen warps do the softmax.
+//
+// 8 bits: the keys' codes are an operand as they lie in the cache.  Queries are two: each entry (its row's largest brought to
+// 2^7 .. 2^8 by a power of two) as e4m3, and what is left of it as e5m2; the remainder of eight bits after the nearest four is
+// a whole number up to 8 of the entry's last unit, which e5m2 holds (three bits, and 2^-16 steps below), so both products add
+// up in one accumulator to that of the bfloat16 query, exact down to 2^-25 of the row's largest entry.  The e4m3 product has
+// twice the rate: two cost what one of bfloat16 does, and no key is converted.  The values' codes become float16, which holds
+// every one of them, once per tile and block by two warps (weights in 8-bit parts would have to be three, and cost the softmax
+// threads, which set the pace, more than they have).  A key's power of two multiplies its column of scores; a value's is added
+// to its key's exponent: w_j = 2^(s_j + e_j - ref), out = sum w_j code_j / sum w_j 2^-e_j, so that the weights fit float16
+// (2^-11 of each at most) whatever the values' scales.  Bfloat16: weights rounded to bfloat16 (2^-8).
+//
+// Masks: only tiles that some row does not see wholly look at them.  In such a tile a value that is not finite is taken out
+// (a product would spread 0 * infinity over all rows) and added to the rows that do see it at the end; of rows of the cache
+// outside the range only zeros reach a product.
+//
+// Every wait on a barrier is bounded; after a timeout the block raises JLX_STATUS_WAIT_TIMEOUT, waits (bounded) for its own
+// copies, frees its tensor memory and returns.
+#include "attention_rows.cuh"
+#include "mbarrier.cuh"
+
+#define DH 128
+#define BQ 128           // query rows per block
+#define BKV 128          // keys per tile
+#define PARTS 4          // softmax threads per query row: each takes BKV / PARTS of a tile's keys and DH / PARTS of O's columns
+#define CP (BKV / PARTS)
+#define SOFTMAX0 4       // first softmax warp
+#define NTHREADS ((SOFTMAX0 + 4 * PARTS) * 32)
+#define AUX 64           // threads that prepare values
+#define GROWTH 6.0f      // how far a row's maximum may outgrow its reference (in powers of two) before O is rescaled
+#define SLOTS 4          // tiles whose scales are kept
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f16_a_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+        "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two float32 operations per instruction (IEEE, as their one-value forms).
+__device__ __forceinline__ uint64_t pack2(float a, float b) { return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// Shared-memory matrix descriptors for tiles whose rows are 128 bytes with the 128-byte swizzle, 8-row groups 1024 bytes
+// apart.  K-major: a row runs along K.  MN-major: along the operand's N direction, rows are K steps; blocks of 64 numbers along
+// N are `lbo_bytes` apart.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t lbo_bytes) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(lbo_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// Instruction descriptors: float32 accumulator, M = 128, N = 128; operand formats a, b (kind::f16: 0 float16, 1 bfloat16;
+// kind::f8f6f4: 0 e4m3, 1 e5m2); A K-major, B K- or MN-major.
+__host__ __device__ constexpr uint32_t make_idesc(uint32_t a, uint32_t b, uint32_t b_mn_major) {
+  return (1u << 4) | (a << 7) | (b << 10) | (b_mn_major << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// Byte offset of 16-byte chunk c (of 8) of row r in a swizzled tile of 128-byte rows.
+__device__ __forceinline__ uint32_t swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+#define HALF_BYTES (128 * 128)  // 128 rows of 128 bytes
+template <bool F8> struct TcTile {
+  static constexpr int Q = 2 * HALF_BYTES;                   // bfloat16: entries 0-63, 64-127; 8 bits: first parts, what is left
+  static constexpr int K = F8 ? HALF_BYTES : 2 * HALF_BYTES;  // a tile of keys, two of them
+  static constexpr int V = 2 * HALF_BYTES;                   // a tile of values as an operand, two of them
+  static constexpr int RAW = F8 ? HALF_BYTES : 0;            // a tile of values' codes, two of them
+  static constexpr int BYTES = F8 ? 2 * BKV : 0;             // the scale bytes of a tile's keys and values, two of them
+  static constexpr int SCALES = F8 ? SLOTS * 3 * BKV * 4 : 0;  // [SLOTS][keys' scales, values' exponents, 2^-exponent]
+  static constexpr int SMEM = Q + 2 * K + 2 * V + 2 * RAW + 2 * BYTES + SCALES + 1024;
+};
+
+template <bool F8>
+__global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __grid_constant__ CUtensorMap map, const RowsParams P, int box_rows) {
+  JLX_TL(TL_ATTN_PREFILL);
+  using T = TcTile<F8>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t *q_p = smem, *k_p = q_p + T::Q, *v_p = k_p + 2 * T::K, *raw_p = v_p + 2 * T::V;
+  uint8_t* bytes_p = raw_p + 2 * T::RAW;
+  float* scales_p = reinterpret_cast<float*>(bytes_p + 2 * T::BYTES);
+  // barriers (each use flips a phase bit; t = a tile's number)
+  enum { B_QREADY = 0,    // Q is in shared memory
+         B_KFULL = 1,     // [2] K of tile t has landed                   stage t % 2, phase t / 2
+         B_KEMPTY = 3,    // [2] the score product of tile t is done
+         B_VFULL = 5,     // [2] V of tile t (codes and scale bytes) has landed
+         B_RAWEMPTY = 7,  // [2] the codes have been read
+         B_VREADY = 9,    // [2] V of tile t is an operand
+         B_VEMPTY = 11,   // [2] the product with P of tile t is done
+         B_SFULL = 13,    // [2] S of tile t is complete
+         B_PREADY = 15,   // P of tile t is in tensor memory, O rescaled   phase t
+         B_ODONE = 16,    // O holds the tiles up to t                     phase t
+         B_MEET = 17,     // [4] the threads of a quarter of the rows have met
+         B_SCALES = 21,   // [SLOTS] the scales of tile t are numbers      slot t % SLOTS, phase t / SLOTS
+         N_BARS = 25 };
+  __shared__ __align__(8) uint64_t bars[N_BARS];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed, any_bad, span[4];
+  __shared__ float xmax[2][PARTS][BQ];  // [meeting parity][part][row]: what the threads of a row exchange
+  __shared__ float q_exp[BQ];           // 8 bits: the power of two that a query row was divided by
+  pdl_launch_dependents_if_small();
+  pdl_wait();
+  const uint32_t bar0 = smem_u32(&bars[0]);
+  auto BAR = [bar0](int i) { return bar0 + 8u * i; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x % P.splits, item_i = blockIdx.x / P.splits;
+  const int tiles_y = gridDim.y / P.Hkv, hk = blockIdx.y / tiles_y, row0 = (blockIdx.y - hk * tiles_y) * BQ;
+  RowsItem it;
+  if (!rows_item(P, item_i, it)) return;
+  const int G = P.Hq / P.Hkv, n_rows = min(it.cnt * G - row0, BQ);
+  if (n_rows <= 0) return;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < N_BARS; ++i) mbar_init(BAR(i), 1);  // a transaction count or a tcgen05.commit each, but:
+    mbar_init(BAR(B_QREADY), 128 * PARTS);
+    mbar_init(BAR(B_PREADY), 128 * PARTS);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(BAR(B_RAWEMPTY + i), AUX);
+      mbar_init(BAR(B_VREADY + i), AUX);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(BAR(B_MEET + i), 32 * PARTS);
+    for (int i = 0; i < SLOTS; ++i) mbar_init(BAR(B_SCALES + i), AUX);
+    failed = any_bad = 0;
+    span[0] = span[2] = 0x7fffffff;
+    span[1] = span[3] = (int)0x80000000;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (threadIdx.x < BQ) {
+    const RowsToken k = rows_token(P, it, row0 + min((int)threadIdx.x, n_rows - 1), hk);
+    const int a = __reduce_min_sync(0xffffffffu, k.lo), b = __reduce_max_sync(0xffffffffu, k.lo);
+    const int c = __reduce_min_sync(0xffffffffu, k.p), d = __reduce_max_sync(0xffffffffu, k.p);
+    if (lane == 0) {
+      atomicMin(&span[0], a);
+      atomicMax(&span[1], b);
+      atomicMin(&span[2], c);
+      atomicMax(&span[3], d);
+    }
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), 512);  // S0, S1 (128 columns each), O (128)
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot, tm_o = tmem + 256;
+  // the item's keys and this block's equal part of their tiles
+  const int first = P.cu_q ? min(span[0], it.base) : span[0], end_all = P.cu_q ? it.base + it.drafted : span[3] + 1;
+  const int full_lo = span[1], full_hi = P.cu_q ? it.base : span[2] + 1;  // keys in between are seen by every row
+  const int start = first / BKV * BKV, per = max((end_all - start + BKV * P.splits - 1) / (BKV * P.splits), 0) * BKV, range0 = start + split * per;
+  const int begin = max(first, range0), end = min(end_all, range0 + per);
+  const int n_tiles = end > begin ? (end - range0 + BKV - 1) / BKV : 0;
+  const int* table = P.block_table + (size_t)it.r * P.bt_stride;
+  const int v_off = P.Hkv * P.page_size;
+  auto masked_tile = [&](int place0) { return place0 < full_lo || place0 + BKV > min(full_hi, end) || place0 < begin; };
+  auto gave_up = [&](bool ok) { return !ok || *(volatile int*)&failed; };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------ copies
+    // Keys are free again after their score product, values after the product with P (or their conversion), which comes a
+    // tile later: each ring advances as soon as its own stage is free.  Lane i has box i of every tile.
+    const int boxes = BKV / box_rows;
+    auto load_tile = [&](int t, int which) {
+      const int st = t & 1, place = range0 + t * BKV + lane * box_rows;
+      const uint32_t bar = BAR((which ? B_VFULL : B_KFULL) + st);
+      if (lane == 0) mbar_expect_tx(bar, BKV * DH * (F8 ? 1 : 2) + (F8 && which ? 2 * BKV : 0));
+      __syncwarp();
+      if (lane < boxes) {
+        const int pi = place / P.page_size;
+        int page = pi < P.bt_stride ? table[pi] : -1;
+        if (page < 0 || page >= P.num_pages) {
+          if (place < end && place + box_rows > begin) atomicOr(P.status, JLX_STATUS_BAD_PAGE);
+          page = 0;  // no page there: every key of the box is masked
+        }
+        const int row = (page * 2 * P.Hkv + hk) * P.page_size + (place - pi * P.page_size);
+        const uint32_t dst = smem_u32(which ? (F8 ? raw_p + st * T::RAW : v_p + st * T::V) : k_p + st * T::K) + lane * box_rows * 128;
+        tma_load_2d(dst, &map, 0, row + which * v_off, bar);
+        if (!F8) tma_load_2d(dst + HALF_BYTES, &map, 64, row + which * v_off, bar);
+        if (F8 && which) {
+          const uint32_t sc = smem_u32(bytes_p + st * T::BYTES) + lane * box_rows;
+          bulk_load(sc, P.scales + row, box_rows, bar);
+          bulk_load(sc + BKV, P.scales + row + v_off, box_rows, bar);
+        }
+      }
+      __syncwarp();
+    };
+    int ik = 0, iv = 0;
+    uint32_t idle = 0;
+    bool ok = true;
+    while ((ik < n_tiles || iv < n_tiles) && ok) {
+      bool go_k = ik < n_tiles && (ik < 2 || mbar_try_wait(BAR(B_KEMPTY + (ik & 1)), ((ik >> 1) - 1) & 1));
+      bool go_v = iv < n_tiles && (iv < 2 || mbar_try_wait(BAR((F8 ? B_RAWEMPTY : B_VEMPTY) + (iv & 1)), ((iv >> 1) - 1) & 1));
+      go_k = __shfl_sync(0xffffffffu, go_k, 0);
+      go_v = __shfl_sync(0xffffffffu, go_v, 0);
+      if (go_k) load_tile(ik++, 0);
+      if (go_v) load_tile(iv++, 1);
+      if (go_k || go_v) idle = 0;
+      else if (++idle >= JLX_WAIT_LIMIT) ok = false;
+      ok = !__any_sync(0xffffffffu, gave_up(ok));
+    }
+    if (!ok) {  // let the copies in flight land before the block's shared memory is given up
+      for (int t = max(0, ik - 2); t < ik; ++t) mbar_wait(BAR(B_KFULL + (t & 1)), (t >> 1) & 1);
+      for (int t = max(0, iv - 2); t < iv; ++t) mbar_wait(BAR(B_VFULL + (t & 1)), (t >> 1) & 1);
+      if (lane == 0) {
+        atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
+        failed = 1;
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------------ products
+    if (lane == 0 && n_tiles > 0) {
+      bool ok = mbar_wait(BAR(B_QREADY), 0);
+      auto issue_qk = [&](int t) {
+        const int st = t & 1;
+        if (ok) ok = mbar_wait(BAR(B_KFULL + st), (t >> 1) & 1);
+        if (gave_up(ok)) { ok = false; return; }
+        tc_fence_after();
+        const uint32_t q_s = smem_u32(q_p), k_s = smem_u32(k_p) + st * T::K;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          if (F8) {  // first parts, then what is left: four steps of 32 entries each
+            const uint32_t off = (kk & 3) * 32;
+            umma_f8(tmem + st * 128, desc_k_major(q_s + (kk >> 2) * HALF_BYTES + off), desc_k_major(k_s + off), make_idesc(kk >> 2, 0, 0), kk != 0);
+          } else {   // steps of 16 entries
+            const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
+            umma_f16(tmem + st * 128, desc_k_major(q_s + off), desc_k_major(k_s + off), make_idesc(1, 1, 0), kk != 0);
+          }
+        }
+        umma_commit(BAR(B_SFULL + st));
+        umma_commit(BAR(B_KEMPTY + st));
+      };
+      issue_qk(0);
+      for (int t = 0; t < n_tiles && ok; ++t) {
+        const int st = t & 1;
+        if (t + 1 < n_tiles) issue_qk(t + 1);
+        if (!ok) break;
+        ok = mbar_wait(BAR(B_PREADY), t & 1);
+        if (ok) ok = mbar_wait(BAR(B_VREADY + st), (t >> 1) & 1);
+        if (gave_up(ok)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t v_s = smem_u32(v_p) + st * T::V;
+#pragma unroll
+        for (int kk = 0; kk < BKV / 16; ++kk)  // P: 16 keys = 8 columns of tensor memory; V: 16 keys = 16 rows of 128 bytes
+          umma_f16_a_tmem(tm_o, tmem + st * 128 + kk * 8, desc_mn_major(v_s + kk * 16 * 128, HALF_BYTES), make_idesc(!F8, !F8, 1), (t | kk) != 0);
+        umma_commit(BAR(B_VEMPTY + st));
+        umma_commit(BAR(B_ODONE));
+      }
+      if (!ok) {
+        atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
+        failed = 1;
+      }
+    }
+  } else if (warp < SOFTMAX0) {
+    // ------------------------------------------------------------------------------ values as an operand
+    const int i0 = threadIdx.x - 64;  // keys i0 and i0 + 64 of every tile
+    bool ok = true;
+    for (int t = 0; t < n_tiles; ++t) {
+      const int st = t & 1, place0 = range0 + t * BKV;
+      ok = mbar_wait(BAR(B_VFULL + st), (t >> 1) & 1);
+      if (F8 && ok && t >= 2) ok = mbar_wait(BAR(B_VEMPTY + st), ((t >> 1) - 1) & 1);
+      if (__any_sync(0xffffffffu, gave_up(ok))) { ok = false; break; }
+      uint8_t* v = v_p + st * T::V;
+      if (F8) {
+        const uint8_t* raw = raw_p + st * T::RAW;
+        float* sc = scales_p + (t % SLOTS) * 3 * BKV;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int i = i0 + u * 64, bk = bytes_p[st * T::BYTES + i], bv = bytes_p[st * T::BYTES + BKV + i];
+          sc[i] = fp8_scale(bk);
+          sc[BKV + i] = bv == FP8_BAD ? __int_as_float(0x7fc00000) : (float)(bv - 127);
+          sc[2 * BKV + i] = __int_as_float((254 - min(bv, 254)) << 23);  // (finite for any byte: a masked key's weight is 0 and stays 0)
+        }
+        mbar_arrive(BAR(B_SCALES + t % SLOTS));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int i = i0 + u * 64;
+          const bool in = place0 + i >= begin && place0 + i < end;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint4 x = *reinterpret_cast<const uint4*>(raw + swizzled(i, c));
+            if (!in) x = make_uint4(0u, 0u, 0u, 0u);
+            uint4 a, b;
+            fp8x4_to_half(x.x, a.x, a.y);
+            fp8x4_to_half(x.y, a.z, a.w);
+            fp8x4_to_half(x.z, b.x, b.y);
+            fp8x4_to_half(x.w, b.z, b.w);
+            uint8_t* half = v + (c >> 2) * HALF_BYTES;
+            *reinterpret_cast<uint4*>(half + swizzled(i, (c & 3) * 2)) = a;
+            *reinterpret_cast<uint4*>(half + swizzled(i, (c & 3) * 2 + 1)) = b;
+          }
+        }
+        fence_async_proxy();
+        mbar_arrive(BAR(B_RAWEMPTY + st));
+      } else if (masked_tile(place0)) {
+        bool bad = false;
+#pragma unroll 1
+        for (int x = i0; x < 2 * BKV * 8; x += AUX) {  // (consecutive threads: chunks of a row)
+          const int i = (x >> 3) & (BKV - 1);
+          uint4* at = reinterpret_cast<uint4*>(v + (x >> 10) * HALF_BYTES + swizzled(i, x & 7));
+          uint32_t w[4] = {at->x, at->y, at->z, at->w};
+          bool here = false;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            if ((w[y] & 0x7f80u) == 0x7f80u) { w[y] &= 0xffff0000u; here = true; }
+            if ((w[y] & 0x7f800000u) == 0x7f800000u) { w[y] &= 0xffffu; here = true; }
+          }
+          if (here) {
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
+            bad = true;
+          }
+        }
+        if (bad) *(volatile int*)&any_bad = 1;
+        fence_async_proxy();
+      }
+      mbar_arrive(BAR(B_VREADY + st));
+    }
+    if (!ok && lane == 0) {
+      atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
+      failed = 1;
+    }
+  } else {
+    // ------------------------------------------------------------------------------ queries, softmax, rescale, store
+    {
+      // four neighbouring threads bring a row's 128 entries into shared memory, 32 each
+      const int i = (threadIdx.x - SOFTMAX0 * 32) >> 2, part = threadIdx.x & 3;
+      const int t = (row0 + min(i, n_rows - 1)) / G, head = hk * G + (row0 + min(i, n_rows - 1)) - t * G;
+      const uint4* src = reinterpret_cast<const uint4*>(P.q + ((size_t)(it.n0 + t) * P.Hq + head) * DH + part * 32);
+      uint4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = src[u];
+      if (F8) {
+        float top = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x[u]);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float2 f = __bfloat1622float2(h[y]);
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = max(min((int)(__float_as_uint(top) >> 23) - 127, 120), -110) - 7;
+        const float in = fp8_pow2(-e);
+        if (part == 0) q_exp[i] = top == INFINITY ? __int_as_float(0x7fc00000) : fp8_pow2(e);  // (no codes for an infinite entry: the scores are NaN)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // 16 entries: a chunk of each part
+          uint32_t hi[4], left[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x[2 * u + (w >> 1)]) + (w & 1) * 2;
+            const float2 f0 = __bfloat1622float2(h[0]), f1 = __bfloat1622float2(h[1]);
+            const float a = f0.x * in, b = f0.y * in, c = f1.x * in, d = f1.y * in;
+            hi[w] = fp8x4_from_float(a, b, c, d);
+            uint32_t back[2];
+            fp8x4_to_half(hi[w], back[0], back[1]);
+            const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&back[0])), g1 = __half22float2(*reinterpret_cast<const __half2*>(&back[1]));
+            left[w] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a - g0.x, b - g0.y), __NV_SATFINITE, __NV_E5M2) |
+                      (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c - g1.x, d - g1.y), __NV_SATFINITE, __NV_E5M2) << 16;
+          }
+          *reinterpret_cast<uint4*>(q_p + swizzled(i, part * 2 + u)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(q_p + HALF_BYTES + swizzled(i, part * 2 + u)) = make_uint4(left[0], left[1], left[2], left[3]);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4*>(q_p + (part >> 1) * HALF_BYTES + swizzled(i, (part & 1) * 4 + u)) = x[u];
+      }
+      fence_async_proxy();
+      mbar_arrive(BAR(B_QREADY));
+    }
+    // A warp reaches the tensor-memory lanes [32 * (warp & 3), +32), so PARTS warps share each quarter of the query rows and
+    // split a tile's keys and the output's columns among them.  The threads of a row meet once per tile to agree on the
+    // row's maximum; each keeps the sum of its own part.
+    const int quarter = warp & 3, part = (warp - SOFTMAX0) >> 2, row = quarter * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const int col0 = part * CP;
+    RowsToken tok = rows_token(P, it, row0 + min(row, n_rows - 1), hk);
+    const bool capped = P.cap_log2 > 0.f, bent = capped || P.slopes;
+    bool ok = mbar_wait(BAR(B_QREADY), 0);  // (every row's power of two has been written)
+    float sc = tok.sc;
+    if (F8) sc *= *(volatile float*)&q_exp[row];
+    float m = ROWS_NEG_BIG, l = 0.f;
+    for (int t = 0; t < n_tiles && ok; ++t) {
+      const int st = t & 1, place0 = range0 + t * BKV, place = place0 + col0;
+      ok = mbar_wait(BAR(B_SFULL + st), (t >> 1) & 1);
+      if (F8 && ok) ok = mbar_wait(BAR(B_SCALES + t % SLOTS), (t / SLOTS) & 1);
+      ok = !__any_sync(0xffffffffu, gave_up(ok));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t s_addr = tmem + st * 128 + lane_addr;
+      uint32_t v[CP];
+      tmem_ld32(s_addr + col0, v);
+      tmem_ld_wait();
+      // base-2 exponents of the weights
+      const float* scp = scales_p + (t % SLOTS) * 3 * BKV + col0;
+      const bool special = masked_tile(place0) || bent;
+      if (F8) {
+        const uint64_t sc2 = pack2(sc, sc);
+#pragma unroll
+        for (int c = 0; c < CP; c += 4) {
+          const float4 ks = *reinterpret_cast<const float4*>(scp + c);
+          const uint64_t f0 = mul2(sc2, pack2(ks.x, ks.y)), f1 = mul2(sc2, pack2(ks.z, ks.w));
+          uint64_t a = pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), b = pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+          if (special) {
+            a = mul2(a, f0);
+            b = mul2(b, f1);
+          } else {
+            const float4 ve = *reinterpret_cast<const float4*>(scp + BKV + c);
+            a = fma2(a, f0, pack2(ve.x, ve.y));
+            b = fma2(b, f1, pack2(ve.z, ve.w));
+          }
+          v[c] = (uint32_t)a; v[c + 1] = (uint32_t)(a >> 32); v[c + 2] = (uint32_t)b; v[c + 3] = (uint32_t)(b >> 32);
+        }
+      } else {
+        const uint64_t sc2 = pack2(sc, sc);
+#pragma unroll
+        for (int c = 0; c < CP; c += 2) {
+          const uint64_t a = mul2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), sc2);
+          v[c] = (uint32_t)a;
+          v[c + 1] = (uint32_t)(a >> 32);
+        }
+      }
+      if (__builtin_expect(special, 0)) {
+        if (capped) {
+#pragma unroll
+          for (int c = 0; c < CP; ++c) {
+            const float x = __uint_as_float(v[c]);
+            v[c] = __float_as_uint(x == x ? P.cap_log2 * cap_tanh(x) : x);
+          }
+        }
+        // which of the 32 keys the row's token sees: those at cached places from lo on (up to its own, or before the tree) ...
+        const int hi = P.cu_q ? min(it.base, end) : min(tok.p + 1, end), from = max(max(tok.lo, begin) - place, 0), to = min(hi - place, CP);
+        uint32_t sees = to > from ? (0xffffffffu >> (32 - (to - from))) << from : 0u;
+        if (P.cu_q && place + CP > it.base) {  // ... and the drafted ones of its mask
+          const int j0 = place - it.base, words = P.words, n = min(it.drafted, end - it.base);
+          const int* mask = P.masks + (size_t)tok.n * words;
+          const int w0 = j0 >> 5, sh = j0 & 31;  // (bits j0 .. j0 + 31 lie in two words)
+          const uint32_t a = w0 >= 0 && w0 < words ? (uint32_t)mask[w0] : 0u, b = w0 + 1 >= 0 && w0 + 1 < words ? (uint32_t)mask[w0 + 1] : 0u;
+          uint32_t bits = __funnelshift_r(a, b, sh);
+          const int cut0 = max(max(-j0, begin - place), 0), cut1 = min(n - j0, CP);
+          bits &= cut1 > cut0 ? (0xffffffffu >> (32 - (cut1 - cut0))) << cut0 : 0u;
+          if (tok.lo > 0)
+            for (uint32_t left = bits; left; left &= left - 1) {
+              const int c = __ffs(left) - 1;
+              if (P.positions[P.cu_q[it.r] + j0 + c] < tok.lo) bits &= ~(1u << c);
+            }
+          sees |= bits;
+        }
+        if (P.slopes) {
+#pragma unroll
+          for (int c = 0; c < CP; ++c) {
+            int key_pos = place + c;
+            if (P.cu_q && key_pos >= it.base) key_pos = key_pos - it.base < it.drafted ? P.positions[P.cu_q[it.r] + key_pos - it.base] : 0;
+            v[c] = __float_as_uint(fmaf(-tok.slope, (float)(tok.p - key_pos), __uint_as_float(v[c])));
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < CP; ++c) {
+          const float x = F8 ? __uint_as_float(v[c]) + scp[BKV + c] : __uint_as_float(v[c]);
+          v[c] = (sees >> c) & 1 ? __float_as_uint(x) : 0xff800000u;
+        }
+      }
+      float mx4[4] = {ROWS_NEG_BIG, ROWS_NEG_BIG, ROWS_NEG_BIG, ROWS_NEG_BIG};  // four chains instead of one long one
+#pragma unroll
+      for (int c = 0; c < CP; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(v[c]));
+      float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      // the row's maximum over all parts (double-buffered by the meeting's parity: a partner may be a tile ahead)
+      const int mp = t & 1;
+      xmax[mp][part][row] = mx;
+      mbar_arrive(BAR(B_MEET + quarter));
+      ok = mbar_wait(BAR(B_MEET + quarter), mp);
+      ok = !__any_sync(0xffffffffu, gave_up(ok));
+      if (!ok) break;
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) mx = fmaxf(mx, xmax[mp][q][row]);
+      mx = fmaxf(m, mx);
+      // While no row of this quarter has grown by more than GROWTH beyond its reference, the references stay, the weights may
+      // exceed 1 (up to 64), and O is not rescaled.  All threads of these rows decide alike: they hold the same references.
+      if (__all_sync(0xffffffffu, mx - m <= GROWTH)) mx = m;
+      const float corr = m == mx ? 1.f : rows_exp2(m - mx);
+      float rs4[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t packed[CP / 2];
+#pragma unroll
+      for (int c = 0; c < CP; c += 4) {
+        const float4 vi = F8 ? *reinterpret_cast<const float4*>(scp + 2 * BKV + c) : make_float4(1.f, 1.f, 1.f, 1.f);
+        const float p0 = rows_exp2(__uint_as_float(v[c]) - mx), p1 = rows_exp2(__uint_as_float(v[c + 1]) - mx);
+        const float p2 = rows_exp2(__uint_as_float(v[c + 2]) - mx), p3 = rows_exp2(__uint_as_float(v[c + 3]) - mx);
+        if (F8) {
+          rs4[0] = fmaf(p0, vi.x, rs4[0]); rs4[1] = fmaf(p1, vi.y, rs4[1]); rs4[2] = fmaf(p2, vi.z, rs4[2]); rs4[3] = fmaf(p3, vi.w, rs4[3]);
+          const __half2 a = __floats2half2_rn(p0, p1), b = __floats2half2_rn(p2, p3);
+          packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&a);
+          packed[(c >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&b);
+        } else {
+          rs4[0] += p0; rs4[1] += p1; rs4[2] += p2; rs4[3] += p3;
+          const __nv_bfloat162 a = __floats2bfloat162_rn(p0, p1), b = __floats2bfloat162_rn(p2, p3);
+          packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&a);
+          packed[(c >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+      }
+      // P over the first half of this S buffer: keys 2c and 2c + 1 in column c (the partners have read their scores: they met
+      // after their loads)
+      tmem_st16(s_addr + part * (CP / 2), packed);
+      l = fmaf(l, corr, (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]));
+      m = mx;
+      // The product of the previous tile must be complete before O is rescaled, and every thread waits for it whether it
+      // rescales or not: a barrier's phase bit tells a waiter the truth only if the waiter has seen the phase before.
+      if (t > 0) {
+        ok = mbar_wait(BAR(B_ODONE), (t - 1) & 1);
+        ok = !__any_sync(0xffffffffu, gave_up(ok));
+        if (!ok) break;
+        if (!__all_sync(0xffffffffu, corr == 1.f)) {
+          tc_fence_after();
+          uint32_t o[32];
+          tmem_ld32(tm_o + lane_addr + part * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+          tmem_st32(tm_o + lane_addr + part * 32, o);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(BAR(B_PREADY));
+    }
+    // the end: the last product, the row's sum (the sum of the parts' sums), the store
+    if (ok && n_tiles > 0) {
+      ok = mbar_wait(BAR(B_ODONE), (n_tiles - 1) & 1);
+      ok = !__any_sync(0xffffffffu, gave_up(ok));
+    }
+    if (ok) {
+      tc_fence_after();
+      const int mp = n_tiles & 1;
+      xmax[mp][part][row] = l;
+      mbar_arrive(BAR(B_MEET + quarter));
+      ok = !__any_sync(0xffffffffu, !mbar_wait(BAR(B_MEET + quarter), mp));
+    }
+    if (ok) {
+      const int mp = n_tiles & 1;
+      float total = 0.f;
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) total += xmax[mp][q][row];
+      uint32_t o[32];
+      if (n_tiles > 0) {
+        tmem_ld32(tm_o + lane_addr + part * 32, o);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] = 0u;
+      }
+      if (!F8 && *(volatile int*)&any_bad && row < n_rows) {  // the values that were taken out, for the rows that see them
+        for (int place = begin; place < end; ++place) {
+          int key_pos;
+          if (!masked_tile(place / BKV * BKV) || !rows_sees(P, it, tok.n, tok.p, tok.lo, place, key_pos)) continue;
+          const int row_c = rows_cache_row(P, table, hk, place);
+          if (row_c < 0) continue;
+          const bf16* vp = reinterpret_cast<const bf16*>(P.pages) + (size_t)(row_c + v_off) * DH + part * 32;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float y = __bfloat162float(vp[c]);
+            if (!isfinite(y)) o[c] = __float_as_uint(__uint_as_float(o[c]) + y);
+          }
+        }
+      }
+      if (row < n_rows) {
+        const size_t at = (size_t)tok.n * P.Hq + tok.head;
+        if (P.splits > 1) {
+          float4* dst = reinterpret_cast<float4*>(P.part_o + (at * P.splits + split) * DH + part * 32);
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            dst[c >> 2] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
+          if (part == 0) P.part_ml[at * P.splits + split] = make_float2(m, total);
+        } else {
+          const float inv = rows_inverse(P, m, total, tok.head);
+          uint4* dst = reinterpret_cast<uint4*>(P.out + at * DH + part * 32);
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            uint4 x;
+            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&x);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) h[u] = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * u]) * inv, __uint_as_float(o[c + 2 * u + 1]) * inv);
+            dst[c >> 3] = x;
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0) {
+      atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
+      failed = 1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// -------------------------------------------------------------------------------------------- host
+template <bool F8>
+static int launch_tc(const RowsParams& P, int box_rows, dim3 grid, cudaStream_t stream) {
+  static unsigned long long allowed = 0;  // a bit per device: the attribute belongs to the device's context
+  int dev = 0;
+  JLX_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !(allowed >> dev & 1)) {
+    JLX_CUDA(cudaFuncSetAttribute(attention_rows_tc_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcTile<F8>::SMEM));
+    if (dev < 64) allowed |= 1ull << dev;
+  }
+  CUtensorMap map;
+  if (int rc = rows_map(P, DH, F8, box_rows, &map)) return rc;
+  JLX_CUDA(jlx_launch_pdl(attention_rows_tc_kernel<F8>, grid, dim3(NTHREADS), TcTile<F8>::SMEM, stream, map, P, box_rows));
+  return 0;
+}
+
+JLX_API int jlx_attention_rows_tc(const RowsArgs* a, cudaStream_t stream) {
+  RowsParams P;
+  if (rows_params(*a, P)) return 1;
+  JLX_REQUIRE(a->dh == DH && a->page_size % 16 == 0 && ((uintptr_t)a->scales & 15) == 0, "attention over rows (tcgen05): needs head size 128, pages of a multiple of 16 tokens and scales on a 16-byte boundary");
+  if (P.n_items == 0) return 0;
+  const int rows = a->max_count * (P.Hq / P.Hkv), box_rows = P.page_size % 64 == 0 ? 64 : P.page_size % 32 == 0 ? 32 : 16;
+  const long long gx = (long long)P.n_items * P.splits, gy = (long long)P.Hkv * ((rows + BQ - 1) / BQ);
+  JLX_REQUIRE(gx < (1ll << 31) && gy <= 65535, "attention over rows: too many items or rows");
+  JLX_REQUIRE(P.splits == 1 || (P.part_o && P.part_ml), "attention over rows: scratch for the ranges is missing");
+  const dim3 grid((unsigned)gx, (unsigned)gy);
+  if (int rc = P.scales ? launch_tc<true>(P, box_rows, grid, stream) : launch_tc<false>(P, box_rows, grid, stream)) return rc;
+  return P.splits > 1 ? launch_rows_join<DH>(P, a->max_count, stream) : 0;
+}

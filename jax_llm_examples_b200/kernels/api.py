@@ -1234,24 +1234,34 @@ def attention_rows_supported(q_dtype: torch.dtype, Hq: int, Hkv: int, dh: int) -
     return q_dtype == torch.bfloat16 and dh in (64, 128) and Hkv > 0 and Hq % Hkv == 0
 
 
+def attention_rows_form(rows: int, dh: int, page_size: int, aligned: bool) -> str:
+    """The kernel for items of up to so many query rows of a KV head ((token, head of the group) pairs)."""
+    if rows <= ROWS_FEW:
+        return "attention_few"
+    return "attention_rows_tc" if dh == 128 and page_size % 16 == 0 and aligned else "attention_rows"
+
+
 @functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
-def attention_rows_plan(max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int) -> int:
+def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int) -> int:
     """Ranges that an item's keys are cut into (equal ones, of the item's own keys)."""
     seen = min(max_kv_len, window + max_count if window else max_kv_len, chunk + max_count if chunk else max_kv_len) + ROWS_TILE  # ranges start at a tile's first key
     rows = max_count * (Hq // Hkv)
-    if rows <= ROWS_FEW:
+    if form == "attention_few":
         # Three blocks share a multiprocessor.  A round of them takes as long as a range and what a block costs besides, as much
         # as 10 tiles (the way to the first tile, the join), a join through scratch 6 tiles more and one for 8 ranges: the
         # number of ranges with the least of it.  (64 requests of 8,000 keys: 225 us with 1 range, 188 with 3, 205 with 6;
         # one of 8,000: 90 with 1, 18.5 with 8, 16.7 with 24, 23.7 with 55.)
-        blocks, places, tiles, splits, least = n_items * Hkv, 3 * sms, -(-seen // ROWS_TILE), 1, 1 << 60
-        for s in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48):
-            cost = -(-blocks * s // places) * (-(-tiles // s) + 10) + (6 + s // 8 if s > ROWS_CLUSTER else 0)
-            if s <= tiles and cost < least:
-                splits, least = s, cost
+        blocks, places, tiles, block, join, share = n_items * Hkv, 3 * sms, -(-seen // ROWS_TILE), 10, 6, 8
+    elif form == "attention_rows_tc":
+        blocks, places, tiles, block, join, share = n_items * Hkv * -(-rows // 128), sms, -(-seen // 128), 4, 3, 4
     else:
-        blocks = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64))
-        splits = max(1, min(3 * sms // blocks, seen // 256))
+        blocks, places, tiles, block, join, share = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64)), 2 * sms, -(-seen // ROWS_TILE), 4, 3, 8
+    splits, least = 1, 1 << 60
+    for s in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48):
+        joined = s > (ROWS_CLUSTER if form == "attention_few" else 1)
+        cost = -(-blocks * s // places) * (-(-tiles // s) + block) + (join + s // share if joined else 0)
+        if s <= tiles and cost < least:
+            splits, least = s, cost
     return splits
 
 
@@ -1288,10 +1298,10 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
         return
     if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
         raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
-    splits = attention_rows_plan(max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
-    few = max_count * (Hq // Hkv) <= ROWS_FEW
+    form = attention_rows_form(max_count * (Hq // Hkv), dh, page_size, scales is None or scales.data_ptr() % 16 == 0)
+    splits = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
     part_o = part_ml = joined = 0
-    if splits > (ROWS_CLUSTER if few else 1):
+    if splits > (ROWS_CLUSTER if form == "attention_few" else 1):
         # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
         scratch = torch.empty(N * Hq * splits * (dh + 2), dtype=torch.float32, device=q.device)
         part_o = scratch.data_ptr()
@@ -1300,8 +1310,7 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     args = _RowsArgs(q_p, pages.data_ptr(), p(scales), block_table.data_ptr(), req_of_token.data_ptr(), positions.data_ptr(), out_p, p(items), p(rows),
                      p(cu_q), p(q_start), p(masks), p(sink), p(slopes), part_o, part_ml, status.data_ptr(), width, R, n_items, max_count, words, N, Hq,
                      Hkv, dh, page_size, P, chunk, window, splits, scale, softcap, attn_scale, floor_scale)
-    name = "attention_few" if few else "attention_rows"
-    _run(name, "jlx_" + name, ctypes.byref(args), _raw_stream(dev))
+    _run(form, "jlx_" + form, ctypes.byref(args), _raw_stream(dev))
     global _launches
     _launches += joined  # the joining kernel
 

@@ -231,8 +231,18 @@ PORTIONS = [
 ]
 
 
+FORMS = ["rule", "attention_rows"]  # the kernel by the sizes, or the one for any page
+
+
+@pytest.fixture
+def form(request, monkeypatch):
+    if request.param != "rule":
+        monkeypatch.setattr(K(), "attention_rows_form", lambda *a: request.param)
+
+
+@pytest.mark.parametrize("form", FORMS, indirect=True)
 @pytest.mark.parametrize("n, held, Hq, Hkv, dh, page, cut, mask", PORTIONS)
-def test_portions(n, held, Hq, Hkv, dh, page, cut, mask):
+def test_portions(form, n, held, Hq, Hkv, dh, page, cut, mask):
     c = Case(n, held, Hq, Hkv, dh, page).to_device()
     assert_close(_attend(c, mask, c.items(cut)), *c.want(**mask))
     assert int(c.status) == 0
@@ -257,7 +267,8 @@ def test_the_planned_length_bounds_nothing(planned):
     assert_close(_attend(c, {}, max_kv=planned), *c.want())
 
 
-def test_rows_of_very_different_scales():
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+def test_rows_of_very_different_scales(form):
     """Keys and values whose rows' scales lie tens of binades apart: a token that sees only small values keeps their digits."""
     c = Case([1, 1, 64], [300, 4, 0], 4, 2, 128, 16, spread=12.0)
     c.rows[..., 0, :, :, :] /= c.rows[..., 0, :, :, :].abs().amax(-1, keepdim=True).clamp(min=1e-30)  # keys of one size: scores stay moderate
@@ -269,24 +280,28 @@ def test_rows_of_very_different_scales():
     assert_close(out, *c.want())
 
 
-def test_nan_rows_reach_those_that_see_them_and_no_other():
-    c = Case([100], [50], 4, 2, 128, 16)
-    place = 50 + 37  # a key and a value, of different heads, in the middle of the portion
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("n", [8, 100])
+def test_nan_rows_reach_those_that_see_them_and_no_other(form, n):
+    c = Case([n], [50], 4, 2, 128, 16)
+    at_token = n * 3 // 8
+    place = 50 + at_token  # a key and a value, of different heads, in the middle of the portion
     page, at = int(c.table[0, place // 16]), place % 16
     c.rows[page, 0, 0, at], c.rows[page, 1, 1, at] = math.nan, math.nan
     c.scales[page, 0, 0, at], c.scales[page, 1, 1, at] = 255, 255
     c.to_device()
     out = _attend(c, {}, c.items(128))
     want, tol = c.want()
-    assert torch.isnan(want[37:]).all() and not torch.isnan(want[:37]).any()
+    assert torch.isnan(want[at_token:]).all() and not torch.isnan(want[:at_token]).any()
     assert_close(out, want, tol)
 
 
-def test_stale_rows_behind_a_request_stay_out():
-    c = Case([5], [60], 4, 2, 64, 64).to_device()
+@pytest.mark.parametrize("n, dh, page", [(5, 64, 64), (2, 128, 16), (40, 128, 64), (40, 64, 16), (3, 128, 5)])
+def test_stale_rows_behind_a_request_stay_out(n, dh, page):
+    c = Case([n], [60], 4, 2, dh, page).to_device()
     c.pages.view(torch.uint8).masked_fill_(~_live(c)[..., None], 0x7f)  # NaN codes, NaN scales
     c.scales.masked_fill_(~_live(c), 255)
-    assert_close(_attend(c, {}, c.items(5)), *c.want())
+    assert_close(_attend(c, {}, c.items(n)), *c.want())
 
 
 def _live(c):
@@ -329,19 +344,22 @@ TREES = [
 ]
 
 
+@pytest.mark.parametrize("form", FORMS, indirect=True)
 @pytest.mark.parametrize("bits8", [False, True])
 @pytest.mark.parametrize("n, held, Hq, Hkv, dh, page, mask", TREES)
-def test_trees(n, held, Hq, Hkv, dh, page, mask, bits8):
+def test_trees(form, n, held, Hq, Hkv, dh, page, mask, bits8):
     c = Case(n, held, Hq, Hkv, dh, page, bits8=bits8).tree().to_device()
     assert_close(_tree(c, mask), *c.want(**mask))
     assert int(c.status) == 0
 
 
+@pytest.mark.parametrize("form", FORMS, indirect=True)
 @pytest.mark.parametrize("bits8", [False, True])
-def test_trees_with_sinks_slopes_and_caps_in_pieces(bits8):
+@pytest.mark.parametrize("cut", [4, 7, 50])
+def test_trees_with_sinks_slopes_and_caps_in_pieces(form, bits8, cut):
     c = Case([50, 9], [900, 64], 8, 2, 128, 64, bits8=bits8).tree().to_device()
     sink, slopes = _extras(8, True, True)
-    out = _tree(c, {}, c.items(7), sink=sink, slopes=slopes, softcap=4.0)  # a tree cut into several items
+    out = _tree(c, {}, c.items(cut), sink=sink, slopes=slopes, softcap=4.0)  # a tree cut into several items
     assert_close(out, *c.want(sink=sink, slopes=slopes, cap=4.0))
 
 
@@ -355,9 +373,10 @@ def test_a_chain_is_a_portion(bits8):
         assert_close(_attend(c, {}, c.items(20)), *c.want())
 
 
+@pytest.mark.parametrize("form", FORMS, indirect=True)
 @pytest.mark.parametrize("bits8", [False, True])
 @pytest.mark.parametrize("sink", [False, True])
-def test_tokens_whose_mask_leaves_nothing_are_zero(bits8, sink):
+def test_tokens_whose_mask_leaves_nothing_are_zero(form, bits8, sink):
     c = Case([6, 40], [0, 0], 4, 2, 128, 16, bits8=bits8).tree()
     c.masks[2] = 0
     c.masks[6 + 33:] = 0
@@ -379,8 +398,9 @@ def test_bits_beyond_a_requests_tokens_mean_nothing(bits8):
 
 
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
-@pytest.mark.parametrize("n, Hq", [(12, 4), (60, 8), (30, 16)])
-def test_infinite_and_nan_rows_of_a_bfloat16_cache_reach_those_that_see_them(n, Hq, bad):
+@pytest.mark.parametrize("n, Hq", [(7, 4), (12, 4), (60, 8), (30, 16)])
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+def test_infinite_and_nan_rows_of_a_bfloat16_cache_reach_those_that_see_them(form, n, Hq, bad):
     """Values that are not finite in a drafted token's row, and behind the last: only its descendants get them, in those entries."""
     c = Case([n, 2], [70, 5], Hq, 2, 128, 16, bits8=False).tree()
     place = 70 + 3
