@@ -9,17 +9,18 @@
 //   O += P V     tcgen05.mma with P in tensor memory and V from shared memory as an MN-major operand
 // S is double-buffered, so the next tile's score product runs while this tile's softmax does; products run in the order of
 // their issue: the score product of tile g + 2, which overwrites the buffer of S_g and P_g, is issued after O += P_g V_g.
-// Warp 0 issues the copies, warp 1 the products, warps 2 and 3 prepare values (below), sixteen warps do the softmax.
+// Warp 0 issues the copies, warp 1 the products, four warps prepare values (below), sixteen do the softmax.
 //
 // 8 bits: the keys' codes are an operand as they lie in the cache.  Queries are two: each entry (its row's largest brought to
 // 2^7 .. 2^8 by a power of two) as e4m3, and what is left of it as e5m2; the remainder of eight bits after the nearest four is
 // a whole number up to 8 of the entry's last unit, which e5m2 holds (three bits, and 2^-16 steps below), so both products add
 // up in one accumulator to that of the bfloat16 query, exact down to 2^-25 of the row's largest entry.  The e4m3 product has
-// twice the rate: two cost what one of bfloat16 does, and no key is converted.  The values' codes become float16, which holds
-// every one of them, once per tile and block by two warps (weights in 8-bit parts would have to be three, and cost the softmax
-// threads, which set the pace, more than they have).  A key's power of two multiplies its column of scores; a value's is added
-// to its key's exponent: w_j = 2^(s_j + e_j - ref), out = sum w_j code_j / sum w_j 2^-e_j, so that the weights fit float16
-// (2^-11 of each at most) whatever the values' scales.  Bfloat16: weights rounded to bfloat16 (2^-8).
+// twice the rate: two cost what one of bfloat16 does, and no key is converted.  A key's power of two multiplies its column of
+// scores.  The values become bfloat16, code times scale, which it holds exactly, once per tile and block: a code's seven bits
+// are a bfloat16 number's exponent and mantissa but for a factor of 2^120, which the multiplication with the scale takes along.
+// (Tried and slower: values' scales kept out of the operand, as exponents added to the keys' scores and taken out of the sum:
+// the three numbers a key that every softmax thread then reads take 1,500 cycles of a tile's shared-memory bandwidth.)
+// Weights are rounded to bfloat16 for the product with the values (2^-8 of each at most); sums are 32-bit.
 //
 // Masks: only tiles that some row does not see wholly look at them.  In such a tile a value that is not finite is taken out
 // (a product would spread 0 * infinity over all rows) and added to the rows that do see it at the end; of rows of the cache
@@ -36,8 +37,8 @@
 #define PARTS 4          // softmax threads per query row: each takes BKV / PARTS of a tile's keys and DH / PARTS of O's columns
 #define CP (BKV / PARTS)
 #define SOFTMAX0 4       // first softmax warp
-#define NTHREADS ((SOFTMAX0 + 4 * PARTS) * 32)
-#define AUX 64           // threads that prepare values
+#define NTHREADS ((SOFTMAX0 + 4 * PARTS + 2) * 32)
+#define AUX 128          // threads that prepare values: warps 2, 3 and the last two (one on each scheduler)
 #define GROWTH 6.0f      // how far a row's maximum may outgrow its reference (in powers of two) before O is rescaled
 #define SLOTS 4          // tiles whose scales are kept
 
@@ -139,12 +140,13 @@ __device__ __forceinline__ uint32_t swizzled(int r, int c) { return r * 128 + ((
 #define HALF_BYTES (128 * 128)  // 128 rows of 128 bytes
 template <bool F8> struct TcTile {
   static constexpr int Q = 2 * HALF_BYTES;                   // bfloat16: entries 0-63, 64-127; 8 bits: first parts, what is left
-  static constexpr int K = F8 ? HALF_BYTES : 2 * HALF_BYTES;  // a tile of keys, two of them
+  static constexpr int K = F8 ? HALF_BYTES : 2 * HALF_BYTES;  // a tile of keys
+  static constexpr int KS = F8 ? 4 : 3;                      // tiles of keys in flight
   static constexpr int V = 2 * HALF_BYTES;                   // a tile of values as an operand, two of them
   static constexpr int RAW = F8 ? HALF_BYTES : 0;            // a tile of values' codes, two of them
   static constexpr int BYTES = F8 ? 2 * BKV : 0;             // the scale bytes of a tile's keys and values, two of them
-  static constexpr int SCALES = F8 ? SLOTS * 3 * BKV * 4 : 0;  // [SLOTS][keys' scales, values' exponents, 2^-exponent]
-  static constexpr int SMEM = Q + 2 * K + 2 * V + 2 * RAW + 2 * BYTES + SCALES + 1024;
+  static constexpr int SCALES = F8 ? SLOTS * BKV * 2 : 0;    // [SLOTS] the keys' scales as bfloat16
+  static constexpr int SMEM = Q + KS * K + 2 * V + 2 * RAW + 2 * BYTES + SCALES + 1024;
 };
 
 template <bool F8>
@@ -153,23 +155,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   using T = TcTile<F8>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t *q_p = smem, *k_p = q_p + T::Q, *v_p = k_p + 2 * T::K, *raw_p = v_p + 2 * T::V;
+  uint8_t *q_p = smem, *k_p = q_p + T::Q, *v_p = k_p + T::KS * T::K, *raw_p = v_p + 2 * T::V;
   uint8_t* bytes_p = raw_p + 2 * T::RAW;
-  float* scales_p = reinterpret_cast<float*>(bytes_p + 2 * T::BYTES);
+  uint16_t* scales_p = reinterpret_cast<uint16_t*>(bytes_p + 2 * T::BYTES);
   // barriers (each use flips a phase bit; t = a tile's number)
   enum { B_QREADY = 0,    // Q is in shared memory
-         B_KFULL = 1,     // [2] K of tile t has landed                   stage t % 2, phase t / 2
-         B_KEMPTY = 3,    // [2] the score product of tile t is done
-         B_VFULL = 5,     // [2] V of tile t (codes and scale bytes) has landed
-         B_RAWEMPTY = 7,  // [2] the codes have been read
-         B_VREADY = 9,    // [2] V of tile t is an operand
-         B_VEMPTY = 11,   // [2] the product with P of tile t is done
-         B_SFULL = 13,    // [2] S of tile t is complete
-         B_PREADY = 15,   // P of tile t is in tensor memory, O rescaled   phase t
-         B_ODONE = 16,    // O holds the tiles up to t                     phase t
-         B_MEET = 17,     // [4] the threads of a quarter of the rows have met
-         B_SCALES = 21,   // [SLOTS] the scales of tile t are numbers      slot t % SLOTS, phase t / SLOTS
-         N_BARS = 25 };
+         B_KFULL = 1,     // [KS] K of tile t has landed                  stage t % KS, phase t / KS
+         B_KEMPTY = 5,    // [KS] the score product of tile t is done
+         B_VFULL = 9,     // [2] V of tile t (codes and scale bytes) has landed   stage t % 2, phase t / 2
+         B_RAWEMPTY = 11, // [2] the codes have been read
+         B_VREADY = 13,   // [2] V of tile t is an operand
+         B_VEMPTY = 15,   // [2] the product with P of tile t is done
+         B_SFULL = 17,    // [2] S of tile t is complete
+         B_PREADY = 19,   // P of tile t is in tensor memory, O rescaled   phase t
+         B_ODONE = 20,    // O holds the tiles up to t                     phase t
+         B_MEET = 21,     // [4] the threads of a quarter of the rows have met
+         B_SCALES = 25,   // [SLOTS] the keys' scales of tile t are there  slot t % SLOTS, phase t / SLOTS
+         N_BARS = 29 };
   __shared__ __align__(8) uint64_t bars[N_BARS];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, any_bad, span[4];
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     // tile later: each ring advances as soon as its own stage is free.  Lane i has box i of every tile.
     const int boxes = BKV / box_rows;
     auto load_tile = [&](int t, int which) {
-      const int st = t & 1, place = range0 + t * BKV + lane * box_rows;
+      const int st = which ? t & 1 : t % T::KS, place = range0 + t * BKV + lane * box_rows;
       const uint32_t bar = BAR((which ? B_VFULL : B_KFULL) + st);
       if (lane == 0) mbar_expect_tx(bar, BKV * DH * (F8 ? 1 : 2) + (F8 && which ? 2 * BKV : 0));
       __syncwarp();
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     uint32_t idle = 0;
     bool ok = true;
     while ((ik < n_tiles || iv < n_tiles) && ok) {
-      bool go_k = ik < n_tiles && (ik < 2 || mbar_try_wait(BAR(B_KEMPTY + (ik & 1)), ((ik >> 1) - 1) & 1));
+      bool go_k = ik < n_tiles && (ik < T::KS || mbar_try_wait(BAR(B_KEMPTY + ik % T::KS), (ik / T::KS - 1) & 1));
       bool go_v = iv < n_tiles && (iv < 2 || mbar_try_wait(BAR((F8 ? B_RAWEMPTY : B_VEMPTY) + (iv & 1)), ((iv >> 1) - 1) & 1));
       go_k = __shfl_sync(0xffffffffu, go_k, 0);
       go_v = __shfl_sync(0xffffffffu, go_v, 0);
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       ok = !__any_sync(0xffffffffu, gave_up(ok));
     }
     if (!ok) {  // let the copies in flight land before the block's shared memory is given up
-      for (int t = max(0, ik - 2); t < ik; ++t) mbar_wait(BAR(B_KFULL + (t & 1)), (t >> 1) & 1);
+      for (int t = max(0, ik - T::KS); t < ik; ++t) mbar_wait(BAR(B_KFULL + t % T::KS), (t / T::KS) & 1);
       for (int t = max(0, iv - 2); t < iv; ++t) mbar_wait(BAR(B_VFULL + (t & 1)), (t >> 1) & 1);
       if (lane == 0) {
         atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
@@ -286,11 +288,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     if (lane == 0 && n_tiles > 0) {
       bool ok = mbar_wait(BAR(B_QREADY), 0);
       auto issue_qk = [&](int t) {
-        const int st = t & 1;
-        if (ok) ok = mbar_wait(BAR(B_KFULL + st), (t >> 1) & 1);
+        const int st = t & 1, sk = t % T::KS;
+        if (ok) ok = mbar_wait(BAR(B_KFULL + sk), (t / T::KS) & 1);
         if (gave_up(ok)) { ok = false; return; }
         tc_fence_after();
-        const uint32_t q_s = smem_u32(q_p), k_s = smem_u32(k_p) + st * T::K;
+        const uint32_t q_s = smem_u32(q_p), k_s = smem_u32(k_p) + sk * T::K;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
           if (F8) {  // first parts, then what is left: four steps of 32 entries each
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
           }
         }
         umma_commit(BAR(B_SFULL + st));
-        umma_commit(BAR(B_KEMPTY + st));
+        umma_commit(BAR(B_KEMPTY + sk));
       };
       issue_qk(0);
       for (int t = 0; t < n_tiles && ok; ++t) {
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         const uint32_t v_s = smem_u32(v_p) + st * T::V;
 #pragma unroll
         for (int kk = 0; kk < BKV / 16; ++kk)  // P: 16 keys = 8 columns of tensor memory; V: 16 keys = 16 rows of 128 bytes
-          umma_f16_a_tmem(tm_o, tmem + st * 128 + kk * 8, desc_mn_major(v_s + kk * 16 * 128, HALF_BYTES), make_idesc(!F8, !F8, 1), (t | kk) != 0);
+          umma_f16_a_tmem(tm_o, tmem + st * 128 + kk * 8, desc_mn_major(v_s + kk * 16 * 128, HALF_BYTES), make_idesc(1, 1, 1), (t | kk) != 0);
         umma_commit(BAR(B_VEMPTY + st));
         umma_commit(BAR(B_ODONE));
       }
@@ -325,9 +327,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         failed = 1;
       }
     }
-  } else if (warp < SOFTMAX0) {
+  } else if (warp < SOFTMAX0 || warp >= SOFTMAX0 + 4 * PARTS) {
     // ------------------------------------------------------------------------------ values as an operand
-    const int i0 = threadIdx.x - 64;  // keys i0 and i0 + 64 of every tile
+    const int i0 = threadIdx.x - (warp < SOFTMAX0 ? 64 : (SOFTMAX0 + 4 * PARTS - 2) * 32);  // the key of every tile
     bool ok = true;
     for (int t = 0; t < n_tiles; ++t) {
       const int st = t & 1, place0 = range0 + t * BKV;
@@ -336,33 +338,55 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       if (__any_sync(0xffffffffu, gave_up(ok))) { ok = false; break; }
       uint8_t* v = v_p + st * T::V;
       if (F8) {
-        const uint8_t* raw = raw_p + st * T::RAW;
-        float* sc = scales_p + (t % SLOTS) * 3 * BKV;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int i = i0 + u * 64, bk = bytes_p[st * T::BYTES + i], bv = bytes_p[st * T::BYTES + BKV + i];
-          sc[i] = fp8_scale(bk);
-          sc[BKV + i] = bv == FP8_BAD ? __int_as_float(0x7fc00000) : (float)(bv - 127);
-          sc[2 * BKV + i] = __int_as_float((254 - min(bv, 254)) << 23);  // (finite for any byte: a masked key's weight is 0 and stays 0)
-        }
+        const int bk = bytes_p[st * T::BYTES + i0], bv = bytes_p[st * T::BYTES + BKV + i0];
+        scales_p[(t % SLOTS) * BKV + i0] = (uint16_t)(bk == FP8_BAD ? 0x7fc0 : bk << 7);
         mbar_arrive(BAR(B_SCALES + t % SLOTS));
+        const uint8_t* raw = raw_p + st * T::RAW;
+        // 2^(120 + e) in two factors: together they leave bfloat16's range only where e > 7.  Rows outside the range (their
+        // codes may be anything) count for nothing, whatever their byte; a row without codes is NaN for all rows that see it:
+        // at once if all do, at the end if some do not.
+        const bool in = place0 + i0 >= begin && place0 + i0 < end;
+        const int e = in ? min(bv, 254) - 127 : 0;
+        uint32_t f = (uint32_t)min(120 + e, 127) + 127, h = (uint32_t)max(e - 7, 0) + 127;
+        f = (f << 7) | (f << 23);
+        h = (h << 7) | (h << 23);
+        uint32_t keep = in ? 0xffffffffu : 0u, all = 0u;
+        if (in && bv == FP8_BAD) {
+          keep = 0u;
+          if (masked_tile(place0)) *(volatile int*)&any_bad = 1;
+          else all = 0x7fc07fc0u;
+        }
+        const __nv_bfloat162 f2 = *reinterpret_cast<const __nv_bfloat162*>(&f), h2 = *reinterpret_cast<const __nv_bfloat162*>(&h);
+        auto widen = [&](uint32_t x) {  // [0, code, 0, code] -> two numbers
+          const uint32_t y = ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u);
+          const __nv_bfloat162 z = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&y), f2);
+          return *reinterpret_cast<const uint32_t*>(&z);
+        };
+        auto further = [&](uint32_t x) {
+          const __nv_bfloat162 z = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), h2);
+          return *reinterpret_cast<const uint32_t*>(&z);
+        };
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int i = i0 + u * 64;
-          const bool in = place0 + i >= begin && place0 + i < end;
+        for (int c = 0; c < 8; ++c) {
+          const uint4 x = *reinterpret_cast<const uint4*>(raw + swizzled(i0, c));
+          const uint32_t w[4] = {x.x & keep, x.y & keep, x.z & keep, x.w & keep};
+          uint32_t o[8];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint4 x = *reinterpret_cast<const uint4*>(raw + swizzled(i, c));
-            if (!in) x = make_uint4(0u, 0u, 0u, 0u);
-            uint4 a, b;
-            fp8x4_to_half(x.x, a.x, a.y);
-            fp8x4_to_half(x.y, a.z, a.w);
-            fp8x4_to_half(x.z, b.x, b.y);
-            fp8x4_to_half(x.w, b.z, b.w);
-            uint8_t* half = v + (c >> 2) * HALF_BYTES;
-            *reinterpret_cast<uint4*>(half + swizzled(i, (c & 3) * 2)) = a;
-            *reinterpret_cast<uint4*>(half + swizzled(i, (c & 3) * 2 + 1)) = b;
+          for (int u = 0; u < 4; ++u) {
+            o[2 * u] = widen(__byte_perm(w[u], 0, 0x1404));
+            o[2 * u + 1] = widen(__byte_perm(w[u], 0, 0x3424));
           }
+          if (__builtin_expect(e > 7, 0)) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) o[u] = further(o[u]);
+          }
+          if (__builtin_expect(all != 0u, 0)) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) o[u] = all;
+          }
+          uint8_t* half = v + (c >> 2) * HALF_BYTES;
+          *reinterpret_cast<uint4*>(half + swizzled(i0, (c & 3) * 2)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(half + swizzled(i0, (c & 3) * 2 + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
         fence_async_proxy();
         mbar_arrive(BAR(B_RAWEMPTY + st));
@@ -468,32 +492,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       tmem_ld32(s_addr + col0, v);
       tmem_ld_wait();
       // base-2 exponents of the weights
-      const float* scp = scales_p + (t % SLOTS) * 3 * BKV + col0;
       const bool special = masked_tile(place0) || bent;
-      if (F8) {
-        const uint64_t sc2 = pack2(sc, sc);
+      const uint64_t sc2 = pack2(sc, sc);
 #pragma unroll
-        for (int c = 0; c < CP; c += 4) {
-          const float4 ks = *reinterpret_cast<const float4*>(scp + c);
-          const uint64_t f0 = mul2(sc2, pack2(ks.x, ks.y)), f1 = mul2(sc2, pack2(ks.z, ks.w));
-          uint64_t a = pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), b = pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
-          if (special) {
-            a = mul2(a, f0);
-            b = mul2(b, f1);
-          } else {
-            const float4 ve = *reinterpret_cast<const float4*>(scp + BKV + c);
-            a = fma2(a, f0, pack2(ve.x, ve.y));
-            b = fma2(b, f1, pack2(ve.z, ve.w));
-          }
-          v[c] = (uint32_t)a; v[c + 1] = (uint32_t)(a >> 32); v[c + 2] = (uint32_t)b; v[c + 3] = (uint32_t)(b >> 32);
-        }
-      } else {
-        const uint64_t sc2 = pack2(sc, sc);
+      for (int c = 0; c < CP; c += 8) {
+        uint4 ks;
+        if (F8) ks = *reinterpret_cast<const uint4*>(scales_p + (t % SLOTS) * BKV + col0 + c);
+        const uint32_t w[4] = {ks.x, ks.y, ks.z, ks.w};
 #pragma unroll
-        for (int c = 0; c < CP; c += 2) {
-          const uint64_t a = mul2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), sc2);
-          v[c] = (uint32_t)a;
-          v[c + 1] = (uint32_t)(a >> 32);
+        for (int u = 0; u < 4; ++u) {
+          uint64_t f = sc2;
+          if (F8) f = mul2(f, (uint64_t)(w[u] << 16) | ((uint64_t)(w[u] & 0xffff0000u) << 32));
+          f = mul2(f, pack2(__uint_as_float(v[c + 2 * u]), __uint_as_float(v[c + 2 * u + 1])));
+          v[c + 2 * u] = (uint32_t)f;
+          v[c + 2 * u + 1] = (uint32_t)(f >> 32);
         }
       }
       if (__builtin_expect(special, 0)) {
@@ -532,8 +544,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         }
 #pragma unroll
         for (int c = 0; c < CP; ++c) {
-          const float x = F8 ? __uint_as_float(v[c]) + scp[BKV + c] : __uint_as_float(v[c]);
-          v[c] = (sees >> c) & 1 ? __float_as_uint(x) : 0xff800000u;
+          v[c] = (sees >> c) & 1 ? v[c] : 0xff800000u;
         }
       }
       float mx4[4] = {ROWS_NEG_BIG, ROWS_NEG_BIG, ROWS_NEG_BIG, ROWS_NEG_BIG};  // four chains instead of one long one
@@ -558,20 +569,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       uint32_t packed[CP / 2];
 #pragma unroll
       for (int c = 0; c < CP; c += 4) {
-        const float4 vi = F8 ? *reinterpret_cast<const float4*>(scp + 2 * BKV + c) : make_float4(1.f, 1.f, 1.f, 1.f);
         const float p0 = rows_exp2(__uint_as_float(v[c]) - mx), p1 = rows_exp2(__uint_as_float(v[c + 1]) - mx);
         const float p2 = rows_exp2(__uint_as_float(v[c + 2]) - mx), p3 = rows_exp2(__uint_as_float(v[c + 3]) - mx);
-        if (F8) {
-          rs4[0] = fmaf(p0, vi.x, rs4[0]); rs4[1] = fmaf(p1, vi.y, rs4[1]); rs4[2] = fmaf(p2, vi.z, rs4[2]); rs4[3] = fmaf(p3, vi.w, rs4[3]);
-          const __half2 a = __floats2half2_rn(p0, p1), b = __floats2half2_rn(p2, p3);
-          packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&a);
-          packed[(c >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&b);
-        } else {
-          rs4[0] += p0; rs4[1] += p1; rs4[2] += p2; rs4[3] += p3;
-          const __nv_bfloat162 a = __floats2bfloat162_rn(p0, p1), b = __floats2bfloat162_rn(p2, p3);
-          packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&a);
-          packed[(c >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&b);
-        }
+        rs4[0] += p0; rs4[1] += p1; rs4[2] += p2; rs4[3] += p3;
+        const __nv_bfloat162 a = __floats2bfloat162_rn(p0, p1), b = __floats2bfloat162_rn(p2, p3);
+        packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&a);
+        packed[(c >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&b);
       }
       // P over the first half of this S buffer: keys 2c and 2c + 1 in column c (the partners have read their scores: they met
       // after their loads)
@@ -623,16 +626,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
 #pragma unroll
         for (int c = 0; c < 32; ++c) o[c] = 0u;
       }
-      if (!F8 && *(volatile int*)&any_bad && row < n_rows) {  // the values that were taken out, for the rows that see them
+      if (*(volatile int*)&any_bad && row < n_rows) {  // the values that were taken out, for the rows that see them
         for (int place = begin; place < end; ++place) {
           int key_pos;
           if (!masked_tile(place / BKV * BKV) || !rows_sees(P, it, tok.n, tok.p, tok.lo, place, key_pos)) continue;
           const int row_c = rows_cache_row(P, table, hk, place);
           if (row_c < 0) continue;
+          if (F8 && P.scales[row_c + v_off] != FP8_BAD) continue;
           const bf16* vp = reinterpret_cast<const bf16*>(P.pages) + (size_t)(row_c + v_off) * DH + part * 32;
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
-            const float y = __bfloat162float(vp[c]);
+            const float y = F8 ? __int_as_float(0x7fc00000) : __bfloat162float(vp[c]);
             if (!isfinite(y)) o[c] = __float_as_uint(__uint_as_float(o[c]) + y);
           }
         }

@@ -61,6 +61,7 @@ class Case:
             self.pages, self.scales = self.rows.to(torch.bfloat16), None
         self.q = (1.5 * torch.randn((self.N, Hq, dh), generator=gen)).to(torch.bfloat16)
         self.bits8, self.device, self.masks = bits8, device, None
+        self.weights = 2.0 ** -11 if bits8 else 2.0 ** -8  # rounding of the weights; served() says otherwise
         self.status = torch.zeros(1, dtype=torch.int32)
         self.scale = dh ** -0.5
 
@@ -90,6 +91,13 @@ class Case:
             if isinstance(v, torch.Tensor) and k != "rows":
                 setattr(self, k, v.to(self.device))
         return self
+
+    def served(self, max_count):
+        """To be called for the items that a kernel gets: the tcgen05 form rounds its weights to bfloat16 over either cache."""
+        from jax_llm_examples_b200.kernels import api as K
+
+        form = K.attention_rows_form(max_count * (self.Hq // self.Hkv), self.dh, self.page, True)
+        self.weights = 2.0 ** -11 if self.bits8 and form != "attention_rows_tc" else 2.0 ** -8
 
     def items(self, cut, which=lambda n: True):
         """(int32 [n, 2], count, largest count)"""
@@ -146,7 +154,7 @@ class Case:
                     w = w / total
                     out[at + i, h] = w @ v[:, h // G]
                     A = w @ v[:, h // G].abs()
-                    rel = (2.0 ** -11 if self.bits8 else 2.0 ** -8) + 2 * (2 * self.dh * 2.0 ** -24 * size + 2.0 ** -18)
+                    rel = self.weights + 2 * (2 * self.dh * 2.0 ** -24 * size + 2.0 ** -18)
                     tol[at + i, h] = 2.0 ** -8 * out[at + i, h].abs() + rel * A
                     if self.bits8:
                         e = v[:, h // G].abs().amax(-1) / 224  # at least the row's power of two

@@ -181,6 +181,7 @@ def _attend(c, mask, items=None, rows=None, out=None, max_kv=None, **kw):
     out = torch.full_like(c.q, 7.0) if out is None else out
     lead = (c.q, c.pages, c.scales, c.table, c.req, c.positions, out, c.scale, mask.get("chunk", 0), mask.get("window", 0), mask.get("temper", 0.0),
             mask.get("floor", 1.0), c.status, max_kv or max(a + b for a, b in zip(c.n, c.held)))
+    c.served(items[2] if items is not None else 1)
     if items is not None:
         kw |= dict(items=items[0], n_items=items[1], max_count=items[2])
     if rows is not None:
@@ -258,7 +259,8 @@ def test_portions_beside_single_tokens_write_their_own_rows_only():
     others = [i for i in range(c.N) if i not in single]
     assert_close(out, want, tol, others)
     _attend(c, {}, rows=torch.tensor(single, dtype=torch.int32, device="cuda"), out=out, sink=sink, slopes=slopes, softcap=5.0)
-    assert_close(out, want, tol)
+    assert_close(out, want, tol, others)
+    assert_close(out, *c.want(sink=sink, slopes=slopes, cap=5.0), single)
 
 
 @pytest.mark.parametrize("planned", [1, 64, 5000, 100000])
@@ -276,8 +278,9 @@ def test_rows_of_very_different_scales(form):
     c.set_rows8(s)
     c.to_device()
     out = _attend(c, {}, rows=torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
+    assert_close(out, *c.want(), [0, 1])
     _attend(c, {}, c.items(64, lambda n: n > 1), out=out)
-    assert_close(out, *c.want())
+    assert_close(out, *c.want(), slice(2, None))
 
 
 @pytest.mark.parametrize("form", FORMS, indirect=True)
@@ -327,6 +330,7 @@ def test_a_bad_page_raises_the_status_and_no_more():
 def _tree(c, mask, items=None, out=None, max_kv=None, **kw):
     out = torch.full_like(c.q, 7.0) if out is None else out
     items = items or c.items(max(c.n))
+    c.served(items[2])
     K().attention_tree(c.q, c.pages, c.table, c.req, c.positions, c.cu_q, c.q_start, c.masks, out, c.scale, mask.get("chunk", 0), mask.get("window", 0),
                        mask.get("temper", 0.0), mask.get("floor", 1.0), c.status, max_kv or max(a + b for a, b in zip(c.n, c.held)), *items, scales=c.scales, **kw)
     return out
@@ -496,6 +500,7 @@ def test_a_step_written_read_and_extended_by_a_tree():
         step.q, step.positions, step.table, step.page, step.masks = q, positions, c.table, 64, c.masks if first else None
         step.rows = (c.pages.float() * torch.exp2(c.scales.float() - 127)[..., None]).double().cpu()
         out = torch.empty_like(q)
+        step.served(n if first else 100)
         if first:
             c.q = q
             _tree(c, {}, out=out)
