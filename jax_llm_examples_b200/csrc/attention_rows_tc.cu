@@ -41,10 +41,14 @@
 #define AUX 128          // threads that prepare values: warps 2, 3 and the last two (one on each scheduler)
 #define GROWTH 6.0f      // how far a row's maximum may outgrow its reference (in powers of two) before O is rescaled
 #define SLOTS 4          // tiles whose scales are kept
+#define AHEAD 3          // tiles that are asked into L2 before shared memory has room for them
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -230,7 +234,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   const int* table = P.block_table + (size_t)it.r * P.bt_stride;
   const int v_off = P.Hkv * P.page_size;
   auto masked_tile = [&](int place0) { return place0 < full_lo || place0 + BKV > min(full_hi, end) || place0 < begin; };
-  auto gave_up = [&](bool ok) { return !ok || *(volatile int*)&failed; };
 
   if (warp == 0) {
     // ------------------------------------------------------------------------------ copies
@@ -261,6 +264,21 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       }
       __syncwarp();
     };
+    // Shared memory holds two tiles of values, the memory's latency under load is longer than a tile takes: the tiles after
+    // them are asked into L2.
+    auto ask_ahead = [&](int t) {
+      const int place = range0 + t * BKV + lane * box_rows;
+      if (t >= n_tiles || lane >= boxes || place >= end || place + box_rows <= begin) return;
+      const int pi = place / P.page_size, page = pi < P.bt_stride ? table[pi] : -1;
+      if (page < 0 || page >= P.num_pages) return;
+      const int row = (page * 2 * P.Hkv + hk) * P.page_size + (place - pi * P.page_size);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        tma_prefetch_2d(&map, 0, row + w * v_off);
+        if (!F8) tma_prefetch_2d(&map, 64, row + w * v_off);
+      }
+    };
+    for (int t = 2; t < 2 + AHEAD; ++t) ask_ahead(t);
     int ik = 0, iv = 0;
     uint32_t idle = 0;
     bool ok = true;
@@ -270,10 +288,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       go_k = __shfl_sync(0xffffffffu, go_k, 0);
       go_v = __shfl_sync(0xffffffffu, go_v, 0);
       if (go_k) load_tile(ik++, 0);
-      if (go_v) load_tile(iv++, 1);
+      if (go_v) {
+        load_tile(iv++, 1);
+        ask_ahead(iv + 1 + AHEAD);
+      }
       if (go_k || go_v) idle = 0;
       else if (++idle >= JLX_WAIT_LIMIT) ok = false;
-      ok = !__any_sync(0xffffffffu, gave_up(ok));
+      ok = __all_sync(0xffffffffu, ok && !*(volatile int*)&failed);
     }
     if (!ok) {  // let the copies in flight land before the block's shared memory is given up
       for (int t = max(0, ik - T::KS); t < ik; ++t) mbar_wait(BAR(B_KFULL + t % T::KS), (t / T::KS) & 1);
@@ -290,7 +311,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       auto issue_qk = [&](int t) {
         const int st = t & 1, sk = t % T::KS;
         if (ok) ok = mbar_wait(BAR(B_KFULL + sk), (t / T::KS) & 1);
-        if (gave_up(ok)) { ok = false; return; }
+        if (!ok) return;
         tc_fence_after();
         const uint32_t q_s = smem_u32(q_p), k_s = smem_u32(k_p) + sk * T::K;
 #pragma unroll
@@ -311,9 +332,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         const int st = t & 1;
         if (t + 1 < n_tiles) issue_qk(t + 1);
         if (!ok) break;
-        ok = mbar_wait(BAR(B_PREADY), t & 1);
-        if (ok) ok = mbar_wait(BAR(B_VREADY + st), (t >> 1) & 1);
-        if (gave_up(ok)) { ok = false; break; }
+        ok = mbar_wait(BAR(B_VREADY + st), (t >> 1) & 1);
+        if (ok) ok = mbar_wait(BAR(B_PREADY), t & 1);
+        if (!ok) break;
         tc_fence_after();
         const uint32_t v_s = smem_u32(v_p) + st * T::V;
 #pragma unroll
@@ -335,7 +356,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       const int st = t & 1, place0 = range0 + t * BKV;
       ok = mbar_wait(BAR(B_VFULL + st), (t >> 1) & 1);
       if (F8 && ok && t >= 2) ok = mbar_wait(BAR(B_VEMPTY + st), ((t >> 1) - 1) & 1);
-      if (__any_sync(0xffffffffu, gave_up(ok))) { ok = false; break; }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       uint8_t* v = v_p + st * T::V;
       if (F8) {
         const int bk = bytes_p[st * T::BYTES + i0], bv = bytes_p[st * T::BYTES + BKV + i0];
@@ -479,12 +501,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     bool ok = mbar_wait(BAR(B_QREADY), 0);  // (every row's power of two has been written)
     float sc = tok.sc;
     if (F8) sc *= *(volatile float*)&q_exp[row];
+    // The row's factor waits for the exponents (raw * sc - ref is one instruction) where it is positive, so that scores have
+    // their maximum where the raw ones have it, and nothing is done to the scores in between.
+    const bool late = sc > 0.f && !bent;
+    const float in = late ? 1.f : sc, out = late ? sc : 1.f;
     float m = ROWS_NEG_BIG, l = 0.f;
     for (int t = 0; t < n_tiles && ok; ++t) {
       const int st = t & 1, place0 = range0 + t * BKV, place = place0 + col0;
       ok = mbar_wait(BAR(B_SFULL + st), (t >> 1) & 1);
       if (F8 && ok) ok = mbar_wait(BAR(B_SCALES + t % SLOTS), (t / SLOTS) & 1);
-      ok = !__any_sync(0xffffffffu, gave_up(ok));
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       const uint32_t s_addr = tmem + st * 128 + lane_addr;
@@ -493,20 +519,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       tmem_ld_wait();
       // base-2 exponents of the weights
       const bool special = masked_tile(place0) || bent;
-      const uint64_t sc2 = pack2(sc, sc);
+      if (F8) {
 #pragma unroll
-      for (int c = 0; c < CP; c += 8) {
-        uint4 ks;
-        if (F8) ks = *reinterpret_cast<const uint4*>(scales_p + (t % SLOTS) * BKV + col0 + c);
-        const uint32_t w[4] = {ks.x, ks.y, ks.z, ks.w};
+        for (int c = 0; c < CP; c += 8) {
+          const uint4 ks = *reinterpret_cast<const uint4*>(scales_p + (t % SLOTS) * BKV + col0 + c);
+          const uint32_t w[4] = {ks.x, ks.y, ks.z, ks.w};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint64_t f = sc2;
-          if (F8) f = mul2(f, (uint64_t)(w[u] << 16) | ((uint64_t)(w[u] & 0xffff0000u) << 32));
-          f = mul2(f, pack2(__uint_as_float(v[c + 2 * u]), __uint_as_float(v[c + 2 * u + 1])));
-          v[c + 2 * u] = (uint32_t)f;
-          v[c + 2 * u + 1] = (uint32_t)(f >> 32);
+          for (int u = 0; u < 4; ++u) {
+            const uint64_t f = mul2((uint64_t)(w[u] << 16) | ((uint64_t)(w[u] & 0xffff0000u) << 32),
+                                    pack2(__uint_as_float(v[c + 2 * u]), __uint_as_float(v[c + 2 * u + 1])));
+            v[c + 2 * u] = (uint32_t)f;
+            v[c + 2 * u + 1] = (uint32_t)(f >> 32);
+          }
         }
+      }
+      if (__builtin_expect(!late, 0)) {
+#pragma unroll
+        for (int c = 0; c < CP; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * in);
       }
       if (__builtin_expect(special, 0)) {
         if (capped) {
@@ -556,11 +585,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       xmax[mp][part][row] = mx;
       mbar_arrive(BAR(B_MEET + quarter));
       ok = mbar_wait(BAR(B_MEET + quarter), mp);
-      ok = !__any_sync(0xffffffffu, gave_up(ok));
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
 #pragma unroll
       for (int q = 0; q < PARTS; ++q) mx = fmaxf(mx, xmax[mp][q][row]);
-      mx = fmaxf(m, mx);
+      mx = fmaxf(m, mx > 0.5f * ROWS_NEG_BIG ? mx * out : ROWS_NEG_BIG);
       // While no row of this quarter has grown by more than GROWTH beyond its reference, the references stay, the weights may
       // exceed 1 (up to 64), and O is not rescaled.  All threads of these rows decide alike: they hold the same references.
       if (__all_sync(0xffffffffu, mx - m <= GROWTH)) mx = m;
@@ -569,8 +598,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       uint32_t packed[CP / 2];
 #pragma unroll
       for (int c = 0; c < CP; c += 4) {
-        const float p0 = rows_exp2(__uint_as_float(v[c]) - mx), p1 = rows_exp2(__uint_as_float(v[c + 1]) - mx);
-        const float p2 = rows_exp2(__uint_as_float(v[c + 2]) - mx), p3 = rows_exp2(__uint_as_float(v[c + 3]) - mx);
+        const float p0 = rows_exp2(fmaf(__uint_as_float(v[c]), out, -mx)), p1 = rows_exp2(fmaf(__uint_as_float(v[c + 1]), out, -mx));
+        const float p2 = rows_exp2(fmaf(__uint_as_float(v[c + 2]), out, -mx)), p3 = rows_exp2(fmaf(__uint_as_float(v[c + 3]), out, -mx));
         rs4[0] += p0; rs4[1] += p1; rs4[2] += p2; rs4[3] += p3;
         const __nv_bfloat162 a = __floats2bfloat162_rn(p0, p1), b = __floats2bfloat162_rn(p2, p3);
         packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&a);
@@ -584,8 +613,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       // The product of the previous tile must be complete before O is rescaled, and every thread waits for it whether it
       // rescales or not: a barrier's phase bit tells a waiter the truth only if the waiter has seen the phase before.
       if (t > 0) {
-        ok = mbar_wait(BAR(B_ODONE), (t - 1) & 1);
-        ok = !__any_sync(0xffffffffu, gave_up(ok));
+        ok = __all_sync(0xffffffffu, mbar_wait(BAR(B_ODONE), (t - 1) & 1));
         if (!ok) break;
         if (!__all_sync(0xffffffffu, corr == 1.f)) {
           tc_fence_after();
@@ -603,15 +631,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     }
     // the end: the last product, the row's sum (the sum of the parts' sums), the store
     if (ok && n_tiles > 0) {
-      ok = mbar_wait(BAR(B_ODONE), (n_tiles - 1) & 1);
-      ok = !__any_sync(0xffffffffu, gave_up(ok));
+      ok = __all_sync(0xffffffffu, mbar_wait(BAR(B_ODONE), (n_tiles - 1) & 1));
     }
     if (ok) {
       tc_fence_after();
       const int mp = n_tiles & 1;
       xmax[mp][part][row] = l;
       mbar_arrive(BAR(B_MEET + quarter));
-      ok = !__any_sync(0xffffffffu, !mbar_wait(BAR(B_MEET + quarter), mp));
+      ok = __all_sync(0xffffffffu, mbar_wait(BAR(B_MEET + quarter), mp));
     }
     if (ok) {
       const int mp = n_tiles & 1;
