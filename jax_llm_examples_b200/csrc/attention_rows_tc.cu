@@ -41,6 +41,7 @@
 #define AUX 128          // threads that prepare values: warps 2, 3 and the last two (one on each scheduler)
 #define GROWTH 6.0f      // how far a row's maximum may outgrow its reference (in powers of two) before O is rescaled
 #define SLOTS 4          // tiles whose scales are kept
+#define ROW_RING 8       // tiles whose places in the cache are known ahead (more than AHEAD + 2)
 #define AHEAD 3          // tiles that are asked into L2 before shared memory has room for them
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -49,6 +50,12 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
 }
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+// Whether the phase is complete, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -154,7 +161,7 @@ template <bool F8> struct TcTile {
 };
 
 template <bool F8>
-__global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __grid_constant__ CUtensorMap map, const RowsParams P, int box_rows) {
+__global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __grid_constant__ CUtensorMap map, const RowsParams P, int box_rows, int row_tiles) {
   JLX_TL(TL_ATTN_PREFILL);
   using T = TcTile<F8>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -180,14 +187,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, any_bad, span[4];
   __shared__ float xmax[2][PARTS][BQ];  // [meeting parity][part][row]: what the threads of a row exchange
+  __shared__ int box_row[ROW_RING][8];  // cache rows of a tile's boxes of keys, by the tile's number
   __shared__ float q_exp[BQ];           // 8 bits: the power of two that a query row was divided by
   pdl_launch_dependents_if_small();
   pdl_wait();
   const uint32_t bar0 = smem_u32(&bars[0]);
   auto BAR = [bar0](int i) { return bar0 + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x % P.splits, item_i = blockIdx.x / P.splits;
-  const int tiles_y = gridDim.y / P.Hkv, hk = blockIdx.y / tiles_y, row0 = (blockIdx.y - hk * tiles_y) * BQ;
+  // an item's ranges, heads and row tiles side by side, then the next item: the items' order (the longest first, say) is the blocks'
+  const int unit = blockIdx.x / P.splits, split = blockIdx.x - unit * P.splits, item_i = unit / (P.Hkv * row_tiles);
+  const int hk = unit % (P.Hkv * row_tiles) / row_tiles, row0 = unit % row_tiles * BQ;
   RowsItem it;
   if (!rows_item(P, item_i, it)) return;
   const int G = P.Hq / P.Hkv, n_rows = min(it.cnt * G - row0, BQ);
@@ -239,20 +248,41 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     // ------------------------------------------------------------------------------ copies
     // Keys are free again after their score product, values after the product with P (or their conversion), which comes a
     // tile later: each ring advances as soon as its own stage is free.  Lane i has box i of every tile.
+    // What a copy needs to know of the block table is fetched a tile ahead of the request into L2, which itself runs AHEAD
+    // tiles ahead of the copies: shared memory holds two tiles of values, and the memory's latency under load is longer than
+    // a tile takes.
     const int boxes = BKV / box_rows;
+    auto find_page = [&](int t) {
+      const int pi = (range0 + t * BKV + lane * box_rows) / P.page_size;
+      return lane < boxes && t < n_tiles && pi < P.bt_stride ? table[pi] : -1;
+    };
+    auto place_tile = [&](int t, int page, bool ask) {
+      if (lane < boxes && t < n_tiles) {
+        const int place = range0 + t * BKV + lane * box_rows;
+        const bool wanted = place < end && place + box_rows > begin;
+        if (page < 0 || page >= P.num_pages) {
+          if (wanted) atomicOr(P.status, JLX_STATUS_BAD_PAGE);
+          page = 0;  // no page there: every key of the box is masked
+        }
+        const int row = (page * 2 * P.Hkv + hk) * P.page_size + place % P.page_size;
+        box_row[t % ROW_RING][lane] = row;
+        if (ask && wanted) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            tma_prefetch_2d(&map, 0, row + w * v_off);
+            if (!F8) tma_prefetch_2d(&map, 64, row + w * v_off);
+          }
+        }
+      }
+      __syncwarp();
+    };
     auto load_tile = [&](int t, int which) {
-      const int st = which ? t & 1 : t % T::KS, place = range0 + t * BKV + lane * box_rows;
+      const int st = which ? t & 1 : t % T::KS;
       const uint32_t bar = BAR((which ? B_VFULL : B_KFULL) + st);
       if (lane == 0) mbar_expect_tx(bar, BKV * DH * (F8 ? 1 : 2) + (F8 && which ? 2 * BKV : 0));
       __syncwarp();
       if (lane < boxes) {
-        const int pi = place / P.page_size;
-        int page = pi < P.bt_stride ? table[pi] : -1;
-        if (page < 0 || page >= P.num_pages) {
-          if (place < end && place + box_rows > begin) atomicOr(P.status, JLX_STATUS_BAD_PAGE);
-          page = 0;  // no page there: every key of the box is masked
-        }
-        const int row = (page * 2 * P.Hkv + hk) * P.page_size + (place - pi * P.page_size);
+        const int row = box_row[t % ROW_RING][lane];
         const uint32_t dst = smem_u32(which ? (F8 ? raw_p + st * T::RAW : v_p + st * T::V) : k_p + st * T::K) + lane * box_rows * 128;
         tma_load_2d(dst, &map, 0, row + which * v_off, bar);
         if (!F8) tma_load_2d(dst + HALF_BYTES, &map, 64, row + which * v_off, bar);
@@ -264,36 +294,35 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       }
       __syncwarp();
     };
-    // Shared memory holds two tiles of values, the memory's latency under load is longer than a tile takes: the tiles after
-    // them are asked into L2.
-    auto ask_ahead = [&](int t) {
-      const int place = range0 + t * BKV + lane * box_rows;
-      if (t >= n_tiles || lane >= boxes || place >= end || place + box_rows <= begin) return;
-      const int pi = place / P.page_size, page = pi < P.bt_stride ? table[pi] : -1;
-      if (page < 0 || page >= P.num_pages) return;
-      const int row = (page * 2 * P.Hkv + hk) * P.page_size + (place - pi * P.page_size);
+    {
+      int pages[AHEAD + 2];
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        tma_prefetch_2d(&map, 0, row + w * v_off);
-        if (!F8) tma_prefetch_2d(&map, 64, row + w * v_off);
-      }
-    };
-    for (int t = 2; t < 2 + AHEAD; ++t) ask_ahead(t);
+      for (int t = 0; t < AHEAD + 2; ++t) pages[t] = find_page(t);
+#pragma unroll
+      for (int t = 0; t < AHEAD + 2; ++t) place_tile(t, pages[t], t >= 2);
+    }
+    int next = AHEAD + 2, page = find_page(next);  // the tile to be placed next
     int ik = 0, iv = 0;
     uint32_t idle = 0;
     bool ok = true;
     while ((ik < n_tiles || iv < n_tiles) && ok) {
-      bool go_k = ik < n_tiles && (ik < T::KS || mbar_try_wait(BAR(B_KEMPTY + ik % T::KS), (ik / T::KS - 1) & 1));
-      bool go_v = iv < n_tiles && (iv < 2 || mbar_try_wait(BAR((F8 ? B_RAWEMPTY : B_VEMPTY) + (iv & 1)), ((iv >> 1) - 1) & 1));
+      // (keys at most AHEAD + 1 tiles before values: their places are known)
+      bool go_k = ik < n_tiles && ik < next && (ik < T::KS || mbar_test(BAR(B_KEMPTY + ik % T::KS), (ik / T::KS - 1) & 1));
+      bool go_v = iv < n_tiles && (iv < 2 || mbar_test(BAR((F8 ? B_RAWEMPTY : B_VEMPTY) + (iv & 1)), ((iv >> 1) - 1) & 1));
       go_k = __shfl_sync(0xffffffffu, go_k, 0);
       go_v = __shfl_sync(0xffffffffu, go_v, 0);
       if (go_k) load_tile(ik++, 0);
       if (go_v) {
         load_tile(iv++, 1);
-        ask_ahead(iv + 1 + AHEAD);
+        place_tile(next, page, true);
+        page = find_page(++next);
       }
-      if (go_k || go_v) idle = 0;
-      else if (++idle >= JLX_WAIT_LIMIT) ok = false;
+      if (go_k || go_v) {
+        idle = 0;
+      } else {
+        __nanosleep(20);
+        if (++idle >= 8 * JLX_WAIT_LIMIT) ok = false;
+      }
       ok = __all_sync(0xffffffffu, ok && !*(volatile int*)&failed);
     }
     if (!ok) {  // let the copies in flight land before the block's shared memory is given up
@@ -706,7 +735,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
 
 // -------------------------------------------------------------------------------------------- host
 template <bool F8>
-static int launch_tc(const RowsParams& P, int box_rows, dim3 grid, cudaStream_t stream) {
+static int launch_tc(const RowsParams& P, int box_rows, int row_tiles, cudaStream_t stream) {
   static unsigned long long allowed = 0;  // a bit per device: the attribute belongs to the device's context
   int dev = 0;
   JLX_CUDA(cudaGetDevice(&dev));
@@ -716,7 +745,9 @@ static int launch_tc(const RowsParams& P, int box_rows, dim3 grid, cudaStream_t 
   }
   CUtensorMap map;
   if (int rc = rows_map(P, DH, F8, box_rows, &map)) return rc;
-  JLX_CUDA(jlx_launch_pdl(attention_rows_tc_kernel<F8>, grid, dim3(NTHREADS), TcTile<F8>::SMEM, stream, map, P, box_rows));
+  const long long blocks = (long long)P.n_items * P.splits * P.Hkv * row_tiles;
+  JLX_REQUIRE(blocks < (1ll << 31), "attention over rows: too many items or rows");
+  JLX_CUDA(jlx_launch_pdl(attention_rows_tc_kernel<F8>, dim3((unsigned)blocks), dim3(NTHREADS), TcTile<F8>::SMEM, stream, map, P, box_rows, row_tiles));
   return 0;
 }
 
@@ -726,10 +757,8 @@ JLX_API int jlx_attention_rows_tc(const RowsArgs* a, cudaStream_t stream) {
   JLX_REQUIRE(a->dh == DH && a->page_size % 16 == 0 && ((uintptr_t)a->scales & 15) == 0, "attention over rows (tcgen05): needs head size 128, pages of a multiple of 16 tokens and scales on a 16-byte boundary");
   if (P.n_items == 0) return 0;
   const int rows = a->max_count * (P.Hq / P.Hkv), box_rows = P.page_size % 64 == 0 ? 64 : P.page_size % 32 == 0 ? 32 : 16;
-  const long long gx = (long long)P.n_items * P.splits, gy = (long long)P.Hkv * ((rows + BQ - 1) / BQ);
-  JLX_REQUIRE(gx < (1ll << 31) && gy <= 65535, "attention over rows: too many items or rows");
   JLX_REQUIRE(P.splits == 1 || (P.part_o && P.part_ml), "attention over rows: scratch for the ranges is missing");
-  const dim3 grid((unsigned)gx, (unsigned)gy);
-  if (int rc = P.scales ? launch_tc<true>(P, box_rows, grid, stream) : launch_tc<false>(P, box_rows, grid, stream)) return rc;
+  const int row_tiles = (rows + BQ - 1) / BQ;
+  if (int rc = P.scales ? launch_tc<true>(P, box_rows, row_tiles, stream) : launch_tc<false>(P, box_rows, row_tiles, stream)) return rc;
   return P.splits > 1 ? launch_rows_join<DH>(P, a->max_count, stream) : 0;
 }
