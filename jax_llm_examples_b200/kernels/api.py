@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes
 import dataclasses
 import functools
+import struct
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
 
 import torch
@@ -1109,9 +1110,9 @@ def attention_prefill_tc(q: torch.Tensor, pages: torch.Tensor, block_table: torc
 FP8 = torch.float8_e4m3fn  # pages in 8 bits: e4m3 codes, and a byte of scale per row (csrc/fp8_rows.cuh)
 
 
-def _ints(what: str, **tensors: "tuple[torch.Tensor | None, int]") -> None:
+def _ints(what: str, *arrays: "tuple[str, torch.Tensor | None, int]") -> None:
     """Index arrays: contiguous int32 with at least so many entries."""
-    for name, (t, n) in tensors.items():
+    for name, t, n in arrays:
         if t is not None and (t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous()):
             raise KernelError(f"{what}: {name} must be contiguous int32 with at least {n} entries")
 
@@ -1127,8 +1128,12 @@ def _same_device(what: str, *tensors: torch.Tensor | None) -> int:
     return dev
 
 
-def _raw_stream(dev: int):
+def _raw_stream(dev: int) -> c_void_p:
     return c_void_p(torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _address(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _cache8(what: str, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, Hkv: int, dh: int) -> None:
@@ -1141,22 +1146,16 @@ def _cache8(what: str, pages: torch.Tensor, scales: torch.Tensor, block_table: t
     _contig(pages, scales, block_table)
 
 
-class _KvFp8Args(ctypes.Structure):  # KvFp8Params in csrc/kv_fp8.cu
-    _fields_ = [("pages", c_void_p), ("scales", c_void_p), ("block_table", c_void_p), ("bt_stride", c_int), ("n_requests", c_int),
-                ("req_of_token", c_void_p), ("places", c_void_p), ("N", c_int), ("Hkv", c_int), ("dh", c_int), ("page_size", c_int),
-                ("num_pages", c_int), ("lanes", c_int), ("status", c_void_p)]
+# What the launchers take as one structure, laid out as in C (packing it costs a call less than a ctypes.Structure does).
+_KV_FP8_ARGS = struct.Struct("@3P2i2P6iPi0P")  # KvFp8Params in csrc/kv_fp8.cu
+_ROPE_FP8_ARGS = struct.Struct("@4Pq4if")  # RopeFp8Args in csrc/kv_fp8.cu
 
 
-class _RopeFp8Args(ctypes.Structure):  # RopeFp8Args in csrc/kv_fp8.cu
-    _fields_ = [("qkv", c_void_p), ("q_out", c_void_p), ("positions", c_void_p), ("inv_freq", c_void_p), ("split_stride", c_longlong), ("in_dtype", c_int),
-                ("splits", c_int), ("Hq", c_int), ("l2norm", c_int), ("eps", c_float)]
-
-
-def _kv_fp8_args(pages, scales, block_table, req_of_token, places, N: int, status) -> _KvFp8Args:
+def _kv_fp8_args(pages, scales, block_table, req_of_token, places, N: int, status) -> bytes:
     P, _, Hkv, page_size, dh = pages.shape
     R, width = block_table.shape
-    return _KvFp8Args(pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), width, R, req_of_token.data_ptr(), places.data_ptr(), N, Hkv, dh,
-                      page_size, P, 0, status.data_ptr())
+    return _KV_FP8_ARGS.pack(pages.data_ptr(), scales.data_ptr(), block_table.data_ptr(), width, R, req_of_token.data_ptr(), places.data_ptr(), N, Hkv,
+                             dh, page_size, P, 0, status.data_ptr(), 0)
 
 
 def kv_store_fp8(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
@@ -1170,12 +1169,12 @@ def kv_store_fp8(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: 
     _contig(k, v)
     N, Hkv, dh = k.shape
     _cache8("kv_store_fp8", pages, scales, block_table, Hkv, dh)
-    _ints("kv_store_fp8", req_of_token=(req_of_token, N), places=(places, N), status=(status, 1))
+    _ints("kv_store_fp8", ("req_of_token", req_of_token, N), ("places", places, N), ("status", status, 1))
     if v.shape != k.shape or v.dtype != k.dtype:
         raise KernelError("kv_store_fp8: keys and values must have one shape and type")
     dev = _same_device("kv_store_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
     args = _kv_fp8_args(pages, scales, block_table, req_of_token, places, N, status)
-    _run("kv_fp8", "jlx_kv_store_fp8", ctypes.byref(args), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
+    _run("kv_fp8", "jlx_kv_store_fp8", args, c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
 
 
 def rope_kv_store_fp8(qkv: torch.Tensor, q_out: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
@@ -1188,7 +1187,7 @@ def rope_kv_store_fp8(qkv: torch.Tensor, q_out: torch.Tensor, pages: torch.Tenso
     N = q_out.shape[0]
     places = positions if places is None else places
     _cache8("rope_kv_store_fp8", pages, scales, block_table, Hkv, dh)
-    _ints("rope_kv_store_fp8", req_of_token=(req_of_token, N), positions=(positions, N), places=(places, N), status=(status, 1))
+    _ints("rope_kv_store_fp8", ("req_of_token", req_of_token, N), ("positions", positions, N), ("places", places, N), ("status", status, 1))
     if q_out.dtype != torch.bfloat16 or tuple(q_out.shape) != (N, Hq, dh) or splits < 1 or qkv.numel() != splits * N * (Hq + 2 * Hkv) * dh:
         raise KernelError(f"rope_kv_store_fp8: {splits} x {N} projected rows of {Hq} + 2 * {Hkv} heads of {dh} and bfloat16 queries do not "
                           f"fit qkv {tuple(qkv.shape)}, q_out {q_out.dtype} {tuple(q_out.shape)}")
@@ -1196,9 +1195,9 @@ def rope_kv_store_fp8(qkv: torch.Tensor, q_out: torch.Tensor, pages: torch.Tenso
         raise KernelError(f"rope_kv_store_fp8: {dh // 2} float32 frequencies are needed")
     dev = _same_device("rope_kv_store_fp8", qkv, q_out, pages, scales, block_table, req_of_token, positions, places, inv_freq, status)
     args = _kv_fp8_args(pages, scales, block_table, req_of_token, places, N, status)
-    rope = _RopeFp8Args(qkv.data_ptr(), q_out.data_ptr(), positions.data_ptr(), None if inv_freq is None else inv_freq.data_ptr(),
-                        0 if splits == 1 else qkv.numel() // splits, code(qkv.dtype), splits, Hq, int(l2norm), eps)
-    _run("kv_fp8", "jlx_rope_kv_store_fp8", ctypes.byref(args), ctypes.byref(rope), _raw_stream(dev))
+    rope = _ROPE_FP8_ARGS.pack(qkv.data_ptr(), q_out.data_ptr(), positions.data_ptr(), _address(inv_freq), 0 if splits == 1 else qkv.numel() // splits,
+                               code(qkv.dtype), splits, Hq, int(l2norm), eps)
+    _run("kv_fp8", "jlx_rope_kv_store_fp8", args, rope, _raw_stream(dev))
 
 
 def kv_load_fp8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, req_of_token: torch.Tensor, places: torch.Tensor,
@@ -1208,25 +1207,19 @@ def kv_load_fp8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Te
     _contig(k, v)
     N, Hkv, dh = k.shape
     _cache8("kv_load_fp8", pages, scales, block_table, Hkv, dh)
-    _ints("kv_load_fp8", req_of_token=(req_of_token, N), places=(places, N), status=(status, 1))
+    _ints("kv_load_fp8", ("req_of_token", req_of_token, N), ("places", places, N), ("status", status, 1))
     if v.shape != k.shape or v.dtype != k.dtype:
         raise KernelError("kv_load_fp8: keys and values must have one shape and type")
     dev = _same_device("kv_load_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
     args = _kv_fp8_args(pages, scales, block_table, req_of_token, places, N, status)
-    _run("kv_fp8", "jlx_kv_load_fp8", ctypes.byref(args), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
+    _run("kv_fp8", "jlx_kv_load_fp8", args, c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
 
 
-class _RowsArgs(ctypes.Structure):  # RowsArgs in csrc/attention_rows.cuh
-    _fields_ = [(n, c_void_p) for n in ("q", "pages", "scales", "block_table", "req_of_token", "positions", "out", "items", "rows", "cu_q", "q_start",
-                                        "masks", "sink", "slopes", "part_o", "part_ml", "status")] + \
-               [(n, c_int) for n in ("bt_stride", "n_requests", "n_items", "max_count", "words", "N", "Hq", "Hkv", "dh", "page_size", "num_pages", "chunk",
-                                     "window", "splits")] + \
-               [(n, c_float) for n in ("scale", "softcap", "attn_scale", "floor_scale")]
-
-
+_ROWS_ARGS = struct.Struct("@17P14i4f")  # RowsArgs in csrc/attention_rows.cuh
 ROWS_TILE = 64  # keys of a tile, csrc/attention_rows.cu and attention_few.cu
 ROWS_FEW = 16  # query rows of an item and KV head that attention_few.cu takes
 ROWS_CLUSTER = 8  # ranges that it joins without scratch
+_ROWS_LAUNCHERS = {form: "jlx_" + form for form in ("attention_few", "attention_rows", "attention_rows_tc")}
 
 
 def attention_rows_supported(q_dtype: torch.dtype, Hq: int, Hkv: int, dh: int) -> bool:
@@ -1281,8 +1274,8 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     if block_table.dtype != torch.int32 or block_table.dim() != 2:
         raise KernelError(f"{what}: the block table must be int32 [requests, pages of one]")
     R, width = block_table.shape
-    _ints(what, req_of_token=(req_of_token, N), positions=(positions, N), items=(items, 2 * n_items), rows=(rows, n_items), status=(status, 1),
-          cu_q=(cu_q, R + 1), q_start=(q_start, R), masks=(masks, N))
+    _ints(what, ("req_of_token", req_of_token, N), ("positions", positions, N), ("items", items, 2 * n_items), ("rows", rows, n_items),
+          ("status", status, 1), ("cu_q", cu_q, R + 1), ("q_start", q_start, R), ("masks", masks, N))
     words = 0
     if masks is not None:
         if masks.dim() != 2 or masks.shape[0] != N:
@@ -1298,7 +1291,8 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
         return
     if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
         raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
-    form = attention_rows_form(max_count * (Hq // Hkv), dh, page_size, scales is None or scales.data_ptr() % 16 == 0)
+    scales_p = _address(scales)
+    form = attention_rows_form(max_count * (Hq // Hkv), dh, page_size, scales_p % 16 == 0)
     splits = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
     part_o = part_ml = joined = 0
     if splits > (ROWS_CLUSTER if form == "attention_few" else 1):
@@ -1306,11 +1300,11 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
         scratch = torch.empty(N * Hq * splits * (dh + 2), dtype=torch.float32, device=q.device)
         part_o = scratch.data_ptr()
         part_ml, joined = part_o + 4 * N * Hq * splits * dh, 1
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    args = _RowsArgs(q_p, pages.data_ptr(), p(scales), block_table.data_ptr(), req_of_token.data_ptr(), positions.data_ptr(), out_p, p(items), p(rows),
-                     p(cu_q), p(q_start), p(masks), p(sink), p(slopes), part_o, part_ml, status.data_ptr(), width, R, n_items, max_count, words, N, Hq,
-                     Hkv, dh, page_size, P, chunk, window, splits, scale, softcap, attn_scale, floor_scale)
-    _run(form, "jlx_" + form, ctypes.byref(args), _raw_stream(dev))
+    args = _ROWS_ARGS.pack(q_p, pages.data_ptr(), scales_p, block_table.data_ptr(), req_of_token.data_ptr(), positions.data_ptr(), out_p,
+                           _address(items), _address(rows), _address(cu_q), _address(q_start), _address(masks), _address(sink), _address(slopes),
+                           part_o, part_ml, status.data_ptr(), width, R, n_items, max_count, words, N, Hq, Hkv, dh, page_size, P, chunk, window, splits,
+                           scale, softcap, attn_scale, floor_scale)
+    _run(form, _ROWS_LAUNCHERS[form], args, _raw_stream(dev))
     global _launches
     _launches += joined  # the joining kernel
 
