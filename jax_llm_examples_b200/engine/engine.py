@@ -78,16 +78,21 @@ class Engine:
     as fit into ``memory_fraction`` of the GPU memory that is free when the engine is made.
     ``max_seq_len``: longest request (sets the block-table width); default ``max_tokens`` (131072 when the
     pool is sized from free memory).
+    ``cache_dtype``: what keys and values are kept in: the activations' type (None), or ``torch.float8_e4m3fn``: 8 bits and a
+    scale byte per token, head and plane, about half the memory and half the bytes a decoded token reads.  For models whose
+    layers all take such a cache (bfloat16, :class:`PagedAttention` with heads of 64 or 128); others are refused.
     """
 
     DEFAULT_MAX_SEQ_LEN = 131072  # longest request when neither max_tokens nor max_seq_len says otherwise
 
     def __init__(self, model: DecoderModel, *, max_tokens: int | None, page_size: int = 64, max_slots: int = 64,
-                 max_seq_len: int | None = None, use_graphs: bool | None = None, memory_fraction: float = 0.9):
+                 max_seq_len: int | None = None, use_graphs: bool | None = None, memory_fraction: float = 0.9,
+                 cache_dtype: torch.dtype | None = None):
+        cache_dtype = self.cache_type(model, cache_dtype)
         if not torch.cuda.is_available():
             raise EngineError("no CUDA device: this engine runs on a GPU only and has no CPU path")
         if max_tokens is None:
-            max_tokens = self.tokens_that_fit(model, page_size, memory_fraction)
+            max_tokens = self.tokens_that_fit(model, page_size, memory_fraction, cache_dtype)
             if max_seq_len is None:  # a pool of millions of tokens: the block tables need not be that wide
                 max_seq_len = min(max_tokens, self.DEFAULT_MAX_SEQ_LEN)
         if page_size <= 0 or max_tokens <= 0:
@@ -98,13 +103,16 @@ class Engine:
         self.max_seq_len = max_seq_len or max_tokens
         self.max_pages_per_request = -(-self.max_seq_len // page_size)
         plan = model.plan
-        K.preload(model.required_libraries())
+        in_8_bits = cache_dtype == K.FP8
+        K.preload(model.required_libraries() + (model.cache8_libraries() if in_8_bits else ()))
         self.manager = CacheManager(page_size, max_slots, self.max_pages_per_request)
         for r in plan.groups:
             self.manager.add_group(r, self.num_pages)
-        dev, dt = self.runtime.device, self.runtime.dtype
-        self.kv = [torch.zeros((self.num_pages, c.planes, c.num_kv_heads, page_size, c.head_dim), dtype=dt, device=dev)
+        dev = self.runtime.device
+        self.cache_dtype = cache_dtype
+        self.kv = [torch.zeros((self.num_pages, c.planes, c.num_kv_heads, page_size, c.head_dim), dtype=cache_dtype, device=dev)
                    for c in plan.caches]
+        self.kv_scales = [torch.zeros(t.shape[:4], dtype=torch.uint8, device=dev) for t in self.kv] if in_8_bits else []
         self.states = [torch.zeros((max_slots, *s.shape), dtype=s.dtype, device=dev) for s in plan.states]
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._ring = _HostRing()
@@ -127,10 +135,21 @@ class Engine:
         self.graph_kernel_launches = 0  # kernels of this package launched through graph replays
 
     @staticmethod
-    def tokens_that_fit(model: DecoderModel, page_size: int = 64, memory_fraction: float = 0.9) -> int:
+    def cache_type(model: DecoderModel, cache_dtype: torch.dtype | None) -> torch.dtype:
+        """The type that a model's keys and values are kept in; refuses one that its layers do not take."""
+        if cache_dtype is None or cache_dtype == model.runtime.dtype:
+            return model.runtime.dtype
+        if cache_dtype != K.FP8 or not model.takes_cache(cache_dtype):
+            raise EngineError(f"keys and values of this model cannot be kept in {cache_dtype} (activations in {model.runtime.dtype}): 8 bits "
+                              "(float8_e4m3fn) are for bfloat16 models whose layers are all paged attention with heads of 64 or 128")
+        return cache_dtype
+
+    @staticmethod
+    def tokens_that_fit(model: DecoderModel, page_size: int = 64, memory_fraction: float = 0.9, cache_dtype: torch.dtype | None = None) -> int:
         """Tokens of cache (whole pages) that fit into this fraction of the device memory now free."""
-        elem = 4 if model.runtime.dtype == torch.float32 else 2
-        per_token = sum(c.planes * c.num_kv_heads * c.head_dim * elem for c in model.plan.caches)
+        cache_dtype = Engine.cache_type(model, cache_dtype)
+        extra = 1 if cache_dtype == K.FP8 else 0  # a row's scale
+        per_token = sum(c.planes * c.num_kv_heads * (c.head_dim * cache_dtype.itemsize + extra) for c in model.plan.caches)
         if per_token == 0:
             raise EngineError("this model keeps no keys and values: give max_tokens")
         free, _ = torch.cuda.mem_get_info(model.runtime.device)
@@ -152,7 +171,7 @@ class Engine:
         return self.manager.committed(slot)
 
     def cache_bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in self.kv + self.states)
+        return sum(t.numel() * t.element_size() for t in self.kv + self.kv_scales + self.states)
 
     # ---------------------------------------------------------------------- step
     def reserve(self, entries: Sequence[StepEntry]) -> None:
@@ -263,13 +282,13 @@ class Engine:
                 torch.cuda.synchronize()
                 before = K.launch_count()
                 with torch.cuda.graph(g, pool=self._graph_pool, capture_error_mode="relaxed"):
-                    logits = self.model.forward(ctx, self.kv, self.states, block_tables)
+                    logits = self.model.forward(ctx, self.kv, self.states, block_tables, self.kv_scales)
                 graph["graph"], graph["logits"], graph["kernels"] = g, logits, K.launch_count() - before
                 g.replay()
                 self.graph_replays += 1
                 self.graph_kernel_launches += graph["kernels"]
             else:
-                logits = self.model.forward(ctx, self.kv, self.states, block_tables)
+                logits = self.model.forward(ctx, self.kv, self.states, block_tables, self.kv_scales)
             self.last_routing = ctx.scratch.get("record_routing", [])
             self.last_scratch = ctx.scratch
         for e, s, n in zip(entries, starts, n_tok):

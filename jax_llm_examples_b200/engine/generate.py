@@ -25,9 +25,9 @@ class Generator:
 
     def __init__(self, model: DecoderModel, *, max_tokens: int, page_size: int = 64, max_slots: int = 64,
                  max_tokens_per_step: int = 2048, max_live: int | None = None, max_seq_len: int | None = None,
-                 seed: int = 0, profile: "bool | str" = False):
+                 seed: int = 0, profile: "bool | str" = False, cache_dtype: torch.dtype | None = None):
         self.engine = Engine(model, max_tokens=max_tokens, page_size=page_size, max_slots=max_slots,
-                             max_seq_len=max_seq_len)
+                             max_seq_len=max_seq_len, cache_dtype=cache_dtype)
         self.sampler = Sampler(seed)
         self.scheduler = Scheduler(self.engine.manager, self._run, max_tokens_per_step=max_tokens_per_step,
                                    max_live=max_live, max_seq_len=self.engine.max_seq_len, on_admit=self._admit)
@@ -95,13 +95,14 @@ class Generator:
 
 
 def generate(model: DecoderModel, prompts: Sequence[Sequence[int]], params: SamplingParams | None = None, *,
-             page_size: int = 64, max_tokens: int | None = None, max_tokens_per_step: int = 2048, seed: int = 0) -> list[list[int]]:
-    """One call: builds a Generator sized for these prompts and runs them."""
+             page_size: int = 64, max_tokens: int | None = None, max_tokens_per_step: int = 2048, seed: int = 0,
+             cache_dtype: torch.dtype | None = None) -> list[list[int]]:
+    """One call: builds a Generator sized for these prompts and runs them (``cache_dtype``: see :class:`Engine`)."""
     params = params or SamplingParams()
     if max_tokens is None:
         max_tokens = sum(-(-(len(p) + params.max_new_tokens) // page_size) * page_size for p in prompts)
     gen = Generator(model, max_tokens=max_tokens, page_size=page_size, max_slots=max(len(prompts), 1),
-                    max_tokens_per_step=max_tokens_per_step, seed=seed)
+                    max_tokens_per_step=max_tokens_per_step, seed=seed, cache_dtype=cache_dtype)
     return gen.generate(prompts, params)
 
 

@@ -28,6 +28,7 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--seed", type=int, default=0, help="seed of random weights, random prompts and sampling")
     ap.add_argument("--write-model", metavar="DIR", help="with --preset: write the random model folder here and exit")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-dtype", choices=["float8_e4m3fn"], default=None, help="keep keys and values in 8 bits (default: in --dtype)")
     ap.add_argument("--prompt", action="append", default=[], help="text prompt (needs tokenizer.json in --model)")
     ap.add_argument("--prompt-ids", action="append", default=[], help='token ids, e.g. "1,2,3"')
     ap.add_argument("--random-prompts", type=int, default=0, help="number of random prompts")
@@ -45,6 +46,8 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--profile-kernels", action="store_true",
                     help="time every kernel launch with CUDA events and print the times by kernel and by op group")
     args = ap.parse_args(argv)
+
+    import torch
 
     import jax_llm_examples_b200 as J
 
@@ -84,7 +87,8 @@ def main(argv: list[str] | None = None) -> int:
     max_tokens = args.max_tokens or sum(-(-(len(p) + args.max_new_tokens) // ps) * ps for p in prompts)
     gen = J.Generator(model, max_tokens=max_tokens, page_size=ps, max_slots=max(len(prompts), 1),
                       max_tokens_per_step=args.max_tokens_per_step, max_live=args.max_live, seed=args.seed,
-                      profile="kernels" if args.profile_kernels else args.verbose)
+                      profile="kernels" if args.profile_kernels else args.verbose,
+                      cache_dtype=getattr(torch, args.cache_dtype) if args.cache_dtype else None)
     t0 = time.time()
     outputs = gen.generate(prompts, params)
     dt = time.time() - t0

@@ -10,6 +10,7 @@ from ..kernels import api as K
 from ..tracing import scope
 from .base import KVNeed, LayerCache, Mixer, PositionEncoding, ProjectedMixer, Rows, Runtime, StepContext, StepShape, register_part
 from .linear import linear
+from .positions import FusedEncoding
 
 # How this part's kernels cut a step's tokens (the planner below is theirs alone; nothing else knows these numbers).
 FLASH_TILE = 16  # query rows per block of the mma.sync flash kernel
@@ -101,6 +102,16 @@ class PagedAttention(Mixer):
     def sub_parts(self):
         return (self.position,)
 
+    kernel_libraries_cache8 = ("kv_fp8", "attention_few", "attention_rows", "attention_rows_tc")
+
+    def takes_cache(self, dtype: torch.dtype, runtime: Runtime) -> bool:
+        if dtype != K.FP8:
+            return super().takes_cache(dtype, runtime)
+        # in 8 bits: by a position encoding that writes them, for the kernels that read them (the subclasses write their pages
+        # themselves, and know no such form)
+        return type(self) is PagedAttention and isinstance(self.position, FusedEncoding) and \
+            K.attention_rows_supported(runtime.dtype, self.n_heads, self.n_kv_heads, self.head_dim)
+
     def step_planners(self):
         return (plan_attention_tiles,)
 
@@ -122,9 +133,29 @@ class PagedAttention(Mixer):
         attn_scale, floor_scale = self.position.query_temperature()
         out = torch.empty_like(q)
         with scope("attention"):
-            self.attend(ctx, q, cache, out, attn_scale, floor_scale)
+            if cache.scales is not None:
+                self._attend_cache8(ctx, q, cache, out, attn_scale, floor_scale)
+            else:
+                self.attend(ctx, q, cache, out, attn_scale, floor_scale)
         with scope("projection"):
             return linear(ctx, out.view(q.shape[0], -1), self.w_o, torch.float32, partials=True)
+
+    def _attend_cache8(self, ctx: StepContext, q, cache: LayerCache, out, attn_scale: float, floor_scale: float) -> None:
+        """Attention over pages in 8 bits: the step's single tokens, its long portions and its short ones."""
+        def call(**which):
+            K.attention_fp8(q, cache.pages, cache.scales, cache.block_table, ctx.req_of_token, ctx.positions, out, self.scale, self.chunk or 0,
+                            self.window or 0, attn_scale, floor_scale, ctx.status, ctx.max_kv_len, sink=self.sink, slopes=self.slopes,
+                            softcap=self.softcap, **which)
+
+        if ctx.max_q_len == 1:
+            call()
+            return
+        count = {name: len(ctx.host_arrays[name]) for name in ("attn_single_rows", "attn_tiles_long", "attn_tiles_short")}
+        for name, most in (("attn_tiles_long", TC_TILE), ("attn_tiles_short", FLASH_TILE)):
+            if count[name]:
+                call(items=ctx.arrays[name], n_items=count[name], max_count=most)
+        if count["attn_single_rows"]:
+            call(rows=ctx.arrays["attn_single_rows"], n_rows=count["attn_single_rows"])
 
     def _split_kv(self, ctx: StepContext, q, cache: LayerCache, out, attn_scale, floor_scale, rows, n_rows: int, diff=None) -> None:
         """Split-KV attention for requests that bring one token: all rows of q, or the listed ones."""

@@ -207,6 +207,7 @@ class LayerCache:
     writes: bool  # False: the layer reads a cache that another layer fills
     state: torch.Tensor | None  # [max_slots, *StateNeed.shape]; the first slab of a mixer that has several
     states: tuple = ()  # all slabs of the run, in the order of the mixer's ``state_needs()``
+    scales: torch.Tensor | None = None  # uint8 [num_pages, 2, Hkv, page_size]: the rows' scales of pages in 8 bits (float8_e4m3fn)
 
 
 @dataclasses.dataclass
@@ -386,6 +387,12 @@ class PositionEncoding(Part):
 
 class Mixer(Part):
     needs_f32_input: bool = False  # True: forward() gets the normed rows unrounded (``h32=``) and no rounded ones
+    # What else an engine has to load for a mixer whose keys and values are kept in 8 bits (:meth:`takes_cache`).
+    kernel_libraries_cache8: tuple[str, ...] = ()
+
+    def takes_cache(self, dtype: torch.dtype, runtime: Runtime) -> bool:
+        """Whether the mixer's keys and values may be kept in this type: the runtime's own, or others it knows."""
+        return dtype == runtime.dtype
 
     def kv_need(self) -> KVNeed | None:
         return None

@@ -134,6 +134,11 @@ class DecoderModel:
             libs.extend(p.required_libraries(self.runtime))
         return tuple(dict.fromkeys(libs))
 
+    def cache8_libraries(self) -> tuple[str, ...]:
+        """What the layers need besides when their keys and values are kept in 8 bits."""
+        mixers = [self.blocks[run.block].mixer for run in self.schedule if run.cache is not None]
+        return tuple(dict.fromkeys(n for m in mixers for n in m.kernel_libraries_cache8))
+
     def parts(self):
         """Every part of the model, parts inside parts included."""
         for top in (*self.blocks, self.final_norm):
@@ -168,9 +173,15 @@ class DecoderModel:
         walk([self.embedding, self.lm_head, self.final_norm, self.blocks])
         return total
 
+    def takes_cache(self, dtype: torch.dtype) -> bool:
+        """Whether every layer's keys and values may be kept in this type."""
+        mixers = [self.blocks[run.block].mixer for run in self.schedule if run.cache is not None]
+        return bool(mixers) and all(m.takes_cache(dtype, self.runtime) for m in mixers)
+
     def forward(self, ctx: StepContext, kv: list[torch.Tensor], states: list[torch.Tensor],
-                block_tables: list[torch.Tensor]) -> torch.Tensor:
-        """Runs the step's tokens through the schedule; returns float32 logits [M, V] at ctx.logit_rows."""
+                block_tables: list[torch.Tensor], kv_scales: "list[torch.Tensor] | None" = None) -> torch.Tensor:
+        """Runs the step's tokens through the schedule; returns float32 logits [M, V] at ctx.logit_rows.  ``kv_scales``: the
+        rows' scales of a cache in 8 bits, one tensor per entry of ``kv``."""
         rt = self.runtime
         for part in self._step_openers:
             part.begin_step(ctx)
@@ -189,7 +200,8 @@ class DecoderModel:
             if run.cache is None:
                 cache = LayerCache(None, None, False, first, slabs)
             else:
-                cache = LayerCache(kv[run.cache], block_tables[self.plan.group_of[run.cache]], run.writes, first, slabs)
+                cache = LayerCache(kv[run.cache], block_tables[self.plan.group_of[run.cache]], run.writes, first, slabs,
+                                   kv_scales[run.cache] if kv_scales else None)
             delta = self.blocks[run.block].forward(ctx, x, delta, cache)
         if ctx.n_logit_rows == 0:
             return torch.empty((0, self.vocab_size), dtype=torch.float32, device=rt.device)

@@ -48,7 +48,9 @@ def wavelength_scaled_frequencies(base: float, dims: int, factor: float, low: fl
     return out.to(torch.float32)
 
 
-class _FusedEncoding(PositionEncoding):
+class FusedEncoding(PositionEncoding):
+    """Rotation, norm and page write in one kernel, into pages of the activations' type or of 8 bits (``cache.scales``)."""
+
     kernel_libraries = ("rope_kv",)
     accepts_partials = True
     inv_freq: torch.Tensor | None = None
@@ -57,13 +59,17 @@ class _FusedEncoding(PositionEncoding):
         rows = as_rows(qkv)
         q = torch.empty((ctx.n_tokens, n_heads, head_dim), dtype=ctx.runtime.dtype, device=rows.data.device)
         l2 = qk_norm_eps is not None and self.norm_applies
+        if cache.writes and cache.scales is not None:
+            K.rope_kv_store_fp8(rows.data, q, cache.pages, cache.scales, cache.block_table, ctx.req_of_token, ctx.positions, self.inv_freq, l2,
+                                qk_norm_eps if l2 else 1.0, n_heads, n_kv_heads, head_dim, ctx.status, rows.splits)
+            return q
         K.rope_kv_store(rows.data, q, cache.pages if cache.writes else None, cache.block_table if cache.writes else None,
                         ctx.req_of_token, ctx.positions, self.inv_freq, l2, qk_norm_eps if l2 else 1.0, n_heads,
                         n_kv_heads, head_dim, ctx.status, rows.splits)
         return q
 
 
-class InterleavedRope(_FusedEncoding):
+class InterleavedRope(FusedEncoding):
     """Rotation of adjacent pairs (2j, 2j+1) by position * f_j (model.py:722-728); the weightless
     q/k norm, where the mixer has one, follows the rotation (model.py:915-917)."""
 
@@ -73,7 +79,7 @@ class InterleavedRope(_FusedEncoding):
         self.inv_freq = inv_freq.to(device=device, dtype=torch.float32).contiguous()
 
 
-class NoPositionWithTemperature(_FusedEncoding):
+class NoPositionWithTemperature(FusedEncoding):
     """No rotation and no q/k norm (model.py:913-917 skip both on these layers).  Queries are scaled by
     1 + attn_scale * ln(1 + floor((p + 1) / floor_scale)); attn_scale = 0 turns that off.  The scale is
     applied to the scores in float32 inside the attention kernel."""

@@ -111,3 +111,34 @@ def test_attention_tree_refuses(no_launch, change, match):
 def test_tensors_that_are_not_on_the_gpu_are_refused(no_launch):
     with pytest.raises(K.KernelError, match="not on the GPU"):
         K.kv_store_fp8(**_store_args())
+
+
+def test_an_engine_keeps_8_bits_only_where_every_layer_takes_them():
+    from types import SimpleNamespace
+
+    import jax_llm_examples_b200 as J
+    from jax_llm_examples_b200.engine.engine import EngineError
+    from jax_llm_examples_b200.parts.attention import GatedPagedAttention, PagedAttention
+    from jax_llm_examples_b200.parts.base import Runtime
+    from jax_llm_examples_b200.parts.positions import NoPositionWithTemperature, UnfusedEncoding
+
+    bf16, f32 = (Runtime(t, torch.device("cpu")) for t in (torch.bfloat16, torch.float32))
+
+    def mixer(dh, position, cls=PagedAttention):
+        return PagedAttention(torch.zeros(4 * dh, 64), torch.zeros(64, 2 * dh), 2, 1, dh, position) if cls is PagedAttention else \
+            GatedPagedAttention(torch.zeros(4 * dh, 64), torch.zeros(64, 2 * dh), 2, 1, dh, dh, 1.0, 1e-5, gate="none")
+
+    fused = NoPositionWithTemperature()
+    assert mixer(64, fused).takes_cache(K.FP8, bf16) and mixer(128, fused).takes_cache(K.FP8, bf16)
+    assert not mixer(32, fused).takes_cache(K.FP8, bf16) and not mixer(64, fused).takes_cache(K.FP8, f32)
+    assert not mixer(64, UnfusedEncoding()).takes_cache(K.FP8, bf16) and not mixer(64, None, GatedPagedAttention).takes_cache(K.FP8, bf16)
+    assert mixer(32, fused).takes_cache(torch.bfloat16, bf16) and not mixer(32, fused).takes_cache(torch.float16, bf16)
+    model = SimpleNamespace(runtime=bf16, takes_cache=lambda t: False)
+    assert J.Engine.cache_type(model, None) == J.Engine.cache_type(model, torch.bfloat16) == torch.bfloat16
+    for t in (K.FP8, torch.float16, torch.float32):
+        with pytest.raises(EngineError, match="cannot be kept"):
+            J.Engine.cache_type(model, t)
+    model.takes_cache = lambda t: True
+    assert J.Engine.cache_type(model, K.FP8) == K.FP8
+    with pytest.raises(EngineError, match="cannot be kept"):
+        J.Engine.cache_type(model, torch.float8_e5m2)
