@@ -107,9 +107,12 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
   const int tiles_y = gridDim.y / P.Hkv, hk = blockIdx.y / tiles_y, row0 = (blockIdx.y - hk * tiles_y) * ROWS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   RowsItem it;
-  if (!rows_item(P, item_i, it)) return;
+  if (!rows_tokens(P, item_i, it)) return;
   const int G = P.Hq / P.Hkv, n_rows = min(it.cnt * G - row0, ROWS);
   if (n_rows <= 0) return;
+  // every warp looks at the rows itself (at most 16): what they see together, and (warp 0) their description for all
+  const RowsToken tok = rows_token(P, it, row0 + min(lane, n_rows - 1), hk);
+  if (!rows_request(P, it)) return;
   const uint32_t bar0 = smem_u32(bars);
   auto FULL = [&](int s) { return bar0 + 8u * s; };
   auto EMPTY = [&](int s) { return bar0 + 8u * (STAGES + s); };
@@ -121,8 +124,6 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
     any_bad = failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // every warp looks at the rows itself (at most 16): what they see together, and (warp 0) their description for all
-  const RowsToken tok = rows_token(P, it, row0 + min(lane, n_rows - 1), hk);
   if (warp == 0 && lane < ROWS) {
     row_tok[lane] = make_int4(tok.n, tok.head, tok.p, tok.lo);
     row_sc[lane] = make_float2(tok.sc, tok.slope);

@@ -54,12 +54,17 @@ struct RowsItem {
   int n0, cnt, r, base, drafted;  // base: keys before the drafted tokens (causal: INT_MAX), drafted: their count
 };
 
-// The item's description; false: nothing to do (a description that points outside the step raises the status).
-__device__ __forceinline__ bool rows_item(const RowsParams& P, int i, RowsItem& it) {
+// The item's tokens, then its request; false: nothing to do (a description that points outside the step raises the status).
+// What a kernel needs of the tokens alone (positions, queries) it asks for in between: a block's way to its first tile is a
+// chain of dependent loads, of 700 cycles and more each.
+__device__ __forceinline__ bool rows_tokens(const RowsParams& P, int i, RowsItem& it) {
   it.n0 = P.items ? P.items[2 * i] : (P.rows ? P.rows[i] : i);
   it.cnt = P.items ? P.items[2 * i + 1] : 1;
   if (it.cnt <= 0) return false;
   if (it.n0 < 0 || it.n0 > P.N - it.cnt) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
+  return true;
+}
+__device__ __forceinline__ bool rows_request(const RowsParams& P, RowsItem& it) {
   it.r = P.req_of_token[it.n0];
   if (it.r < 0 || it.r >= P.n_requests) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
   it.base = P.cu_q ? P.q_start[it.r] : 0x7fffffff;
@@ -71,6 +76,7 @@ __device__ __forceinline__ bool rows_item(const RowsParams& P, int i, RowsItem& 
   }
   return true;
 }
+__device__ __forceinline__ bool rows_item(const RowsParams& P, int i, RowsItem& it) { return rows_tokens(P, i, it) && rows_request(P, it); }
 
 __device__ __forceinline__ int rows_first_key(const RowsParams& P, int p) {
   int s = 0;
@@ -89,7 +95,7 @@ __device__ __forceinline__ RowsToken rows_token(const RowsParams& P, const RowsI
   RowsToken k;
   k.n = it.n0 + t;
   k.head = hk * G + (row - t * G);
-  k.p = P.positions[k.n];
+  k.p = P.positions[k.n];  // (by itself: what comes first waits for nothing else)
   k.lo = rows_first_key(P, k.p);
   k.sc = P.scale_log2;
   if (P.attn_scale != 0.f) k.sc *= 1.f + P.attn_scale * log1pf(floorf(((float)k.p + 1.f) / P.floor_scale));

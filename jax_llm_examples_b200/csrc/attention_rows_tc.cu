@@ -198,9 +198,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   const int unit = blockIdx.x / P.splits, split = blockIdx.x - unit * P.splits, item_i = unit / (P.Hkv * row_tiles);
   const int hk = unit % (P.Hkv * row_tiles) / row_tiles, row0 = unit % row_tiles * BQ;
   RowsItem it;
-  if (!rows_item(P, item_i, it)) return;
+  if (!rows_tokens(P, item_i, it)) return;
   const int G = P.Hq / P.Hkv, n_rows = min(it.cnt * G - row0, BQ);
   if (n_rows <= 0) return;
+  // asked for now, needed after the request's description: the tokens' positions, and the queries (four neighbouring threads of
+  // the softmax warps bring a row's 128 entries into shared memory, 32 each)
+  const bool softmax = warp >= SOFTMAX0 && warp < SOFTMAX0 + 4 * PARTS;
+  const int q_row = (threadIdx.x - SOFTMAX0 * 32) >> 2, q_part = threadIdx.x & 3;
+  int p_mine = 0;
+  uint4 q_mine[4];
+  if (threadIdx.x < BQ) p_mine = P.positions[it.n0 + (row0 + min((int)threadIdx.x, n_rows - 1)) / G];
+  if (softmax) {
+    const int row = row0 + min(q_row, n_rows - 1), t = row / G, head = hk * G + row - t * G;
+    const uint4* src = reinterpret_cast<const uint4*>(P.q + ((size_t)(it.n0 + t) * P.Hq + head) * DH + q_part * 32);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) q_mine[u] = src[u];
+  }
+  if (!rows_request(P, it)) return;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < N_BARS; ++i) mbar_init(BAR(i), 1);  // a transaction count or a tcgen05.commit each, but:
@@ -219,9 +233,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   }
   __syncthreads();
   if (threadIdx.x < BQ) {
-    const RowsToken k = rows_token(P, it, row0 + min((int)threadIdx.x, n_rows - 1), hk);
-    const int a = __reduce_min_sync(0xffffffffu, k.lo), b = __reduce_max_sync(0xffffffffu, k.lo);
-    const int c = __reduce_min_sync(0xffffffffu, k.p), d = __reduce_max_sync(0xffffffffu, k.p);
+    const int lo = rows_first_key(P, p_mine);
+    const int a = __reduce_min_sync(0xffffffffu, lo), b = __reduce_max_sync(0xffffffffu, lo);
+    const int c = __reduce_min_sync(0xffffffffu, p_mine), d = __reduce_max_sync(0xffffffffu, p_mine);
     if (lane == 0) {
       atomicMin(&span[0], a);
       atomicMax(&span[1], b);
@@ -340,6 +354,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       auto issue_qk = [&](int t) {
         const int st = t & 1, sk = t % T::KS;
         if (ok) ok = mbar_wait(BAR(B_KFULL + sk), (t / T::KS) & 1);
+        if (F8 && ok) ok = mbar_wait(BAR(B_SCALES + t % SLOTS), (t / SLOTS) & 1);  // (whoever sees S complete may read the scales)
         if (!ok) return;
         tc_fence_after();
         const uint32_t q_s = smem_u32(q_p), k_s = smem_u32(k_p) + sk * T::K;
@@ -377,7 +392,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         failed = 1;
       }
     }
-  } else if (warp < SOFTMAX0 || warp >= SOFTMAX0 + 4 * PARTS) {
+  } else if (!softmax) {
     // ------------------------------------------------------------------------------ values as an operand
     const int i0 = threadIdx.x - (warp < SOFTMAX0 ? 64 : (SOFTMAX0 + 4 * PARTS - 2) * 32);  // the key of every tile
     bool ok = true;
@@ -471,13 +486,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   } else {
     // ------------------------------------------------------------------------------ queries, softmax, rescale, store
     {
-      // four neighbouring threads bring a row's 128 entries into shared memory, 32 each
-      const int i = (threadIdx.x - SOFTMAX0 * 32) >> 2, part = threadIdx.x & 3;
-      const int t = (row0 + min(i, n_rows - 1)) / G, head = hk * G + (row0 + min(i, n_rows - 1)) - t * G;
-      const uint4* src = reinterpret_cast<const uint4*>(P.q + ((size_t)(it.n0 + t) * P.Hq + head) * DH + part * 32);
-      uint4 x[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = src[u];
+      const int i = q_row, part = q_part;
+      const uint4 (&x)[4] = q_mine;
       if (F8) {
         float top = 0.f;
 #pragma unroll
@@ -538,7 +548,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     for (int t = 0; t < n_tiles && ok; ++t) {
       const int st = t & 1, place0 = range0 + t * BKV, place = place0 + col0;
       ok = mbar_wait(BAR(B_SFULL + st), (t >> 1) & 1);
-      if (F8 && ok) ok = mbar_wait(BAR(B_SCALES + t % SLOTS), (t / SLOTS) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();

@@ -284,6 +284,29 @@ def test_rows_of_very_different_scales(form):
 
 
 @pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("places", [[700], [130, 500, 890], [3], [905]])
+def test_scores_that_leap(form, bits8, places):
+    """Keys whose scores swamp all before them, tiles apart, and a value for each to tell them by."""
+    c = Case([30], [900], 8, 2, 128, 16, bits8=False).tree()
+    for i, place in enumerate(places):
+        page, at = int(c.table[0, place // 16]), place % 16
+        c.rows[page, 0, :, at] *= 64.0 * 4.0 ** i
+        c.rows[page, 1, :, at] = 96.0 + 32 * i  # (held exactly in either type)
+    if bits8:
+        c.rows, scales = hold(c.rows)
+        c.set_rows8(scales)
+        c.bits8 = True
+    else:
+        c.pages = c.rows.to(torch.bfloat16)
+    c.to_device()
+    out = _tree(c, {})
+    want, tol = c.want()
+    assert ((want > 95).all(-1) & (want < 161).all(-1)).any()
+    assert_close(out, want, tol)
+
+
+@pytest.mark.parametrize("form", FORMS, indirect=True)
 @pytest.mark.parametrize("n", [8, 100])
 def test_nan_rows_reach_those_that_see_them_and_no_other(form, n):
     c = Case([n], [50], 4, 2, 128, 16)
