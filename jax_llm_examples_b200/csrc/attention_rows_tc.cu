@@ -1,5 +1,5 @@
 // Grouped-query attention of many query rows of an item over the paged cache on the 5th-generation tensor cores (tcgen05), head
-// size 128: drafted trees and prompt portions, over a cache in bfloat16 or in 8 bits (attention_rows.cuh has mask and formula).
+// sizes 64 and 128: drafted trees and prompt portions, over a cache in bfloat16 or in 8 bits (attention_rows.cuh has mask and formula).
 //
 // A block takes 128 query rows of one item and KV head, (token, head of the group) pairs token by token, so that every key is
 // read once for 128 / G tokens' heads together, and one range of their keys in tiles of 128.  Per tile:
@@ -31,10 +31,9 @@
 #include "attention_rows.cuh"
 #include "mbarrier.cuh"
 
-#define DH 128
 #define BQ 128           // query rows per block
 #define BKV 128          // keys per tile
-#define PARTS 4          // softmax threads per query row: each takes BKV / PARTS of a tile's keys and DH / PARTS of O's columns
+#define PARTS 4          // softmax threads per query row: each takes BKV / PARTS of a tile's keys and an equal part of O's columns
 #define CP (BKV / PARTS)
 #define SOFTMAX0 4       // first softmax warp
 #define NTHREADS ((SOFTMAX0 + 4 * PARTS + 2) * 32)
@@ -96,6 +95,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -129,41 +135,48 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return d;
 }
 
-// Shared-memory matrix descriptors for tiles whose rows are 128 bytes with the 128-byte swizzle, 8-row groups 1024 bytes
-// apart.  K-major: a row runs along K.  MN-major: along the operand's N direction, rows are K steps; blocks of 64 numbers along
-// N are `lbo_bytes` apart.
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
-  return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory matrix descriptors for tiles whose rows are 128 (or 64) bytes with the swizzle of that many, 8-row groups side
+// by side.  K-major: a row runs along K.  MN-major: along the operand's N direction, rows are K steps; blocks of 64 numbers
+// along N are `lbo_bytes` apart.
+template <int ROW> __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(8 * ROW >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)(ROW == 128 ? 2 : 4) << 61);
 }
 __device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t lbo_bytes) {
   return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(lbo_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// Instruction descriptors: float32 accumulator, M = 128, N = 128; operand formats a, b (kind::f16: 0 float16, 1 bfloat16;
+// Instruction descriptors: float32 accumulator, M = 128, N = n; operand formats a, b (kind::f16: 0 float16, 1 bfloat16;
 // kind::f8f6f4: 0 e4m3, 1 e5m2); A K-major, B K- or MN-major.
-__host__ __device__ constexpr uint32_t make_idesc(uint32_t a, uint32_t b, uint32_t b_mn_major) {
-  return (1u << 4) | (a << 7) | (b << 10) | (b_mn_major << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+__host__ __device__ constexpr uint32_t make_idesc(uint32_t a, uint32_t b, uint32_t b_mn_major, uint32_t n) {
+  return (1u << 4) | (a << 7) | (b << 10) | (b_mn_major << 16) | ((n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-// Byte offset of 16-byte chunk c (of 8) of row r in a swizzled tile of 128-byte rows.
-__device__ __forceinline__ uint32_t swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+// Byte offset of 16-byte chunk c of row r in a swizzled tile of rows of ROW bytes.
+template <int ROW> __device__ __forceinline__ uint32_t swizzled(int r, int c) {
+  return ROW == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
 
 #define HALF_BYTES (128 * 128)  // 128 rows of 128 bytes
-template <bool F8> struct TcTile {
-  static constexpr int Q = 2 * HALF_BYTES;                   // bfloat16: entries 0-63, 64-127; 8 bits: first parts, what is left
-  static constexpr int K = F8 ? HALF_BYTES : 2 * HALF_BYTES;  // a tile of keys
+template <int DH, bool F8> struct TcTile {
+  static constexpr int ROW = F8 ? DH : 128;                  // bytes of a row of queries or keys as the score product sees it
+  static constexpr int HALVES = F8 ? 1 : DH / 64;            // bfloat16: entries 0-63, 64-127 lie in tiles of their own
+  static constexpr int PART = 128 * ROW;                     // such a tile
+  static constexpr int Q = F8 ? 2 * PART : HALVES * PART;    // 8 bits: first parts, what is left
+  static constexpr int K = HALVES * PART;                    // a tile of keys
   static constexpr int KS = F8 ? 4 : 3;                      // tiles of keys in flight
-  static constexpr int V = 2 * HALF_BYTES;                   // a tile of values as an operand, two of them
-  static constexpr int RAW = F8 ? HALF_BYTES : 0;            // a tile of values' codes, two of them
+  static constexpr int V = DH / 64 * HALF_BYTES;             // a tile of values as an operand, two of them
+  static constexpr int RAW = F8 ? PART : 0;                  // a tile of values' codes, two of them
   static constexpr int BYTES = F8 ? 2 * BKV : 0;             // the scale bytes of a tile's keys and values, two of them
   static constexpr int SCALES = F8 ? SLOTS * BKV * 2 : 0;    // [SLOTS] the keys' scales as bfloat16
   static constexpr int SMEM = Q + KS * K + 2 * V + 2 * RAW + 2 * BYTES + SCALES + 1024;
+  static constexpr int STEPS = F8 ? 2 * DH / 32 : DH / 16;   // score products of a tile
+  static constexpr int OC = DH / PARTS;                      // O's columns of a softmax thread
 };
 
-template <bool F8>
+template <int DH, bool F8>
 __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __grid_constant__ CUtensorMap map, const RowsParams P, int box_rows, int row_tiles) {
   JLX_TL(TL_ATTN_PREFILL);
-  using T = TcTile<F8>;
+  using T = TcTile<DH, F8>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *q_p = smem, *k_p = q_p + T::Q, *v_p = k_p + T::KS * T::K, *raw_p = v_p + 2 * T::V;
@@ -202,17 +215,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   const int G = P.Hq / P.Hkv, n_rows = min(it.cnt * G - row0, BQ);
   if (n_rows <= 0) return;
   // asked for now, needed after the request's description: the tokens' positions, and the queries (four neighbouring threads of
-  // the softmax warps bring a row's 128 entries into shared memory, 32 each)
+  // the softmax warps bring a row into shared memory)
   const bool softmax = warp >= SOFTMAX0 && warp < SOFTMAX0 + 4 * PARTS;
   const int q_row = (threadIdx.x - SOFTMAX0 * 32) >> 2, q_part = threadIdx.x & 3;
   int p_mine = 0;
-  uint4 q_mine[4];
+  uint4 q_mine[DH / 32];
   if (threadIdx.x < BQ) p_mine = P.positions[it.n0 + (row0 + min((int)threadIdx.x, n_rows - 1)) / G];
   if (softmax) {
     const int row = row0 + min(q_row, n_rows - 1), t = row / G, head = hk * G + row - t * G;
-    const uint4* src = reinterpret_cast<const uint4*>(P.q + ((size_t)(it.n0 + t) * P.Hq + head) * DH + q_part * 32);
+    const uint4* src = reinterpret_cast<const uint4*>(P.q + ((size_t)(it.n0 + t) * P.Hq + head) * DH + q_part * (DH / 4));
 #pragma unroll
-    for (int u = 0; u < 4; ++u) q_mine[u] = src[u];
+    for (int u = 0; u < DH / 32; ++u) q_mine[u] = src[u];
   }
   if (!rows_request(P, it)) return;
 
@@ -284,7 +297,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             tma_prefetch_2d(&map, 0, row + w * v_off);
-            if (!F8) tma_prefetch_2d(&map, 64, row + w * v_off);
+            if (T::HALVES == 2) tma_prefetch_2d(&map, 64, row + w * v_off);
           }
         }
       }
@@ -297,9 +310,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       __syncwarp();
       if (lane < boxes) {
         const int row = box_row[t % ROW_RING][lane];
-        const uint32_t dst = smem_u32(which ? (F8 ? raw_p + st * T::RAW : v_p + st * T::V) : k_p + st * T::K) + lane * box_rows * 128;
+        const uint32_t dst = smem_u32(which ? (F8 ? raw_p + st * T::RAW : v_p + st * T::V) : k_p + st * T::K) + lane * box_rows * T::ROW;
         tma_load_2d(dst, &map, 0, row + which * v_off, bar);
-        if (!F8) tma_load_2d(dst + HALF_BYTES, &map, 64, row + which * v_off, bar);
+        if (T::HALVES == 2) tma_load_2d(dst + HALF_BYTES, &map, 64, row + which * v_off, bar);
         if (F8 && which) {
           const uint32_t sc = smem_u32(bytes_p + st * T::BYTES) + lane * box_rows;
           bulk_load(sc, P.scales + row, box_rows, bar);
@@ -359,13 +372,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         tc_fence_after();
         const uint32_t q_s = smem_u32(q_p), k_s = smem_u32(k_p) + sk * T::K;
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          if (F8) {  // first parts, then what is left: four steps of 32 entries each
-            const uint32_t off = (kk & 3) * 32;
-            umma_f8(tmem + st * 128, desc_k_major(q_s + (kk >> 2) * HALF_BYTES + off), desc_k_major(k_s + off), make_idesc(kk >> 2, 0, 0), kk != 0);
+        for (int kk = 0; kk < T::STEPS; ++kk) {
+          if (F8) {  // first parts, then what is left: steps of 32 entries
+            const int part = kk / (DH / 32);
+            const uint32_t off = kk % (DH / 32) * 32;
+            umma_f8(tmem + st * 128, desc_k_major<T::ROW>(q_s + part * T::PART + off), desc_k_major<T::ROW>(k_s + off), make_idesc(part, 0, 0, BKV), kk != 0);
           } else {   // steps of 16 entries
             const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
-            umma_f16(tmem + st * 128, desc_k_major(q_s + off), desc_k_major(k_s + off), make_idesc(1, 1, 0), kk != 0);
+            umma_f16(tmem + st * 128, desc_k_major<T::ROW>(q_s + off), desc_k_major<T::ROW>(k_s + off), make_idesc(1, 1, 0, BKV), kk != 0);
           }
         }
         umma_commit(BAR(B_SFULL + st));
@@ -383,7 +397,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         const uint32_t v_s = smem_u32(v_p) + st * T::V;
 #pragma unroll
         for (int kk = 0; kk < BKV / 16; ++kk)  // P: 16 keys = 8 columns of tensor memory; V: 16 keys = 16 rows of 128 bytes
-          umma_f16_a_tmem(tm_o, tmem + st * 128 + kk * 8, desc_mn_major(v_s + kk * 16 * 128, HALF_BYTES), make_idesc(1, 1, 1), (t | kk) != 0);
+          umma_f16_a_tmem(tm_o, tmem + st * 128 + kk * 8, desc_mn_major(v_s + kk * 16 * 128, HALF_BYTES), make_idesc(1, 1, 1, DH), (t | kk) != 0);
         umma_commit(BAR(B_VEMPTY + st));
         umma_commit(BAR(B_ODONE));
       }
@@ -433,8 +447,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
           return *reinterpret_cast<const uint32_t*>(&z);
         };
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint4 x = *reinterpret_cast<const uint4*>(raw + swizzled(i0, c));
+        for (int c = 0; c < DH / 16; ++c) {
+          const uint4 x = *reinterpret_cast<const uint4*>(raw + swizzled<T::ROW>(i0, c));
           const uint32_t w[4] = {x.x & keep, x.y & keep, x.z & keep, x.w & keep};
           uint32_t o[8];
 #pragma unroll
@@ -451,17 +465,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
             for (int u = 0; u < 8; ++u) o[u] = all;
           }
           uint8_t* half = v + (c >> 2) * HALF_BYTES;
-          *reinterpret_cast<uint4*>(half + swizzled(i0, (c & 3) * 2)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(half + swizzled(i0, (c & 3) * 2 + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(half + swizzled<128>(i0, (c & 3) * 2)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(half + swizzled<128>(i0, (c & 3) * 2 + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
         fence_async_proxy();
         mbar_arrive(BAR(B_RAWEMPTY + st));
       } else if (masked_tile(place0)) {
         bool bad = false;
 #pragma unroll 1
-        for (int x = i0; x < 2 * BKV * 8; x += AUX) {  // (consecutive threads: chunks of a row)
+        for (int x = i0; x < DH / 64 * BKV * 8; x += AUX) {  // (consecutive threads: chunks of a row)
           const int i = (x >> 3) & (BKV - 1);
-          uint4* at = reinterpret_cast<uint4*>(v + (x >> 10) * HALF_BYTES + swizzled(i, x & 7));
+          uint4* at = reinterpret_cast<uint4*>(v + (x >> 10) * HALF_BYTES + swizzled<128>(i, x & 7));
           uint32_t w[4] = {at->x, at->y, at->z, at->w};
           bool here = false;
 #pragma unroll
@@ -487,11 +501,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     // ------------------------------------------------------------------------------ queries, softmax, rescale, store
     {
       const int i = q_row, part = q_part;
-      const uint4 (&x)[4] = q_mine;
+      const uint4 (&x)[DH / 32] = q_mine;
       if (F8) {
         float top = 0.f;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < DH / 32; ++u) {
           const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x[u]);
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
@@ -505,7 +519,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         const float in = fp8_pow2(-e);
         if (part == 0) q_exp[i] = top == INFINITY ? __int_as_float(0x7fc00000) : fp8_pow2(e);  // (no codes for an infinite entry: the scores are NaN)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {  // 16 entries: a chunk of each part
+        for (int u = 0; u < DH / 64; ++u) {  // 16 entries: a chunk of each part
           uint32_t hi[4], left[4];
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -519,12 +533,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
             left[w] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a - g0.x, b - g0.y), __NV_SATFINITE, __NV_E5M2) |
                       (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c - g1.x, d - g1.y), __NV_SATFINITE, __NV_E5M2) << 16;
           }
-          *reinterpret_cast<uint4*>(q_p + swizzled(i, part * 2 + u)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(q_p + HALF_BYTES + swizzled(i, part * 2 + u)) = make_uint4(left[0], left[1], left[2], left[3]);
+          *reinterpret_cast<uint4*>(q_p + swizzled<T::ROW>(i, part * (DH / 64) + u)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(q_p + T::PART + swizzled<T::ROW>(i, part * (DH / 64) + u)) = make_uint4(left[0], left[1], left[2], left[3]);
         }
       } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4*>(q_p + (part >> 1) * HALF_BYTES + swizzled(i, (part & 1) * 4 + u)) = x[u];
+        for (int u = 0; u < DH / 32; ++u) {
+          const int c = part * (DH / 32) + u;
+          *reinterpret_cast<uint4*>(q_p + (c >> 3) * HALF_BYTES + swizzled<128>(i, c & 7)) = x[u];
+        }
       }
       fence_async_proxy();
       mbar_arrive(BAR(B_QREADY));
@@ -655,12 +672,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         if (!ok) break;
         if (!__all_sync(0xffffffffu, corr == 1.f)) {
           tc_fence_after();
-          uint32_t o[32];
-          tmem_ld32(tm_o + lane_addr + part * 32, o);
+          uint32_t o[T::OC];
+          if (T::OC == 32) tmem_ld32(tm_o + lane_addr + part * T::OC, o);
+          else tmem_ld16(tm_o + lane_addr + part * T::OC, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
-          tmem_st32(tm_o + lane_addr + part * 32, o);
+          for (int c = 0; c < T::OC; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+          if (T::OC == 32) tmem_st32(tm_o + lane_addr + part * T::OC, o);
+          else tmem_st16(tm_o + lane_addr + part * T::OC, o);
         }
       }
       tmem_st_wait();
@@ -683,13 +702,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       float total = 0.f;
 #pragma unroll
       for (int q = 0; q < PARTS; ++q) total += xmax[mp][q][row];
-      uint32_t o[32];
+      uint32_t o[T::OC];
       if (n_tiles > 0) {
-        tmem_ld32(tm_o + lane_addr + part * 32, o);
+        if (T::OC == 32) tmem_ld32(tm_o + lane_addr + part * T::OC, o);
+        else tmem_ld16(tm_o + lane_addr + part * T::OC, o);
         tmem_ld_wait();
       } else {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = 0u;
+        for (int c = 0; c < T::OC; ++c) o[c] = 0u;
       }
       if (*(volatile int*)&any_bad && row < n_rows) {  // the values that were taken out, for the rows that see them
         for (int place = begin; place < end; ++place) {
@@ -698,9 +718,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
           const int row_c = rows_cache_row(P, table, hk, place);
           if (row_c < 0) continue;
           if (F8 && P.scales[row_c + v_off] != FP8_BAD) continue;
-          const bf16* vp = reinterpret_cast<const bf16*>(P.pages) + (size_t)(row_c + v_off) * DH + part * 32;
+          const bf16* vp = reinterpret_cast<const bf16*>(P.pages) + (size_t)(row_c + v_off) * DH + part * T::OC;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
+          for (int c = 0; c < T::OC; ++c) {
             const float y = F8 ? __int_as_float(0x7fc00000) : __bfloat162float(vp[c]);
             if (!isfinite(y)) o[c] = __float_as_uint(__uint_as_float(o[c]) + y);
           }
@@ -709,16 +729,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       if (row < n_rows) {
         const size_t at = (size_t)tok.n * P.Hq + tok.head;
         if (P.splits > 1) {
-          float4* dst = reinterpret_cast<float4*>(P.part_o + (at * P.splits + split) * DH + part * 32);
+          float4* dst = reinterpret_cast<float4*>(P.part_o + (at * P.splits + split) * DH + part * T::OC);
 #pragma unroll
-          for (int c = 0; c < 32; c += 4)
+          for (int c = 0; c < T::OC; c += 4)
             dst[c >> 2] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
           if (part == 0) P.part_ml[at * P.splits + split] = make_float2(m, total);
         } else {
           const float inv = rows_inverse(P, m, total, tok.head);
-          uint4* dst = reinterpret_cast<uint4*>(P.out + at * DH + part * 32);
+          uint4* dst = reinterpret_cast<uint4*>(P.out + at * DH + part * T::OC);
 #pragma unroll
-          for (int c = 0; c < 32; c += 8) {
+          for (int c = 0; c < T::OC; c += 8) {
             uint4 x;
             __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&x);
 #pragma unroll
@@ -743,31 +763,33 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
 }
 
 // -------------------------------------------------------------------------------------------- host
-template <bool F8>
+template <int DH, bool F8>
 static int launch_tc(const RowsParams& P, int box_rows, int row_tiles, cudaStream_t stream) {
   static unsigned long long allowed = 0;  // a bit per device: the attribute belongs to the device's context
   int dev = 0;
   JLX_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !(allowed >> dev & 1)) {
-    JLX_CUDA(cudaFuncSetAttribute(attention_rows_tc_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcTile<F8>::SMEM));
+    JLX_CUDA(cudaFuncSetAttribute(attention_rows_tc_kernel<DH, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcTile<DH, F8>::SMEM));
     if (dev < 64) allowed |= 1ull << dev;
   }
   CUtensorMap map;
   if (int rc = rows_map(P, DH, F8, box_rows, &map)) return rc;
   const long long blocks = (long long)P.n_items * P.splits * P.Hkv * row_tiles;
   JLX_REQUIRE(blocks < (1ll << 31), "attention over rows: too many items or rows");
-  JLX_CUDA(jlx_launch_pdl(attention_rows_tc_kernel<F8>, dim3((unsigned)blocks), dim3(NTHREADS), TcTile<F8>::SMEM, stream, map, P, box_rows, row_tiles));
+  JLX_CUDA(jlx_launch_pdl(attention_rows_tc_kernel<DH, F8>, dim3((unsigned)blocks), dim3(NTHREADS), TcTile<DH, F8>::SMEM, stream, map, P, box_rows, row_tiles));
   return 0;
 }
 
 JLX_API int jlx_attention_rows_tc(const RowsArgs* a, cudaStream_t stream) {
   RowsParams P;
   if (rows_params(*a, P)) return 1;
-  JLX_REQUIRE(a->dh == DH && a->page_size % 16 == 0 && ((uintptr_t)a->scales & 15) == 0, "attention over rows (tcgen05): needs head size 128, pages of a multiple of 16 tokens and scales on a 16-byte boundary");
+  JLX_REQUIRE(a->page_size % 16 == 0 && ((uintptr_t)a->scales & 15) == 0, "attention over rows (tcgen05): needs pages of a multiple of 16 tokens and scales on a 16-byte boundary");
   if (P.n_items == 0) return 0;
   const int rows = a->max_count * (P.Hq / P.Hkv), box_rows = P.page_size % 64 == 0 ? 64 : P.page_size % 32 == 0 ? 32 : 16;
   JLX_REQUIRE(P.splits == 1 || (P.part_o && P.part_ml), "attention over rows: scratch for the ranges is missing");
   const int row_tiles = (rows + BQ - 1) / BQ;
-  if (int rc = P.scales ? launch_tc<true>(P, box_rows, row_tiles, stream) : launch_tc<false>(P, box_rows, row_tiles, stream)) return rc;
-  return P.splits > 1 ? launch_rows_join<DH>(P, a->max_count, stream) : 0;
+  const int rc = a->dh == 128 ? (P.scales ? launch_tc<128, true>(P, box_rows, row_tiles, stream) : launch_tc<128, false>(P, box_rows, row_tiles, stream))
+                              : (P.scales ? launch_tc<64, true>(P, box_rows, row_tiles, stream) : launch_tc<64, false>(P, box_rows, row_tiles, stream));
+  if (rc || P.splits == 1) return rc;
+  return a->dh == 128 ? launch_rows_join<128>(P, a->max_count, stream) : launch_rows_join<64>(P, a->max_count, stream);
 }

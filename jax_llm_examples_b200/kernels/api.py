@@ -1227,11 +1227,11 @@ def attention_rows_supported(q_dtype: torch.dtype, Hq: int, Hkv: int, dh: int) -
     return q_dtype == torch.bfloat16 and dh in (64, 128) and Hkv > 0 and Hq % Hkv == 0
 
 
-def attention_rows_form(rows: int, dh: int, page_size: int, aligned: bool) -> str:
+def attention_rows_form(rows: int, page_size: int, aligned: bool) -> str:
     """The kernel for items of up to so many query rows of a KV head ((token, head of the group) pairs)."""
     if rows <= ROWS_FEW:
         return "attention_few"
-    return "attention_rows_tc" if dh == 128 and page_size % 16 == 0 and aligned else "attention_rows"
+    return "attention_rows_tc" if page_size % 16 == 0 and aligned else "attention_rows"
 
 
 @functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
@@ -1292,7 +1292,7 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
         raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
     scales_p = _address(scales)
-    form = attention_rows_form(max_count * (Hq // Hkv), dh, page_size, scales_p % 16 == 0)
+    form = attention_rows_form(max_count * (Hq // Hkv), page_size, scales_p % 16 == 0)
     splits = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
     part_o = part_ml = joined = 0
     if splits > (ROWS_CLUSTER if form == "attention_few" else 1):

@@ -96,7 +96,7 @@ class Case:
         """To be called for the items that a kernel gets: the tcgen05 form rounds its weights to bfloat16 over either cache."""
         from jax_llm_examples_b200.kernels import api as K
 
-        form = K.attention_rows_form(max_count * (self.Hq // self.Hkv), self.dh, self.page, True)
+        form = K.attention_rows_form(max_count * (self.Hq // self.Hkv), self.page, True)
         self.weights = 2.0 ** -11 if self.bits8 and form != "attention_rows_tc" else 2.0 ** -8
 
     def items(self, cut, which=lambda n: True):
