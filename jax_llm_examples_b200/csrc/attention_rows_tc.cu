@@ -594,10 +594,19 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       }
       if (__builtin_expect(special, 0)) {
         if (capped) {
+          // the polynomial where no score of the warp lies outside its range (a NaN does: it keeps to the general form)
+          float far = 0.f;
 #pragma unroll
-          for (int c = 0; c < CP; ++c) {
-            const float x = __uint_as_float(v[c]);
-            v[c] = __float_as_uint(x == x ? P.cap_log2 * cap_tanh(x) : x);
+          for (int c = 0; c < CP; ++c) far = __uint_as_float(v[c]) == __uint_as_float(v[c]) ? fmaxf(far, fabsf(__uint_as_float(v[c]))) : INFINITY;
+          if (!__any_sync(0xffffffffu, far > 1.f)) {
+#pragma unroll
+            for (int c = 0; c < CP; ++c) v[c] = __float_as_uint(P.cap_log2 * cap_tanh_small(__uint_as_float(v[c])));
+          } else {
+#pragma unroll
+            for (int c = 0; c < CP; ++c) {
+              const float x = __uint_as_float(v[c]);
+              v[c] = __float_as_uint(x == x ? P.cap_log2 * cap_tanh(x) : x);
+            }
           }
         }
         // which of the 32 keys the row's token sees: those at cached places from lo on (up to its own, or before the tree) ...
