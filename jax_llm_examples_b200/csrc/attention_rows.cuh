@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowsPara
 // What the callers hand over (_RowsArgs in kernels/api.py).
 struct RowsArgs {
   const void *q, *pages, *scales, *block_table, *req_of_token, *positions, *out, *items, *rows, *cu_q, *q_start, *masks, *sink, *slopes, *part_o, *part_ml, *status;
-  int bt_stride, n_requests, n_items, max_count, words, N, Hq, Hkv, dh, page_size, num_pages, chunk, window, splits;
+  int bt_stride, n_requests, n_items, max_count, words, N, Hq, Hkv, dh, page_size, num_pages, chunk, window, splits, row_block;
   float scale, softcap, attn_scale, floor_scale;
 };
 

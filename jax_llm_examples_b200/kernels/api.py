@@ -1215,7 +1215,7 @@ def kv_load_fp8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Te
     _run("kv_fp8", "jlx_kv_load_fp8", args, c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
 
 
-_ROWS_ARGS = struct.Struct("@17P14i4f")  # RowsArgs in csrc/attention_rows.cuh
+_ROWS_ARGS = struct.Struct("@17P15i4f")  # RowsArgs in csrc/attention_rows.cuh
 ROWS_TILE = 64  # keys of a tile, csrc/attention_rows.cu and attention_few.cu
 ROWS_FEW = 16  # query rows of an item and KV head that attention_few.cu takes
 ROWS_CLUSTER = 8  # ranges that it joins without scratch
@@ -1235,8 +1235,8 @@ def attention_rows_form(rows: int, page_size: int, aligned: bool) -> str:
 
 
 @functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
-def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int) -> int:
-    """Ranges that an item's keys are cut into (equal ones, of the item's own keys)."""
+def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int) -> "tuple[int, int]":
+    """(Ranges that an item's keys are cut into: equal ones, of the item's own keys; query rows of a block of ``attention_rows_tc``.)"""
     seen = min(max_kv_len, window + max_count if window else max_kv_len, chunk + max_count if chunk else max_kv_len) + ROWS_TILE  # ranges start at a tile's first key
     rows = max_count * (Hq // Hkv)
     if form == "attention_few":
@@ -1246,7 +1246,7 @@ def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_i
         # one of 8,000: 90 with 1, 18.5 with 8, 16.7 with 24, 23.7 with 55.)
         blocks, places, tiles, block, join, share = n_items * Hkv, 3 * sms, -(-seen // ROWS_TILE), 10, 6, 8
     elif form == "attention_rows_tc":
-        blocks, places, tiles, block, join, share = n_items * Hkv * -(-rows // 128), sms, -(-seen // 128), 4, 3, 4
+        return _rows_tc_plan(-(-seen // 128), n_items * Hkv, rows, sms)
     else:
         blocks, places, tiles, block, join, share = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64)), 2 * sms, -(-seen // ROWS_TILE), 4, 3, 8
     splits, least = 1, 1 << 60
@@ -1255,7 +1255,34 @@ def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_i
         cost = -(-blocks * s // places) * (-(-tiles // s) + block) + (join + s // share if joined else 0)
         if s <= tiles and cost < least:
             splits, least = s, cost
-    return splits
+    return splits, 0
+
+
+def _rows_tc_plan(tiles: int, units: int, rows: int, sms: int) -> "tuple[int, int]":
+    """(Ranges, rows of a block: 128 or 256) for `units` (item, KV head) pairs of `rows` query rows over `tiles` tiles of keys: the
+    pair with the least time, in tiles of 128 rows.  A tile of 256 rows takes 1.9; a block takes 4 besides its tiles, a join 4 and
+    one for 4 ranges.  A multiprocessor holds one block: up to two rounds of them take as long as their longest, more of them as
+    long as all their work (and then tiles of 128 rows take 1.1: they fetch every key twice as often).
+    (1 request, 64 rows a KV head and 8,000 keys: 37 us with 6 ranges of 128 rows, 48 with 8 of 256; 2,048 tokens after 1,500, five
+    heads on a KV head: 207 us with 256 rows, 230 with 128; with 2 ranges 268 and 300.)"""
+    splits, row_block, least = 1, 128, 1e30
+    for b in (128, 256):
+        if b - 128 >= rows:
+            continue
+        full, rest = divmod(rows, b)
+        for s in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48):
+            if s > tiles:
+                break
+            blocks, range_ = units * s * (full + (rest > 0)), -(-tiles // s)
+            if blocks <= 2 * sms:
+                cost = -(-blocks // sms) * (range_ * (1.9 if b == 256 else 1.0) + 4)
+            else:
+                whole, part = range_ * (1.9 if b == 256 else 1.1) + 4, range_ * (1.9 if rest > 128 else 1.1) + 4
+                cost = units * s * (full * whole + (rest > 0) * part) / sms + whole / 2
+            cost += 4 + s // 4 if s > 1 else 0
+            if cost < least:
+                splits, row_block, least = s, b, cost
+    return splits, row_block
 
 
 def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, positions, out, scale, chunk, window, attn_scale, floor_scale, status,
@@ -1293,7 +1320,7 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
         raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
     scales_p = _address(scales)
     form = attention_rows_form(max_count * (Hq // Hkv), page_size, scales_p % 16 == 0)
-    splits = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
+    splits, row_block = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
     part_o = part_ml = joined = 0
     if splits > (ROWS_CLUSTER if form == "attention_few" else 1):
         # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
@@ -1303,7 +1330,7 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     args = _ROWS_ARGS.pack(q_p, pages.data_ptr(), scales_p, block_table.data_ptr(), req_of_token.data_ptr(), positions.data_ptr(), out_p,
                            _address(items), _address(rows), _address(cu_q), _address(q_start), _address(masks), _address(sink), _address(slopes),
                            part_o, part_ml, status.data_ptr(), width, R, n_items, max_count, words, N, Hq, Hkv, dh, page_size, P, chunk, window, splits,
-                           scale, softcap, attn_scale, floor_scale)
+                           row_block, scale, softcap, attn_scale, floor_scale)
     _run(form, _ROWS_LAUNCHERS[form], args, _raw_stream(dev))
     global _launches
     _launches += joined  # the joining kernel
