@@ -170,7 +170,7 @@ template <int DH, bool F8> struct TcTile {
   static constexpr int V = DH / 64 * HALF_BYTES;             // a tile of values as an operand, two of them
   static constexpr int VS = F8 && DH == 64 ? 3 : 2;          // tiles of values in flight (8 bits: of their codes)
   static constexpr int RAW = F8 ? PART : 0;                  // a tile of values' codes
-  static constexpr int SCALES = F8 ? SLOTS * BKV * 3 : 0;    // [SLOTS] the keys' scales as bfloat16; [SLOTS] the values' bytes
+  static constexpr int SCALES = F8 ? SLOTS * BKV * 5 : 0;    // [SLOTS] the keys' scales; [SLOTS] the values' bytes
   static constexpr int SMEM = 2 * Q + KS * K + 2 * V + VS * RAW + SCALES + 1024;
   static constexpr int STEPS = F8 ? 2 * DH / 32 : DH / 16;   // score products of a tile
   static constexpr int OC = DH / PARTS;                      // columns of its group's O that a softmax thread rescales
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *q_p = smem, *k_p = q_p + 2 * T::Q, *v_p = k_p + T::KS * T::K, *raw_p = v_p + 2 * T::V;
-  uint16_t* scales_p = reinterpret_cast<uint16_t*>(raw_p + T::VS * T::RAW);
+  float* scales_p = reinterpret_cast<float*>(raw_p + T::VS * T::RAW);
   uint8_t* bytes_p = reinterpret_cast<uint8_t*>(scales_p + SLOTS * BKV);
   // barriers (each use flips a phase bit; t = a tile's number)
   enum { B_QREADY = 0,    // Q is in shared memory
@@ -409,13 +409,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       if (t + 1 < n_tiles) fetch(t + 1, page, k_next, v_next);
       if (t >= SLOTS) ok = __all_sync(0xffffffffu, mbar_wait(BAR(B_SCFREE + t % SLOTS), (t / SLOTS - 1) & 1));
       if (!ok) break;
-      uint32_t w[2];
+      uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t a = (k >> (16 * i)) & 0xff, b = (k >> (16 * i + 8)) & 0xff;
-        w[i] = (a == FP8_BAD ? 0x7fc0u : a << 7) | (b == FP8_BAD ? 0x7fc0u : b << 7) << 16;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = (k >> (8 * i)) & 0xff;
+        w[i] = a == FP8_BAD ? 0x7fc00000u : a << 23;
       }
-      *reinterpret_cast<uint2*>(scales_p + (t % SLOTS) * BKV + lane * 4) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint4*>(scales_p + (t % SLOTS) * BKV + lane * 4) = make_uint4(w[0], w[1], w[2], w[3]);
       *reinterpret_cast<uint32_t*>(bytes_p + (t % SLOTS) * BKV + lane * 4) = v;
       mbar_arrive(BAR(B_SCALES + t % SLOTS));
       k = k_next;
@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             float x = __uint_as_float(v[c]) * in;
-            if (F8) x *= __uint_as_float((uint32_t)scales_p[(t % SLOTS) * BKV + c0 + c] << 16);
+            if (F8) x *= scales_p[(t % SLOTS) * BKV + c0 + c];
             v[c] = __float_as_uint(x);
           }
           if (capped) {
@@ -702,12 +702,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       tmem_ld_wait();
       if (F8 && !special) {
 #pragma unroll
-        for (int c = 0; c < CP; c += 8) {
-          const uint4 ks = *reinterpret_cast<const uint4*>(scales_p + (t % SLOTS) * BKV + col0 + c);
-          const uint32_t w[4] = {ks.x, ks.y, ks.z, ks.w};
+        for (int c = 0; c < CP; c += 4) {
+          const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(scales_p + (t % SLOTS) * BKV + col0 + c);
+          const uint64_t w[2] = {ks.x, ks.y};
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const uint64_t f = mul2((uint64_t)(w[u] << 16) | ((uint64_t)(w[u] & 0xffff0000u) << 32),
+          for (int u = 0; u < 2; ++u) {
+            const uint64_t f = mul2(w[u],
                                     pack2(__uint_as_float(v[c + 2 * u]), __uint_as_float(v[c + 2 * u + 1])));
             v[c + 2 * u] = (uint32_t)f;
             v[c + 2 * u + 1] = (uint32_t)(f >> 32);
@@ -733,12 +733,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       // rescaled, which takes 700 cycles and more.  All threads of these rows decide alike: they hold the same references.
       if (__all_sync(0xffffffffu, mx - m <= GROWTH)) mx = m;
       const float corr = m == mx ? 1.f : rows_exp2(m - mx);
+      const uint64_t out2 = pack2(out, out), mx2 = pack2(-mx, -mx);
       float rs4[4] = {0.f, 0.f, 0.f, 0.f};
       uint32_t packed[CP / 2];
 #pragma unroll
       for (int c = 0; c < CP; c += 4) {
-        const float p0 = rows_exp2(fmaf(__uint_as_float(v[c]), out, -mx)), p1 = rows_exp2(fmaf(__uint_as_float(v[c + 1]), out, -mx));
-        const float p2 = rows_exp2(fmaf(__uint_as_float(v[c + 2]), out, -mx)), p3 = rows_exp2(fmaf(__uint_as_float(v[c + 3]), out, -mx));
+        const uint64_t e0 = fma2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), out2, mx2), e1 = fma2(pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), out2, mx2);
+        const float p0 = rows_exp2(__uint_as_float((uint32_t)e0)), p1 = rows_exp2(__uint_as_float((uint32_t)(e0 >> 32)));
+        const float p2 = rows_exp2(__uint_as_float((uint32_t)e1)), p3 = rows_exp2(__uint_as_float((uint32_t)(e1 >> 32)));
         rs4[0] += p0; rs4[1] += p1; rs4[2] += p2; rs4[3] += p3;
         const __nv_bfloat162 a = __floats2bfloat162_rn(p0, p1), b = __floats2bfloat162_rn(p2, p3);
         packed[c >> 1] = *reinterpret_cast<const uint32_t*>(&a);
