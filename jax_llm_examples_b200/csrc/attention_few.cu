@@ -130,7 +130,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(con
   }
   const int lo_min = __reduce_min_sync(0xffffffffu, tok.lo), lo_max = __reduce_max_sync(0xffffffffu, tok.lo);
   const int p_min = __reduce_min_sync(0xffffffffu, tok.p), p_max = __reduce_max_sync(0xffffffffu, tok.p);
-  const int first = P.cu_q ? min(lo_min, it.base) : lo_min, end_all = P.cu_q ? it.base + it.drafted : p_max + 1;
+  const int first = P.cu_q ? min(lo_min, it.base) : lo_min, end_all = rows_end(P, it, p_max);
   const int full_lo = lo_max, full_hi = P.cu_q ? it.base : p_min + 1;  // keys in between are seen by every row
   // equal ranges of whole tiles (an item's own: a short request's blocks are as short as each other)
   const int start = first / KT * KT, per = max((end_all - start + KT * P.splits - 1) / (KT * P.splits), 0) * KT, range0 = start + split * per;

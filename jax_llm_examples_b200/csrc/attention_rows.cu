@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
   }
   __syncthreads();
   // the item's keys and this block's range of them
-  const int first = P.cu_q ? min(span[0], it.base) : span[0], end_all = P.cu_q ? it.base + it.drafted : span[3] + 1;
+  const int first = P.cu_q ? min(span[0], it.base) : span[0], end_all = rows_end(P, it, span[3]);
   const int full_lo = span[1], full_hi = P.cu_q ? it.base : span[2] + 1;  // keys in between are seen by every row
   // equal ranges of whole tiles (an item's own: a short request's blocks are as short as each other)
   const int start = first / KT * KT, per = max((end_all - start + KT * P.splits - 1) / (KT * P.splits), 0) * KT, range0 = start + split * per;

@@ -64,6 +64,8 @@ __device__ __forceinline__ bool rows_tokens(const RowsParams& P, int i, RowsItem
   if (it.n0 < 0 || it.n0 > P.N - it.cnt) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
   return true;
 }
+// Keys that a request's row of the block table can hold.
+__device__ __forceinline__ int rows_capacity(const RowsParams& P) { return (int)min((long long)P.bt_stride * P.page_size, 0x7f000000ll); }
 __device__ __forceinline__ bool rows_request(const RowsParams& P, RowsItem& it) {
   it.r = P.req_of_token[it.n0];
   if (it.r < 0 || it.r >= P.n_requests) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
@@ -71,7 +73,7 @@ __device__ __forceinline__ bool rows_request(const RowsParams& P, RowsItem& it) 
   it.drafted = 0;
   if (P.cu_q) {
     const int first = P.cu_q[it.r], end = P.cu_q[it.r + 1];
-    if (first < 0 || end > P.N || it.n0 < first || it.n0 + it.cnt > end || it.base < 0) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
+    if (first < 0 || end > P.N || it.n0 < first || it.n0 + it.cnt > end || it.base < 0 || it.base > rows_capacity(P) - (end - first)) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
     it.drafted = end - first;
   }
   return true;
@@ -82,7 +84,15 @@ __device__ __forceinline__ int rows_first_key(const RowsParams& P, int p) {
   int s = 0;
   if (P.chunk > 0) s = p - p % P.chunk;
   if (P.window > 0) s = max(s, p - P.window + 1);
-  return s;
+  return max(s, 0);
+}
+
+// The place behind the last key that the item's rows see (the highest of their positions is p_max).
+__device__ __forceinline__ int rows_end(const RowsParams& P, const RowsItem& it, int p_max) {
+  if (P.cu_q) return it.base + it.drafted;
+  if (p_max < rows_capacity(P)) return p_max + 1;
+  atomicOr(P.status, JLX_STATUS_BAD_PAGE);
+  return rows_capacity(P);
 }
 
 // What a query row needs to know of its token.

@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   tc_fence_after();
   const uint32_t tmem = tmem_slot, tm_o = tmem + 256;
   // the item's keys and this block's equal part of their tiles
-  const int first = P.cu_q ? min(span[0], it.base) : span[0], end_all = P.cu_q ? it.base + it.drafted : span[3] + 1;
+  const int first = P.cu_q ? min(span[0], it.base) : span[0], end_all = rows_end(P, it, span[3]);
   const int full_lo = span[1], full_hi = P.cu_q ? it.base : span[2] + 1;  // keys in between are seen by every row
   const int start = first / BKV * BKV, per = max((end_all - start + BKV * P.splits - 1) / (BKV * P.splits), 0) * BKV, range0 = start + split * per;
   const int begin = max(first, range0), end = min(end_all, range0 + per);

@@ -488,6 +488,122 @@ def test_two_streams_at_once_and_a_captured_call():
         assert_close(out, *c.want())
 
 
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 12])
+@pytest.mark.parametrize("row_block", [128, 256])
+@pytest.mark.parametrize("n, held, dh, mask", [
+    (60, 700, 128, {}),  # 300 rows: 256 and 44, or 128, 128 and 44
+    (26, 100, 64, {}),  # 130 rows on one tile of keys and on two
+    (51, 1000, 64, dict(window=300)),
+    (52, 129, 128, dict(chunk=128)),  # 260 rows
+])
+def test_rows_of_a_block_and_ranges(monkeypatch, n, held, dh, mask, row_block, splits, bits8):
+    """Either number of rows, with fewer tiles of keys than ranges and with ranges of one tile, two and more."""
+    monkeypatch.setattr(K(), "attention_rows_plan", lambda *a: (splits, row_block))
+    c = Case([n, 3], [held, 5], 5, 1, dh, 64, bits8=bits8).tree().to_device()
+    assert_close(_tree(c, mask), *c.want(**mask))
+    if bits8:
+        c = Case([n, 3], [held, 5], 5, 1, dh, 48).to_device()
+        sink, _ = _extras(5, True, False)
+        assert_close(_attend(c, mask, c.items(n), sink=sink), *c.want(sink=sink, **mask))
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("cut", [1, 40])
+@pytest.mark.parametrize("bits8", [False, True])
+def test_a_cache_past_31_bits(bits8, cut):
+    """Pages that begin more than 2^31 bytes (and, in 16 bits, numbers) behind the cache's start."""
+    c = Case([40], [300], 8, 1, 128, 64, bits8=bits8).tree().to_device()
+    pool = torch.empty((2 ** 31 // (2 * 64 * 128) + 100 + c.P, *c.pages.shape[1:]), dtype=c.pages.dtype, device="cuda")
+    at = pool.shape[0] - c.P
+    pool.view(torch.uint8)[at:] = c.pages.view(torch.uint8)
+    if bits8:
+        scales = torch.zeros((pool.shape[0], *c.scales.shape[1:]), dtype=torch.uint8, device="cuda")
+        scales[at:] = c.scales
+        c.scales = scales
+    c.pages = pool
+    c.table = torch.where(c.table >= 0, c.table + at, c.table)
+    table, c.table = c.table, c.table - at  # (want() reads the small pool)
+    want, tol = c.want()
+    c.table = table
+    c.served(cut)
+    assert_close(_tree(c, {}, c.items(cut)), want, tol)
+    if bits8:
+        x = torch.randn(40, 1, 128, device="cuda")
+        ko, vo = torch.empty_like(x), torch.empty_like(x)
+        K().kv_store_fp8(x, -x, pool, c.scales, c.table, c.req, c.places, c.status)
+        K().kv_load_fp8(pool, c.scales, c.table, c.req, c.places, ko, vo, c.status)
+        assert torch.equal(ko.cpu().double(), hold(x.cpu())[0]) and torch.equal(vo, -ko)
+    assert int(c.status) == 0
+
+
+def test_ranges_of_many_rows_on_two_streams_and_in_two_graphs():
+    """The calls whose ranges are joined through scratch: at once on two streams, and captured twice and replayed in turn with an eager call."""
+    cases = [Case([60], [3000 + 64 * i], 10, 2, 128, 64, seed=i, bits8=i > 0).tree(seed=i).to_device() for i in range(2)]
+    cases.append(Case([1], [9000], 8, 2, 128, 64).to_device())  # single tokens in more ranges than a cluster joins
+    items = {id(c): c.items(max(c.n)) for c in cases}  # (made before the captures)
+    call = lambda c, out: _tree(c, {}, items[id(c)], out=out) if c.masks is not None else _attend(c, {}, out=out)  # noqa: E731
+    for c in cases:
+        form = K().attention_rows_form(max(c.n) * (c.Hq // c.Hkv), c.page, True)
+        joined = K().ROWS_CLUSTER if form == "attention_few" else 1
+        sms = torch.cuda.get_device_properties(0).multi_processor_count
+        assert K().attention_rows_plan(form, c.held[0] + c.n[0], 0, 0, 1, max(c.n), c.Hq, c.Hkv, sms)[0] > joined
+    want = [c.want() for c in cases]
+    sides = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        for c, s in zip(cases, sides):
+            with torch.cuda.stream(s):
+                outs.append(call(c, torch.zeros_like(c.q)))
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert_close(out, *want[i % 3])
+    graphs = []
+    for c in cases + cases:
+        out, g = torch.zeros_like(c.q), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(c, out)
+        graphs.append((g, out))
+    for _ in range(2):
+        for g, out in graphs:
+            out.zero_()
+            g.replay()
+            eager = call(cases[0], torch.zeros_like(cases[0].q))
+    torch.cuda.synchronize()
+    assert_close(eager, *want[0])
+    for i, (_, out) in enumerate(graphs):
+        assert_close(out, *want[i % 3])
+
+
+@pytest.mark.parametrize("n", [1, 9, 40])
+def test_scales_that_do_not_start_on_16_bytes(n):
+    c = Case([n], [200], 8, 2, 128, 64).to_device()
+    c.scales = torch.cat([c.scales.new_zeros(1), c.scales.flatten()])[1:].view(c.scales.shape)
+    assert c.scales.data_ptr() % 16
+    c.weights = 2.0 ** -11
+    out = torch.full_like(c.q, 7.0)
+    items = c.items(n)
+    K().attention_fp8(c.q, c.pages, c.scales, c.table, c.req, c.positions, out, c.scale, 0, 0, 0.0, 1.0, c.status, 200 + n, items=items[0], n_items=items[1],
+                      max_count=items[2])
+    assert_close(out, *c.want())
+
+
+def test_steps_of_no_tokens_and_rows_asked_for_twice():
+    c = Case([3, 1], [20, 30], 4, 2, 64, 16).to_device()
+    none = c.q[:0]
+    K().attention_fp8(none, c.pages, c.scales, c.table, c.req[:0], c.positions[:0], torch.empty_like(none), c.scale, 0, 0, 0.0, 1.0, c.status, 1)
+    k = torch.empty(0, 2, 64, device="cuda")
+    K().kv_store_fp8(k, k, c.pages, c.scales, c.table, c.req[:0], c.places[:0], c.status)
+    K().kv_load_fp8(c.pages, c.scales, c.table, c.req[:0], c.places[:0], k, torch.empty_like(k), c.status)
+    out = _attend(c, {}, (torch.zeros((1, 2), dtype=torch.int32, device="cuda"), 0, 1))
+    assert (out == 7).all()
+    _attend(c, {}, (torch.tensor([[0, 3], [1, 2], [0, 0]], dtype=torch.int32, device="cuda"), 3, 3), out=out)  # rows 1 and 2 twice; an item of none
+    _attend(c, {}, rows=torch.tensor([3, 3, 3], dtype=torch.int32, device="cuda"), out=out)
+    assert_close(out, *c.want())
+    assert int(c.status) == 0
+
+
 def test_a_description_that_points_outside_the_step_is_refused_by_the_kernel():
     c = Case([4], [20], 4, 2, 64, 16).tree().to_device()
     for items in ([[2, 3]], [[-1, 2]], [[0, 9]]):
@@ -497,6 +613,33 @@ def test_a_description_that_points_outside_the_step_is_refused_by_the_kernel():
     c.status.zero_()
     out = _attend(c, {}, rows=torch.tensor([1, 77], dtype=torch.int32, device="cuda"))
     assert int(c.status) == 1 and (out[0] == 7).all() and not (out[1] == 7).all()
+
+
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("n", [2, 40])
+@pytest.mark.parametrize("far", [10 ** 4, 2 ** 31 - 1])
+def test_positions_that_the_table_cannot_hold_raise_the_status(form, n, far):
+    c = Case([n, n], [20, 30], 8, 2, 64, 16).to_device()
+    c.positions[n - 1] = far
+    out = _attend(c, {}, c.items(n))
+    assert int(c.status) == 1
+    c.positions[n - 1] = 20 + n - 1
+    assert_close(out, *c.want(), slice(n, None))  # the other request's rows
+    c.status.zero_()
+    c.positions[:n] = -5000  # before the first key: nothing is seen
+    out = _attend(c, dict(chunk=512), c.items(n))
+    assert not out[:n].any() and int(c.status) == 0
+
+
+@pytest.mark.parametrize("n", [2, 40])
+@pytest.mark.parametrize("far", [10 ** 4, 2 ** 31 - 1])
+def test_trees_that_the_table_cannot_hold_raise_the_status(n, far):
+    c = Case([n, n], [20, 30], 8, 2, 64, 16).tree().to_device()
+    c.q_start[0] = far
+    out = _tree(c, {})
+    assert int(c.status) == 1
+    c.q_start[0] = 20
+    assert_close(out, *c.want(), slice(n, None))
 
 
 def test_head_sizes_without_a_kernel_are_refused():
