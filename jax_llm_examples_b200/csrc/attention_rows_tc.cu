@@ -243,16 +243,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   if (!rows_request(P, it)) return;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < N_BARS; ++i) mbar_init(BAR(i), 1);  // a transaction count or a tcgen05.commit each, but:
-    mbar_init(BAR(B_QREADY), 256 * PARTS);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(BAR(B_PREADY + i), 128 * PARTS);
-      mbar_init(BAR(B_VREADY + i), AUX);
+    for (int i = 0; i < N_BARS; ++i) {
+      int count = 1;  // a transaction count or a tcgen05.commit, but:
+      if (i == B_QREADY) count = 256 * PARTS;
+      if (i >= B_PREADY && i < B_PREADY + 2) count = 128 * PARTS;
+      if ((i >= B_RAWEMPTY && i < B_RAWEMPTY + 3) || (i >= B_VREADY && i < B_VREADY + 2)) count = AUX;
+      if (i >= B_MEET && i < B_MEET + 8) count = 32 * PARTS;
+      if (i >= B_END && i < B_END + 4) count = 64 * PARTS;
+      if (i >= B_SCALES && i < B_SCALES + SLOTS) count = 32;
+      mbar_init(BAR(i), count);
     }
-    for (int i = 0; i < 3; ++i) mbar_init(BAR(B_RAWEMPTY + i), AUX);
-    for (int i = 0; i < 8; ++i) mbar_init(BAR(B_MEET + i), 32 * PARTS);
-    for (int i = 0; i < 4; ++i) mbar_init(BAR(B_END + i), 64 * PARTS);
-    for (int i = 0; i < SLOTS; ++i) mbar_init(BAR(B_SCALES + i), 32);
     failed = any_bad = 0;
     item_s[0] = it.r;
     item_s[1] = it.base;
