@@ -15,13 +15,14 @@
 // prepare values (below).
 //
 // What bounds it: a group's turn of about 4,500 cycles, of which 1,250 are the exponentials (1,024 at the unit's rate), 1,000 the
-// rest of the softmax, 600 (8 bits) the keys' scales and 1,800 the wait for the two products (1,024 at the unit's rate) behind the
-// other group's; so 2,250 a tile of 128 by 128, where exponentials and products alone would take 1,024 side by side.  Measured
-// (B200): 2,048 tokens after 1,500, 40 heads on 8 of 128, 8 bits: 201 us, 527 TFLOP/s, 32 % of the bfloat16 peak; trees of 32
-// tokens on 8 requests of up to 8,192 keys, bfloat16: 96 us; of 64 on 16 of up to 12,000, 32 heads, 8 bits: 286 us, 531 TFLOP/s.
-// (One group of sixteen warps on 128 rows with two buffers of scores: 227, 114 and 325 us.  One block per multiprocessor that
-// takes equal shares of all tiles: 247, 112 and 293 with that one group; its join and the change from piece to piece cost what
-// the shares gained.  Copies asked into L2 ahead, and scale bytes as small bulk copies: 20 % slower each.)
+// rest of the softmax, 600 (8 bits) the keys' scales and 1,800 the wait for the two products: their 16 instructions are accepted
+// one in 95 cycles from one thread, 1,520 a tile.  So 2,250 a tile of 128 by 128, where exponentials and products would take
+// 1,024 each, side by side.  Measured (B200): 2,048 tokens after 1,500, 40 heads on 8 of 128, 8 bits: 187 us, 566 TFLOP/s, 34 %
+// of the bfloat16 peak; trees of 32 tokens on 8 requests of up to 8,192 keys, bfloat16: 96 us, 339 TFLOP/s; of 64 tokens on 16
+// requests of up to 12,000, 32 heads, 8 bits: 278 us, 547 TFLOP/s.
+// Tried and slower: one group of sixteen warps on 128 rows with two buffers of scores (227, 114 and 325 us); then one block per
+// multiprocessor that takes an equal share of all tiles (247, 112 and 293: its join and the change from piece to piece cost what
+// the shares gained); a warp for each group's products beside one for all copies (228, 108 and 357).
 //
 // 8 bits: the keys' codes are an operand as they lie in the cache.  Queries are two: each entry (its row's largest brought to
 // 2^7 .. 2^8 by a power of two) as e4m3, and what is left of it as e5m2; the remainder of eight bits after the nearest four is

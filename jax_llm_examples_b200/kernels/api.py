@@ -1111,17 +1111,20 @@ FP8 = torch.float8_e4m3fn  # pages in 8 bits: e4m3 codes, and a byte of scale pe
 
 
 def _ints(what: str, *arrays: "tuple[str, torch.Tensor | None, int]") -> None:
-    """Index arrays: contiguous int32 with at least so many entries."""
+    """Index arrays: int32 with at least so many entries (:func:`_placed` looks at where and how they lie)."""
     for name, t, n in arrays:
-        if t is not None and (t.dtype is not torch.int32 or t.numel() < n or not t.is_contiguous()):
+        if t is not None and (t.dtype is not torch.int32 or t.numel() < n):
             raise KernelError(f"{what}: {name} must be contiguous int32 with at least {n} entries")
 
 
-def _same_device(what: str, *tensors: torch.Tensor | None) -> int:
-    """The current device, to whose stream a launch goes: tensors of another device, or of none, have no place in it."""
+def _placed(what: str, *tensors: torch.Tensor | None) -> int:
+    """The current device, to whose stream a launch goes: tensors of another device, or of none, have no place in it, nor have
+    tensors that are not contiguous."""
     dev = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.get_device() != dev:
+        if t is not None and (t.get_device() != dev or not t.is_contiguous()):
+            if not t.is_contiguous():
+                raise KernelError(f"{what}: a kernel was given a tensor that is not contiguous")
             if not t.is_cuda:
                 raise KernelError(f"{what}: a kernel was given a tensor that is not on the GPU; there is no CPU path")
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
@@ -1137,13 +1140,13 @@ def _address(t: torch.Tensor | None) -> int:
 
 
 def _cache8(what: str, pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, Hkv: int, dh: int) -> None:
-    if pages.dtype != FP8 or pages.dim() != 5 or pages.shape[1] != 2 or pages.shape[2] != Hkv or pages.shape[4] != dh:
+    shape = pages.shape
+    if pages.dtype is not FP8 or len(shape) != 5 or shape[1] != 2 or shape[2] != Hkv or shape[4] != dh:
         raise KernelError(f"{what}: pages must be float8_e4m3fn [pages, 2, {Hkv}, page size, {dh}], not {pages.dtype} {tuple(pages.shape)}")
-    if scales.dtype != torch.uint8 or scales.shape != pages.shape[:4]:
+    if scales.dtype is not torch.uint8 or scales.shape != shape[:4]:
         raise KernelError(f"{what}: scales must be uint8 {tuple(pages.shape[:4])}, a byte per row of the pages")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
         raise KernelError(f"{what}: the block table must be int32 [requests, pages of one]")
-    _contig(pages, scales, block_table)
 
 
 # What the launchers take as one structure, laid out as in C (packing it costs a call less than a ctypes.Structure does).
@@ -1166,13 +1169,12 @@ def kv_store_fp8(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: 
     one call are distinct.  A row's entries are kept as x * 2^-e rounded to e4m3, its byte as e + 127, e the smallest whole
     number (at least -60) with max |x| <= 448 * 2^e.  A row with an infinity or a NaN, or above 448 * 2^60, gets byte 255 and
     reads back as NaN.  A place without a page is left out and raises the status."""
-    _contig(k, v)
     N, Hkv, dh = k.shape
     _cache8("kv_store_fp8", pages, scales, block_table, Hkv, dh)
     _ints("kv_store_fp8", ("req_of_token", req_of_token, N), ("places", places, N), ("status", status, 1))
     if v.shape != k.shape or v.dtype != k.dtype:
         raise KernelError("kv_store_fp8: keys and values must have one shape and type")
-    dev = _same_device("kv_store_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
+    dev = _placed("kv_store_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
     args = _kv_fp8_args(pages, scales, block_table, req_of_token, places, N, status)
     _run("kv_fp8", "jlx_kv_store_fp8", args, c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
 
@@ -1183,7 +1185,6 @@ def rope_kv_store_fp8(qkv: torch.Tensor, q_out: torch.Tensor, pages: torch.Tenso
     """:func:`rope_kv_store` into a cache in 8 bits (:func:`kv_store_fp8`), quantised from the 32-bit keys and values.  qkv:
     [N, (Hq + 2 Hkv) * dh] projected rows (float32 or bfloat16), or ``splits`` float32 partials of them; q_out: bfloat16
     [N, Hq, dh].  ``places`` (None: the positions): where the rows are kept, for drafted tokens whose position is not their place."""
-    _contig(qkv, q_out, inv_freq)
     N = q_out.shape[0]
     places = positions if places is None else places
     _cache8("rope_kv_store_fp8", pages, scales, block_table, Hkv, dh)
@@ -1193,7 +1194,7 @@ def rope_kv_store_fp8(qkv: torch.Tensor, q_out: torch.Tensor, pages: torch.Tenso
                           f"fit qkv {tuple(qkv.shape)}, q_out {q_out.dtype} {tuple(q_out.shape)}")
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != dh // 2):
         raise KernelError(f"rope_kv_store_fp8: {dh // 2} float32 frequencies are needed")
-    dev = _same_device("rope_kv_store_fp8", qkv, q_out, pages, scales, block_table, req_of_token, positions, places, inv_freq, status)
+    dev = _placed("rope_kv_store_fp8", qkv, q_out, pages, scales, block_table, req_of_token, positions, places, inv_freq, status)
     args = _kv_fp8_args(pages, scales, block_table, req_of_token, places, N, status)
     rope = _ROPE_FP8_ARGS.pack(qkv.data_ptr(), q_out.data_ptr(), positions.data_ptr(), _address(inv_freq), 0 if splits == 1 else qkv.numel() // splits,
                                code(qkv.dtype), splits, Hq, int(l2norm), eps)
@@ -1204,13 +1205,12 @@ def kv_load_fp8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Te
                 k: torch.Tensor, v: torch.Tensor, status: torch.Tensor) -> None:
     """The rows that a cache in 8 bits keeps at the listed places, as numbers: k, v [N, Hkv, dh] (float32 or bfloat16, exact in
     both).  A place without a page gives zeros and raises the status."""
-    _contig(k, v)
     N, Hkv, dh = k.shape
     _cache8("kv_load_fp8", pages, scales, block_table, Hkv, dh)
     _ints("kv_load_fp8", ("req_of_token", req_of_token, N), ("places", places, N), ("status", status, 1))
     if v.shape != k.shape or v.dtype != k.dtype:
         raise KernelError("kv_load_fp8: keys and values must have one shape and type")
-    dev = _same_device("kv_load_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
+    dev = _placed("kv_load_fp8", k, v, pages, scales, block_table, req_of_token, places, status)
     args = _kv_fp8_args(pages, scales, block_table, req_of_token, places, N, status)
     _run("kv_fp8", "jlx_kv_load_fp8", args, c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
 
@@ -1290,30 +1290,35 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     N, Hq, dh = q.shape
     P, two, Hkv, page_size, dh2 = pages.shape
     out_p, q_p = out.data_ptr(), q.data_ptr()
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or out.shape != q.shape or (out_p == q_p and N):
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or out.shape != q.shape or (out_p == q_p and N):
         raise KernelError(f"{what}: queries and output must be bfloat16 [N, Hq, dh], and not the same rows")
     if dh2 != dh or two != 2:
         raise KernelError(f"{what}: cache pages {tuple(pages.shape)} and queries {tuple(q.shape)} disagree")
     if scales is not None:
         _cache8(what, pages, scales, block_table, Hkv, dh)
-    elif pages.dtype != torch.bfloat16:
+    elif pages.dtype is not torch.bfloat16:
         raise KernelError(f"{what}: pages must be bfloat16, or float8_e4m3fn with scales")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+    elif block_table.dtype is not torch.int32 or block_table.dim() != 2:
         raise KernelError(f"{what}: the block table must be int32 [requests, pages of one]")
     R, width = block_table.shape
-    _ints(what, ("req_of_token", req_of_token, N), ("positions", positions, N), ("items", items, 2 * n_items), ("rows", rows, n_items),
-          ("status", status, 1), ("cu_q", cu_q, R + 1), ("q_start", q_start, R), ("masks", masks, N))
-    words = 0
+    _ints(what, ("req_of_token", req_of_token, N), ("positions", positions, N), ("status", status, 1))
+    if items is not None or rows is not None:
+        _ints(what, ("items", items, 2 * n_items), ("rows", rows, n_items))
+    words = cu_q_p = q_start_p = masks_p = 0
     if masks is not None:
+        _ints(what, ("cu_q", cu_q, R + 1), ("q_start", q_start, R), ("masks", masks, N))
         if masks.dim() != 2 or masks.shape[0] != N:
             raise KernelError(f"{what}: masks must be int32 [{N}, words], a bit per drafted token of the request")
-        words = masks.shape[1]
+        words, cu_q_p, q_start_p, masks_p = masks.shape[1], cu_q.data_ptr(), q_start.data_ptr(), masks.data_ptr()
     if max_kv_len < 1 or max_count < 1 or n_items < 0 or (items is None and rows is None and n_items > N):
         raise KernelError(f"{what}: {n_items} items of up to {max_count} tokens over {max_kv_len} keys")
-    _check_sink(sink, Hq)
-    _check_sink(slopes, Hq, "slopes")
-    _contig(q, pages, block_table, out)
-    dev = _same_device(what, q, pages, scales, block_table, req_of_token, positions, out, items, rows, cu_q, q_start, masks, sink, slopes, status)
+    if sink is not None:
+        _check_sink(sink, Hq)
+    if slopes is not None:
+        _check_sink(slopes, Hq, "slopes")
+    dev = _placed(what, q, pages, scales, block_table, req_of_token, positions, out, status, items, rows)
+    if masks is not None or sink is not None or slopes is not None:
+        _placed(what, cu_q, q_start, masks, sink, slopes)
     if N == 0 or n_items == 0:
         return
     if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
@@ -1328,7 +1333,7 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
         part_o = scratch.data_ptr()
         part_ml, joined = part_o + 4 * N * Hq * splits * dh, 1
     args = _ROWS_ARGS.pack(q_p, pages.data_ptr(), scales_p, block_table.data_ptr(), req_of_token.data_ptr(), positions.data_ptr(), out_p,
-                           _address(items), _address(rows), _address(cu_q), _address(q_start), _address(masks), _address(sink), _address(slopes),
+                           _address(items), _address(rows), cu_q_p, q_start_p, masks_p, _address(sink), _address(slopes),
                            part_o, part_ml, status.data_ptr(), width, R, n_items, max_count, words, N, Hq, Hkv, dh, page_size, P, chunk, window, splits,
                            row_block, scale, softcap, attn_scale, floor_scale)
     _run(form, _ROWS_LAUNCHERS[form], args, _raw_stream(dev))
