@@ -139,6 +139,12 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return d;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Shared-memory matrix descriptors for tiles whose rows are 128 (or 64) bytes with the swizzle of that many, 8-row groups side
 // by side.  K-major: a row runs along K.  MN-major: along the operand's N direction, rows are K steps; blocks of 64 numbers
 // along N are `lbo_bytes` apart.
@@ -451,9 +457,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
         uint32_t f = (uint32_t)min(120 + e, 127) + 127, h = (uint32_t)max(e - 7, 0) + 127;
         f = (f << 7) | (f << 23);
         h = (h << 7) | (h << 23);
-        uint32_t keep = in ? 0xffffffffu : 0u, all = 0u;
+        if (!in || bv == FP8_BAD) f = 0u;  // (every code is a finite number to the product)
+        uint32_t all = 0u;
         if (in && bv == FP8_BAD) {
-          keep = 0u;
           if (masked_tile(place0)) *(volatile int*)&any_bad = 1;
           else all = 0x7fc07fc0u;
         }
@@ -478,7 +484,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
           uint8_t* half = v + (c0 >> 2) * HALF_BYTES;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const uint32_t w[4] = {x[c].x & keep, x[c].y & keep, x[c].z & keep, x[c].w & keep};
+            const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
             uint32_t o[8];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -717,7 +723,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       }
       float mx4[4] = {ROWS_NEG_BIG, ROWS_NEG_BIG, ROWS_NEG_BIG, ROWS_NEG_BIG};  // four chains instead of one long one
 #pragma unroll
-      for (int c = 0; c < CP; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(v[c]));
+      for (int c = 0; c < CP; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       // the row's maximum over all parts (double-buffered by the meeting's parity: a partner may be a tile ahead)
       const int mp = turn & 1;
