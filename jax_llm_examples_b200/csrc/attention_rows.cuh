@@ -26,7 +26,7 @@ struct RowsParams {
   const void* pages;       // [P, 2, Hkv, page, DH] bfloat16, or e4m3 codes
   const uint8_t* scales;   // [P, 2, Hkv, page] with codes
   const int* block_table;
-  int bt_stride, n_requests;
+  int bt_stride, n_requests, max_count;
   const int* req_of_token;
   const int* positions;
   bf16* out;               // [N, Hq, DH]
@@ -61,7 +61,7 @@ __device__ __forceinline__ bool rows_tokens(const RowsParams& P, int i, RowsItem
   it.n0 = P.items ? P.items[2 * i] : (P.rows ? P.rows[i] : i);
   it.cnt = P.items ? P.items[2 * i + 1] : 1;
   if (it.cnt <= 0) return false;
-  if (it.n0 < 0 || it.n0 > P.N - it.cnt) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
+  if (it.n0 < 0 || it.n0 > P.N - it.cnt || it.cnt > P.max_count) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return false; }
   return true;
 }
 // Keys that a request's row of the block table can hold.
@@ -199,7 +199,7 @@ static int rows_params(const RowsArgs& a, RowsParams& P) {
   JLX_REQUIRE(!a.cu_q == !a.masks && !a.cu_q == !a.q_start && (!a.cu_q || (a.items && a.words > 0)), "attention over rows: a tree needs its offsets, cached lengths, masks and items");
   JLX_REQUIRE((long long)a.max_count * a.Hq < (1ll << 30), "attention over rows: an item has too many rows");
   P.q = (const bf16*)a.q; P.pages = a.pages; P.scales = (const uint8_t*)a.scales; P.block_table = (const int*)a.block_table; P.bt_stride = a.bt_stride;
-  P.n_requests = a.n_requests; P.req_of_token = (const int*)a.req_of_token; P.positions = (const int*)a.positions; P.out = (bf16*)a.out;
+  P.n_requests = a.n_requests; P.max_count = a.max_count; P.req_of_token = (const int*)a.req_of_token; P.positions = (const int*)a.positions; P.out = (bf16*)a.out;
   P.items = (const int*)a.items; P.rows = (const int*)a.rows; P.n_items = a.n_items; P.cu_q = (const int*)a.cu_q; P.q_start = (const int*)a.q_start;
   P.masks = (const int*)a.masks; P.words = a.words; P.N = a.N; P.Hq = a.Hq; P.Hkv = a.Hkv; P.page_size = a.page_size; P.num_pages = a.num_pages;
   P.scale_log2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E;

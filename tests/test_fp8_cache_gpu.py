@@ -307,6 +307,31 @@ def test_scores_that_leap(form, bits8, places):
 
 
 @pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("n", [3, 30, 70])
+@pytest.mark.parametrize("steps", [[5.0, 5.0, 5.0], [12.0, 12.0, 15.0], [17.0, 5.0, 15.5], [-40.0, 15.0, 30.0]])
+def test_scores_that_climb(form, bits8, n, steps):
+    """The largest score of every row climbs by these powers of two, tiles apart: within what a reference may be outgrown by, and beyond."""
+    c = Case([n], [900], 4, 1, 128, 16, bits8=False, spread=0.0).tree()
+    c.q[:] = c.q[0, 0]
+    c.rows[:, 0] *= 0.25
+    top = 0.0
+    for place, step in zip((150, 420, 800), steps):
+        top += step
+        page, at = int(c.table[0, place // 16]), place % 16
+        c.rows[page, 0, 0, at] = c.q[0, 0].double() * (top / (c.scale * math.log2(math.e) * float((c.q[0, 0].double() ** 2).sum())))
+    c.rows = c.rows.to(torch.bfloat16).double()
+    if bits8:
+        c.rows, scales = hold(c.rows)
+        c.set_rows8(scales)
+        c.bits8 = True
+    else:
+        c.pages = c.rows.to(torch.bfloat16)
+    c.to_device()
+    assert_close(_tree(c, {}), *c.want())
+
+
+@pytest.mark.parametrize("form", FORMS, indirect=True)
 @pytest.mark.parametrize("n", [8, 100])
 def test_nan_rows_reach_those_that_see_them_and_no_other(form, n):
     c = Case([n], [50], 4, 2, 128, 16)
@@ -610,6 +635,10 @@ def test_a_description_that_points_outside_the_step_is_refused_by_the_kernel():
         c.status.zero_()
         _tree(c, {}, (torch.tensor(items, dtype=torch.int32, device="cuda"), 1, 9))
         assert int(c.status) == 1
+    for most in (1, 3):  # an item of more tokens than the call was sized for
+        c.status.zero_()
+        out = _tree(c, {}, (torch.tensor([[0, 4]], dtype=torch.int32, device="cuda"), 1, most))
+        assert int(c.status) == 1 and (out == 7).all()
     c.status.zero_()
     out = _attend(c, {}, rows=torch.tensor([1, 77], dtype=torch.int32, device="cuda"))
     assert int(c.status) == 1 and (out[0] == 7).all() and not (out[1] == 7).all()
