@@ -6,7 +6,10 @@
 // A row of dh entries belongs to `lanes` neighbouring threads of a warp (the power of two that covers dh / 8), eight entries
 // each: 16 bytes of bfloat16 (or 2 x 16 of float32) in, 8 bytes of codes out; the row's largest magnitude and the norm's sum
 // of squares meet by shuffles, so a row is read once and nothing passes through shared memory but a token's angles.
-// Both directions move bytes and little else: what bounds them is the memory, and for a decode step's few rows the launch.
+// What bounds them: for a prompt's rows behind rotation and norm the issue slots (240 instructions a warp and two rows, 76 % of the
+// rate: 4,096 tokens of 40 + 2 x 8 heads of 128 take 29 us, 3.7 TB/s; half the angles' loads kept in registers, packed arithmetic or
+// six blocks a multiprocessor are slower: registers and the warps they cost); for plain writing and reading back the memory (7 us
+// for the same tokens back); for a decode step's few rows the launch.
 #include "fp8_rows.cuh"
 
 struct KvFp8Params {
@@ -89,7 +92,9 @@ __device__ __forceinline__ void kv_fp8_write(const KvFp8Params& P, long long row
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
   }
-  for (int o = P.lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < P.lanes) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (!mine || !keep) return;
   const bool bad = top > __float_as_uint(FP8_LIMIT);
   const int e = bad ? 0 : fp8_row_exp(__uint_as_float(top));
@@ -205,6 +210,7 @@ rope_kv_store_fp8_kernel(const TI* __restrict__ qkv, int splits, long long split
     }
     __syncthreads();
   }
+  const float per_entry = 1.f / (float)P.dh;
   // (whole warps stay in the loop: the shuffles need every lane)
   for (int h0 = blockIdx.y * TURNS * step; h0 < rows; h0 += gridDim.y * TURNS * step) {
     if (h0 != blockIdx.y * TURNS * step) fetch(h0);
@@ -245,9 +251,11 @@ rope_kv_store_fp8_kernel(const TI* __restrict__ qkv, int splits, long long split
         for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
       }
       if (l2norm) {
-        for (int o = P.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          if (o < P.lanes) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (!is_v) {
-          const float inv = rsqrtf(ss / (float)P.dh + eps);
+          const float inv = rsqrtf(fmaf(ss, per_entry, eps));
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] *= inv;
         }
