@@ -1227,24 +1227,34 @@ def attention_rows_supported(q_dtype: torch.dtype, Hq: int, Hkv: int, dh: int) -
     return q_dtype == torch.bfloat16 and dh in (64, 128) and Hkv > 0 and Hq % Hkv == 0
 
 
-def attention_rows_form(rows: int, page_size: int, aligned: bool) -> str:
-    """The kernel for items of up to so many query rows of a KV head ((token, head of the group) pairs)."""
-    if rows <= ROWS_FEW:
+def attention_rows_form(rows: int, page_size: int, aligned: bool, keys: int = 0, units: int = 0) -> str:
+    """The kernel for items of up to so many query rows of a KV head ((token, head of the group) pairs).  ``keys``, ``units``: of a
+    cache in 8 bits, the keys that an item sees and the (item, KV head) pairs.
+
+    Few items of up to 64 rows take ``attention_few`` in groups of 16 as long as those are at most 32: its way to the first tile
+    and its join are shorter than the tcgen05 kernel's.  (8 bits, 40 heads on 8 of 128, a tree of 8 on one request, 24 groups: 12.7
+    us for 19.0 at 900 keys, 19.1 for 24.9 at 5,000, but 35.3 for 25.1 at 8,000; on two requests, 48 groups: 21.3 for 19.0.  Over
+    a bfloat16 cache 24 groups take 21.0 for 18.0.)"""
+    if rows <= ROWS_FEW or (rows <= 4 * ROWS_FEW and 0 < keys <= 5120 and units * -(-rows // ROWS_FEW) <= 32):
         return "attention_few"
     return "attention_rows_tc" if page_size % 16 == 0 and aligned else "attention_rows"
+
+
+def _keys_seen(max_kv_len: int, chunk: int, window: int, max_count: int) -> int:
+    return min(max_kv_len, window + max_count if window else max_kv_len, chunk + max_count if chunk else max_kv_len)
 
 
 @functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
 def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int) -> "tuple[int, int]":
     """(Ranges that an item's keys are cut into: equal ones, of the item's own keys; query rows of a block of ``attention_rows_tc``.)"""
-    seen = min(max_kv_len, window + max_count if window else max_kv_len, chunk + max_count if chunk else max_kv_len) + ROWS_TILE  # ranges start at a tile's first key
+    seen = _keys_seen(max_kv_len, chunk, window, max_count) + ROWS_TILE  # ranges start at a tile's first key
     rows = max_count * (Hq // Hkv)
     if form == "attention_few":
         # Three blocks share a multiprocessor.  A round of them takes as long as a range and what a block costs besides, as much
         # as 10 tiles (the way to the first tile, the join), a join through scratch 6 tiles more and one for 8 ranges: the
         # number of ranges with the least of it.  (64 requests of 8,000 keys: 225 us with 1 range, 188 with 3, 205 with 6;
         # one of 8,000: 90 with 1, 18.5 with 8, 16.7 with 24, 23.7 with 55.)
-        blocks, places, tiles, block, join, share = n_items * Hkv, 3 * sms, -(-seen // ROWS_TILE), 10, 6, 8
+        blocks, places, tiles, block, join, share = n_items * Hkv * -(-rows // ROWS_FEW), 3 * sms, -(-seen // ROWS_TILE), 10, 6, 8
     elif form == "attention_rows_tc":
         return _rows_tc_plan(-(-seen // 128), n_items * Hkv, rows, sms)
     else:
@@ -1324,7 +1334,8 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
         raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
     scales_p = _address(scales)
-    form = attention_rows_form(max_count * (Hq // Hkv), page_size, scales_p % 16 == 0)
+    keys = 0 if scales is None else _keys_seen(max_kv_len, chunk, window, max_count)
+    form = attention_rows_form(max_count * (Hq // Hkv), page_size, scales_p % 16 == 0, keys, n_items * Hkv)
     splits, row_block = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
     part_o = part_ml = joined = 0
     if splits > (ROWS_CLUSTER if form == "attention_few" else 1):

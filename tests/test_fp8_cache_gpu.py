@@ -232,12 +232,15 @@ PORTIONS = [
 ]
 
 
-FORMS = ["rule", "attention_rows"]  # the kernel by the sizes, or the one for any page
+FORMS = ["rule", "attention_rows", "attention_rows_tc", "attention_few"]  # the kernel by the sizes, or the one named where it can
 
 
 @pytest.fixture
 def form(request, monkeypatch):
-    if request.param != "rule":
+    rule = K().attention_rows_form
+    if request.param == "attention_rows_tc":
+        monkeypatch.setattr(K(), "attention_rows_form", lambda rows, page, aligned, *a: request.param if page % 16 == 0 and aligned else rule(rows, page, aligned))
+    elif request.param != "rule":
         monkeypatch.setattr(K(), "attention_rows_form", lambda *a: request.param)
 
 
