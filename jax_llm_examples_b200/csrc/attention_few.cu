@@ -95,9 +95,10 @@ template <int DH, bool F8, int NG> struct FewTile {
   static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + 1024;  // (up to 1 KB for the alignment)
 };
 
-// NG: groups of 8 query rows (1, 2).
+// NG: groups of 8 query rows (1, 2).  Registers for as many blocks of a multiprocessor as its shared memory has room for (heads of
+// 128 in bfloat16, two groups: 209 registers and one block otherwise, six requests of 4,000 keys 25 us for 20).
 template <int DH, bool F8, int NG>
-__global__ void __launch_bounds__((CONSUMERS + 1) * 32) attention_few_kernel(const __grid_constant__ CUtensorMap map, const RowsParams P, int clustered, int box_rows) {
+__global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2 : 3) attention_few_kernel(const __grid_constant__ CUtensorMap map, const RowsParams P, int clustered, int box_rows) {
   JLX_TL(TL_ATTN_DECODE);
   using T = FewTile<DH, F8, NG>;
   constexpr int CH = T::CH, STAGES = T::STAGES, ROWS = 8 * NG;
@@ -631,6 +632,41 @@ static int launch_few(const RowsParams& P, dim3 grid, cudaStream_t stream) {
   cfg.numAttrs = clustered ? 2 : 1;
   JLX_CUDA(cudaLaunchKernelEx(&cfg, attention_few_kernel<DH, F8, NG>, map, P, clustered, box_rows));
   return 0;
+}
+
+template <int DH, bool F8, int NG>
+static int few_places(int splits) {
+  using T = FewTile<DH, F8, NG>;
+  int dev = 0, sms = 0, n = 0;
+  bool ok = cudaFuncSetAttribute(attention_few_kernel<DH, F8, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM) == cudaSuccess;
+  if (splits > 1 && splits <= MAX_CLUSTER) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits);
+    cfg.blockDim = dim3((CONSUMERS + 1) * 32);
+    cfg.dynamicSmemBytes = T::SMEM;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    ok = ok && cudaOccupancyMaxActiveClusters(&n, attention_few_kernel<DH, F8, NG>, &cfg) == cudaSuccess;
+    n *= splits;
+  } else {
+    ok = ok && cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
+         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_few_kernel<DH, F8, NG>, (CONSUMERS + 1) * 32, T::SMEM) == cudaSuccess;
+    n *= sms;
+  }
+  if (!ok) cudaGetLastError();
+  return ok && n > 0 ? n : 1;
+}
+
+// Blocks that the current device holds at once of the kernel for so many rows of a KV head, with ranges in clusters where they
+// are joined there (what plans ranges asks once per kind).
+JLX_API int jlx_attention_few_places(int dh, int bits8, int rows, int splits) {
+  if (dh == 128)
+    return bits8 ? (rows <= 8 ? few_places<128, true, 1>(splits) : few_places<128, true, 2>(splits)) : (rows <= 8 ? few_places<128, false, 1>(splits) : few_places<128, false, 2>(splits));
+  return bits8 ? (rows <= 8 ? few_places<64, true, 1>(splits) : few_places<64, true, 2>(splits)) : (rows <= 8 ? few_places<64, false, 1>(splits) : few_places<64, false, 2>(splits));
 }
 
 JLX_API int jlx_attention_few(const RowsArgs* a, cudaStream_t stream) {

@@ -1219,6 +1219,7 @@ _ROWS_ARGS = struct.Struct("@17P15i4f")  # RowsArgs in csrc/attention_rows.cuh
 ROWS_TILE = 64  # keys of a tile, csrc/attention_rows.cu and attention_few.cu
 ROWS_FEW = 16  # query rows of an item and KV head that attention_few.cu takes
 ROWS_CLUSTER = 8  # ranges that it joins without scratch
+ROWS_SPLITS = (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48)  # numbers of ranges to choose from
 _ROWS_LAUNCHERS = {form: "jlx_" + form for form in ("attention_few", "attention_rows", "attention_rows_tc")}
 
 
@@ -1245,27 +1246,38 @@ def _keys_seen(max_kv_len: int, chunk: int, window: int, max_count: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
-def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int) -> "tuple[int, int]":
-    """(Ranges that an item's keys are cut into: equal ones, of the item's own keys; query rows of a block of ``attention_rows_tc``.)"""
+def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int,
+                        places: "tuple[int, ...] | None" = None) -> "tuple[int, int]":
+    """(Ranges that an item's keys are cut into: equal ones, of the item's own keys; query rows of a block of ``attention_rows_tc``.)
+    ``places``: blocks of ``attention_few`` that the device holds at once, for each of ROWS_SPLITS (None: three a multiprocessor)."""
     seen = _keys_seen(max_kv_len, chunk, window, max_count) + ROWS_TILE  # ranges start at a tile's first key
     rows = max_count * (Hq // Hkv)
     if form == "attention_few":
-        # Three blocks share a multiprocessor.  A round of them takes as long as a range and what a block costs besides, as much
-        # as 10 tiles (the way to the first tile, the join), a join through scratch 6 tiles more and one for 8 ranges: the
-        # number of ranges with the least of it.  (64 requests of 8,000 keys: 225 us with 1 range, 188 with 3, 205 with 6;
-        # one of 8,000: 90 with 1, 18.5 with 8, 16.7 with 24, 23.7 with 55.)
-        blocks, places, tiles, block, join, share = n_items * Hkv * -(-rows // ROWS_FEW), 3 * sms, -(-seen // ROWS_TILE), 10, 6, 8
+        # A round of blocks, as many as the device holds, takes as long as a range and what a block costs besides, as much as 10 tiles
+        # (the way to the first tile, the join), a join through scratch 6 tiles more and one for 8 ranges: the number of ranges
+        # with the least of it.  (64 requests of 8,000 keys: 225 us with 1 range, 188 with 3, 205 with 6; one of 8,000: 90 with 1,
+        # 18.5 with 8, 16.7 with 24, 23.7 with 55.  Six requests of 4,000 over a bfloat16 cache, two blocks a multiprocessor: 18.8
+        # with 5 ranges, 27 with 8, which would suit three.)
+        blocks, tiles, block, join, share = n_items * Hkv * -(-rows // ROWS_FEW), -(-seen // ROWS_TILE), 10, 6, 8
+        places = places or (3 * sms,) * len(ROWS_SPLITS)
     elif form == "attention_rows_tc":
         return _rows_tc_plan(-(-seen // 128), n_items * Hkv, rows, sms)
     else:
-        blocks, places, tiles, block, join, share = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64)), 2 * sms, -(-seen // ROWS_TILE), 4, 3, 8
+        blocks, tiles, block, join, share = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64)), -(-seen // ROWS_TILE), 4, 3, 8
+        places = (2 * sms,) * len(ROWS_SPLITS)
     splits, least = 1, 1 << 60
-    for s in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48):
+    for s, held in zip(ROWS_SPLITS, places):
         joined = s > (ROWS_CLUSTER if form == "attention_few" else 1)
-        cost = -(-blocks * s // places) * (-(-tiles // s) + block) + (join + s // share if joined else 0)
+        cost = -(-blocks * s // held) * (-(-tiles // s) + block) + (join + s // share if joined else 0)
         if s <= tiles and cost < least:
             splits, least = s, cost
     return splits, 0
+
+
+@functools.lru_cache(maxsize=None)
+def _few_places(dev: int, dh: int, bits8: bool, rows: int) -> "tuple[int, ...]":
+    """Blocks of ``attention_few`` that the (current) device holds at once, by the number of ranges."""
+    return tuple(library("attention_few").jlx_attention_few_places(c_int(dh), c_int(int(bits8)), c_int(rows), c_int(s)) for s in ROWS_SPLITS)
 
 
 def _rows_tc_plan(tiles: int, units: int, rows: int, sms: int) -> "tuple[int, int]":
@@ -1280,7 +1292,7 @@ def _rows_tc_plan(tiles: int, units: int, rows: int, sms: int) -> "tuple[int, in
         if b - 128 >= rows:
             continue
         full, rest = divmod(rows, b)
-        for s in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48):
+        for s in ROWS_SPLITS:
             if s > tiles:
                 break
             blocks, range_ = units * s * (full + (rest > 0)), -(-tiles // s)
@@ -1336,7 +1348,8 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     scales_p = _address(scales)
     keys = 0 if scales is None else _keys_seen(max_kv_len, chunk, window, max_count)
     form = attention_rows_form(max_count * (Hq // Hkv), page_size, scales_p % 16 == 0, keys, n_items * Hkv)
-    splits, row_block = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count())
+    places = _few_places(dev, dh, scales is not None, 8 if max_count * (Hq // Hkv) <= 8 else ROWS_FEW) if form == "attention_few" else None
+    splits, row_block = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count(), places)
     part_o = part_ml = joined = 0
     if splits > (ROWS_CLUSTER if form == "attention_few" else 1):
         # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
