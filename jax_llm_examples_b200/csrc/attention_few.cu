@@ -1,5 +1,5 @@
-// Grouped-query attention of up to 16 query rows of an item and KV head over the paged cache, held in bfloat16 or in 8 bits:
-// single decoded tokens and small drafted trees (attention_rows.cuh has mask and formula), head sizes 64 and 128.  It reads
+// Grouped-query attention of up to 16 query rows a block of an item and KV head over the paged cache, held in bfloat16 or in 8
+// bits: single decoded tokens and small drafted trees (attention_rows.cuh has mask and formula), head sizes 64 and 128.  It reads
 // every key once and computes little with it: bytes bound it, and the instructions that stand between a byte and a product.
 //
 // A block takes one range of an item's keys, in tiles of 64: a warp of its own fetches them up to STAGES tiles ahead, by TMA
@@ -34,8 +34,8 @@
 // and each reads its share of the others' there, no second kernel and no scratch.  More ranges than that go through scratch.
 //
 // What bounds it: in long caches the instructions between a byte and a product (a tile's 280 a warp), in short ones a block's way to its first tile (page, position, key: 2 us) and the launch.  Measured
-// (B200, 40 heads on 8 of 128, 8 bits): 64 requests of up to 8,192 keys 162 us, 5.06 TB/s, 77 % of the copy rate; 8 of up to
-// 30,000 81 us, 4.87 TB/s; one of 700 14 us with its call, 8.4 on the device.
+// (B200, 40 heads on 8 of 128, 8 bits): 64 requests of up to 8,192 keys 156 us, 5.25 TB/s, 80 % of the copy rate; 8 of up to
+// 30,000 79 us, 4.99 TB/s; one of 700 13 us with its call, 8.4 on the device.
 // Tried and slower: 8-bit score products (the conversion of queries' remainders costs more than the codes'), a reference taken
 // from the tile before with a second pass where it fails, exponentials by a polynomial.
 #include <cooperative_groups.h>

@@ -28,8 +28,7 @@
 //
 // Pages that hold no whole boxes of 16 rows, and scales that start off a 16-byte boundary, come here; the rest goes to the
 // tcgen05 kernel, which is 1.6 to 5.7 times as fast.  Measured (B200, pages of 24): 2,048 tokens after 1,500, 40 heads on 8 of 128,
-// 8 bits: 1,089 us, 97 TFLOP/s (188 us there); trees of 32 tokens on 8 requests, bfloat16: 448 us (89); of 8 on one request: 27 us
-// (17.5).  Its mma.sync products and the conversion of codes in every warp bound it.
+// 8 bits: 1,089 us, 97 TFLOP/s (188 us there); trees of 32 tokens on 8 requests, bfloat16: 448 us (89).  Its mma.sync products and the conversion of codes in every warp bound it.
 #include "attention_rows.cuh"
 #include "mbarrier.cuh"
 #include "mma_sync.cuh"

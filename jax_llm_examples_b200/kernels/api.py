@@ -1228,15 +1228,16 @@ def attention_rows_supported(q_dtype: torch.dtype, Hq: int, Hkv: int, dh: int) -
     return q_dtype == torch.bfloat16 and dh in (64, 128) and Hkv > 0 and Hq % Hkv == 0
 
 
-def attention_rows_form(rows: int, page_size: int, aligned: bool, keys: int = 0, units: int = 0) -> str:
-    """The kernel for items of up to so many query rows of a KV head ((token, head of the group) pairs).  ``keys``, ``units``: of a
-    cache in 8 bits, the keys that an item sees and the (item, KV head) pairs.
+def attention_rows_form(rows: int, page_size: int, aligned: bool, keys: int = 0, units: int = 0, bits8: bool = False) -> str:
+    """The kernel for items of up to so many query rows of a KV head ((token, head of the group) pairs).  ``keys``, ``units``: the
+    keys that an item sees and the (item, KV head) pairs.
 
-    Few items of up to 64 rows take ``attention_few`` in groups of 16 as long as those are at most 32: its way to the first tile
-    and its join are shorter than the tcgen05 kernel's.  (8 bits, 40 heads on 8 of 128, a tree of 8 on one request, 24 groups: 12.7
-    us for 19.0 at 900 keys, 19.1 for 24.9 at 5,000, but 35.3 for 25.1 at 8,000; on two requests, 48 groups: 21.3 for 19.0.  Over
-    a bfloat16 cache 24 groups take 21.0 for 18.0.)"""
-    if rows <= ROWS_FEW or (rows <= 4 * ROWS_FEW and 0 < keys <= 5120 and units * -(-rows // ROWS_FEW) <= 32):
+    Items of up to 64 rows take ``attention_few`` in groups of 16 while groups times keys are few: its way to the first tile and
+    its join are shorter than the tcgen05 kernel's, but each group fetches the keys anew.  (40 heads on 8 of 128, trees of 8.  8
+    bits: one request, 24 groups, 12.7 us for 19.0 at 900 keys, 19.1 for 24.9 at 5,000; four requests, 96 groups, 17.7 for 20.8 at
+    1,000, 39.4 for 31.0 at 4,000.  A bfloat16 cache: 12.8 for 18.9 and 19.1 for 23.1; 18.9 for 18.8 and 35.8 for 29.0.)"""
+    groups = units * -(-rows // ROWS_FEW)
+    if rows <= ROWS_FEW or (rows <= 4 * ROWS_FEW and 0 < keys <= 5120 and groups * keys <= (262144 if bits8 else 163840)):
         return "attention_few"
     return "attention_rows_tc" if page_size % 16 == 0 and aligned else "attention_rows"
 
@@ -1346,8 +1347,8 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
         raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
     scales_p = _address(scales)
-    keys = 0 if scales is None else _keys_seen(max_kv_len, chunk, window, max_count)
-    form = attention_rows_form(max_count * (Hq // Hkv), page_size, scales_p % 16 == 0, keys, n_items * Hkv)
+    keys = _keys_seen(max_kv_len, chunk, window, max_count)
+    form = attention_rows_form(max_count * (Hq // Hkv), page_size, scales_p % 16 == 0, keys, n_items * Hkv, scales is not None)
     places = _few_places(dev, dh, scales is not None, 8 if max_count * (Hq // Hkv) <= 8 else ROWS_FEW) if form == "attention_few" else None
     splits, row_block = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count(), places)
     part_o = part_ml = joined = 0
