@@ -27,8 +27,9 @@
 // that do see it at the end (a product would spread 0 * infinity over all rows).  In 8 bits only a row's scale can say NaN.
 //
 // Pages that hold no whole boxes of 16 rows, and scales that start off a 16-byte boundary, come here; the rest goes to the
-// tcgen05 kernel, which is 1.6 to 5.7 times as fast.  Measured (B200, pages of 24): 2,048 tokens after 1,500, 40 heads on 8 of 128,
-// 8 bits: 1,089 us, 97 TFLOP/s (188 us there); trees of 32 tokens on 8 requests, bfloat16: 448 us (89).  Its mma.sync products and the conversion of codes in every warp bound it.
+// tcgen05 kernel, which is up to 5.7 times as fast.  Measured (B200, pages of 24): 2,048 tokens after 1,500, 40 heads on 8 of 128,
+// 8 bits: 1,089 us, 97 TFLOP/s (188 us there); trees of 32 tokens on 8 requests, bfloat16: 448 us (89).  Its mma.sync products and
+// the conversion of codes in every warp bound it.
 #include "attention_rows.cuh"
 #include "mbarrier.cuh"
 #include "mma_sync.cuh"
