@@ -255,7 +255,9 @@ rope_kv_store_fp8_kernel(const TI* __restrict__ qkv, int splits, long long split
         for (int o = 16; o > 0; o >>= 1)
           if (o < P.lanes) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (!is_v) {
-          const float inv = rsqrtf(fmaf(ss, per_entry, eps));
+          // (a Newton step on the reciprocal root, which is off by two units otherwise: fewer entries cross a rounding border)
+          const float mean = fmaf(ss, per_entry, eps), root = rsqrtf(mean), step = fmaf(-mean * root, root, 1.f);
+          const float inv = fabsf(step) < 1.f ? fmaf(0.5f * root, step, root) : root;  // (not of an infinite sum)
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] *= inv;
         }
