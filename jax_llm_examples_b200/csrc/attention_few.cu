@@ -348,6 +348,8 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
           }
         }
         if (any) any_bad = 1;
+        // (the stage's next copies are writes of the asynchronous proxy: these stores have to be ordered before them, too)
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
       // ---- S^T: two keys (g, g + 8) x two rows per thread and group; two chains of products

@@ -1,0 +1,84 @@
+"""The 8-bit cache and the attention over rows at the ends of their format and their calls, against 64 bits (fp8_helpers.py)."""
+
+import math
+
+import pytest
+import torch
+
+from .fp8_helpers import Case, assert_close, hold
+
+pytestmark = pytest.mark.gpu
+
+
+def K():
+    from jax_llm_examples_b200.kernels import api
+
+    return api
+
+
+FORMS = ["rule", "attention_rows", "attention_rows_tc", "attention_few"]  # the kernel by the sizes, or the one named
+
+
+@pytest.fixture
+def form(request, monkeypatch):
+    if request.param != "rule":
+        monkeypatch.setattr(K(), "attention_rows_form", lambda *a: request.param)
+    return request.param
+
+
+def _call(c, mask=None, items=None, out=None, rows=None, **kw):
+    """The causal call over 8 bits or, where the case is a tree, the tree's, with the case's bound for the kernel that serves it."""
+    mask, out = mask or {}, torch.full_like(c.q, 7.0) if out is None else out
+    keys = max(a + b for a, b in zip(c.n, c.held))
+    most = items[2] if items is not None else 1
+    n_items = items[1] if items is not None else (rows.numel() if rows is not None else c.N)
+    seen = K()._keys_seen(keys, mask.get("chunk", 0), mask.get("window", 0), most)
+    aligned = c.scales is None or c.scales.data_ptr() % 16 == 0
+    kernel = K().attention_rows_form(most * (c.Hq // c.Hkv), c.page, aligned, seen, n_items * c.Hkv, c.bits8)
+    c.weights = 2.0 ** -11 if c.bits8 and kernel != "attention_rows_tc" else 2.0 ** -8
+    how = (c.scale, mask.get("chunk", 0), mask.get("window", 0), mask.get("temper", 0.0), mask.get("floor", 1.0), c.status, keys)
+    if c.masks is not None:
+        items = items or c.items(max(c.n))
+        K().attention_tree(c.q, c.pages, c.table, c.req, c.positions, c.cu_q, c.q_start, c.masks, out, *how, *items, scales=c.scales, **kw)
+    else:
+        if items is not None:
+            kw |= dict(items=items[0], n_items=items[1], max_count=items[2])
+        if rows is not None:
+            kw |= dict(rows=rows, n_rows=rows.numel())
+        K().attention_fp8(c.q, c.pages, c.scales, c.table, c.req, c.positions, out, *how, **kw)
+    return out
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("mask", [dict(window=70), dict(window=901), dict(chunk=1000), dict(window=3000)])
+def test_a_masked_first_tile_and_the_tiles_after_it(mask, dh, page):
+    """The first tile's stage, with what lies before the window taken out of it, is filled again: large values stand there."""
+    c = Case([1, 1, 1], [4010, 2999, 3333], 8, 2, dh, page)
+    for r in range(3):
+        p = c.held[r]
+        lo = max(p - p % mask["chunk"] if "chunk" in mask else 0, p - mask["window"] + 1 if "window" in mask else 0)
+        before = torch.arange(max(lo - 64, 0), lo)
+        pages = c.table[r, before // page].long()
+        c.pages.view(torch.uint8)[pages, :, :, before % page] = 0x7e  # 448
+        c.scales[pages, :, :, before % page] = 127 + 60
+    c.to_device()
+    want, tol = c.want(**mask)
+    first = _call(c, mask)
+    assert_close(first, want, tol)
+    for _ in range(20):
+        assert torch.equal(_call(c, mask), first)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_a_masked_first_tile_of_a_bfloat16_cache(page):
+    c = Case([3, 2], [3001, 2600], 8, 2, 128, page, bits8=False).tree()
+    for r in range(2):
+        before = torch.arange(c.held[r] - 900 - 64, c.held[r] - 900)
+        c.pages[c.table[r, before // page].long(), :, :, before % page] = math.inf
+    c.to_device()
+    want, tol = c.want(window=900)
+    first = _call(c, dict(window=900))
+    assert_close(first, want, tol)
+    for _ in range(20):
+        assert torch.equal(_call(c, dict(window=900)), first)
