@@ -17,7 +17,7 @@
 #include "common.cuh"
 
 #define FP8_MIN_EXP (-60)
-#define FP8_LIMIT 5.1650969690842e20f  // 448 * 2^60
+#define FP8_LIMIT 0x1.cp68f  // 448 * 2^60, to the last bit
 #define FP8_BAD 255
 
 // 2^e for -126 <= e <= 127

@@ -23,3 +23,12 @@ def test_values_changed_in_a_stage_are_fenced_before_it_is_filled_again(name, st
     at = code.index(stores)
     between = code[at:code.index(release, at)]
     assert "fence.proxy.async" in between or "fence_async_proxy()" in between
+
+
+def test_the_largest_row_that_is_held_is_448_times_2_to_the_60():
+    """The kernels' limit is the format's: 448 * 2^60, to the last bit of a 32-bit number."""
+    import numpy as np
+
+    text = re.search(r"#define FP8_LIMIT (\S+?)f\s", (CSRC / "fp8_rows.cuh").read_text() + "\n").group(1)
+    value = float.fromhex(text) if text.lower().startswith("0x") else float(text)
+    assert np.float32(value) == np.float32(448 * 2.0 ** 60)

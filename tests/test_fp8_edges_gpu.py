@@ -82,3 +82,25 @@ def test_a_masked_first_tile_of_a_bfloat16_cache(page):
     assert_close(first, want, tol)
     for _ in range(20):
         assert torch.equal(_call(c, dict(window=900)), first)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_at_the_largest_scale_and_one_step_above(dtype):
+    """448 * 2^60 is held, the next number of the type is not, nor is what lies just above the limit."""
+    limit = 448 * 2.0 ** 60
+    step = torch.finfo(dtype).eps * 2.0 ** 68  # (448 * 2^60 lies in [2^68, 2^69))
+    tops = [limit, limit + step, limit + 2 * step, limit + 20 * step, limit - step, 2.0 * limit, -limit, -limit - step]
+    c = Case([len(tops)], [2], 2, 2, 64, 16).to_device()
+    k, v = torch.randn(len(tops), 2, 64, dtype=torch.float64), torch.randn(len(tops), 2, 64, dtype=torch.float64)
+    for i, top in enumerate(tops):
+        k[i, 0, 7], v[i, 1, 63] = top, -top
+    k, v = k.to(dtype), v.to(dtype)
+    assert float(k[1, 0, 7]) > limit and float(k[0, 0, 7]) == limit
+    K().kv_store_fp8(k.cuda(), v.cuda(), c.pages, c.scales, c.table, c.req, c.places, c.status)
+    _, want = hold(torch.stack([k, v], 1))
+    assert torch.equal(c.scales[c.table[0, 0].long()][:, :, 2:2 + len(tops)].permute(2, 0, 1).cpu(), want)
+    ko, vo = torch.empty_like(k, device="cuda"), torch.empty_like(v, device="cuda")
+    K().kv_load_fp8(c.pages, c.scales, c.table, c.req, c.places, ko, vo, c.status)
+    for got, x in ((ko, k), (vo, v)):
+        x, _ = hold(x)
+        assert torch.equal(torch.isnan(got).cpu(), torch.isnan(x)) and torch.equal(torch.nan_to_num(got.cpu().double()), torch.nan_to_num(x))
