@@ -386,7 +386,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
       float ks0 = 1.f, ks1 = 1.f, ve0 = 0.f, ve1 = 0.f, vi0 = 1.f, vi1 = 1.f;  // keys' scales; values' exponents and 2^-exponent
       if (F8) {
         const uint8_t* sp = scales_of(st) + kg;
-        const int bk0 = sp[0], bk1 = sp[8], bv0 = sp[KT], bv1 = sp[KT + 8];
+        const int bk0 = sp[0], bk1 = sp[8], bv0 = fp8_weight_byte(sp[KT]), bv1 = fp8_weight_byte(sp[KT + 8]);
         ks0 = fp8_scale(bk0);
         ks1 = fp8_scale(bk1);
         ve0 = bv0 == FP8_BAD ? __int_as_float(0x7fc00000) : (float)(bv0 - 127);

@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
       sc[tid] = fp8_scale(byte);
     } else {
       const bool bad = byte == FP8_BAD;
-      const int e = byte == 0 ? 0 : byte - 127;
+      const int e = fp8_weight_byte(byte) - 127;
       sc[tid] = bad ? __int_as_float(0x7fc00000) : (float)e;
       sc[tid + KT] = bad ? 1.f : fp8_pow2(max(-60, min(60, -e)));
     }

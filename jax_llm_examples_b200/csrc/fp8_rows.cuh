@@ -29,8 +29,12 @@ __device__ __forceinline__ int fp8_row_exp(float amax) {
   return max((int)(b >> 23) - 127 - 8 + ((b & 0x7fffff) > 0x600000), FP8_MIN_EXP);
 }
 
-// What a scale byte stands for (255: NaN).  Byte 0, a row that was never written, gives 0.
+// What a scale byte stands for (255: NaN).  Byte 0, a row that was never written (no row is kept with it; its codes are 0), gives 0.
 __device__ __forceinline__ float fp8_scale(int byte) { return byte == FP8_BAD ? __int_as_float(0x7fc00000) : __int_as_float(byte << 23); }
+// The byte whose exponent goes into the weights of the values: a row that was never written is one of zeros, which is kept with
+// the smallest scale.  (With 2^-127 its weight would leave the 32-bit range and its share of the softmax's sum be lost, with 2^0
+// it could set the reference of rows that hold far smaller values.)
+__device__ __forceinline__ int fp8_weight_byte(int byte) { return byte == 0 ? FP8_MIN_EXP + 127 : byte; }
 
 // Four codes -> two pairs of float16 (exact: float16 holds every e4m3 number).
 __device__ __forceinline__ void fp8x4_to_half(uint32_t codes, uint32_t& lo, uint32_t& hi) {

@@ -104,3 +104,23 @@ def test_rows_at_the_largest_scale_and_one_step_above(dtype):
     for got, x in ((ko, k), (vo, v)):
         x, _ = hold(x)
         assert torch.equal(torch.isnan(got).cpu(), torch.isnan(x)) and torch.equal(torch.nan_to_num(got.cpu().double()), torch.nan_to_num(x))
+
+
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("n", [1, 3, 40])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 14, 2.0 ** -50])
+def test_keys_that_were_never_written_count_as_zeros(form, n, size):
+    """Scale byte 0, as the cache begins: a key of zeros, whose score is 0, and a value of zeros, in the sum like any other, whatever
+    the scales of the values beside it."""
+    c = Case([n], [300], 4, 2, 128, 16)
+    c.rows[:, 1] *= size
+    c.rows, scales = hold(c.rows)
+    c.set_rows8(scales)
+    for place in range(3, 300, 5):
+        page, at = int(c.table[0, place // 16]), place % 16
+        c.rows[page, :, :, at] = 0.0
+        c.pages.view(torch.uint8)[page, :, :, at] = 0
+        c.scales[page, :, :, at] = 0
+    c.q *= 0.02  # scores close to each other: every key has its share of the sum
+    c.to_device()
+    assert_close(_call(c, items=c.items(n)), *c.want())
