@@ -1,4 +1,4 @@
-// What the two kernels of attention over rows (attention_rows.cu, attention_rows_tc.cu) share.
+// What the three kernels of attention over rows (attention_few.cu, attention_rows.cu, attention_rows_tc.cu) share.
 //
 // A work item is a stretch of a request's tokens; its query rows are (token, head of the KV head's group) pairs, token by
 // token, row r = token * G + head: a tile of rows packs a few tokens' heads, so that one read of a key serves all of them.
@@ -124,11 +124,17 @@ __device__ __forceinline__ bool rows_sees(const RowsParams& P, const RowsItem& i
   return ((P.masks[(size_t)n * P.words + (j >> 5)] >> (j & 31)) & 1) && key_pos >= lo;
 }
 
+// Keys whose page the table does not name (below 0, or beyond the pool) raise the status where some row sees them, and are keys
+// and values of zeros in every kernel: rows_cache_row says -1, a TMA box starts behind the cache's last row, where all it brings is
+// zeros, and the scales' bytes are 0.
+__device__ __forceinline__ bool rows_page_there(const RowsParams& P, int page) { return page >= 0 && page < P.num_pages; }
+__device__ __forceinline__ int rows_behind(const RowsParams& P) { return P.num_pages * 2 * P.Hkv * P.page_size; }  // (fits: the launcher looks)
+
 // The flat row of the key at `place` in the cache (values: Hkv * page_size further), or -1.
 __device__ __forceinline__ int rows_cache_row(const RowsParams& P, const int* table, int hk, int place) {
   const int pi = place / P.page_size;
   const int page = pi < P.bt_stride ? table[pi] : -1;
-  if (page < 0 || page >= P.num_pages) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return -1; }
+  if (!rows_page_there(P, page)) { atomicOr(P.status, JLX_STATUS_BAD_PAGE); return -1; }
   return (page * 2 * P.Hkv + hk) * P.page_size + (place - pi * P.page_size);
 }
 

@@ -37,7 +37,7 @@
 //
 // Masks: only tiles that some row does not see wholly look at them.  In such a tile a value that is not finite is taken out
 // (a product would spread 0 * infinity over all rows) and added to the rows that do see it at the end; of rows of the cache
-// outside the range only zeros reach a product.
+// outside the range finite numbers reach a product at most, with weights of zero (8 bits: zeros).
 //
 // Every wait on a barrier is bounded; after a timeout the block raises JLX_STATUS_WAIT_TIMEOUT, waits (bounded) for its own
 // copies, frees its tensor memory and returns.
@@ -311,11 +311,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     bool ok = true;
     for (; t < n_tiles; ++t) {
       const int place = range0 + t * BKV + lane * box_rows, st = t % stages;
-      if (page < 0 || page >= P.num_pages) {
-        if (lane < boxes && place < end && place + box_rows > begin) atomicOr(P.status, JLX_STATUS_BAD_PAGE);
-        page = 0;  // no page there: every key of the box is masked
-      }
-      const int row = (page * 2 * P.Hkv + hk) * P.page_size + place % P.page_size + off;
+      const bool there = rows_page_there(P, page);
+      if (!there && lane < boxes && place < end && place + box_rows > begin) atomicOr(P.status, JLX_STATUS_BAD_PAGE);
+      const int row = there ? (page * 2 * P.Hkv + hk) * P.page_size + place % P.page_size + off : rows_behind(P);
       page = page_next;
       page_next = find_page(t + 2);
       if (t >= stages) ok = mbar_wait(BAR((which ? (F8 ? B_RAWEMPTY : B_VEMPTY) : B_KEMPTY) + st), (t / stages - 1) & 1);
@@ -403,7 +401,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     };
     auto fetch = [&](int t, int page, uint32_t& k, uint32_t& v) {
       const int place = range0 + t * BKV + lane * 4;
-      const uint8_t* src = P.scales + (size_t)(((page < 0 || page >= P.num_pages ? 0 : page) * 2 * P.Hkv + hk) * P.page_size + place % P.page_size);
+      k = v = 0u;
+      if (!rows_page_there(P, page)) return;
+      const uint8_t* src = P.scales + (size_t)((page * 2 * P.Hkv + hk) * P.page_size + place % P.page_size);
       k = *reinterpret_cast<const uint32_t*>(src);
       v = *reinterpret_cast<const uint32_t*>(src + v_off);
     };

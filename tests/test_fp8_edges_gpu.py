@@ -26,19 +26,27 @@ def form(request, monkeypatch):
     return request.param
 
 
-def _call(c, mask=None, items=None, out=None, rows=None, **kw):
-    """The causal call over 8 bits or, where the case is a tree, the tree's, with the case's bound for the kernel that serves it."""
-    mask, out = mask or {}, torch.full_like(c.q, 7.0) if out is None else out
-    keys = max(a + b for a, b in zip(c.n, c.held))
+def _serve(c, mask=None, items=None, rows=None):
+    """Holds the case to the bound of the kernel that serves these items (to be called before the case is asked for it)."""
+    mask = mask or {}
+    if c.masks is not None:
+        items = items or c.items(max(c.n))
     most = items[2] if items is not None else 1
     n_items = items[1] if items is not None else (rows.numel() if rows is not None else c.N)
-    seen = K()._keys_seen(keys, mask.get("chunk", 0), mask.get("window", 0), most)
+    seen = K()._keys_seen(max(a + b for a, b in zip(c.n, c.held)), mask.get("chunk", 0), mask.get("window", 0), most)
     aligned = c.scales is None or c.scales.data_ptr() % 16 == 0
     kernel = K().attention_rows_form(most * (c.Hq // c.Hkv), c.page, aligned, seen, n_items * c.Hkv, c.bits8)
     c.weights = 2.0 ** -11 if c.bits8 and kernel != "attention_rows_tc" else 2.0 ** -8
-    how = (c.scale, mask.get("chunk", 0), mask.get("window", 0), mask.get("temper", 0.0), mask.get("floor", 1.0), c.status, keys)
+    return items
+
+
+def _call(c, mask=None, items=None, out=None, rows=None, **kw):
+    """The causal call over 8 bits or, where the case is a tree, the tree's."""
+    mask, out = mask or {}, torch.full_like(c.q, 7.0) if out is None else out
+    items = _serve(c, mask, items, rows)
+    how = (c.scale, mask.get("chunk", 0), mask.get("window", 0), mask.get("temper", 0.0), mask.get("floor", 1.0), c.status,
+           max(a + b for a, b in zip(c.n, c.held)))
     if c.masks is not None:
-        items = items or c.items(max(c.n))
         K().attention_tree(c.q, c.pages, c.table, c.req, c.positions, c.cu_q, c.q_start, c.masks, out, *how, *items, scales=c.scales, **kw)
     else:
         if items is not None:
@@ -63,6 +71,7 @@ def test_a_masked_first_tile_and_the_tiles_after_it(mask, dh, page):
         c.pages.view(torch.uint8)[pages, :, :, before % page] = 0x7e  # 448
         c.scales[pages, :, :, before % page] = 127 + 60
     c.to_device()
+    _serve(c, mask)
     want, tol = c.want(**mask)
     first = _call(c, mask)
     assert_close(first, want, tol)
@@ -77,6 +86,7 @@ def test_a_masked_first_tile_of_a_bfloat16_cache(page):
         before = torch.arange(c.held[r] - 900 - 64, c.held[r] - 900)
         c.pages[c.table[r, before // page].long(), :, :, before % page] = math.inf
     c.to_device()
+    _serve(c, dict(window=900))
     want, tol = c.want(window=900)
     first = _call(c, dict(window=900))
     assert_close(first, want, tol)
@@ -124,3 +134,61 @@ def test_keys_that_were_never_written_count_as_zeros(form, n, size):
     c.q *= 0.02  # scores close to each other: every key has its share of the sum
     c.to_device()
     assert_close(_call(c, items=c.items(n)), *c.want())
+
+
+def _with_a_stranger_in_page_0(c):
+    """Page 0 belongs to none of the case's requests, and holds values that would show in any output."""
+    spare = next(p for p in range(1, c.P) if not (c.table == p).any())
+    c.rows[spare] = c.rows[0]
+    c.pages.view(torch.uint8)[spare] = c.pages.view(torch.uint8)[0]
+    c.table[c.table == 0] = spare
+    c.pages[0] = torch.full_like(c.pages[0], 300.0 if c.bits8 else 5e4)
+    if c.bits8:
+        c.scales[spare] = c.scales[0]
+        c.scales[0] = 127 + 12
+    return c
+
+
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("n, page, dh", [(1, 64, 128), (2, 16, 64), (40, 64, 64), (40, 16, 128), (90, 48, 128)])
+@pytest.mark.parametrize("what", ["none", "too high"])
+def test_a_missing_page_counts_as_keys_of_zeros(form, what, n, page, dh, bits8):
+    """A request whose table names no page for some of its keys: the status says so, zeros stand in for them in every kernel, and no
+    other request's rows enter its output."""
+    c = _with_a_stranger_in_page_0(Case([n, n], [700, 333], 4, 2, dh, page, bits8=bits8).tree())
+    for entry in (0, 300 // page, 640 // page):
+        c.rows[int(c.table[0, entry])] = 0.0
+    _serve(c)
+    want, tol = c.want()
+    for entry in (0, 300 // page, 640 // page):
+        c.table[0, entry] = -1 if what == "none" else c.P + entry
+    c.to_device()
+    assert_close(_call(c), want, tol)
+    assert int(c.status) == 1
+    if bits8:
+        c.masks = None
+        c.positions = c.places.clone()
+        c.status.zero_()
+        table, c.table = c.table, c.table.clamp(0, c.P - 1)
+        for entry in (0, 300 // page, 640 // page):  # (the oracle reads them as zeros: from a page of its own)
+            c.table[0, entry] = 0
+        c.rows[0] = 0.0
+        _serve(c, items=c.items(n))
+        want, tol = c.want()
+        c.table = table
+        assert_close(_call(c, items=c.items(n)), want, tol)
+        assert int(c.status) == 1
+
+
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("n, page", [(1, 64), (3, 16), (60, 32)])
+def test_pages_given_back_behind_a_window_are_not_asked_for(form, n, page, bits8):
+    c = _with_a_stranger_in_page_0(Case([n], [2000], 4, 2, 128, page, bits8=bits8).tree())
+    _serve(c, dict(window=700))
+    want, tol = c.want(window=700)
+    c.table[0, :(2000 - 700 + 1) // page] = -1
+    c.to_device()
+    assert_close(_call(c, dict(window=700)), want, tol)
+    assert int(c.status) == 0
