@@ -572,7 +572,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
       *reinterpret_cast<float4*>(merged + (size_t)row * T::LD + d) = acc;
       if (d == 0) merged_ml[row] = make_float2(mm, ll);
     } else {
-      const size_t at = (size_t)k.x * P.Hq + k.y;
+      const size_t at = rows_part_token(P, item_i, k.x, it.n0) * P.Hq + k.y;
       *reinterpret_cast<float4*>(P.part_o + (at * P.splits + split) * DH + d) = acc;
       if (d == 0) P.part_ml[at * P.splits + split] = make_float2(mm, ll);
     }

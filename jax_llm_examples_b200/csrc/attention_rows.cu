@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
         if (!isfinite(x[3])) acc.w += x[3];
       }
     }
-    const size_t at = (size_t)tok.x * P.Hq + tok.y;
+    const size_t at = (P.splits > 1 ? rows_part_token(P, item_i, tok.x, it.n0) : (size_t)tok.x) * P.Hq + tok.y;
     if (P.splits > 1) {
       *reinterpret_cast<float4*>(P.part_o + (at * P.splits + split) * DH + d) = acc;
       if (d == 0) P.part_ml[at * P.splits + split] = make_float2(mm, ll);

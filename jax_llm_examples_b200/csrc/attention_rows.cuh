@@ -45,8 +45,9 @@ struct RowsParams {
   const float* sink;       // [Hq] or null
   const float* slopes;     // [Hq] or null
   int splits;              // ranges that an item's keys are cut into
-  float* part_o;           // [N, Hq, splits, DH]: sums of weighted values against the maximum
-  float2* part_ml;         // [N, Hq, splits]: (maximum, sum of weights)
+  int part_items;          // scratch rows are tokens: this many for every item, or (0) the step's N (whichever are fewer)
+  float* part_o;           // [tokens, Hq, splits, DH]: sums of weighted values against the maximum
+  float2* part_ml;         // [tokens, Hq, splits]: (maximum, sum of weights)
   int* status;
 };
 
@@ -150,6 +151,11 @@ __device__ __forceinline__ float rows_inverse(const RowsParams& P, float m, floa
   return l == 0.f ? 0.f : 1.f / l;
 }
 
+// The scratch's token for token row n of an item whose tokens begin at n0.
+__device__ __forceinline__ size_t rows_part_token(const RowsParams& P, int item, int n, int n0) {
+  return P.part_items ? (size_t)item * P.part_items + (n - n0) : (size_t)n;
+}
+
 // Joins the ranges of a row from scratch: a warp per row, DH / 32 entries a lane.
 template <int DH>
 __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowsParams P) {
@@ -161,8 +167,8 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowsPara
   const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
   if (row >= it.cnt * P.Hq) return;
   const int head = row % P.Hq;
-  const size_t at = (size_t)it.n0 * P.Hq + row;
-  const float2* ml = P.part_ml + at * P.splits;
+  const size_t at = (size_t)it.n0 * P.Hq + row, kept = rows_part_token(P, blockIdx.x, it.n0, it.n0) * P.Hq + row;
+  const float2* ml = P.part_ml + kept * P.splits;
   float m = ROWS_NEG_BIG;
   for (int s = lane; s < P.splits; s += 32) m = fmaxf(m, ml[s].x);
   m = warp_max(m);
@@ -170,7 +176,7 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowsPara
   float acc[E], l = 0.f;
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.f;
-  const float* po = P.part_o + at * P.splits * DH + lane * E;
+  const float* po = P.part_o + kept * P.splits * DH + lane * E;
 #pragma unroll 4
   for (int s = 0; s < P.splits; ++s) {
     const float2 x = ml[s];
@@ -186,10 +192,10 @@ __global__ void __launch_bounds__(256) attention_rows_join_kernel(const RowsPara
 }
 
 // -------------------------------------------------------------------------------------------- host
-// What the callers hand over (_RowsArgs in kernels/api.py).
+// What the callers hand over (_ROWS_ARGS in kernels/api.py).
 struct RowsArgs {
   const void *q, *pages, *scales, *block_table, *req_of_token, *positions, *out, *items, *rows, *cu_q, *q_start, *masks, *sink, *slopes, *part_o, *part_ml, *status;
-  int bt_stride, n_requests, n_items, max_count, words, N, Hq, Hkv, dh, page_size, num_pages, chunk, window, splits, row_block;
+  int bt_stride, n_requests, n_items, max_count, words, N, Hq, Hkv, dh, page_size, num_pages, chunk, window, splits, row_block, part_items;
   float scale, softcap, attn_scale, floor_scale;
 };
 
@@ -202,6 +208,7 @@ static int rows_params(const RowsArgs& a, RowsParams& P) {
   JLX_REQUIRE(a.softcap >= 0.f && a.chunk >= 0 && a.window >= 0, "attention: the score cap, chunk and window must not be negative (0: none)");
   JLX_REQUIRE(a.splits >= 1 && a.splits <= 4096, "attention over rows: %d ranges", a.splits);
   JLX_REQUIRE((((uintptr_t)a.part_o & 15) | ((uintptr_t)a.part_ml & 7)) == 0, "attention over rows: scratch for the ranges is not aligned");
+  JLX_REQUIRE(a.part_items == 0 || a.part_items >= a.max_count, "attention over rows: the scratch holds %d tokens an item, of %d", a.part_items, a.max_count);
   JLX_REQUIRE(!a.cu_q == !a.masks && !a.cu_q == !a.q_start && (!a.cu_q || (a.items && a.words > 0)), "attention over rows: a tree needs its offsets, cached lengths, masks and items");
   JLX_REQUIRE((long long)a.max_count * a.Hq < (1ll << 30), "attention over rows: an item has too many rows");
   P.q = (const bf16*)a.q; P.pages = a.pages; P.scales = (const uint8_t*)a.scales; P.block_table = (const int*)a.block_table; P.bt_stride = a.bt_stride;
@@ -212,7 +219,7 @@ static int rows_params(const RowsArgs& a, RowsParams& P) {
   P.cap_log2 = a.softcap > 0.f ? a.softcap * LOG2E : 0.f;
   P.chunk = a.chunk; P.window = a.window; P.attn_scale = a.attn_scale; P.floor_scale = a.floor_scale;
   P.sink = (const float*)a.sink; P.slopes = (const float*)a.slopes; P.splits = a.splits;
-  P.part_o = (float*)a.part_o; P.part_ml = (float2*)a.part_ml; P.status = (int*)a.status;
+  P.part_items = a.part_items; P.part_o = (float*)a.part_o; P.part_ml = (float2*)a.part_ml; P.status = (int*)a.status;
   return 0;
 }
 

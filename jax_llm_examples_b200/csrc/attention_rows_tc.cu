@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
   __shared__ float xmax[2][2][PARTS][BQ];  // [meeting parity][group][part][row]: what the threads of a row exchange
   __shared__ float ends[2][BQ];            // [group][row]: the references at the end
   __shared__ int4 toks[BROWS];          // the rows' tokens: index, position, first key, slope
-  __shared__ int item_s[3];
+  __shared__ int item_s[4];
   __shared__ float q_exp[BROWS];           // 8 bits: the power of two that a query row was divided by
   pdl_launch_dependents_if_small();
   pdl_wait();
@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
     item_s[0] = it.r;
     item_s[1] = it.base;
     item_s[2] = it.drafted;
+    item_s[3] = it.n0;
     span[0] = span[2] = 0x7fffffff;
     span[1] = span[3] = (int)0x80000000;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -618,6 +619,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       it.r = x[0];
       it.base = x[1];
       it.drafted = x[2];
+      it.n0 = x[3];
       return it;
     };
     const bool capped = P.cap_log2 > 0.f, bent = capped || P.slopes;
@@ -800,7 +802,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       const int col_end = col + (by_rows ? T::OC : T::OE);
       const RowsToken tok = token();
       const RowsItem it = item();
-      const size_t at = (size_t)tok.n * P.Hq + tok.head;
+      const size_t at = (P.splits > 1 ? rows_part_token(P, item_i, tok.n, it.n0) : (size_t)tok.n) * P.Hq + tok.head;
       const float inv = P.splits > 1 ? 1.f : rows_inverse(P, m, total, tok.head);
       if (P.splits > 1 && col == 0 && block_row < n_rows) P.part_ml[at * P.splits + split] = make_float2(m, total);
 #pragma unroll 1

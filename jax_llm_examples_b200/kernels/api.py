@@ -1215,10 +1215,11 @@ def kv_load_fp8(pages: torch.Tensor, scales: torch.Tensor, block_table: torch.Te
     _run("kv_fp8", "jlx_kv_load_fp8", args, c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), code(k.dtype), _raw_stream(dev))
 
 
-_ROWS_ARGS = struct.Struct("@17P15i4f")  # RowsArgs in csrc/attention_rows.cuh
+_ROWS_ARGS = struct.Struct("@17P16i4f")  # RowsArgs in csrc/attention_rows.cuh
 ROWS_TILE = 64  # keys of a tile, csrc/attention_rows.cu and attention_few.cu
 ROWS_FEW = 16  # query rows of an item and KV head that attention_few.cu takes
 ROWS_CLUSTER = 8  # ranges that it joins without scratch
+ROWS_SCRATCH = 256 << 20  # bytes that the ranges of a call may take: many rows fill the device without ranges
 ROWS_SPLITS = (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48)  # numbers of ranges to choose from
 _ROWS_LAUNCHERS = {form: "jlx_" + form for form in ("attention_few", "attention_rows", "attention_rows_tc")}
 
@@ -1248,9 +1249,10 @@ def _keys_seen(max_kv_len: int, chunk: int, window: int, max_count: int) -> int:
 
 @functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
 def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_items: int, max_count: int, Hq: int, Hkv: int, sms: int,
-                        places: "tuple[int, ...] | None" = None) -> "tuple[int, int]":
+                        places: "tuple[int, ...] | None" = None, most: int = 1 << 30) -> "tuple[int, int]":
     """(Ranges that an item's keys are cut into: equal ones, of the item's own keys; query rows of a block of ``attention_rows_tc``.)
-    ``places``: blocks of ``attention_few`` that the device holds at once, for each of ROWS_SPLITS (None: three a multiprocessor)."""
+    ``places``: blocks of ``attention_few`` that the device holds at once, for each of ROWS_SPLITS (None: three a multiprocessor).
+    ``most``: ranges that there is scratch for, where they are joined through it."""
     seen = _keys_seen(max_kv_len, chunk, window, max_count) + ROWS_TILE  # ranges start at a tile's first key
     rows = max_count * (Hq // Hkv)
     if form == "attention_few":
@@ -1262,7 +1264,7 @@ def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_i
         blocks, tiles, block, join, share = n_items * Hkv * -(-rows // ROWS_FEW), -(-seen // ROWS_TILE), 10, 6, 8
         places = places or (3 * sms,) * len(ROWS_SPLITS)
     elif form == "attention_rows_tc":
-        return _rows_tc_plan(-(-seen // 128), n_items * Hkv, rows, sms)
+        return _rows_tc_plan(-(-seen // 128), n_items * Hkv, rows, sms, most)
     else:
         blocks, tiles, block, join, share = n_items * Hkv * -(-rows // (32 if rows <= 32 else 64)), -(-seen // ROWS_TILE), 4, 3, 8
         places = (2 * sms,) * len(ROWS_SPLITS)
@@ -1270,7 +1272,7 @@ def attention_rows_plan(form: str, max_kv_len: int, chunk: int, window: int, n_i
     for s, held in zip(ROWS_SPLITS, places):
         joined = s > (ROWS_CLUSTER if form == "attention_few" else 1)
         cost = -(-blocks * s // held) * (-(-tiles // s) + block) + (join + s // share if joined else 0)
-        if s <= tiles and cost < least:
+        if s <= tiles and cost < least and not (joined and s > most):
             splits, least = s, cost
     return splits, 0
 
@@ -1281,7 +1283,7 @@ def _few_places(dev: int, dh: int, bits8: bool, rows: int) -> "tuple[int, ...]":
     return tuple(library("attention_few").jlx_attention_few_places(c_int(dh), c_int(int(bits8)), c_int(rows), c_int(s)) for s in ROWS_SPLITS)
 
 
-def _rows_tc_plan(tiles: int, units: int, rows: int, sms: int) -> "tuple[int, int]":
+def _rows_tc_plan(tiles: int, units: int, rows: int, sms: int, most: int) -> "tuple[int, int]":
     """(Ranges, rows of a block: 128 or 256) for `units` (item, KV head) pairs of `rows` query rows over `tiles` tiles of keys: the
     pair with the least time, in tiles of 128 rows.  A tile of 256 rows takes 1.9; a block takes 4 besides its tiles, a join 4 and
     one for 4 ranges.  A multiprocessor holds one block: up to two rounds of them take as long as their longest, more of them as
@@ -1294,7 +1296,7 @@ def _rows_tc_plan(tiles: int, units: int, rows: int, sms: int) -> "tuple[int, in
             continue
         full, rest = divmod(rows, b)
         for s in ROWS_SPLITS:
-            if s > tiles:
+            if s > min(tiles, max(most, 1)):
                 break
             blocks, range_ = units * s * (full + (rest > 0)), -(-tiles // s)
             if blocks <= 2 * sms:
@@ -1350,17 +1352,19 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     keys = _keys_seen(max_kv_len, chunk, window, max_count)
     form = attention_rows_form(max_count * (Hq // Hkv), page_size, scales_p % 16 == 0, keys, n_items * Hkv, scales is not None)
     places = _few_places(dev, dh, scales is not None, 8 if max_count * (Hq // Hkv) <= 8 else ROWS_FEW) if form == "attention_few" else None
-    splits, row_block = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count(), places)
+    tokens = min(N, n_items * max_count)  # in the scratch: those of every item, or the step's
+    most = min(ROWS_SPLITS[-1], ROWS_SCRATCH // (tokens * Hq * (dh + 2) * 4))
+    splits, row_block = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count(), places, most)
     part_o = part_ml = joined = 0
     if splits > (ROWS_CLUSTER if form == "attention_few" else 1):
         # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
-        scratch = torch.empty(N * Hq * splits * (dh + 2), dtype=torch.float32, device=q.device)
+        scratch = torch.empty(tokens * Hq * splits * (dh + 2), dtype=torch.float32, device=q.device)
         part_o = scratch.data_ptr()
-        part_ml, joined = part_o + 4 * N * Hq * splits * dh, 1
+        part_ml, joined = part_o + 4 * tokens * Hq * splits * dh, 1
     args = _ROWS_ARGS.pack(q_p, pages.data_ptr(), scales_p, block_table.data_ptr(), req_of_token.data_ptr(), positions.data_ptr(), out_p,
                            _address(items), _address(rows), cu_q_p, q_start_p, masks_p, _address(sink), _address(slopes),
                            part_o, part_ml, status.data_ptr(), width, R, n_items, max_count, words, N, Hq, Hkv, dh, page_size, P, chunk, window, splits,
-                           row_block, scale, softcap, attn_scale, floor_scale)
+                           row_block, max_count if tokens < N else 0, scale, softcap, attn_scale, floor_scale)
     _run(form, _ROWS_LAUNCHERS[form], args, _raw_stream(dev))
     global _launches
     _launches += joined  # the joining kernel

@@ -32,3 +32,45 @@ def test_the_largest_row_that_is_held_is_448_times_2_to_the_60():
     text = re.search(r"#define FP8_LIMIT (\S+?)f\s", (CSRC / "fp8_rows.cuh").read_text() + "\n").group(1)
     value = float.fromhex(text) if text.lower().startswith("0x") else float(text)
     assert np.float32(value) == np.float32(448 * 2.0 ** 60)
+
+
+# (kept heads, rows of a step, its items or single rows, keys of the longest request)
+SCRATCH = [
+    # one decoded token behind a long context beside a prompt's portion
+    (40, 8, 128, 2049, dict(rows=1), 30000), (40, 8, 128, 8193, dict(rows=1), 131072), (16, 2, 64, 2050, dict(rows=2), 131072),
+    # short portions beside a long one, and drafted trees of one request out of many tokens
+    (40, 8, 128, 2100, dict(items=3, most=16), 30000), (32, 8, 128, 5000, dict(items=1, most=64), 131072),
+    # one list of portions of very different lengths, sized by the longest
+    (40, 8, 128, 2250, dict(items=101, most=2048), 30000),
+    # portions of many rows a KV head, whole
+    (64, 1, 128, 8192, dict(items=1, most=8192), 131072), (64, 1, 64, 16384, dict(items=1, most=16384), 131072), (40, 8, 128, 8192, dict(items=64, most=128), 8192),
+]
+
+
+@pytest.mark.parametrize("page", [64, 24])
+@pytest.mark.parametrize("Hq, Hkv, dh, N, served, keys", SCRATCH)
+def test_scratch_for_ranges_is_sized_by_the_rows_that_a_call_serves_and_bounded(monkeypatch, Hq, Hkv, dh, N, served, keys, page):
+    import torch
+
+    from jax_llm_examples_b200.kernels import api as K
+
+    asked, ran = [], []
+    monkeypatch.setattr(K, "_placed", lambda *a: 0)
+    monkeypatch.setattr(K, "_raw_stream", lambda dev: None)
+    monkeypatch.setattr(K, "sm_count", lambda: 148)
+    monkeypatch.setattr(K, "_few_places", lambda *a: (444,) * len(K.ROWS_SPLITS))
+    monkeypatch.setattr(K, "_run", lambda lib, fn, args, stream: ran.append(K._ROWS_ARGS.unpack(args)))
+    q = torch.zeros((N, Hq, dh), dtype=torch.bfloat16)
+    pages = torch.zeros((2, 2, Hkv, page, dh), dtype=torch.uint8).view(K.FP8)
+    ints = torch.zeros(N, dtype=torch.int32)
+    items, most = served.get("items", 0), served.get("most", 1)
+    out, pairs = torch.empty_like(q), torch.zeros((items, 2), dtype=torch.int32) if items else None
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda n, **kw: asked.append(n * 4) or empty(0, **kw))
+    K.attention_fp8(q, pages, torch.zeros((2, 2, Hkv, page), dtype=torch.uint8), torch.zeros((1, 2), dtype=torch.int32), ints, ints, out, 1.0, 0, 0, 0.0, 1.0,
+                    torch.zeros(1, dtype=torch.int32), keys, items=pairs, n_items=items, max_count=most, rows=ints if "rows" in served else None,
+                    n_rows=served.get("rows", 0))
+    assert len(ran) == 1
+    rows = min(N, served["rows"] if "rows" in served else items * most)
+    for n in asked:
+        assert n <= 256 << 20 and n <= rows * Hq * max(K.ROWS_SPLITS) * (dh + 2) * 4

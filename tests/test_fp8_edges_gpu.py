@@ -192,3 +192,39 @@ def test_pages_given_back_behind_a_window_are_not_asked_for(form, n, page, bits8
     c.to_device()
     assert_close(_call(c, dict(window=700)), want, tol)
     assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("form", ["attention_rows", "attention_rows_tc", "attention_few"], indirect=True)
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("cut", [3, 14])
+def test_ranges_of_a_few_items_of_a_step_are_joined_from_scratch_of_their_own(monkeypatch, form, bits8, cut):
+    """Items that are far fewer than the step's tokens, in pieces of any order, some shorter than the call was sized for."""
+    monkeypatch.setattr(K(), "attention_rows_plan", lambda *a: (12, 128))
+    c = Case([14, 200, 9], [900, 0, 1500], 8, 2, 128, 64, bits8=bits8).tree().to_device()
+    items = c.items(cut, lambda n: n != 200)
+    items = (items[0].flip(0).contiguous(), *items[1:])
+    assert items[1] * items[2] < c.N
+    out = _call(c, items=items)
+    ours = [i for i in range(c.N) if not 14 <= i < 214]
+    assert_close(out, *c.want(), ours)
+    assert (out[14:214] == 7).all() and int(c.status) == 0
+
+
+def test_one_token_behind_a_long_context_beside_a_portion_takes_little_memory():
+    """40 heads on 8 of 128, 30,000 keys: the ranges of one row, not of the portion's 2,048 others."""
+    c = Case([2048, 1], [0, 30000], 40, 8, 128, 64).to_device()
+    row = torch.tensor([2048], dtype=torch.int32, device="cuda")
+    out = torch.full_like(c.q, 7.0)
+    _call(c, out=out, rows=row)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    _call(c, out=out, rows=row)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before <= 64 << 20
+    alone = Case([1], [30000], 40, 8, 128, 64).to_device()
+    alone.pages, alone.scales, alone.P, alone.rows, alone.q = c.pages, c.scales, c.P, c.rows, c.q[2048:].contiguous()
+    alone.table = c.table[1:].contiguous()
+    got = _call(alone)
+    assert torch.equal(got[0], out[2048]) and (out[:2048] == 7).all()
+    assert_close(got, *alone.want())
