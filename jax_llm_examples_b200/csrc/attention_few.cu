@@ -28,7 +28,7 @@
 //
 // The reference `ref` of a row's exponents is not its running maximum: it moves, with a rescaling of the outputs, only when a
 // score outgrows it by 2^GROWTH (weights up to 64: no trouble for float16 or a 32-bit sum), so a tile costs one vote instead of
-// a maximum over all its keys.
+// a maximum over all its keys.  Over a bfloat16 cache it moves by as much beyond the headroom that keeps large values' sums finite.
 //
 // Ranges of one item (few items, long contexts) are a thread-block cluster of up to 8: they leave their sums in shared memory
 // and each reads its share of the others' there, no second kernel and no scratch.  More ranges than that go through scratch.
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (F8) x[ng][e] = x[ng][e] == -INFINITY ? x[ng][e] : x[ng][e] + (e < 2 ? ve0 : ve1);  // (a masked key's scale may be anything)
-          grown |= x[ng][e] > m[ng][e & 1] + GROWTH;
+          grown |= x[ng][e] > m[ng][e & 1] + (F8 ? GROWTH : -ROWS_HEADROOM);
         }
       if (__builtin_expect(__any_sync(0xffffffffu, grown), 0)) {
 #pragma unroll
@@ -440,9 +440,10 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
           float corr[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(m[ng][c], fmaxf(x[ng][c], x[ng][c + 2]));
+            float mx = fmaxf(x[ng][c], x[ng][c + 2]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            mx = fmaxf(m[ng][c], F8 ? mx : mx + (ROWS_HEADROOM + GROWTH));
             corr[c] = rows_exp2(m[ng][c] - mx);
             m[ng][c] = mx;
             l[ng][c] *= corr[c];

@@ -334,10 +334,11 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
+      const float ref[2] = {F8 ? m[0] : m[0] + ROWS_HEADROOM, F8 ? m[1] : m[1] + ROWS_HEADROOM};
       const float2 vi = F8 ? *reinterpret_cast<const float2*>(sck + 2 * KT + i * 8) : make_float2(1.f, 1.f);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float w = (seen >> (i * 4 + e)) & 1 ? rows_exp2(s[i][e] - m[e >> 1]) : 0.f;
+        const float w = (seen >> (i * 4 + e)) & 1 ? rows_exp2(s[i][e] - ref[e >> 1]) : 0.f;
         s[i][e] = w;
         sum[e >> 1] = F8 ? fmaf(w, (e & 1) ? vi.y : vi.x, sum[e >> 1]) : sum[e >> 1] + w;
       }
@@ -413,8 +414,8 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
       }
     }
     if (t4 == 0) {
-      rows_ml[warp * 16 + g] = make_float2(m[0], l[0]);
-      rows_ml[warp * 16 + g + 8] = make_float2(m[1], l[1]);
+      rows_ml[warp * 16 + g] = make_float2(F8 ? m[0] : m[0] + ROWS_HEADROOM, l[0]);
+      rows_ml[warp * 16 + g + 8] = make_float2(F8 ? m[1] : m[1] + ROWS_HEADROOM, l[1]);
     }
   }
   __syncthreads();

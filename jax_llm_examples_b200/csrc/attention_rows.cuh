@@ -19,6 +19,10 @@
 #include "softcap.cuh"
 
 #define ROWS_NEG_BIG (-1.0e30f)
+// Over a bfloat16 cache, whose values may be as large as 32 bits go, a row's weights are at most 2^-ROWS_HEADROOM against the
+// reference of its exponents: the sum of weighted values stays below the largest of them for 2^24 keys, and overflows no sooner
+// than the average does.  (Values below 2^-100 lose digits by it.  Codes of 8 bits need none: they are below 2^69.)
+#define ROWS_HEADROOM 24.0f
 #define LOG2E 1.4426950408889634f
 
 struct RowsParams {

@@ -736,11 +736,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       if (!ok) break;
 #pragma unroll
       for (int q = 0; q < PARTS; ++q) mx = fmaxf(mx, xmax[mp][group][q][row]);
-      mx = fmaxf(m, mx > 0.5f * ROWS_NEG_BIG ? mx * out : ROWS_NEG_BIG);
-      // While no row of this quarter has grown by more than GROWTH beyond its reference, the references stay, the weights may
-      // exceed 1 (up to 2^16: 32-bit sums and bfloat16 weights lose nothing by it, and values below 2^100 do not overflow), and O is not
-      // rescaled, which takes 700 cycles and more.  All threads of these rows decide alike: they hold the same references.
-      if (__all_sync(0xffffffffu, mx - m <= GROWTH)) mx = m;
+      // While no row of this quarter has grown by more than GROWTH beyond its reference, the references stay and O is not
+      // rescaled, which takes 700 cycles and more.  All threads of these rows decide alike: they hold the same references.  8 bits:
+      // the weights may exceed 1 (up to 2^16: 32-bit sums and bfloat16 weights lose nothing by it).  Bfloat16 caches: a new
+      // reference lies that much above what the headroom for large values asks for.
+      mx = mx > 0.5f * ROWS_NEG_BIG ? mx * out + (F8 ? 0.f : ROWS_HEADROOM) : ROWS_NEG_BIG;
+      const float top = mx;
+      mx = fmaxf(m, mx);
+      if (__all_sync(0xffffffffu, mx - m <= (F8 ? GROWTH : 0.f))) mx = m;
+      else if (!F8) mx = fmaxf(m, top + GROWTH);
       const float corr = m == mx ? 1.f : rows_exp2(m - mx);
       const uint64_t out2 = pack2(out, out), mx2 = pack2(-mx, -mx);
       float rs4[4] = {0.f, 0.f, 0.f, 0.f};

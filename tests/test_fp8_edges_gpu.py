@@ -228,3 +228,25 @@ def test_one_token_behind_a_long_context_beside_a_portion_takes_little_memory():
     got = _call(alone)
     assert torch.equal(got[0], out[2048]) and (out[:2048] == 7).all()
     assert_close(got, *alone.want())
+
+
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("n", [3, 60])
+@pytest.mark.parametrize("steps", [[5.0, 5.0], [15.0, 15.5], [3.0, 14.0], [40.0, 5.5]])
+def test_large_values_of_a_bfloat16_cache_are_averaged_not_lost(form, n, steps):
+    """Values of 2^126, a quarter of what the type holds, behind scores that climb: an average of them is finite."""
+    c = Case([n], [900], 4, 1, 128, 16, bits8=False, spread=0.0).tree()
+    c.q[:] = c.q[0, 0]
+    c.rows[:, 0] *= 0.02
+    top = 0.0
+    for place, step in zip((300, 700), steps):
+        top += step
+        page, at = int(c.table[0, place // 16]), place % 16
+        c.rows[page, 0, 0, at] = c.q[0, 0].double() * (top / (c.scale * math.log2(math.e) * float((c.q[0, 0].double() ** 2).sum())))
+    c.rows[:, 1] = c.rows[:, 1].sign() * 2.0 ** 126 * torch.where(c.rows[:, 1].abs() > 1, 1.0, 0.5)
+    c.pages = c.rows.to(torch.bfloat16)
+    c.rows = c.pages.double()
+    c.to_device()
+    out = _call(c)
+    assert torch.isfinite(out).all()
+    assert_close(out, *c.want())
