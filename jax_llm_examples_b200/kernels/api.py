@@ -1380,10 +1380,12 @@ def attention_fp8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, bl
     portions of prompts, of any length.  Without items: single tokens, the first n_rows of the listed ``rows``, or all.  Only the
     served rows of ``out`` are written.  ``max_kv_len``: keys of the longest request (it sizes the work, and bounds nothing)."""
     n = n_items if items is not None else (n_rows if rows is not None else q.shape[0])
+    if items is not None and rows is not None:
+        raise KernelError("attention_fp8: a call serves items or single rows, not both")
     if scales is None:
         raise KernelError("attention_fp8: a cache in 8 bits has scales")
     _attention_rows("attention_fp8", q, pages, scales, block_table, req_of_token, positions, out, scale, chunk, window, attn_scale, floor_scale,
-                    status, max_kv_len, items, None if items is not None else rows, n, max_count if items is not None else 1, None, None, None,
+                    status, max_kv_len, items, rows, n, max_count if items is not None else 1, None, None, None,
                     sink, slopes, softcap)
 
 

@@ -74,3 +74,25 @@ def test_scratch_for_ranges_is_sized_by_the_rows_that_a_call_serves_and_bounded(
     rows = min(N, served["rows"] if "rows" in served else items * most)
     for n in asked:
         assert n <= 256 << 20 and n <= rows * Hq * max(K.ROWS_SPLITS) * (dh + 2) * 4
+
+
+def _attend_args(**change):
+    import torch
+
+    from .fp8_helpers import Case
+
+    c = Case([3], [5], 4, 2, 64, 16, device="cpu")
+    a = dict(q=c.q, pages=c.pages, scales=c.scales, block_table=c.table, req_of_token=c.req, positions=c.positions, out=torch.empty_like(c.q),
+             scale=0.125, chunk=0, window=0, attn_scale=0.0, floor_scale=1.0, status=c.status, max_kv_len=8)
+    return {**a, **change}
+
+
+def test_items_and_single_rows_in_one_call_are_refused(monkeypatch):
+    """One of the two would be left out of the output, and the caller not told."""
+    import torch
+
+    from jax_llm_examples_b200.kernels import api as K
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(K.KernelError, match="items or single rows"):
+        K.attention_fp8(**_attend_args(items=torch.zeros((1, 2), dtype=torch.int32), n_items=1, max_count=3, rows=torch.zeros(1, dtype=torch.int32), n_rows=1))
