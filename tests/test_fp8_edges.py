@@ -96,3 +96,17 @@ def test_items_and_single_rows_in_one_call_are_refused(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     with pytest.raises(K.KernelError, match="items or single rows"):
         K.attention_fp8(**_attend_args(items=torch.zeros((1, 2), dtype=torch.int32), n_items=1, max_count=3, rows=torch.zeros(1, dtype=torch.int32), n_rows=1))
+
+
+def test_an_output_that_shares_memory_with_the_queries_is_refused(monkeypatch):
+    """Blocks read queries while others write outputs."""
+    import torch
+
+    from jax_llm_examples_b200.kernels import api as K
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    room = torch.zeros(5 * 4 * 64, dtype=torch.bfloat16)
+    q = room[:3 * 256].view(3, 4, 64)
+    for first in (0, 1, 2):
+        with pytest.raises(K.KernelError, match="not the same rows"):
+            K.attention_fp8(**_attend_args(q=q, out=room[first * 256:(first + 3) * 256].view(3, 4, 64)))
