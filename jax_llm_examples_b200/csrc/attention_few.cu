@@ -14,10 +14,11 @@
 //
 // 8 bits: codes go to the tensor cores as float16, which holds every one of them; no number of the cache is rounded.  A key's
 // power of two multiplies its row of scores.  A value's is added to its key's exponent: with a_j = s_j + e_j the weights
-// w_j = 2^(a_j - ref) and the sum  sum w_j 2^-e_j  give  out = sum w_j code_j / sum w_j 2^-e_j,  so that the weights fit
-// float16 (2^-11 of each at most) whatever the values' scales, and a key of small values loses nothing to a neighbour's large
-// ones.  (Scales lie within 2^-60 .. 2^60: no product leaves the 32-bit range.)  Queries are brought to float16 by a power of
-// two per row, which makes the largest entry 2^7 .. 2^8: exact down to 2^-25 of it.
+// w_j = 2^(a_j - ref) and the sum  sum w_j 2^-e_j  give  out = sum w_j code_j / sum w_j 2^-e_j,  so that float16 rounds each
+// weight by 2^-11 of it at most, or by 2^-25 where it is below 2^-14: keys whose weight times scale is below 2^-25 of the
+// row's largest add to the sum and no longer to the values, of which they are at most as small a part.  (Scales lie within
+// 2^-60 .. 2^60: no product leaves the 32-bit range.)  Queries are brought to float16 by a power of two per row, which makes the
+// largest entry 2^7 .. 2^8: entries above 2^-24 of it are exact, smaller ones off by 2^-32 of it at most.
 // Bfloat16 caches: probabilities are rounded to bfloat16 for the product with the values (2^-8 of each at most).  Sums and
 // outputs are 32-bit in both.
 //

@@ -110,3 +110,14 @@ def test_an_output_that_shares_memory_with_the_queries_is_refused(monkeypatch):
     for first in (0, 1, 2):
         with pytest.raises(K.KernelError, match="not the same rows"):
             K.attention_fp8(**_attend_args(q=q, out=room[first * 256:(first + 3) * 256].view(3, 4, 64)))
+
+
+def test_what_two_8_bit_parts_hold_of_a_query():
+    """An e4m3 part and what is left of it in e5m2, of every bfloat16 number up to 2^8: exact from 2^-6 on, off by 2^-14 at most below."""
+    import torch
+
+    a = torch.arange(0x7F80, dtype=torch.int16).view(torch.bfloat16).float()
+    a = a[a < 256]
+    first = a.to(torch.float8_e4m3fn).float()
+    off = (a.double() - first.double() - (a - first).to(torch.float8_e5m2).double()).abs()
+    assert not off[a >= 2.0 ** -6].any() and off.max() == 2.0 ** -14

@@ -250,3 +250,42 @@ def test_large_values_of_a_bfloat16_cache_are_averaged_not_lost(form, n, steps):
     out = _call(c)
     assert torch.isfinite(out).all()
     assert_close(out, *c.want())
+
+
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("top", [2.0 ** 10, 2.0 ** 13, 2.0 ** 16, 2.0 ** 20])
+@pytest.mark.parametrize("n, Hq, dh", [(2, 4, 128), (40, 8, 64), (70, 4, 128)])
+def test_queries_with_one_entry_far_above_the_others(form, top, n, Hq, dh):
+    """The large entry meets keys of zero: the scores are those of the small ones.  What the operands lose of an entry: nothing down
+    to 2^-13 of the row's largest and 2^-21 of that below it (two 8-bit parts), 2^-32 of it (float16).  The values are +-1, so
+    that a score's error d adds 2 d to an output's."""
+    c = Case([n], [300], Hq, 2, dh, 16, spread=0.0)
+    c.rows[:, 0, ..., 5] = 0.0
+    c.rows[:, 1] = c.rows[:, 1].sign()
+    c.rows, scales = hold(c.rows)
+    c.set_rows8(scales)
+    c.q[..., 5] = top
+    c.to_device()
+    items = c.items(n)
+    out = _call(c, items=items)
+    want, tol = c.want()
+    part = 2.0 ** -21 if c.weights == 2.0 ** -8 else 2.0 ** -32
+    size = float(c.rows[:, 0].abs().sum(-1).max()) * c.scale
+    tol = tol + 2 * part * top * size
+    assert_close(out, want, tol)
+
+
+@pytest.mark.parametrize("n, held, Hq, Hkv, dh, page, mask", [
+    ([20], [300], 4, 2, 64, 16, {}), ([5, 13], [700, 64], 8, 2, 128, 64, {}), ([8, 3, 8], [1000, 0, 333], 40, 8, 128, 64, {}), ([60], [900], 2, 2, 128, 48, dict(window=200)),
+    ([16, 16], [2000, 100], 12, 3, 64, 32, dict(chunk=512)),
+])
+def test_few_items_of_17_to_64_rows_keep_float16s_digits(n, held, Hq, Hkv, dh, page, mask):
+    """8-bit items that the rule sends to the few-rows kernel, held to its own bound, as portions and as trees."""
+    c = Case(n, held, Hq, Hkv, dh, page).to_device()
+    out = _call(c, mask, c.items(max(n)))
+    assert c.weights == 2.0 ** -11 and 16 < max(n) * (Hq // Hkv) <= 64
+    assert_close(out, *c.want(**mask))
+    c = Case(n, held, Hq, Hkv, dh, page).tree().to_device()
+    out = _call(c, mask)
+    assert c.weights == 2.0 ** -11
+    assert_close(out, *c.want(**mask))
