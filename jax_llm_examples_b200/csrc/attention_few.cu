@@ -96,6 +96,11 @@ template <int DH, bool F8, int NG> struct FewTile {
   static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + 1024;  // (up to 1 KB for the alignment)
 };
 
+// The scales of a box whose page is missing: copied like any other's.  (What the fetching warp does between a free stage and its
+// copies counts: fewer bytes to wait for in such tiles, with plain stores of zeros, took 87 us for 78 with 8 requests of up to
+// 30,000 keys, copies from a row of their own 82, a branch around them 80.)
+__device__ __align__(16) uint8_t no_scales[KT];
+
 // NG: groups of 8 query rows (1, 2).  Registers for as many blocks of a multiprocessor as its shared memory has room for (heads of
 // 128 in bfloat16, two groups: 209 registers and one block otherwise, six requests of 4,000 keys 25 us for 20).
 template <int DH, bool F8, int NG>
@@ -170,30 +175,21 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
         if (t >= STAGES) ok = mbar_wait(EMPTY(s), (t / STAGES - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const int place = range0 + t * KT + lane * box_rows;
-        const bool box = lane < boxes, there = box && rows_page_there(P, page);
-        if (box && !there) {
-          if (place < end && place + box_rows > begin) atomicOr(P.status, JLX_STATUS_BAD_PAGE);
-          if (F8) {  // its scales' bytes: ordinary stores, before the arrival below, and before a later tile's copies into their places
-            for (int i = 0; i < 2 * box_rows; i += 16) {
-              const int w = i >= box_rows;
-              *reinterpret_cast<uint4*>(scales_of(s) + w * KT + lane * box_rows + i - w * box_rows) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          }
-        }
-        const int copied = __popc(__ballot_sync(0xffffffffu, there));
-        if (F8 && copied != boxes) __syncwarp();  // (the other lanes' stores come with lane 0's arrival)
-        if (lane == 0) mbar_expect_tx(FULL(s), 2 * T::BYTES + (F8 ? 2 * box_rows * copied : 0));
+        if (lane == 0) mbar_expect_tx(FULL(s), 2 * T::BYTES + T::SCALE_BYTES);
         __syncwarp();
-        if (box) {
-          const int row = there ? (page * 2 * P.Hkv + hk) * P.page_size + place % P.page_size : rows_behind(P), to_v = there ? v_off : 0;
+        if (lane < boxes) {
+          const int place = range0 + t * KT + lane * box_rows;
+          const bool there = rows_page_there(P, page);
+          if (!there && place < end && place + box_rows > begin) atomicOr(P.status, JLX_STATUS_BAD_PAGE);
+          if (!there) page = P.num_pages;
+          const int row = (page * 2 * P.Hkv + hk) * P.page_size + place % P.page_size, to_v = there ? v_off : 0;
+          const uint8_t* bytes = there ? P.scales + row : no_scales;
           const uint32_t dst = smem_u32(k_tile(s)) + lane * box_rows * (CH == 4 ? 64 : 128);
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
 #pragma unroll
-            for (int h = 0; h < (CH + 7) / 8; ++h) tma_load_2d(dst + w * T::BYTES + h * KT * 128, &map, h * 128 / T::ELEM, row + w * to_v, FULL(s));
-            if (F8 && there) bulk_load(smem_u32(scales_of(s)) + w * KT + lane * box_rows, P.scales + row + w * v_off, box_rows, FULL(s));
+            for (int h = 0; h < (CH + 7) / 8; ++h) tma_load_2d(dst + w * T::BYTES + h * KT * 128, &map, h * 128 / T::ELEM, row + w * v_off, FULL(s));
+            if (F8) bulk_load(smem_u32(scales_of(s)) + w * KT + lane * box_rows, bytes + w * to_v, box_rows, FULL(s));
           }
         }
         page = find_page(t + 1);

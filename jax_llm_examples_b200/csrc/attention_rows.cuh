@@ -130,10 +130,9 @@ __device__ __forceinline__ bool rows_sees(const RowsParams& P, const RowsItem& i
 }
 
 // Keys whose page the table does not name (below 0, or beyond the pool) raise the status where some row sees them, and are keys
-// and values of zeros in every kernel: rows_cache_row says -1, a TMA box starts behind the cache's last row, where all it brings is
-// zeros, and the scales' bytes are 0.
+// and values of zeros in every kernel: rows_cache_row says -1, a TMA box is asked for from page num_pages, behind the cache, where all
+// it brings is zeros, and the scales' bytes are 0.
 __device__ __forceinline__ bool rows_page_there(const RowsParams& P, int page) { return page >= 0 && page < P.num_pages; }
-__device__ __forceinline__ int rows_behind(const RowsParams& P) { return P.num_pages * 2 * P.Hkv * P.page_size; }  // (fits: the launcher looks)
 
 // The flat row of the key at `place` in the cache (values: Hkv * page_size further), or -1.
 __device__ __forceinline__ int rows_cache_row(const RowsParams& P, const int* table, int hk, int place) {
@@ -206,7 +205,7 @@ struct RowsArgs {
 static int rows_params(const RowsArgs& a, RowsParams& P) {
   JLX_REQUIRE(a.Hkv > 0 && a.Hq > 0 && a.Hq % a.Hkv == 0 && (a.dh == 64 || a.dh == 128), "attention over rows: %d query heads on %d of %d entries (64 or 128) are not supported", a.Hq, a.Hkv, a.dh);
   JLX_REQUIRE(a.N > 0 && a.n_items >= 0 && a.max_count > 0 && a.page_size > 0 && a.num_pages > 0 && a.bt_stride > 0 && a.n_requests > 0, "attention over rows: bad sizes");
-  JLX_REQUIRE((long long)a.num_pages * 2 * a.Hkv * a.page_size < (1ll << 31), "attention over rows: cache too large for 32-bit rows");
+  JLX_REQUIRE(((long long)a.num_pages + 1) * 2 * a.Hkv * a.page_size < (1ll << 31), "attention over rows: cache too large for 32-bit rows");
   JLX_REQUIRE((((uintptr_t)a.q | (uintptr_t)a.pages | (uintptr_t)a.out) & 15) == 0, "attention over rows: q, pages and out must be 16-byte aligned");
   JLX_REQUIRE(a.attn_scale == 0.f || a.floor_scale > 0.f, "attention: floor_scale must be positive");
   JLX_REQUIRE(a.softcap >= 0.f && a.chunk >= 0 && a.window >= 0, "attention: the score cap, chunk and window must not be negative (0: none)");

@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       const int place = range0 + t * BKV + lane * box_rows, st = t % stages;
       const bool there = rows_page_there(P, page);
       if (!there && lane < boxes && place < end && place + box_rows > begin) atomicOr(P.status, JLX_STATUS_BAD_PAGE);
-      const int row = there ? (page * 2 * P.Hkv + hk) * P.page_size + place % P.page_size + off : rows_behind(P);
+      if (!there) page = P.num_pages;
+      const int row = (page * 2 * P.Hkv + hk) * P.page_size + place % P.page_size + off;
       page = page_next;
       page_next = find_page(t + 2);
       if (t >= stages) ok = mbar_wait(BAR((which ? (F8 ? B_RAWEMPTY : B_VEMPTY) : B_KEMPTY) + st), (t / stages - 1) & 1);
