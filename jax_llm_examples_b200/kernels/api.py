@@ -1315,7 +1315,7 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     N, Hq, dh = q.shape
     P, two, Hkv, page_size, dh2 = pages.shape
     out_p, q_p = out.data_ptr(), q.data_ptr()
-    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or out.shape != q.shape or abs(out_p - q_p) < 2 * q.numel():
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or out.shape != q.shape or -2 * N * Hq * dh < out_p - q_p < 2 * N * Hq * dh:
         raise KernelError(f"{what}: queries and output must be bfloat16 [N, Hq, dh], and not the same rows")
     if dh2 != dh or two != 2:
         raise KernelError(f"{what}: cache pages {tuple(pages.shape)} and queries {tuple(q.shape)} disagree")
@@ -1352,8 +1352,10 @@ def _attention_rows(what: str, q, pages, scales, block_table, req_of_token, posi
     keys = _keys_seen(max_kv_len, chunk, window, max_count)
     form = attention_rows_form(max_count * (Hq // Hkv), page_size, scales_p % 16 == 0, keys, n_items * Hkv, scales is not None)
     places = _few_places(dev, dh, scales is not None, 8 if max_count * (Hq // Hkv) <= 8 else ROWS_FEW) if form == "attention_few" else None
-    tokens = min(N, n_items * max_count)  # in the scratch: those of every item, or the step's
-    most = min(ROWS_SPLITS[-1], ROWS_SCRATCH // (tokens * Hq * (dh + 2) * 4))
+    tokens = n_items * max_count  # in the scratch: those of every item, or the step's
+    tokens = tokens if tokens < N else N
+    one = tokens * Hq * (dh + 2) * 4  # bytes of a range
+    most = ROWS_SPLITS[-1] if one <= ROWS_SCRATCH // ROWS_SPLITS[-1] else ROWS_SCRATCH // one
     splits, row_block = attention_rows_plan(form, max_kv_len, chunk, window, n_items, max_count, Hq, Hkv, sm_count(), places, most)
     part_o = part_ml = joined = 0
     if splits > (ROWS_CLUSTER if form == "attention_few" else 1):
