@@ -113,7 +113,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
   __shared__ __align__(8) uint64_t bars[2 * STAGES];
   __shared__ int4 row_tok[ROWS];   // (token, head, position, first key) of the block's rows
   __shared__ float2 row_sc[ROWS];  // (score factor, slope)
-  __shared__ int any_bad, failed;
+  __shared__ int any_bad;
   pdl_launch_dependents_if_small();
   pdl_wait();
   const int split = blockIdx.x % P.splits, item_i = blockIdx.x / P.splits;
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
       mbar_init(FULL(s), box_rows ? 1 : F8 ? 33 : 32);  // TMA's bytes; else every lane's copies, and the scales' store
       mbar_init(EMPTY(s), CONSUMERS);
     }
-    any_bad = failed = 0;
+    any_bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0 && lane < ROWS) {
@@ -249,10 +249,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
     cp_async_commit();
     cp_async_wait<0>();  // nothing is in flight when the ring is used for something else
     }
-    if (!ok && lane == 0) {
-      atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
-      failed = 1;
-    }
+    if (!ok && lane == 0) atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
   } else {
     // ------------------------------------------------------------------------------ the computing warps
     // queries: column g of group ng is row 8 ng + g, its entries in the order of the scores' contraction
@@ -496,10 +493,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
       __syncwarp();
       if (lane == 0) mbar_arrive(EMPTY(st));
     }
-    if (!ok && lane == 0) {
-      atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
-      failed = 1;
-    }
+    if (!ok && lane == 0) atomicOr(P.status, JLX_STATUS_WAIT_TIMEOUT);
   }
   __syncthreads();  // the ring is free: the warps leave their rows in it
 
