@@ -35,8 +35,8 @@
 // and each reads its share of the others' there, no second kernel and no scratch.  More ranges than that go through scratch.
 //
 // What bounds it: in long caches the instructions between a byte and a product (a tile's 280 a warp), in short ones a block's way to its first tile (page, position, key: 2 us) and the launch.  Measured
-// (B200, 40 heads on 8 of 128, 8 bits): 64 requests of up to 8,192 keys 156 us, 5.25 TB/s, 80 % of the copy rate; 8 of up to
-// 30,000 79 us, 4.99 TB/s; one of 700 13 us with its call, 8.4 on the device.
+// (B200, 40 heads on 8 of 128, 8 bits): 64 requests of up to 8,192 keys 153 us, 5.35 TB/s, 82 % of the copy rate; 8 of up to
+// 30,000 78 us, 5.05 TB/s; one of 700 13 us with its call, 8.4 on the device.
 // Tried and slower: 8-bit score products (the conversion of queries' remainders costs more than the codes'), a reference taken
 // from the tile before with a second pass where it fails, exponentials by a polynomial.
 #include <cooperative_groups.h>
@@ -527,6 +527,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
     *reinterpret_cast<__nv_bfloat162*>(&v.y) = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
     *reinterpret_cast<uint2*>(P.out + ((size_t)k.x * P.Hq + k.y) * DH + d) = v;
   };
+  const int part_shift = rows_part_shift(P, item_i, it.n0);
   for (int idx = tid; idx < n_rows * Q4; idx += (CONSUMERS + 1) * 32) {
     const int row = idx / Q4, d = (idx - row * Q4) * 4;
     float mm = ROWS_NEG_BIG, ll = 0.f;
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__((CONSUMERS + 1) * 32, DH == 128 && NG == 2 ? 2
       *reinterpret_cast<float4*>(merged + (size_t)row * T::LD + d) = acc;
       if (d == 0) merged_ml[row] = make_float2(mm, ll);
     } else {
-      const size_t at = rows_part_token(P, item_i, k.x, it.n0) * P.Hq + k.y;
+      const size_t at = (size_t)(k.x + part_shift) * P.Hq + k.y;
       *reinterpret_cast<float4*>(P.part_o + (at * P.splits + split) * DH + d) = acc;
       if (d == 0) P.part_ml[at * P.splits + split] = make_float2(mm, ll);
     }

@@ -28,8 +28,8 @@
 // that do see it at the end (a product would spread 0 * infinity over all rows).  In 8 bits only a row's scale can say NaN.
 //
 // Pages that hold no whole boxes of 16 rows, and scales that start off a 16-byte boundary, come here; the rest goes to the
-// tcgen05 kernel, which is up to 5.7 times as fast.  Measured (B200, pages of 24): 2,048 tokens after 1,500, 40 heads on 8 of 128,
-// 8 bits: 1,089 us, 97 TFLOP/s (188 us there); trees of 32 tokens on 8 requests, bfloat16: 448 us (89).  Its mma.sync products and
+// tcgen05 kernel, which is up to 5.9 times as fast.  Measured (B200, pages of 24): 2,048 tokens after 1,500, 40 heads on 8 of 128,
+// 8 bits: 1,089 us, 97 TFLOP/s (185 us there); trees of 32 tokens on 8 requests, bfloat16: 448 us (94).  Its mma.sync products and
 // the conversion of codes in every warp bound it.
 #include "attention_rows.cuh"
 #include "mbarrier.cuh"
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
   __shared__ int4 row_tok[16 * WM];  // (token, head, position, first key) of the block's rows
   __shared__ int2 row_sc[16 * WM];   // (score factor, slope)
   __shared__ int span[4];            // smallest and largest first key, smallest and largest position of the rows
-  __shared__ int any_bad;
+  __shared__ int any_bad, first_token;  // (the item's first token: kept in a register it made the kernel 8 % slower)
   pdl_launch_dependents_if_small();
   pdl_wait();
   const int split = blockIdx.x % P.splits, item_i = blockIdx.x / P.splits;
@@ -90,7 +90,10 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
   if (n_rows <= 0) return;
 
   if (tid < 4) span[tid] = (tid & 1) ? (int)0x80000000 : 0x7fffffff;
-  if (tid == 0) any_bad = 0;
+  if (tid == 0) {
+    any_bad = 0;
+    first_token = it.n0;
+  }
   __syncthreads();
   if (tid < 16 * WM) {
     const RowsToken k = rows_token(P, it, row0 + min(tid, n_rows - 1), hk);
@@ -420,6 +423,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
     }
   }
   __syncthreads();
+  const int part_shift = P.splits > 1 ? rows_part_shift(P, blockIdx.x / P.splits, first_token) : 0;
   for (int idx = tid; idx < n_rows * (DH / 4); idx += 128) {
     const int row = idx / (DH / 4), d = (idx - row * (DH / 4)) * 4, w0 = (row >> 4) * WK, i = row & 15;
     float mm = ROWS_NEG_BIG, ll = 0.f;
@@ -450,7 +454,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const RowsParams P)
         if (!isfinite(x[3])) acc.w += x[3];
       }
     }
-    const size_t at = (P.splits > 1 ? rows_part_token(P, item_i, tok.x, it.n0) : (size_t)tok.x) * P.Hq + tok.y;
+    const size_t at = (size_t)(tok.x + part_shift) * P.Hq + tok.y;
     if (P.splits > 1) {
       *reinterpret_cast<float4*>(P.part_o + (at * P.splits + split) * DH + d) = acc;
       if (d == 0) P.part_ml[at * P.splits + split] = make_float2(mm, ll);

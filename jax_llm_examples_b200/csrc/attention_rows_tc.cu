@@ -17,9 +17,9 @@
 // What bounds it: a group's turn of about 4,500 cycles, of which 1,250 are the exponentials (1,024 at the unit's rate), 1,000 the
 // rest of the softmax, 600 (8 bits) the keys' scales and 1,800 the wait for the two products: their 16 instructions are accepted
 // one in 95 cycles from one thread, 1,520 a tile.  So 2,250 a tile of 128 by 128, where exponentials and products would take
-// 1,024 each, side by side.  Measured (B200): 2,048 tokens after 1,500, 40 heads on 8 of 128, 8 bits: 187 us, 566 TFLOP/s, 34 %
-// of the bfloat16 peak; trees of 32 tokens on 8 requests of up to 8,192 keys, bfloat16: 96 us, 339 TFLOP/s; of 64 tokens on 16
-// requests of up to 12,000, 32 heads, 8 bits: 278 us, 547 TFLOP/s.
+// 1,024 each, side by side.  Measured (B200): 2,048 tokens after 1,500, 40 heads on 8 of 128, 8 bits: 185 us, 571 TFLOP/s, 34 %
+// of the bfloat16 peak; trees of 32 tokens on 8 requests of up to 8,192 keys, bfloat16: 94 us, 347 TFLOP/s; of 64 tokens on 16
+// requests of up to 12,000, 32 heads, 8 bits: 275 us, 551 TFLOP/s.
 // Tried and slower: one group of sixteen warps on 128 rows with two buffers of scores (227, 114 and 325 us); then one block per
 // multiprocessor that takes an equal share of all tiles (247, 112 and 293: its join and the change from piece to piece cost what
 // the shares gained); a warp for each group's products beside one for all copies (228, 108 and 357).
@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_rows_tc_kernel(const __
       const int col_end = col + (by_rows ? T::OC : T::OE);
       const RowsToken tok = token();
       const RowsItem it = item();
-      const size_t at = (P.splits > 1 ? rows_part_token(P, item_i, tok.n, it.n0) : (size_t)tok.n) * P.Hq + tok.head;
+      const size_t at = (size_t)(tok.n + (P.splits > 1 ? rows_part_shift(P, item_i, it.n0) : 0)) * P.Hq + tok.head;
       const float inv = P.splits > 1 ? 1.f : rows_inverse(P, m, total, tok.head);
       if (P.splits > 1 && col == 0 && block_row < n_rows) P.part_ml[at * P.splits + split] = make_float2(m, total);
 #pragma unroll 1

@@ -1380,7 +1380,9 @@ def attention_fp8(q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, bl
     """:func:`attention_generic` over a cache in 8 bits (:func:`kv_store_fp8`), on the tensor cores: q, out bfloat16 [N, Hq, dh],
     dh 64 or 128.  ``items``: int32 [n_items, 2] = (first token row, count <= max_count), consecutive tokens of one request each:
     portions of prompts, of any length.  Without items: single tokens, the first n_rows of the listed ``rows``, or all.  Only the
-    served rows of ``out`` are written.  ``max_kv_len``: keys of the longest request (it sizes the work, and bounds nothing)."""
+    served rows of ``out`` are written.  ``max_kv_len``: keys of the longest request (it sizes the work, and bounds nothing).
+    Keys without a page raise the status and count as zeros.  The softmax's weights are rounded for the product with the values:
+    to float16 in calls of few rows, to bfloat16 in the others (:func:`attention_rows_form`)."""
     n = n_items if items is not None else (n_rows if rows is not None else q.shape[0])
     if items is not None and rows is not None:
         raise KernelError("attention_fp8: a call serves items or single rows, not both")
