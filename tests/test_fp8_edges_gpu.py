@@ -21,8 +21,11 @@ FORMS = ["rule", "attention_rows", "attention_rows_tc", "attention_few"]  # the 
 
 @pytest.fixture
 def form(request, monkeypatch):
-    if request.param != "rule":
-        monkeypatch.setattr(K(), "attention_rows_form", lambda *a: request.param)
+    rule = K().attention_rows_form
+    if request.param != "rule":  # (the tcgen05 kernel where it can)
+        monkeypatch.setattr(K(), "attention_rows_form",
+                            lambda rows, page, aligned, *a: rule(rows, page, aligned, *a) if request.param == "attention_rows_tc" and (page % 16 or not aligned)
+                            else request.param)
     return request.param
 
 
@@ -151,7 +154,7 @@ def _with_a_stranger_in_page_0(c):
 
 @pytest.mark.parametrize("form", FORMS, indirect=True)
 @pytest.mark.parametrize("bits8", [False, True])
-@pytest.mark.parametrize("n, page, dh", [(1, 64, 128), (2, 16, 64), (40, 64, 64), (40, 16, 128), (90, 48, 128)])
+@pytest.mark.parametrize("n, page, dh", [(1, 64, 128), (2, 16, 64), (40, 64, 64), (40, 16, 128), (90, 48, 128), (3, 24, 128), (40, 7, 64)])
 @pytest.mark.parametrize("what", ["none", "too high"])
 def test_a_missing_page_counts_as_keys_of_zeros(form, what, n, page, dh, bits8):
     """A request whose table names no page for some of its keys: the status says so, zeros stand in for them in every kernel, and no
@@ -289,3 +292,46 @@ def test_few_items_of_17_to_64_rows_keep_float16s_digits(n, held, Hq, Hkv, dh, p
     out = _call(c, mask)
     assert c.weights == 2.0 ** -11
     assert_close(out, *c.want(**mask))
+
+
+def test_a_few_rows_of_a_step_on_two_streams_and_in_graphs():
+    """Scratch that holds the served rows alone: calls at once on two streams, captured ones replayed with other queries, a row twice."""
+    cases = [Case([1, 600, 1], [9000 + 700 * i, 0, 8000], 8, 2, 128, 64, seed=i).to_device() for i in range(2)]
+    rows = torch.tensor([601, 0, 601], dtype=torch.int32, device="cuda")
+    served, others = [0, 601], slice(1, 601)
+    seen = K()._keys_seen(9702, 0, 0, 1)
+    form = K().attention_rows_form(4, 64, True, seen, 6, True)
+    assert form == "attention_few" and K().attention_rows_plan(form, 9702, 0, 0, 3, 1, 8, 2, 148)[0] > K().ROWS_CLUSTER
+
+    def want(c):
+        one = Case([1, 1], [c.held[0], c.held[2]], 8, 2, 128, 64)
+        one.rows, one.table, one.q = c.rows, c.table[[0, 2]].contiguous(), c.q[served].contiguous()
+        return one.want()
+
+    sides = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        for c, s in zip(cases, sides):
+            with torch.cuda.stream(s):
+                outs.append(_call(c, rows=rows))
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert_close(out[served], *want(cases[i % 2]))
+        assert (out[others] == 7).all()
+    graphs = []
+    for c in cases:
+        out, g = torch.full_like(c.q, 7.0), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            _call(c, rows=rows, out=out)
+        graphs.append((g, out))
+        c.q.mul_(0.5)
+    for _ in range(2):
+        for (g, _), c in zip(graphs, cases):
+            g.replay()
+            eager = _call(c, rows=rows)
+    torch.cuda.synchronize()
+    for (_, out), c in zip(graphs, cases):
+        assert_close(out[served], *want(c))
+        assert (out[others] == 7).all()
+    assert torch.equal(eager, graphs[-1][1])
