@@ -28,7 +28,7 @@
 // 2^7 .. 2^8 by a power of two) as e4m3, and what is left of it as e5m2; the remainder of eight bits after the nearest four is
 // a whole number up to 8 of the entry's last unit, which e5m2 holds (three bits), so both products add up in one accumulator to
 // that of the bfloat16 query.  That is exact for entries from 2^-6 on, 2^-13 of the row's largest; below, e4m3's steps no longer
-// shrink, the remainder has up to five bits, and an entry is off by up to 2^-14: 2^-21 of the row's largest.  The e4m3 product
+// shrink, the remainder has up to eight bits, and an entry is off by up to 2^-14: 2^-21 of the row's largest.  The e4m3 product
 // has twice the rate: two cost what one of bfloat16 does, and no key is converted.  A key's power of two multiplies its column
 // of scores.  The values become bfloat16, code times scale, which it holds exactly, once per tile and block: a code's seven bits
 // are a bfloat16 number's exponent and mantissa but for a factor of 2^120, which the multiplication with the scale takes along.
