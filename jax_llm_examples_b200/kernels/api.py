@@ -1498,6 +1498,108 @@ def gemm_stream(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, status: tor
     return used.value
 
 
+# ------------------------------------------------------------- low-rank adapters beside a shared projection
+ADAPTER_MAX_RANK = 256  # csrc/adapters.cu
+_ADAPTER_ARGS = struct.Struct("@10P3q10i")  # AdapterArgs in csrc/adapters.cu
+
+
+@dataclasses.dataclass(frozen=True)
+class AdapterPlan:
+    """Which rows of a step use which adapter (:func:`adapter_plan`): the rows sorted by adapter, cut into tiles of one each."""
+
+    rows: int
+    adapters: int
+    tile_rows: int
+    order: torch.Tensor  # int32 [rows]
+    tiles: torch.Tensor  # int32 [tiles, 3] = (adapter or -1, first entry of order, count <= tile_rows)
+
+
+def adapter_plan(adapter_of_row, adapters: int, device=None) -> AdapterPlan:
+    """The plan of a step whose row n uses adapter ``adapter_of_row[n]`` of so many, or none (-1): made once on the host and used by
+    every layer's :func:`adapter_add`.  ``device``: the current one if not given."""
+    ids = torch.as_tensor(adapter_of_row, dtype=torch.int64, device="cpu").reshape(-1)
+    if adapters < 1 or (ids.numel() and not -1 <= int(ids.min()) <= int(ids.max()) < adapters):
+        raise KernelError(f"adapter_plan: rows name adapters outside 0 .. {adapters - 1} (-1: none)")
+    order = torch.sort(ids, stable=True).indices
+    used, counts = torch.unique_consecutive(ids[order], return_counts=True)
+    # tiles of 16 rows where no adapter has more: a decode step's
+    tile_rows = 16 if not counts.numel() or int(counts.max()) <= 16 else 64
+    per = -(-counts // tile_rows)
+    within = torch.arange(int(per.sum())) - torch.repeat_interleave(per.cumsum(0) - per, per)
+    tiles = torch.stack([torch.repeat_interleave(used, per), torch.repeat_interleave(counts.cumsum(0) - counts, per) + within * tile_rows,
+                         (torch.repeat_interleave(counts, per) - within * tile_rows).clamp(max=tile_rows)], 1)
+    both = torch.cat([order, tiles.reshape(-1)]).to(torch.int32).to("cuda" if device is None else device)
+    return AdapterPlan(ids.numel(), adapters, tile_rows, both[:ids.numel()], both[ids.numel():].view(-1, 3))
+
+
+def _rows_of(what: str, name: str, t: torch.Tensor, n: int, width: int, written: bool = False) -> int:
+    """Elements between the rows of t [n, width], rows of contiguous entries (maybe a column range of wider ones)."""
+    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width or (width > 1 and t.stride(1) != 1) or (written and n > 1 and t.stride(0) < width):
+        raise KernelError(f"{what}: {name} must be [{n}, {width}] with rows of contiguous entries, not {tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0) if n > 1 else width
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors' rows share bytes.  (Column ranges of the same rows, side by side, do not.)"""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else t.data_ptr()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if a.dim() == b.dim() == 2 and a.shape[0] > 1 and b.shape[0] > 1:
+        wide = a.stride(0) * a.element_size()
+        if wide and wide == b.stride(0) * b.element_size():
+            at, aw, bw = (b0 - a0) % wide, a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+            return not (at >= aw and at + bw <= wide)
+    return True
+
+
+def adapter_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: AdapterPlan, y: torch.Tensor, out: torch.Tensor | None = None,
+                scale: torch.Tensor | None = None, ranks: torch.Tensor | None = None) -> None:
+    """out[n] = y[n] + scale[e] (x[n] a[e]^T) b[e]^T for row n's adapter e in ``plan`` (no adapter: out[n] = y[n]): what low-rank
+    adapters of many requests add to a shared projection's rows.  x: [N, K]; a: [E, r, K]; b: [E, No, r]; all float32 or all
+    bfloat16, r up to ADAPTER_MAX_RANK; y, out: [N, No], float32 or bfloat16 (``out`` None: y itself), for instance the first of a product's
+    split-K partials.  x, y and out may be column ranges of wider rows.  scale: float32 [E] or None (1); ranks: int32 [E] or
+    None (r): adapter e uses the first ranks[e] rows of a[e] and columns of b[e], and what lies behind is not used."""
+    out = y if out is None else out
+    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+        raise KernelError(f"adapter_add: matrices a {tuple(a.shape)} and b {tuple(b.shape)} are not [E, r, K] and [E, No, r]")
+    (E, r, K), No, N = a.shape, b.shape[1], x.shape[0]
+    if x.dtype != a.dtype or x.dtype != b.dtype or y.dtype != out.dtype:
+        raise KernelError("adapter_add: x, a and b must have one type, and so must y and out")
+    if plan.rows != N or plan.adapters != E:
+        raise KernelError(f"adapter_add: the plan is for {plan.rows} rows and {plan.adapters} adapters, not {N} and {E}")
+    if not 0 < r <= ADAPTER_MAX_RANK or K < 1 or No < 1:
+        raise KernelError(f"adapter_add: rank {r} (up to {ADAPTER_MAX_RANK}), {K} and {No} entries a row are not supported")
+    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != E):
+        raise KernelError(f"adapter_add: scale must be float32 [{E}]")
+    if ranks is not None and (ranks.dtype != torch.int32 or ranks.numel() != E):
+        raise KernelError(f"adapter_add: ranks must be int32 [{E}]")
+    types = code(x.dtype), code(y.dtype)
+    ld = _rows_of("adapter_add", "x", x, N, K), _rows_of("adapter_add", "y", y, N, No), _rows_of("adapter_add", "out", out, N, No, True)
+    dev = _placed("adapter_add", a, b, plan.order, plan.tiles, scale, ranks)
+    for t in (x, y, out):
+        if t.get_device() != dev:
+            raise KernelError(f"adapter_add: a tensor is on {t.device}, the current device is cuda:{dev}")
+    same = out.data_ptr() == y.data_ptr() and ld[1] == ld[2]
+    if any(_overlap(out, t) for t in (x, a, b)) or not (same or not _overlap(out, y)):
+        raise KernelError("adapter_add: out shares memory with an operand (only y itself may be written over)")
+    if N == 0:
+        return
+    args = [x.data_ptr(), a.data_ptr(), b.data_ptr(), y.data_ptr(), out.data_ptr(), plan.order.data_ptr(), plan.tiles.data_ptr(), _address(scale),
+            _address(ranks), 0, *ld, N, N, E, r, K, No, plan.tiles.shape[0], plan.tile_rows, *types]
+    packed = _ADAPTER_ARGS.pack(*args)
+    plain = not library("adapters").jlx_adapters_fast(packed)
+    if plain:
+        # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
+        low = torch.empty(N * r, dtype=torch.float32, device=x.device)
+        args[9] = low.data_ptr()
+        packed = _ADAPTER_ARGS.pack(*args)
+    _run("adapters", "jlx_adapters", packed, sm_count(), _raw_stream(dev))
+    global _launches
+    _launches += plain  # two kernels
+
+
 # --------------------------------------------------------------------------------------- MoE
 ROUTER_WEIGHT_FORMS = {"sigmoid": 0, "softmax_of_chosen": 1, "softmax_normalized": 2, "sigmoid_corrected": 3}  # csrc/moe.cu
 ROUTER_MAX_GROUPS = 64

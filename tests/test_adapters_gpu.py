@@ -1,0 +1,151 @@
+"""Low-rank adapters of many requests beside a shared projection, against the definition in 64 bits.
+
+What a result may be off by: the sums of K products and of r, in 32 bits, by 2^-23 of the magnitudes' sum an addition (the tensor
+cores cut, not round); between the products bfloat16 operands pass as two bfloat16 numbers, off by 2^-16, for 32-bit outputs as
+three, off by 2^-24; the last rounding by 2^-8 or 2^-24 of the result."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def K():
+    from jax_llm_examples_b200.kernels import api
+
+    return api
+
+
+class Step:
+    def __init__(self, of_row, E, r, k, n, dtype=BF, out_dtype=BF, mixed=False, seed=0, wide=0):
+        gen = torch.Generator().manual_seed(seed)
+        N = len(of_row)
+        rand = lambda *s: torch.randn(s, generator=gen)  # noqa: E731
+        rows = lambda w, t: torch.cat([rand(N, w) * torch.exp(rand(N, 1)), rand(N, wide)], 1).to(t).cuda()[:, :w]  # noqa: E731
+        self.of_row, self.x, self.y = of_row, rows(k, dtype), rows(n, out_dtype)
+        self.a, self.b = (rand(E, r, k) * k ** -0.5).to(dtype).cuda(), (rand(E, n, r)).to(dtype).cuda()
+        self.scale = (0.5 + torch.rand(E, generator=gen)).cuda()
+        self.ranks = torch.tensor([max(0, r - 5 * (e % 4)) for e in range(E)], dtype=torch.int32).cuda() if mixed else None
+        self.plan = K().adapter_plan(of_row, E)
+
+    def run(self, out=None):
+        out = torch.full_like(self.y, float("nan")) if out is None else out
+        K().adapter_add(self.x, self.a, self.b, self.plan, self.y, out, scale=self.scale, ranks=self.ranks)
+        return out
+
+    def want(self):
+        """(The definition, how far a result may be off.)"""
+        y = self.y.double()
+        out, off = y.clone(), torch.zeros_like(y)
+        k, r = self.a.shape[2], self.a.shape[1]
+        between = 0.0 if self.x.dtype == F32 else 2.0 ** -24 if self.y.dtype == F32 else 2.0 ** -16
+        for n, e in enumerate(self.of_row):
+            if e < 0:
+                continue
+            m = r if self.ranks is None else int(self.ranks[e])
+            a, b, x, s = self.a[e, :m].double(), self.b[e, :, :m].double(), self.x[n].double(), self.scale[e].double()
+            out[n] += s * (b @ (a @ x))
+            off[n] = (b.abs() @ (a.abs() @ x.abs())) * s * ((k + r + 4) * 2.0 ** -23 + between)
+        rounds = 2.0 ** -8 if self.y.dtype == BF else 2.0 ** -23  # (32 bits: the addition of y, too)
+        return out, off * (1 + rounds) + rounds * out.abs() + (2.0 ** -24 * y.abs())
+
+    def check(self, got):
+        want, off = self.want()
+        assert bool(((got.double() - want).abs() <= off).all()), float(((got.double() - want).abs() / off).max())
+        none = torch.tensor([e < 0 for e in self.of_row]).cuda()
+        assert torch.equal(got[none], self.y[none])
+
+
+ROWS = {
+    "one": [0], "bare": [-1], "few": [2, 0, 2, -1, 0], "tile": [1] * 16, "tile and one": [1] * 17, "own each": list(range(24)), "shared": [0, 1, 2, -1] * 16,
+    "portions": [3] * 100 + [0] * 64 + [-1] * 33 + [2] * 31 + [1], "steps beside a portion": [4] * 129 + [0, 1, 2, 3, -1, 1, 2],
+}
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("r, k, n, dtype, out_dtype", [
+    (16, 256, 320, BF, BF), (8, 72, 40, BF, F32), (64, 1000, 264, BF, F32), (24, 520, 1032, BF, BF), (128, 264, 128, BF, BF), (200, 136, 96, BF, F32),
+    (256, 512, 64, BF, BF), (13, 100, 77, BF, BF), (1, 8, 8, BF, F32), (4, 129, 33, F32, F32), (64, 512, 300, F32, F32), (16, 64, 64, F32, BF), (8, 1, 1, BF, BF),
+    (32, 2048, 24, BF, BF),
+])
+def test_rows_of_many_adapters(rows, r, k, n, dtype, out_dtype):
+    step = Step(ROWS[rows], 24, r, k, n, dtype, out_dtype, seed=r + k)
+    step.check(step.run())
+
+
+@pytest.mark.parametrize("r", [8, 16, 40, 128, 13])
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+def test_ranks_of_their_own_and_nothing_read_behind_them(r, out_dtype):
+    step = Step(ROWS["steps beside a portion"], 5, r, 264, 136, BF, out_dtype, mixed=True, seed=r)
+    for e in range(5):
+        step.a[e, int(step.ranks[e]):] = float("nan")
+        step.b[e, :, int(step.ranks[e]):] = float("inf")
+    step.check(step.run())
+
+
+@pytest.mark.parametrize("wide", [8, 3])
+@pytest.mark.parametrize("rows", ["few", "portions"])
+def test_column_ranges_of_wider_rows_and_in_place(wide, rows):
+    step = Step(ROWS[rows], 6, 16, 256, 160, wide=wide)
+    want, off = step.want()
+    base = step.y._base if step.y._base is not None else step.y
+    behind = base[:, 160:].clone()
+    K().adapter_add(step.x, step.a, step.b, step.plan, step.y, scale=step.scale)
+    assert bool(((step.y.double() - want).abs() <= off).all())
+    assert torch.equal(base[:, 160:], behind)
+
+
+def test_the_first_of_split_partials():
+    step = Step(ROWS["shared"], 4, 16, 512, 256, BF, F32)
+    parts = torch.stack([step.y, torch.randn_like(step.y)])
+    other, step.y = parts[1].clone(), parts[0]
+    want, off = step.want()
+    K().adapter_add(step.x, step.a, step.b, step.plan, parts[0], scale=step.scale)
+    assert bool(((parts[0].double() - want).abs() <= off).all()) and torch.equal(parts[1], other)
+
+
+@pytest.mark.parametrize("dtype, r", [(BF, 16), (BF, 13), (F32, 8)])
+def test_what_is_not_finite_stays_in_its_row(dtype, r):
+    step = Step([0, 1, 0, 2, 1, -1], 3, r, 264, 136, dtype, dtype)
+    step.x[0, 5], step.x[1, 3] = float("nan"), float("inf")
+    step.b[2] = float("nan")
+    got = step.run()
+    assert bool(got[0].isnan().all()) and bool(got[3].isnan().all()) and not bool(got[1].isfinite().any())
+    for n in (2, 4, 5):
+        assert bool(got[n].isfinite().all())
+
+
+@pytest.mark.parametrize("r, dtype", [(16, BF), (64, BF), (5, F32)])
+def test_the_same_bits_every_time_on_any_stream_and_in_a_graph(r, dtype):
+    step = Step(ROWS["portions"], 4, r, 520, 264, dtype, dtype)
+    want = step.run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [step.run() for _ in range(3)]
+    side.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    outs = [torch.zeros_like(want) for _ in range(2)]
+    graphs = []
+    for out in outs:  # two graphs, replayed beside each other
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step.run(out)
+        graphs.append(g)
+    for g in graphs:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            g.replay()
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_no_rows_and_counted_launches():
+    step = Step([], 2, 8, 64, 64)
+    before = K().launch_count()
+    assert step.run().shape == (0, 64) and K().launch_count() == before
+    Step([0, 1], 2, 8, 64, 64).run()
+    assert K().launch_count() == before + 1
+    Step([0, 1], 2, 8, 63, 64).run()
+    assert K().launch_count() == before + 3
