@@ -1426,6 +1426,85 @@ def tree_masks(parents) -> "tuple[list[int], list[list[int]]]":
     return depth, [[signed(b >> (32 * w) & 0xFFFFFFFF) for w in range(words)] for b in bits]
 
 
+# ------------------------------------------------- a cache kept to a budget: weights, choice, moving the kept rows
+_WEIGHTS_ARGS = struct.Struct("@4P2i")  # WeightsArgs in csrc/attention_weights.cuh
+WEIGHTS_FEW = 16  # query rows of a request and KV head that attention_weights.cu takes
+WEIGHTS_KEYS = 16  # keys of a tile there
+WEIGHTS_HELD = 200 << 10  # bytes of scores that a block keeps in shared memory
+
+
+@functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
+def attention_weights_plan(keys: int, pairs: int, rows: int, sms: int) -> "tuple[int, int, bool]":
+    """(Ranges that a request's keys are cut into, the most keys of one, whether its scores fit shared memory) for so many (request,
+    KV head) pairs of up to so many query rows."""
+    row = 4 * (8 if rows <= 8 else 16)
+    most = lambda s: -(-(keys + WEIGHTS_KEYS) // (WEIGHTS_KEYS * s)) * WEIGHTS_KEYS  # noqa: E731  (ranges start at a tile's first key)
+    splits = 1
+    while splits < 8 and ((pairs * splits < 4 * sms and keys >= 256 * splits) or most(splits) * row > 72 << 10):
+        splits *= 2
+    return splits, most(splits), most(splits) * row <= WEIGHTS_HELD
+
+
+def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor, positions: torch.Tensor, out: torch.Tensor,
+                      scale: float, chunk: int, window: int, attn_scale: float, floor_scale: float, status: torch.Tensor, max_kv_len: int,
+                      max_count: int, scales: torch.Tensor | None = None, sink: torch.Tensor | None = None, slopes: torch.Tensor | None = None,
+                      softcap: float = 0.0, add: torch.Tensor | None = None) -> None:
+    """The weights that every cached key receives: out[r, h, j] = add[r, h, j] + the sum of the softmax weights that request r's
+    query rows, the tokens cu_q[r] .. cu_q[r + 1] of ``q`` with all heads of KV head h's group, give to the key at place j.  Mask, scores and
+    softmax are those of the attention entry points with the same arguments (causal by ``positions``; a row that sees nothing
+    gives nothing).  q: bfloat16 [N, Hq, dh], dh 64 or 128; pages: bfloat16, or float8_e4m3fn with ``scales``; out: float32
+    [R, Hkv, width], written whole; add: float32 of that shape (out itself, to add to what earlier steps left) or None (zeros).
+    ``max_kv_len``, ``max_count``: keys and query tokens of the longest request; a request with more, or with keys beyond ``width``, raises the
+    status and gives nothing.  Keys without a page raise the status and count as zeros.  The order of all sums is fixed."""
+    what = "attention_weights"
+    N, Hq, dh = q.shape
+    P, two, Hkv, page_size, dh2 = pages.shape
+    if q.dtype is not torch.bfloat16:
+        raise KernelError(f"{what}: queries must be bfloat16 [N, Hq, dh]")
+    if dh2 != dh or two != 2:
+        raise KernelError(f"{what}: cache pages {tuple(pages.shape)} and queries {tuple(q.shape)} disagree")
+    if scales is not None:
+        _cache8(what, pages, scales, block_table, Hkv, dh)
+    elif pages.dtype is not torch.bfloat16:
+        raise KernelError(f"{what}: pages must be bfloat16, or float8_e4m3fn with scales")
+    elif block_table.dtype is not torch.int32 or block_table.dim() != 2:
+        raise KernelError(f"{what}: the block table must be int32 [requests, pages of one]")
+    R, width = block_table.shape
+    _ints(what, ("cu_q", cu_q, R + 1), ("positions", positions, N), ("status", status, 1))
+    if out.dtype is not torch.float32 or out.dim() != 3 or out.shape[:2] != (R, Hkv):
+        raise KernelError(f"{what}: out must be float32 [{R}, {Hkv}, places], not {out.dtype} {tuple(out.shape)}")
+    if add is not None and (add.dtype is not torch.float32 or add.shape != out.shape or (add.data_ptr() != out.data_ptr() and _overlap(add, out))):
+        raise KernelError(f"{what}: add must be float32 {tuple(out.shape)}, out itself or apart from it")
+    if max_kv_len < 1 or max_count < 1:
+        raise KernelError(f"{what}: {max_count} tokens of a request over {max_kv_len} keys")
+    if sink is not None:
+        _check_sink(sink, Hq)
+    if slopes is not None:
+        _check_sink(slopes, Hq, "slopes")
+    dev = _placed(what, q, pages, scales, block_table, cu_q, positions, out, add, status, sink, slopes)
+    if out.numel() == 0:
+        return
+    if N == 0:
+        if add is None:
+            out.zero_()
+        elif add.data_ptr() != out.data_ptr():
+            out.copy_(add)
+        return
+    if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
+        raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
+    rows, keys = max_count * (Hq // Hkv), _keys_seen(max_kv_len, chunk, window, max_count)
+    if rows > WEIGHTS_FEW:
+        raise KernelError(f"{what}: {rows} query rows of a KV head are not supported (up to {WEIGHTS_FEW})")
+    splits, most, fits = attention_weights_plan(keys, R * Hkv, rows, sm_count())
+    # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
+    scratch = None if fits else torch.empty(R * Hkv * splits * most * (8 if rows <= 8 else 16), dtype=torch.float32, device=q.device)
+    args = _ROWS_ARGS.pack(q.data_ptr(), pages.data_ptr(), _address(scales), block_table.data_ptr(), 0, positions.data_ptr(), 0, 0, 0, 0, 0, 0, _address(sink),
+                           _address(slopes), 0, 0, status.data_ptr(), width, R, R, max_count, 0, N, Hq, Hkv, dh, page_size, P, chunk, window, splits, 0, 0,
+                           scale, softcap, attn_scale, floor_scale)
+    more = _WEIGHTS_ARGS.pack(cu_q.data_ptr(), _address(add), out.data_ptr(), _address(scratch), out.shape[2], max_kv_len)
+    _run("attention_weights", "jlx_attention_weights", args, more, rows, splits, most, _raw_stream(dev))
+
+
 # ------------------------------------------------------------------------------------- GEMMs
 GEMM_FORMS = {"rule": 0, "general": 1, "tile": 2, "rows": 3}  # csrc/gemm_simt.cu
 

@@ -1,0 +1,219 @@
+"""The weights that cached keys receive, from few query rows, against the definition in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from .budget_helpers import received
+from .fp8_helpers import Case, assert_close, two_to
+
+pytestmark = pytest.mark.gpu
+
+
+def K():
+    from jax_llm_examples_b200.kernels import api
+
+    return api
+
+
+def run(c, width=None, add=None, out=None, cu_q=None, max_kv=None, max_count=None, status=None, chunk=0, window=0, temper=0.0, floor=1.0, sink=None, slopes=None,
+        cap=0.0):
+    width = width or max(a + b for a, b in zip(c.n, c.held))
+    out = torch.full((len(c.n), c.Hkv, width), math.nan, device="cuda") if out is None else out
+    K().attention_weights(c.q, c.pages, c.table, c.cu_q if cu_q is None else cu_q, c.positions, out, c.scale, chunk, window, temper, floor,
+                          c.status if status is None else status, max_kv or max(a + b for a, b in zip(c.n, c.held)), max_count or max(c.n), scales=c.scales,
+                          sink=sink, slopes=slopes, softcap=cap, add=add)
+    return out
+
+
+# (tokens of each request, keys before them, query heads, KV heads, head size, page)
+STEPS = {
+    "one of one": ([1], [0], 8, 8, 128, 16),
+    "one": ([1], [699], 40, 8, 128, 64),
+    "ragged": ([1, 1, 1, 1, 1], [0, 15, 16, 300, 1023], 40, 8, 128, 64),
+    "small heads": ([1, 1, 1], [64, 517, 90], 16, 4, 64, 48),
+    "group of 16": ([1, 1], [333, 12], 32, 2, 128, 16),
+    "no group": ([1, 1], [250, 77], 6, 6, 64, 7),
+    "three tokens": ([3, 3, 1], [100, 513, 31], 16, 4, 128, 32),
+    "long": ([1], [9000], 8, 2, 128, 64),
+    "some without": ([1, 0, 2, 0], [5, 40, 700, 0], 8, 4, 64, 16),
+}
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("step", STEPS)
+def test_few_rows(step, bits8):
+    n, held, Hq, Hkv, dh, page = STEPS[step]
+    c = Case(n, held, Hq, Hkv, dh, page, seed=len(step), bits8=bits8).to_device()
+    want, tol = received(c)
+    assert_close(run(c), want, tol)
+    assert int(c.status) == 0
+
+
+MASKS = {
+    "chunk": dict(chunk=128), "window": dict(window=77), "both": dict(chunk=256, window=100), "temperature": dict(temper=0.1, floor=64.0), "cap": dict(cap=5.0),
+    "sink": dict(sink=True), "slopes": dict(slopes=True), "all": dict(window=200, temper=0.2, floor=32.0, cap=20.0, sink=True, slopes=True),
+}
+
+
+def _masks(c, mask):
+    gen = torch.Generator().manual_seed(3)
+    a = dict(MASKS[mask])
+    if a.get("sink"):
+        a["sink"] = torch.randn(c.Hq, generator=gen).cuda()
+    if a.get("slopes"):
+        a["slopes"] = (0.1 * torch.rand(c.Hq, generator=gen)).cuda()
+    return a
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("mask", MASKS)
+def test_masks_and_scores_of_few_rows(mask, bits8):
+    c = Case([1, 2, 1], [400, 300, 20], 16, 4, 64, 16, seed=5, bits8=bits8).to_device()
+    a = _masks(c, mask)
+    want, tol = received(c, **a)
+    assert_close(run(c, **a), want, tol)
+
+
+@pytest.mark.parametrize("n", [[1, 1]])
+def test_adds_to_what_is_there_and_writes_every_place(n):
+    c = Case(n, [130, 57], 8, 4, 128, 16, bits8=False).to_device()
+    width = 200
+    add = torch.rand((2, 4, width), generator=torch.Generator().manual_seed(1)).cuda()
+    want, tol = received(c, add=add, width=width)
+    assert_close(run(c, width=width, add=add), want, tol)
+    assert torch.equal(run(c, width=width, add=add)[:, :, 150:], add[:, :, 150:])
+    assert_close(run(c, width=width), *received(c, width=width))
+    there = add.clone()
+    run(c, width=width, add=there, out=there)
+    assert_close(there, want, tol)
+
+
+def test_a_row_that_sees_nothing_gives_nothing():
+    c = Case([1, 1], [50, 60], 8, 4, 64, 16, bits8=False)
+    c.positions[0] = -1
+    c.to_device()
+    want, tol = received(c)
+    assert float(want[0].sum()) == 0
+    for sink in (None, torch.zeros(8, device="cuda")):
+        got = run(c, sink=sink)
+        assert float(got[0].abs().sum()) == 0 and not bool(got.isnan().any())
+    assert_close(run(c), want, tol)
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("n", [[1, 1]])
+def test_what_is_masked_may_be_anything(n, bits8):
+    """Keys behind the last one and before the window hold infinities and NaN."""
+    c = Case(n, [200, 100], 8, 4, 128, 16, seed=2, bits8=bits8)
+    window = 60
+    want, tol = received(c, window=window)
+    for r in range(2):
+        for place in list(range(c.held[r] - window)) + list(range(c.held[r] + c.n[r], -(-(c.held[r] + c.n[r]) // 16) * 16)):
+            page = int(c.table[r, place // 16])
+            if bits8:
+                c.scales[page, :, :, place % 16] = 255
+            else:
+                c.pages[page, :, :, place % 16] = math.nan if place % 2 else math.inf
+    c.to_device()
+    assert_close(run(c, window=window), want, tol)
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("n", [[1, 1]])
+def test_a_visible_nan_spoils_its_rows_only(n, bits8):
+    c = Case(n, [90, 100], 8, 4, 64, 16, seed=2, bits8=bits8)
+    page, at = int(c.table[1, 2]), 5
+    if bits8:
+        c.scales[page, 0, 1, at] = 255
+    else:
+        c.pages[page, 0, 1, at] = math.nan
+    c.to_device()
+    got = run(c)
+    assert bool(got[1, 1, :c.held[1] + 1].isnan().all())
+    bad = got.isnan()
+    bad[1, 1] = False
+    assert not bool(bad.any())
+
+
+@pytest.mark.parametrize("n", [[1, 1]])
+def test_missing_pages_are_zeros_and_raise_the_status(n):
+    c = Case(n, [100, 100], 8, 4, 128, 16, bits8=False)
+    c.rows[c.table[0, 1].long()] = 0
+    want, tol = received(c)
+    c.table[0, 1] = 10000
+    c.to_device()
+    assert_close(run(c), want, tol)
+    assert int(c.status) == 1
+    c.status.zero_()
+    # beyond what any row sees nothing is looked at
+    c.table[0, -1] = -5
+    c.table[0, 1] = 3
+    run(c)
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("n", [[1, 1]])
+def test_more_than_the_call_was_sized_for_gives_nothing(n):
+    c = Case(n, [2000, 30], 8, 4, 128, 16, bits8=False).to_device()
+    want, tol = received(c)
+    add = torch.rand_like(want, dtype=torch.float32).cuda()
+    for change in (dict(max_kv=100), dict(cu_q=torch.tensor([0, c.N + 1, c.N], dtype=torch.int32).cuda())):
+        c.status.zero_()
+        got = run(c, add=add, **change)
+        assert torch.equal(got[0], add[0]) and int(c.status) == 1
+    c.status.zero_()
+    got = run(c, width=100)
+    assert float(got[0].abs().sum()) == 0 and int(c.status) == 1
+    assert_close(got[1], want[1, :, :100], tol[1, :, :100])
+
+
+def test_a_range_too_long_for_shared_memory():
+    c = Case([1], [60000], 4, 1, 64, 64, bits8=False, spread=0.3).to_device()
+    _, _, fits = K().attention_weights_plan(60001, 1, 4, 148)
+    assert not fits
+    want, tol = received(c)
+    assert_close(run(c), want, tol)
+
+
+@pytest.mark.parametrize("n", [[1, 1, 1]])
+def test_the_same_bits_every_time_on_any_stream_and_in_graphs(n):
+    c = Case(n, [700, 100, 1300], 16, 4, 128, 64, bits8=False).to_device()
+    want = run(c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [run(c) for _ in range(3)]
+    side.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    outs, graphs = [torch.zeros_like(want) for _ in range(2)], []
+    for out in outs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(c, out=out)
+        graphs.append(g)
+    for g in graphs:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            g.replay()
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_keys_that_were_never_written_weigh_as_zeros():
+    c = Case([1], [40], 8, 4, 64, 16, bits8=True)
+    page = int(c.table[0, 1])
+    c.scales[page], c.pages[page] = 0, torch.zeros_like(c.pages[page].float()).to(c.pages.dtype)
+    c.rows[page] = 0
+    want, tol = received(c)
+    assert_close(run(c.to_device()), want, tol)
+
+
+def test_extremes_of_an_8_bit_rows_scale():
+    c = Case([1], [100], 8, 4, 128, 16, bits8=True, seed=4)
+    for i, e in enumerate((-60, -30, 6)):
+        c.scales[int(c.table[0, i])] = e + 127
+        c.rows[int(c.table[0, i])] = c.pages[int(c.table[0, i])].double() * two_to(torch.tensor(e))
+    want, tol = received(c)
+    assert_close(run(c.to_device()), want, tol)
