@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(THREADS) attention_weights_kernel(const Weight
   // equal ranges of whole tiles
   const int per = max((end_all - start + KT * P.splits - 1) / (KT * P.splits), 0) * KT, range0 = start + split * per;
   const int begin = max(first, range0), end = min(end_all, range0 + per), tiles = end > begin ? (end - range0 + KT - 1) / KT : 0;
-  if (per > P.buf_keys || end_all > P.W.width || it.cnt * G > ROWS) {  // more keys than the call was sized for: the whole cluster leaves
+  if (end_all > min(P.W.max_kv, P.W.width) || per > P.buf_keys || it.cnt * G > ROWS) {  // more keys than the call was sized for: the whole cluster leaves
     if (tid == 0) atomicOr(P.R.status, JLX_STATUS_BAD_PAGE);
     weights_copy(P, row, 0, P.W.width, everyone, all);
     return;

@@ -1430,6 +1430,7 @@ def tree_masks(parents) -> "tuple[list[int], list[list[int]]]":
 _WEIGHTS_ARGS = struct.Struct("@4P2i")  # WeightsArgs in csrc/attention_weights.cuh
 WEIGHTS_FEW = 16  # query rows of a request and KV head that attention_weights.cu takes
 WEIGHTS_KEYS = 16  # keys of a tile there
+WEIGHTS_TILE = 128  # keys, and query rows, of a tile in attention_weights_tc.cu
 WEIGHTS_HELD = 200 << 10  # bytes of scores that a block keeps in shared memory
 
 
@@ -1443,6 +1444,14 @@ def attention_weights_plan(keys: int, pairs: int, rows: int, sms: int) -> "tuple
     while splits < 8 and ((pairs * splits < 4 * sms and keys >= 256 * splits) or most(splits) * row > 72 << 10):
         splits *= 2
     return splits, most(splits), most(splits) * row <= WEIGHTS_HELD
+
+
+def _weights_shares(units: int, tiles: int, blocks: int) -> int:
+    """Blocks that share the tiles passing by one of so many units, for about so many blocks in all."""
+    shares = 1
+    while shares < 8 and units * shares < blocks and tiles >= 4 * shares:
+        shares *= 2
+    return shares
 
 
 def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor, positions: torch.Tensor, out: torch.Tensor,
@@ -1493,16 +1502,25 @@ def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.T
     if not attention_rows_supported(q.dtype, Hq, Hkv, dh):
         raise KernelError(f"{what}: {Hq} query heads on {Hkv} of {dh} entries (64 or 128) are not supported")
     rows, keys = max_count * (Hq // Hkv), _keys_seen(max_kv_len, chunk, window, max_count)
+    # scratch is made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
     if rows > WEIGHTS_FEW:
-        raise KernelError(f"{what}: {rows} query rows of a KV head are not supported (up to {WEIGHTS_FEW})")
-    splits, most, fits = attention_weights_plan(keys, R * Hkv, rows, sm_count())
-    # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
-    scratch = None if fits else torch.empty(R * Hkv * splits * most * (8 if rows <= 8 else 16), dtype=torch.float32, device=q.device)
+        q_tiles = -(-rows // WEIGHTS_TILE)
+        scratch = torch.empty(_up4(2 * N * Hq) + 4 * R * q_tiles, dtype=torch.float32, device=q.device)
+    else:
+        splits, most, fits = attention_weights_plan(keys, R * Hkv, rows, sm_count())
+        scratch = None if fits else torch.empty(R * Hkv * splits * most * (8 if rows <= 8 else 16), dtype=torch.float32, device=q.device)
     args = _ROWS_ARGS.pack(q.data_ptr(), pages.data_ptr(), _address(scales), block_table.data_ptr(), 0, positions.data_ptr(), 0, 0, 0, 0, 0, 0, _address(sink),
-                           _address(slopes), 0, 0, status.data_ptr(), width, R, R, max_count, 0, N, Hq, Hkv, dh, page_size, P, chunk, window, splits, 0, 0,
+                           _address(slopes), 0, 0, status.data_ptr(), width, R, R, max_count, 0, N, Hq, Hkv, dh, page_size, P, chunk, window, 1, 0, 0,
                            scale, softcap, attn_scale, floor_scale)
     more = _WEIGHTS_ARGS.pack(cu_q.data_ptr(), _address(add), out.data_ptr(), _address(scratch), out.shape[2], max_kv_len)
-    _run("attention_weights", "jlx_attention_weights", args, more, rows, splits, most, _raw_stream(dev))
+    if rows <= WEIGHTS_FEW:
+        _run("attention_weights", "jlx_attention_weights", args, more, rows, splits, most, _raw_stream(dev))
+        return
+    blocks = 4 * sm_count()  # two rounds of them
+    _run("attention_weights_tc", "jlx_attention_weights_tc", args, more, _weights_shares(R * Hkv * q_tiles, -(-keys // WEIGHTS_TILE), blocks),
+         _weights_shares(R * Hkv * -(-max_kv_len // WEIGHTS_TILE), q_tiles, blocks), _raw_stream(dev))
+    global _launches
+    _launches += 1  # two kernels
 
 
 # ------------------------------------------------------------------------------------- GEMMs

@@ -1,4 +1,4 @@
-"""The weights that cached keys receive, from few query rows, against the definition in 64 bits."""
+"""The weights that cached keys receive, from single tokens, last tokens of prompts and whole portions, against the definition in 64 bits."""
 
 import math
 
@@ -76,7 +76,7 @@ def test_masks_and_scores_of_few_rows(mask, bits8):
     assert_close(run(c, **a), want, tol)
 
 
-@pytest.mark.parametrize("n", [[1, 1]])
+@pytest.mark.parametrize("n", [[1, 1], [2, 1]])
 def test_adds_to_what_is_there_and_writes_every_place(n):
     c = Case(n, [130, 57], 8, 4, 128, 16, bits8=False).to_device()
     width = 200
@@ -103,7 +103,7 @@ def test_a_row_that_sees_nothing_gives_nothing():
 
 
 @pytest.mark.parametrize("bits8", [False, True])
-@pytest.mark.parametrize("n", [[1, 1]])
+@pytest.mark.parametrize("n", [[1, 1], [40, 3]])
 def test_what_is_masked_may_be_anything(n, bits8):
     """Keys behind the last one and before the window hold infinities and NaN."""
     c = Case(n, [200, 100], 8, 4, 128, 16, seed=2, bits8=bits8)
@@ -121,7 +121,7 @@ def test_what_is_masked_may_be_anything(n, bits8):
 
 
 @pytest.mark.parametrize("bits8", [False, True])
-@pytest.mark.parametrize("n", [[1, 1]])
+@pytest.mark.parametrize("n", [[1, 1], [20, 2]])
 def test_a_visible_nan_spoils_its_rows_only(n, bits8):
     c = Case(n, [90, 100], 8, 4, 64, 16, seed=2, bits8=bits8)
     page, at = int(c.table[1, 2]), 5
@@ -137,7 +137,7 @@ def test_a_visible_nan_spoils_its_rows_only(n, bits8):
     assert not bool(bad.any())
 
 
-@pytest.mark.parametrize("n", [[1, 1]])
+@pytest.mark.parametrize("n", [[1, 1], [30, 1]])
 def test_missing_pages_are_zeros_and_raise_the_status(n):
     c = Case(n, [100, 100], 8, 4, 128, 16, bits8=False)
     c.rows[c.table[0, 1].long()] = 0
@@ -154,7 +154,7 @@ def test_missing_pages_are_zeros_and_raise_the_status(n):
     assert int(c.status) == 0
 
 
-@pytest.mark.parametrize("n", [[1, 1]])
+@pytest.mark.parametrize("n", [[1, 1], [30, 30]])
 def test_more_than_the_call_was_sized_for_gives_nothing(n):
     c = Case(n, [2000, 30], 8, 4, 128, 16, bits8=False).to_device()
     want, tol = received(c)
@@ -177,7 +177,7 @@ def test_a_range_too_long_for_shared_memory():
     assert_close(run(c), want, tol)
 
 
-@pytest.mark.parametrize("n", [[1, 1, 1]])
+@pytest.mark.parametrize("n", [[1, 1, 1], [70, 3, 33]])
 def test_the_same_bits_every_time_on_any_stream_and_in_graphs(n):
     c = Case(n, [700, 100, 1300], 16, 4, 128, 64, bits8=False).to_device()
     want = run(c)
@@ -217,3 +217,73 @@ def test_extremes_of_an_8_bit_rows_scale():
         c.rows[int(c.table[0, i])] = c.pages[int(c.table[0, i])].double() * two_to(torch.tensor(e))
     want, tol = received(c)
     assert_close(run(c.to_device()), want, tol)
+
+
+# ------------------------------------------------------------------------------------------------------------- many rows
+MANY = {
+    "one tile": ([16], [0], 8, 1, 128, 16),
+    "a portion": ([150], [0], 10, 2, 128, 64),
+    "behind others": ([77], [300], 8, 4, 64, 48),
+    "ragged": ([40, 1, 0, 130, 33], [500, 129, 7, 0, 63], 8, 2, 128, 32),
+    "one row too many": ([17], [400], 4, 4, 64, 7),
+    "group of 5": ([52, 26], [260, 1000], 10, 2, 128, 64),
+    "short requests": ([9] * 6, [3 * i for i in range(6)], 16, 4, 64, 16),
+    "long": ([20], [5000], 4, 2, 128, 64),
+}
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("step", MANY)
+def test_many_rows(step, bits8):
+    n, held, Hq, Hkv, dh, page = MANY[step]
+    c = Case(n, held, Hq, Hkv, dh, page, seed=len(step), bits8=bits8).to_device()
+    assert max(n) * Hq // Hkv > K().WEIGHTS_FEW
+    want, tol = received(c)
+    assert_close(run(c), want, tol)
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("mask", MASKS)
+def test_masks_and_scores_of_many_rows(mask, bits8):
+    c = Case([150, 2, 40], [200, 300, 20], 8, 4, 64, 16, seed=5, bits8=bits8).to_device()
+    a = _masks(c, mask)
+    want, tol = received(c, **a)
+    assert_close(run(c, **a), want, tol)
+
+
+def test_only_the_last_rows_of_a_prompt():
+    c = Case([100, 64], [50, 0], 8, 4, 64, 16, bits8=False).to_device()
+    want, tol = received(c, rows=32)
+    q, p = torch.cat([c.q[68:100], c.q[132:]]), torch.cat([c.positions[68:100], c.positions[132:]])
+    c.q, c.positions, c.cu_q = q.contiguous(), p.contiguous(), torch.tensor([0, 32, 64], dtype=torch.int32).cuda()
+    assert_close(run(c, max_count=32), want, tol)
+
+
+def test_positions_in_any_order():
+    c = Case([90], [0], 8, 2, 64, 16, bits8=False)
+    c.positions = c.positions[torch.randperm(90, generator=torch.Generator().manual_seed(1))].contiguous()
+    c.positions[7] = -3
+    want, tol = received(c)
+    assert_close(run(c.to_device()), want, tol)
+
+
+def test_pages_that_a_window_has_left_behind_are_not_asked_for():
+    c = Case([40, 1], [500, 300], 8, 4, 64, 16, bits8=False)
+    for r in range(2):
+        c.table[r, :(c.held[r] - 64) // 16] = -1
+    want, tol = received(Case([40, 1], [500, 300], 8, 4, 64, 16, bits8=False), window=64)
+    c.to_device()
+    assert_close(run(c, window=64), want, tol)
+    assert int(c.status) == 0
+
+
+def test_a_few_rows_as_many_rows_gives_them(monkeypatch):
+    """Either kernel on the same rows."""
+    c = Case([2, 4], [300, 129], 8, 2, 128, 16, bits8=False).to_device()
+    want, tol = received(c)
+    few = run(c)
+    monkeypatch.setattr(K(), "WEIGHTS_FEW", 0)
+    many = run(c)
+    assert_close(few, want, tol)
+    assert_close(many, want, tol)
