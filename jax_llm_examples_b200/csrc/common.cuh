@@ -19,6 +19,7 @@ enum {
   JLX_STATUS_BAD_TOKEN = 2,     // a token id outside the vocabulary
   JLX_STATUS_BAD_EXPERT = 4,    // a routed expert index outside the expert count
   JLX_STATUS_WAIT_TIMEOUT = 8,  // a bounded wait on a barrier gave up
+  JLX_STATUS_BAD_LENGTH = 16,   // a length or a number of places outside its array
 };
 
 static thread_local char jlx_error_text[512] = "";

@@ -1,0 +1,339 @@
+// A paged cache kept to a budget: which places a request and KV head keep (kv_choose), and moving the kept rows of keys and values to the
+// front of the request's pages or of other pages (kv_compact).
+//
+// kv_choose, of a request's L places and n = min(keep, L): the last `recent` ones, then the first `first` ones, as far as n goes, then of the
+// rest those with the largest sums; ties go to the lowest place; NaN counts as the lowest sum, -0 as 0.  Places come in ascending
+// order.  A sum becomes a whole number of 32 bits with the same order; the bits of the smallest kept one are found eight at a time
+// by counting (a digit's count of the places that share the digits before it), and one pass over the places writes what is above it
+// and the first so many that equal it.  A cluster of blocks serves a request and KV head, each with a stretch of the places in
+// shared memory: the sums are read from memory once.
+//
+// kv_compact moves rows bit for bit.  Into other pages every row is on its own.  In place, row i's new place is at or before its old
+// one: a block takes a column of 32 bytes of one plane's rows through all places in order, some hundreds at a time, all loads of
+// which precede all stores; a later row's source lies behind what has been written.
+//
+// Both are bound by bytes, few in the first, so there by the chain of its passes.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+#define THREADS 512
+#define WARPS (THREADS / 32)
+#define MAX_CLUSTER 8
+#define HELD (200 * 1024 / 4)  // sums that a block holds in shared memory at most
+
+struct ChooseArgs {  // _CHOOSE_ARGS in kernels/api.py
+  const float* sums;   // [R, H, width]
+  const int* lengths;  // [R]
+  const int* keep;     // [R]
+  int* places;         // [R, H, most]
+  int* counts;         // [R]
+  int* status;
+  int R, H, width, most, first, recent;
+};
+
+// Larger numbers for larger sums; 0 for NaN (no number has it).
+__device__ __forceinline__ uint32_t ordered(float x) {
+  if (x != x) return 0u;
+  const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// The sum of a number over the threads before this one, and over all of them.
+__device__ __forceinline__ int2 block_scan(int v, int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const int s = warp_sums[w];
+    before += w < warp ? s : 0;
+    all += s;
+  }
+  return make_int2(before + x - v, all);
+}
+
+// per: places of a block.  HOLDS: they are kept in shared memory (else read again from memory in every pass).
+template <bool HOLDS>
+__global__ void __launch_bounds__(THREADS) kv_choose_kernel(const ChooseArgs P, int per) {
+  JLX_TL(TL_OTHER);
+  extern __shared__ uint32_t held[];
+  __shared__ int count[256], warp_sums[WARPS], found[2], mine[2];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks(), me = cluster.block_rank(), tid = threadIdx.x;
+  pdl_launch_dependents_if_small();
+  pdl_wait();
+  const int row = blockIdx.y, r = row / P.H;
+  int L = P.lengths[r], n = P.keep[r];
+  if (L < 0 || L > P.width || n < 0 || min(n, L) > P.most) {
+    if (tid == 0) atomicOr(P.status, JLX_STATUS_BAD_LENGTH);
+    L = min(max(L, 0), P.width);
+  }
+  n = min(min(max(n, 0), L), P.most);
+  const int recent = min(P.recent, n), first = min(P.first, n - recent), want = n - recent - first;  // want: chosen by their sums
+  if (me == 0 && tid == 0 && row == r * P.H) P.counts[r] = n;
+  const float* sums = P.sums + (size_t)row * P.width;
+  int* places = P.places + (size_t)row * P.most;
+  for (int i = n + me * THREADS + tid; i < P.most; i += blocks * THREADS) places[i] = -1;
+  // this block's places [p0, p1); of them [q0, q1) are a matter of choice
+  const int p0 = min(me * per, L), p1 = min(p0 + per, L), q0 = min(max(p0, first), p1), q1 = max(min(p1, L - recent), q0);
+  auto key = [&](int p) { return HOLDS ? held[p - p0] : ordered(sums[p]); };
+  if (HOLDS)
+    for (int p = q0 + tid; p < q1; p += THREADS) held[p - p0] = ordered(sums[p]);
+  __syncthreads();
+  // the smallest sum that is chosen, and how many of the places with just that one
+  uint32_t edge = 0u, mask = 0u;
+  int left = want;
+  if (want > 0 && want < L - recent - first) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) count[tid] = 0;
+      __syncthreads();
+      for (int p = q0 + tid; p < q1; p += THREADS) {
+        const uint32_t k = key(p);
+        if ((k & mask) == edge) atomicAdd(&count[k >> shift & 255], 1);
+      }
+      cluster.sync();
+      // digits from the largest: thread i has digit 255 - i
+      int c = 0;
+      if (tid < 256)
+        for (int q = 0; q < blocks; ++q) c += *cluster.map_shared_rank(&count[255 - tid], q);
+      const int above = block_scan(c, warp_sums).x;
+      if (tid < 256 && above < left && above + c >= left) {
+        found[0] = 255 - tid;
+        found[1] = left - above;
+      }
+      cluster.sync();  // (the counts have been read everywhere)
+      edge |= (uint32_t)found[0] << shift;
+      mask |= 255u << shift;
+      left = found[1];
+    }
+  }
+  const bool all = want >= L - recent - first;
+  // ---- how many of this block's places are above the edge, and how many equal it
+  auto above_edge = [&](uint32_t k) { return all || (want > 0 && k > edge); };
+  auto at_edge = [&](uint32_t k) { return !all && want > 0 && k == edge; };
+  int a = 0, e = 0;
+  for (int p = q0 + tid; p < q1; p += THREADS) {
+    const uint32_t k = key(p);
+    a += above_edge(k);
+    e += at_edge(k);
+  }
+  a = block_scan(a, warp_sums).y;
+  e = block_scan(e, warp_sums).y;
+  if (tid == 0) {
+    mine[0] = a;
+    mine[1] = e;
+  }
+  cluster.sync();
+  int equal = 0, at = 0;  // places equal to the edge, and kept places, before this block's
+  for (int q = 0; q < me; ++q) {
+    const int qa = *cluster.map_shared_rank(&mine[0], q), qe = *cluster.map_shared_rank(&mine[1], q);
+    const int forced0 = min(q * per, L), forced1 = min(forced0 + per, L);
+    at += qa + max(min(left, equal + qe) - min(left, equal), 0);
+    at += max(min(forced1, first) - forced0, 0) + max(forced1 - max(forced0, L - recent), 0);
+    equal += qe;
+  }
+  // ---- in order, THREADS at a time
+  for (int base = p0; base < p1; base += THREADS) {
+    const int p = base + tid;
+    bool keep = false, same = false;
+    if (p < p1) {
+      if (p < first || p >= L - recent) {
+        keep = true;
+      } else {
+        const uint32_t k = key(p);
+        keep = above_edge(k);
+        same = at_edge(k);
+      }
+    }
+    const int2 s = block_scan(same, warp_sums);
+    keep |= same && equal + s.x < left;
+    const int2 k = block_scan(keep, warp_sums);
+    if (keep) places[at + k.x] = p;
+    equal += s.y;
+    at += k.y;
+  }
+  cluster.sync();  // (a block's shared memory stays until the others have read it)
+}
+
+// -------------------------------------------------------------------------------------------- moving
+struct CompactArgs {  // _COMPACT_ARGS in kernels/api.py
+  uint8_t* pages;         // [P, 2, H, page, row_bytes]
+  uint8_t* scales;        // [P, 2, H, page] or null
+  const int* table;       // [R, table_width] where the rows are
+  const int* into;        // [R, into_width] where they go
+  const int* places;      // [R, H, most]
+  const int* counts;      // [R]
+  const float* sums;      // [R, H, width] or null
+  float* sums_out;        // [R, H, out_width]
+  int* status;
+  int R, H, page, num_pages, row_bytes, table_width, into_width, most, width, out_width;
+};
+
+// The flat row of a place's key (values H * page further), or -1.
+__device__ __forceinline__ int compact_row(const CompactArgs& P, const int* table, int width, int h, int place) {
+  const int pi = place < 0 ? width : place / P.page;
+  const int page = pi < width ? table[pi] : -1;
+  return page >= 0 && page < P.num_pages ? (page * 2 * P.H + h) * P.page + (place - pi * P.page) : -1;
+}
+// Where row i of head h comes from and goes to; false (and the status): a page is missing, or (in place) the row would move back.
+__device__ __forceinline__ bool compact_move(const CompactArgs& P, int r, int h, int i, bool in_place, int& src, int& dst) {
+  const int place = P.places[((size_t)r * P.H + h) * P.most + i];
+  src = compact_row(P, P.table + (size_t)r * P.table_width, P.table_width, h, place);
+  dst = compact_row(P, P.into + (size_t)r * P.into_width, P.into_width, h, i);
+  if (src < 0 || dst < 0 || (in_place && place < i)) {
+    atomicOr(P.status, JLX_STATUS_BAD_PAGE);
+    return false;
+  }
+  return true;
+}
+__device__ __forceinline__ int compact_count(const CompactArgs& P, int r) { return min(max(P.counts[r], 0), P.most); }
+
+// Sums of a request and head: a block, all loads of a stretch before its stores (sums and sums_out may be one).
+__device__ __forceinline__ void compact_sums(const CompactArgs& P, int row) {
+  const int r = row / P.H, n = min(compact_count(P, r), P.out_width);
+  const float* from = P.sums + (size_t)row * P.width;
+  float* to = P.sums_out + (size_t)row * P.out_width;
+  const bool in_place = to == from;
+  for (int base = 0; base < P.out_width; base += THREADS) {
+    const int i = base + threadIdx.x;
+    float v = 0.f;
+    if (i < n) {
+      const int place = P.places[(size_t)row * P.most + i];
+      if (place >= 0 && place < P.width && !(in_place && place < i)) v = from[place];
+      else atomicOr(P.status, JLX_STATUS_BAD_PAGE);
+    }
+    if (in_place) __syncthreads();
+    if (i < P.out_width) to[i] = v;
+    if (in_place) __syncthreads();
+  }
+}
+
+// Into other pages: 16 bytes a thread, a row's chunks side by side.  The last grid row moves sums.
+__global__ void __launch_bounds__(THREADS) kv_compact_kernel(const CompactArgs P, int rows_per_block) {
+  JLX_TL(TL_KV_STORE);
+  pdl_launch_dependents_if_small();
+  pdl_wait();
+  const int row = blockIdx.y, r = row / P.H, h = row - r * P.H;
+  if (blockIdx.x == gridDim.x - 1) {
+    if (P.sums) compact_sums(P, row);
+    return;
+  }
+  const int n = compact_count(P, r), chunks = P.row_bytes / 16;
+  const int i0 = blockIdx.x * rows_per_block, i1 = min(i0 + rows_per_block, n);
+  for (int x = threadIdx.x; x < (i1 - i0) * chunks; x += THREADS) {
+    const int i = i0 + x / chunks, c = x - (i - i0) * chunks;
+    int src, dst;
+    if (!compact_move(P, r, h, i, false, src, dst)) continue;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const size_t s = (size_t)src + w * P.H * P.page, d = (size_t)dst + w * P.H * P.page;
+      reinterpret_cast<uint4*>(P.pages)[d * chunks + c] = reinterpret_cast<const uint4*>(P.pages)[s * chunks + c];
+      if (P.scales && c == 0) P.scales[d] = P.scales[s];
+    }
+  }
+}
+
+// In place: a block has a column of 16 or 32 bytes of a plane (grid x: the columns, the scales, the sums).
+__global__ void __launch_bounds__(THREADS) kv_compact_in_place_kernel(const CompactArgs P, int columns) {
+  JLX_TL(TL_KV_STORE);
+  constexpr int AT_ONCE = 4;
+  pdl_launch_dependents_if_small();
+  pdl_wait();
+  const int row = blockIdx.y, r = row / P.H, h = row - r * P.H;
+  if (blockIdx.x == 2 * columns + 2) {
+    if (P.sums) compact_sums(P, row);
+    return;
+  }
+  const int n = compact_count(P, r), plane = blockIdx.x & 1, column = blockIdx.x >> 1;
+  const size_t off = (size_t)plane * P.H * P.page;
+  if (column == columns) {  // a byte a row
+    if (!P.scales) return;
+    for (int base = 0; base < n; base += THREADS) {
+      const int i = base + threadIdx.x;
+      int src, dst;
+      const bool moves = i < n && compact_move(P, r, h, i, true, src, dst);
+      const uint8_t v = moves ? P.scales[src + off] : 0;
+      __syncthreads();
+      if (moves) P.scales[dst + off] = v;
+      __syncthreads();
+    }
+    return;
+  }
+  const int chunks = P.row_bytes / 16, wide = P.row_bytes % 32 == 0 ? 2 : 1, per = THREADS / wide;
+  const int c = column * wide + threadIdx.x % wide, first = threadIdx.x / wide;
+  for (int base = 0; base < n; base += per * AT_ONCE) {
+    uint4 v[AT_ONCE];
+    int to[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = base + u * per + first;
+      int src, dst;
+      to[u] = -1;
+      if (i < n && compact_move(P, r, h, i, true, src, dst)) {
+        to[u] = dst;
+        v[u] = reinterpret_cast<const uint4*>(P.pages)[((size_t)src + off) * chunks + c];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+      if (to[u] >= 0) reinterpret_cast<uint4*>(P.pages)[((size_t)to[u] + off) * chunks + c] = v[u];
+    __syncthreads();
+  }
+}
+
+// -------------------------------------------------------------------------------------------- host
+JLX_API int jlx_kv_choose(const ChooseArgs* args, int cluster, void* stream_) {
+  const ChooseArgs& P = *args;
+  JLX_REQUIRE(P.R > 0 && P.H > 0 && P.width > 0 && P.most >= 0 && P.first >= 0 && P.recent >= 0, "kv_choose: bad sizes");
+  JLX_REQUIRE(cluster >= 1 && cluster <= MAX_CLUSTER, "kv_choose: %d blocks a row", cluster);
+  JLX_REQUIRE((long long)P.R * P.H <= 65535, "kv_choose: %d requests of %d KV heads are too many for a launch", P.R, P.H);
+  const int per = ((P.width + cluster - 1) / cluster + 3) / 4 * 4;
+  const bool holds = per <= HELD;
+  const size_t smem = holds ? (size_t)per * 4 : 0;
+  auto kernel = holds ? kv_choose_kernel<true> : kv_choose_kernel<false>;
+  if (smem > 40 * 1024) JLX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster, P.R * P.H);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream_;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  JLX_CUDA(cudaLaunchKernelEx(&cfg, kernel, P, per));
+  return 0;
+}
+
+JLX_API int jlx_kv_compact(const CompactArgs* args, int in_place, void* stream_) {
+  const CompactArgs& P = *args;
+  cudaStream_t stream = (cudaStream_t)stream_;
+  JLX_REQUIRE(P.R > 0 && P.H > 0 && P.page > 0 && P.num_pages > 0 && P.row_bytes > 0 && P.row_bytes % 16 == 0 && P.most > 0, "kv_compact: bad sizes");
+  JLX_REQUIRE(((uintptr_t)P.pages & 15) == 0, "kv_compact: pages must be 16-byte aligned");
+  JLX_REQUIRE(((long long)P.num_pages + 1) * 2 * P.H * P.page < (1ll << 31), "kv_compact: cache too large for 32-bit rows");
+  JLX_REQUIRE((long long)P.R * P.H <= 65535, "kv_compact: %d requests of %d KV heads are too many for a launch", P.R, P.H);
+  if (in_place) {
+    const int columns = P.row_bytes % 32 == 0 ? P.row_bytes / 32 : P.row_bytes / 16;
+    JLX_CUDA(jlx_launch_pdl(kv_compact_in_place_kernel, dim3(2 * columns + 3, P.R * P.H), dim3(THREADS), 0, stream, P, columns));
+    return 0;
+  }
+  const int rows_per_block = 128;
+  JLX_CUDA(jlx_launch_pdl(kv_compact_kernel, dim3((P.most + rows_per_block - 1) / rows_per_block + 1, P.R * P.H), dim3(THREADS), 0, stream, P, rows_per_block));
+  return 0;
+}

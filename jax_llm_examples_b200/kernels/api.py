@@ -23,6 +23,7 @@ STATUS_BITS = {
     2: "a token id was outside the vocabulary",
     4: "a routed expert index was outside the expert count",
     8: "a bounded wait inside a kernel gave up",
+    16: "a length or a number of places lay outside its array",
 }
 
 
@@ -1521,6 +1522,85 @@ def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.T
          _weights_shares(R * Hkv * -(-max_kv_len // WEIGHTS_TILE), q_tiles, blocks), _raw_stream(dev))
     global _launches
     _launches += 1  # two kernels
+
+
+_CHOOSE_ARGS = struct.Struct("@6P6i")  # ChooseArgs in csrc/kv_budget.cu
+_COMPACT_ARGS = struct.Struct("@9P10i")  # CompactArgs in csrc/kv_budget.cu
+
+
+def kv_choose(sums: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor, places: torch.Tensor, counts: torch.Tensor, status: torch.Tensor,
+              first: int = 0, recent: int = 0) -> None:
+    """Which places every request and KV head keep.  sums: float32 [R, Hkv, width] (:func:`attention_weights`); lengths: int32 [R],
+    places that a request has; keep: int32 [R], how many of them are kept; places: int32 [R, Hkv, most]; counts: int32 [R].
+    Of a request's length L, counts[r] = min(keep[r], L) places are kept: the last ``recent``, then the first ``first`` as far as that
+    goes, then those with the largest sums (ties: the lowest place; NaN counts as the lowest sum).  They stand in ascending order
+    in places[r, h], followed by -1.  A length outside 0 .. width, or a number to keep that ``places`` has no room for, is cut to it and
+    raises the status."""
+    what = "kv_choose"
+    if sums.dtype is not torch.float32 or sums.dim() != 3:
+        raise KernelError(f"{what}: sums must be float32 [requests, KV heads, places], not {sums.dtype} {tuple(sums.shape)}")
+    R, H, width = sums.shape
+    _ints(what, ("lengths", lengths, R), ("keep", keep, R), ("places", places, 0), ("counts", counts, R), ("status", status, 1))
+    if places.dim() != 3 or places.shape[:2] != (R, H):
+        raise KernelError(f"{what}: places must be int32 [{R}, {H}, places], not {tuple(places.shape)}")
+    if first < 0 or recent < 0:
+        raise KernelError(f"{what}: the first {first} and the last {recent} places cannot be kept")
+    dev = _placed(what, sums, lengths, keep, places, counts, status)
+    if R * H == 0:
+        return
+    if width == 0:
+        raise KernelError(f"{what}: sums have no places")
+    args = _CHOOSE_ARGS.pack(sums.data_ptr(), lengths.data_ptr(), keep.data_ptr(), places.data_ptr(), counts.data_ptr(), status.data_ptr(), R, H, width,
+                             places.shape[2], min(first, width), min(recent, width))
+    blocks = 1
+    while blocks < 8 and (R * H * blocks < sm_count() and width >= 2048 * blocks or width > 16384 * blocks):
+        blocks *= 2
+    _run("kv_budget", "jlx_kv_choose", args, blocks, _raw_stream(dev))
+
+
+def kv_compact(pages: torch.Tensor, block_table: torch.Tensor, places: torch.Tensor, counts: torch.Tensor, status: torch.Tensor,
+               into: torch.Tensor | None = None, scales: torch.Tensor | None = None, sums: torch.Tensor | None = None,
+               sums_out: torch.Tensor | None = None) -> None:
+    """The kept rows of keys and values move to the front: row i < counts[r] of request r and KV head h comes from place
+    places[r, h, i] (:func:`kv_choose`) and goes to place i, in the pages that ``into`` (int32 [R, pages of one]) names; without it in the
+    request's own, where places[r, h, i] >= i is needed (ascending places are).  pages: [P, 2, Hkv, page size, dh] of any type whose
+    rows are whole 16 bytes, with ``scales`` in 8 bits; pages of ``into`` are none that the call reads rows from.  ``sums``: float32
+    [R, Hkv, width], moved alike into ``sums_out`` [R, Hkv, width of its own] (None: sums itself), whose other entries become 0.
+    Rows behind the kept ones stay as they were.  A row whose place or page is missing, or that would move back, is left out and raises
+    the status.  Keys keep the rotation of the position that they were written at; the request's next token lies at place counts[r]."""
+    what = "kv_compact"
+    if pages.dim() != 5 or pages.shape[1] != 2 or (scales is None) != (pages.dtype is not FP8):
+        raise KernelError(f"{what}: pages must be [pages, 2, KV heads, page size, entries], with scales if and only if they are float8_e4m3fn")
+    P, _, H, page_size, dh = pages.shape
+    if scales is not None:
+        _cache8(what, pages, scales, block_table, H, dh)
+    if places.dim() != 3 or places.shape[1] != H:
+        raise KernelError(f"{what}: places must be int32 [requests, {H}, places], not {tuple(places.shape)}")
+    R, _, most = places.shape
+    _ints(what, ("block_table", block_table, 0), ("into", into, 0), ("places", places, 0), ("counts", counts, R), ("status", status, 1))
+    if any(t is not None and (t.dim() != 2 or t.shape[0] != R) for t in (block_table, into)):
+        raise KernelError(f"{what}: block tables must be int32 [{R}, pages of one]")
+    if dh * pages.element_size() % 16 or pages.data_ptr() % 16:
+        raise KernelError(f"{what}: rows of {dh} entries of {pages.dtype} are not whole 16 bytes on 16-byte boundaries")
+    if sums is None and sums_out is not None:
+        raise KernelError(f"{what}: sums_out without sums")
+    sums_out = sums if sums_out is None else sums_out
+    if sums is not None:
+        if any(t.dtype is not torch.float32 or t.dim() != 3 or t.shape[:2] != (R, H) for t in (sums, sums_out)):
+            raise KernelError(f"{what}: sums must be float32 [{R}, {H}, places]")
+        if _overlap(sums, sums_out) and not (sums.data_ptr() == sums_out.data_ptr() and sums.shape == sums_out.shape):
+            raise KernelError(f"{what}: sums_out must be sums itself or apart from it")
+    dev = _placed(what, pages, block_table, places, counts, status, into, scales, sums, sums_out)
+    if most == 0 and sums_out is not None:
+        sums_out.zero_()
+    if R * H == 0 or P * page_size == 0 or most == 0:
+        return
+    into_t = block_table if into is None else into
+    args = _COMPACT_ARGS.pack(pages.data_ptr(), _address(scales), block_table.data_ptr(), into_t.data_ptr(), places.data_ptr(), counts.data_ptr(), _address(sums),
+                              _address(sums_out), status.data_ptr(), R, H, page_size, P, dh * pages.element_size(), block_table.shape[1], into_t.shape[1], most,
+                              0 if sums is None else sums.shape[2], 0 if sums is None else sums_out.shape[2])
+    in_place = into is None or into.data_ptr() == block_table.data_ptr()
+    _run("kv_budget", "jlx_kv_compact", args, int(in_place), _raw_stream(dev))
 
 
 # ------------------------------------------------------------------------------------- GEMMs

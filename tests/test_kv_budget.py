@@ -1,0 +1,122 @@
+"""A cache kept to a budget, host side: refusals before anything is launched, and the rules on sizes."""
+
+import pytest
+import torch
+
+from jax_llm_examples_b200.kernels import api as K
+
+from .fp8_helpers import Case
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+
+
+I32 = torch.int32
+
+
+def _weights(**change):
+    c = Case([3], [5], 4, 2, 64, 16, device="cpu", bits8=False)
+    a = dict(q=c.q, pages=c.pages, block_table=c.table, cu_q=c.cu_q, positions=c.positions, out=torch.zeros(1, 2, 8), scale=0.125, chunk=0, window=0,
+             attn_scale=0.0, floor_scale=1.0, status=c.status, max_kv_len=8, max_count=3)
+    return {**a, **change}
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(), "not on the GPU"),
+    (dict(q=torch.zeros(3, 4, 64)), "bfloat16"),
+    (dict(q=torch.zeros(3, 4, 32, dtype=torch.bfloat16)), "disagree"),
+    (dict(pages=torch.zeros(4, 2, 2, 16, 64)), "pages"),
+    (dict(scales=torch.zeros((4, 2, 2, 16), dtype=torch.uint8)), "float8"),
+    (dict(block_table=torch.zeros((1, 2), dtype=torch.int64)), "block table"),
+    (dict(cu_q=torch.zeros(1, dtype=I32)), "cu_q"),
+    (dict(positions=torch.zeros(3)), "positions"),
+    (dict(out=torch.zeros(1, 2, 8, dtype=torch.bfloat16)), "out"),
+    (dict(out=torch.zeros(2, 2, 8)), "out"),
+    (dict(add=torch.zeros(1, 2, 9)), "add"),
+    (dict(add=torch.zeros(1, 2, 8, dtype=torch.float64)), "add"),
+    (dict(max_kv_len=0), "keys"),
+    (dict(max_count=0), "tokens"),
+    (dict(sink=torch.zeros(3)), "sink"),
+    (dict(slopes=torch.zeros(4, dtype=torch.bfloat16)), "slopes"),
+    (dict(q=torch.zeros((3, 64, 4), dtype=torch.bfloat16).transpose(1, 2)), "contiguous"),
+])
+def test_weights_refuse(no_launch, change, match):
+    with pytest.raises(K.KernelError, match=match):
+        K.attention_weights(**_weights(**change))
+
+
+def test_weights_are_not_added_over_shifted_memory(no_launch):
+    both = torch.zeros(24)
+    with pytest.raises(K.KernelError, match="add"):
+        K.attention_weights(**_weights(out=both[:16].view(1, 2, 8), add=both[4:20].view(1, 2, 8)))
+
+
+@pytest.mark.parametrize("keys", [1, 15, 16, 700, 8192, 30000, 131072])
+@pytest.mark.parametrize("pairs", [1, 8, 64, 512])
+@pytest.mark.parametrize("rows", [1, 8, 16])
+def test_ranges_hold_all_keys(keys, pairs, rows):
+    splits, most, fits = K.attention_weights_plan(keys, pairs, rows, 148)
+    assert 1 <= splits <= 8 and most % K.WEIGHTS_KEYS == 0
+    # a first key anywhere within a tile
+    assert splits * most >= keys + K.WEIGHTS_KEYS - 1 and fits == (most * (32 if rows <= 8 else 64) <= K.WEIGHTS_HELD)
+
+
+def _choose(**change):
+    a = dict(sums=torch.zeros(2, 3, 10), lengths=torch.ones(2, dtype=I32), keep=torch.ones(2, dtype=I32), places=torch.zeros((2, 3, 4), dtype=I32),
+             counts=torch.zeros(2, dtype=I32), status=torch.zeros(1, dtype=I32))
+    return {**a, **change}
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(), "not on the GPU"),
+    (dict(sums=torch.zeros(2, 3, 10, dtype=torch.bfloat16)), "sums"),
+    (dict(sums=torch.zeros(2, 30)), "sums"),
+    (dict(lengths=torch.ones(1, dtype=I32)), "lengths"),
+    (dict(keep=torch.ones(2)), "keep"),
+    (dict(places=torch.zeros((2, 2, 4), dtype=I32)), "places"),
+    (dict(places=torch.zeros((2, 3, 4))), "places"),
+    (dict(counts=torch.zeros(1, dtype=I32)), "counts"),
+    (dict(first=-1), "first"),
+    (dict(recent=-1), "last"),
+    (dict(sums=torch.zeros(2, 10, 3).transpose(1, 2)), "contiguous"),
+])
+def test_choosing_refuses(no_launch, change, match):
+    with pytest.raises(K.KernelError, match=match):
+        K.kv_choose(**_choose(**change))
+
+
+def _compact(**change):
+    a = dict(pages=torch.zeros(4, 2, 3, 16, 64), block_table=torch.zeros((2, 2), dtype=I32), places=torch.zeros((2, 3, 4), dtype=I32),
+             counts=torch.zeros(2, dtype=I32), status=torch.zeros(1, dtype=I32))
+    return {**a, **change}
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(), "not on the GPU"),
+    (dict(pages=torch.zeros(4, 3, 16, 64)), "pages"),
+    (dict(pages=torch.zeros(4, 2, 3, 16, 64).to(torch.float8_e4m3fn)), "scales"),
+    (dict(scales=torch.zeros((4, 2, 3, 16), dtype=torch.uint8)), "scales"),
+    (dict(pages=torch.zeros(4, 2, 3, 16, 6, dtype=torch.bfloat16)), "16 bytes"),
+    (dict(places=torch.zeros((2, 2, 4), dtype=I32)), "places"),
+    (dict(places=torch.zeros((2, 3, 4), dtype=torch.int64)), "places"),
+    (dict(counts=torch.zeros(1, dtype=I32)), "counts"),
+    (dict(block_table=torch.zeros((1, 2), dtype=I32)), "block tables"),
+    (dict(into=torch.zeros((1, 2), dtype=I32)), "block tables"),
+    (dict(into=torch.zeros((2, 2), dtype=torch.int64)), "into"),
+    (dict(sums_out=torch.zeros(2, 3, 9)), "without sums"),
+    (dict(sums=torch.zeros(2, 2, 9)), "sums"),
+    (dict(sums=torch.zeros(2, 3, 9), sums_out=torch.zeros(2, 3, 9, dtype=torch.bfloat16)), "sums"),
+])
+def test_moving_refuses(no_launch, change, match):
+    with pytest.raises(K.KernelError, match=match):
+        K.kv_compact(**_compact(**change))
+
+
+def test_sums_move_within_themselves_or_apart(no_launch):
+    one = torch.zeros(100)
+    with pytest.raises(K.KernelError, match="apart"):
+        K.kv_compact(**_compact(sums=one[:54].view(2, 3, 9), sums_out=one[6:60].view(2, 3, 9)))
+    with pytest.raises(K.KernelError, match="apart"):
+        K.kv_compact(**_compact(sums=one[:54].view(2, 3, 9), sums_out=one[:48].view(2, 3, 8)))
