@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(THREADS) attention_weights_kernel(const Weight
           for (int c = 0; c < 2; ++c) {
             v[c] = s[ng][2 * h + c] * sc[ng][c];
             if (F8) v[c] *= ks[a][h];
-            if (P.R.cap_log2 > 0.f) v[c] = P.R.cap_log2 * cap_tanh(v[c]);
+            if (P.R.cap_log2 > 0.f) v[c] = P.R.cap_log2 * weights_tanh(v[c]);
             if (P.R.slopes) v[c] -= slope[ng][c] * (float)(pos[ng][c] - place);
             if (place < lo[ng][c] || place > pos[ng][c] || place < begin || place >= end) v[c] = -INFINITY;
             m[ng][c] = fmaxf(m[ng][c], v[c]);

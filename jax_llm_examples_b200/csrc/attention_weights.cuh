@@ -51,3 +51,18 @@ __device__ __forceinline__ uint32_t weights_widen(uint32_t x, uint32_t select) {
   const __nv_bfloat162 z = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&f));
   return *reinterpret_cast<const uint32_t*>(&z);
 }
+
+// tanh for capped scores, whose weights go out in 32 bits (the other attention kernels round theirs to 16 and take softcap.cuh's):
+// |x| <= 1: x p(x^2), p of degree 7 with the smallest largest relative error against tanh(x) / x on [0, 1] (fitted by iteratively
+// reweighted least squares in a Chebyshev basis: 4.2e-9, 1.1e-7 with its roundings); beyond as there.
+__device__ __forceinline__ float weights_tanh(float x) {
+  const float u = x * x;
+  float p = fmaf(-0.00035334538551978767f, u, 0.0022822292521595955f);
+  p = fmaf(p, u, -0.007917444221675396f);
+  p = fmaf(p, u, 0.021464819088578224f);
+  p = fmaf(p, u, -0.05387091264128685f);
+  p = fmaf(p, u, 0.1333215981721878f);
+  p = fmaf(p, u, -0.33333277702331543f);
+  p = fmaf(p, u, 1.f);
+  return fabsf(x) <= 1.f ? p * x : cap_tanh_large(x);
+}

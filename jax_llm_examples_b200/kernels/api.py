@@ -1431,7 +1431,7 @@ def tree_masks(parents) -> "tuple[list[int], list[list[int]]]":
 _WEIGHTS_ARGS = struct.Struct("@4P2i")  # WeightsArgs in csrc/attention_weights.cuh
 WEIGHTS_FEW = 16  # query rows of a request and KV head that attention_weights.cu takes
 WEIGHTS_KEYS = 16  # keys of a tile there
-WEIGHTS_TILE = 128  # keys, and query rows, of a tile in attention_weights_tc.cu
+WEIGHTS_TILE = 128  # keys, or query rows, of a tile in attention_weights_tc.cu
 WEIGHTS_HELD = 200 << 10  # bytes of scores that a block keeps in shared memory
 
 
@@ -1447,10 +1447,12 @@ def attention_weights_plan(keys: int, pairs: int, rows: int, sms: int) -> "tuple
     return splits, most(splits), most(splits) * row <= WEIGHTS_HELD
 
 
-def _weights_shares(units: int, tiles: int, blocks: int) -> int:
-    """Blocks that share the tiles passing by one of so many units, for about so many blocks in all."""
+@functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
+def _weights_shares(units: int, tiles: int, places: int) -> int:
+    """Blocks that share the tiles passing by one of so many units, where the device holds ``places`` blocks: so many that a unit's share is no
+    more than a block's of all the work.  (The longest units come first and the short ones fill up behind them.)"""
     shares = 1
-    while shares < 8 and units * shares < blocks and tiles >= 4 * shares:
+    while shares < 8 and tiles > shares * max(units * tiles // places, 4):
         shares *= 2
     return shares
 
@@ -1517,9 +1519,11 @@ def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.T
     if rows <= WEIGHTS_FEW:
         _run("attention_weights", "jlx_attention_weights", args, more, rows, splits, most, _raw_stream(dev))
         return
-    blocks = 4 * sm_count()  # two rounds of them
-    _run("attention_weights_tc", "jlx_attention_weights_tc", args, more, _weights_shares(R * Hkv * q_tiles, -(-keys // WEIGHTS_TILE), blocks),
-         _weights_shares(R * Hkv * -(-max_kv_len // WEIGHTS_TILE), q_tiles, blocks), _raw_stream(dev))
+    places, k_tiles, passes = 2 * sm_count(), -(-out.shape[2] // WEIGHTS_TILE), -(-rows // WEIGHTS_TILE)
+    keys_shares = _weights_shares(R * Hkv * -(-max_kv_len // WEIGHTS_TILE), passes, places)
+    key_tiles = max(1, min(8, R * Hkv * k_tiles // (4 * places))) if keys_shares == 1 and passes <= 32 else 1
+    _run("attention_weights_tc", "jlx_attention_weights_tc", args, more, _weights_shares(R * Hkv * q_tiles, -(-keys // WEIGHTS_TILE), places), keys_shares,
+         key_tiles, _raw_stream(dev))
     global _launches
     _launches += 1  # two kernels
 
