@@ -18,7 +18,7 @@ struct WeightsArgs {  // _WEIGHTS_ARGS in kernels/api.py
 struct WeightsParams {
   RowsParams R;        // (its items, rows, cu_q, masks and parts are not used; max_count is the most tokens of a request)
   WeightsArgs W;
-  int splits, buf_keys;
+  int splits, buf_keys, rows, page_shift;  // rows: the most of a request and KV head; page_shift: the page size's logarithm, -1 if it is no power of two
 };
 
 // Request r's tokens; false: it has none, or they lie outside the step (the status says so).

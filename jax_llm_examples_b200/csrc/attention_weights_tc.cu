@@ -732,7 +732,8 @@ JLX_API int jlx_attention_weights_tc(const RowsArgs* rows_args, const WeightsArg
   T.key_tiles = key_tiles;
   if (int e = rows_params(*rows_args, T.P.R)) return e;
   T.P.W = *args;
-  T.P.buf_keys = 0;
+  T.P.buf_keys = T.P.rows = 0;
+  T.P.page_shift = -1;
   const RowsParams& R = T.P.R;
   JLX_REQUIRE(rows_splits >= 1 && rows_splits <= MAX_SPLITS && keys_splits >= 1 && keys_splits <= MAX_SPLITS, "attention_weights: %d and %d blocks share tiles", rows_splits, keys_splits);
   JLX_REQUIRE((long long)R.n_requests * R.Hkv * MAX_SPLITS < (1ll << 31), "attention_weights: %d requests of %d KV heads are too many for a launch", R.n_requests, R.Hkv);

@@ -1432,17 +1432,17 @@ _WEIGHTS_ARGS = struct.Struct("@4P2i")  # WeightsArgs in csrc/attention_weights.
 WEIGHTS_FEW = 16  # query rows of a request and KV head that attention_weights.cu takes
 WEIGHTS_KEYS = 16  # keys of a tile there
 WEIGHTS_TILE = 128  # keys, or query rows, of a tile in attention_weights_tc.cu
-WEIGHTS_HELD = 200 << 10  # bytes of scores that a block keeps in shared memory
+WEIGHTS_HELD = 100 << 10  # bytes of scores that a block keeps in shared memory
 
 
 @functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
 def attention_weights_plan(keys: int, pairs: int, rows: int, sms: int) -> "tuple[int, int, bool]":
     """(Ranges that a request's keys are cut into, the most keys of one, whether its scores fit shared memory) for so many (request,
     KV head) pairs of up to so many query rows."""
-    row = 4 * (8 if rows <= 8 else 16)
+    row = 8 * -(-rows // 2)  # bytes of a key's scores
     most = lambda s: -(-(keys + WEIGHTS_KEYS) // (WEIGHTS_KEYS * s)) * WEIGHTS_KEYS  # noqa: E731  (ranges start at a tile's first key)
     splits = 1
-    while splits < 8 and ((pairs * splits < 4 * sms and keys >= 256 * splits) or most(splits) * row > 72 << 10):
+    while splits < 16 and ((pairs * splits < 8 * sms and keys >= 128 * splits) or most(splits) * row > 48 << 10):
         splits *= 2
     return splits, most(splits), most(splits) * row <= WEIGHTS_HELD
 
@@ -1511,7 +1511,7 @@ def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.T
         scratch = torch.empty(_up4(2 * N * Hq) + 4 * R * q_tiles, dtype=torch.float32, device=q.device)
     else:
         splits, most, fits = attention_weights_plan(keys, R * Hkv, rows, sm_count())
-        scratch = None if fits else torch.empty(R * Hkv * splits * most * (8 if rows <= 8 else 16), dtype=torch.float32, device=q.device)
+        scratch = None if fits else torch.empty(R * Hkv * splits * most * -(-rows // 2) * 2, dtype=torch.float32, device=q.device)
     args = _ROWS_ARGS.pack(q.data_ptr(), pages.data_ptr(), _address(scales), block_table.data_ptr(), 0, positions.data_ptr(), 0, 0, 0, 0, 0, 0, _address(sink),
                            _address(slopes), 0, 0, status.data_ptr(), width, R, R, max_count, 0, N, Hq, Hkv, dh, page_size, P, chunk, window, 1, 0, 0,
                            scale, softcap, attn_scale, floor_scale)

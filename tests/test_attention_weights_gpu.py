@@ -169,10 +169,13 @@ def test_more_than_the_call_was_sized_for_gives_nothing(n):
     assert_close(got[1], want[1, :, :100], tol[1, :, :100])
 
 
-def test_a_range_too_long_for_shared_memory():
-    c = Case([1], [60000], 4, 1, 64, 64, bits8=False, spread=0.3).to_device()
-    _, _, fits = K().attention_weights_plan(60001, 1, 4, 148)
-    assert not fits
+@pytest.mark.parametrize("bits8", [False, True])
+def test_ranges_too_long_for_shared_memory(monkeypatch, bits8):
+    """Their scores go through scratch: at the size where they do, and as if shared memory were small."""
+    assert not K().attention_weights_plan(500000, 1, 8, 148)[2]
+    plan = K().attention_weights_plan
+    monkeypatch.setattr(K(), "attention_weights_plan", lambda *a: (*plan(*a)[:2], False))
+    c = Case([1, 2], [9000, 333], 8, 2, 64, 64, bits8=bits8).to_device()
     want, tol = received(c)
     assert_close(run(c), want, tol)
 

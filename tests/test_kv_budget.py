@@ -58,9 +58,9 @@ def test_weights_are_not_added_over_shifted_memory(no_launch):
 @pytest.mark.parametrize("rows", [1, 8, 16])
 def test_ranges_hold_all_keys(keys, pairs, rows):
     splits, most, fits = K.attention_weights_plan(keys, pairs, rows, 148)
-    assert 1 <= splits <= 8 and most % K.WEIGHTS_KEYS == 0
+    assert 1 <= splits <= 16 and most % K.WEIGHTS_KEYS == 0
     # a first key anywhere within a tile
-    assert splits * most >= keys + K.WEIGHTS_KEYS - 1 and fits == (most * (32 if rows <= 8 else 64) <= K.WEIGHTS_HELD)
+    assert splits * most >= keys + K.WEIGHTS_KEYS - 1 and fits == (most * 8 * -(-rows // 2) <= K.WEIGHTS_HELD)
 
 
 def _choose(**change):
