@@ -31,7 +31,7 @@ namespace cg = cooperative_groups;
 #define THREADS 256
 #define WARPS (THREADS / 32)
 #define MAX_RANK 256
-#define MAX_CLUSTER 8
+#define MAX_CLUSTER 16  // (more than 8 blocks are not portable; this is sm_100a only)
 
 struct AdapterArgs {  // _ADAPTER_ARGS in kernels/api.py
   const void *x, *a, *b, *y;
@@ -111,11 +111,12 @@ template <> struct Eight<float> {
 // MT: tiles of 16 rows.  NT: tiles of 8 ranks that a warp has; the block's warps are WR groups of them (WR * NT * 8 >= r) times
 // WK cuts of K.  PARTS: bfloat16 numbers that a 32-bit sum between the products becomes.
 template <int MT, int NT, int WR, typename TY>
-__global__ void __launch_bounds__(THREADS) adapters_kernel(const AdapterArgs P) {
+__global__ void __launch_bounds__(THREADS, WR * NT * 8 > 128 ? 1 : 2) adapters_kernel(const AdapterArgs P) {
   JLX_TL(TL_OTHER);
   constexpr int ROWS = 16 * MT, WK = WARPS / WR, RC = WR * NT * 8, LD = low_stride(RC);
   constexpr int PARTS = sizeof(TY) == 4 ? 3 : 2;
   constexpr int STEPS = (RC + 31) / 32;  // of 32 ranks in the second product (the last one may be short)
+  constexpr bool EARLY = MT == 1 && STEPS <= 2;  // room in registers for what the next 32 columns need
   extern __shared__ __align__(16) uint8_t smem_raw[];
   float* meet = reinterpret_cast<float*>(smem_raw);                  // [max(WK / 2, 1)][ROWS][RC]: the warps' sums; then [ROWS][RC] of the block
   bf16* low = reinterpret_cast<bf16*>(meet + (WK > 1 ? WK / 2 : 1) * ROWS * RC);  // [PARTS][ROWS][LD]
@@ -133,6 +134,38 @@ __global__ void __launch_bounds__(THREADS) adapters_kernel(const AdapterArgs P) 
   const bf16 *x = reinterpret_cast<const bf16*>(P.x), *a = reinterpret_cast<const bf16*>(P.a), *b = reinterpret_cast<const bf16*>(P.b);
   const TY* y = reinterpret_cast<const TY*>(P.y);
   TY* out = reinterpret_cast<TY*>(P.out);
+
+  // what a warp takes of B (and, of few rows, of y) for 32 columns
+  const int units = (P.No + 31) / 32, per_u = (units + blocks - 1) / blocks, u0 = me * per_u, u1 = min(u0 + per_u, units);
+  const int col_g = (g >> 1) * 8 + (g & 1);
+  struct B {
+    uint4 b[STEPS][4];
+    Eight<TY> y[EARLY ? 2 : 1];
+  };
+  B first;
+  auto fetch_b = [&](int u, B& f) {
+    if (u >= u1) return;
+    if (t.e >= 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = u * 32 + col_g + j * 2;
+        const bf16* br = b + ((size_t)t.e * P.No + n) * P.r;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          const int k = s * 32 + t4 * 8;
+          f.b[s][j] = n < P.No && k < t.rank ? *reinterpret_cast<const uint4*>(br + k) : make_uint4(0, 0, 0, 0);
+          if (t.rank & 7) f.b[s][j] = first_of(f.b[s][j], t.rank - k);
+        }
+      }
+    }
+    if (EARLY) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int n = row_s[h * 8 + g], col = u * 32 + t4 * 8;
+        if (n >= 0 && col < P.No) f.y[h].load(y + (size_t)n * P.ldy + col);
+      }
+    }
+  };
 
   if (t.e >= 0) {
     // ---- x A^T over this block's part of K
@@ -153,26 +186,48 @@ __global__ void __launch_bounds__(THREADS) adapters_kernel(const AdapterArgs P) 
       }
     const int rank0 = wr * NT * 8 + g;
     const bf16* ar = a + ((size_t)t.e * P.r + rank0) * P.K + t4 * 8;
-#pragma unroll 2
-    for (int c = c0 + wk; c < c1; c += WK) {
+    struct Step {
+      uint4 x[MT][2], a[NT];
+    };
+    auto fetch = [&](int c, Step& f) {
       const int k = c * 32;
-      const bool in = k + t4 * 8 < P.K;
-      uint4 xf[MT][2], af[NT];
+      const bool in = c < c1 && k + t4 * 8 < P.K;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) af[n] = in && rank0 + n * 8 < t.rank ? *reinterpret_cast<const uint4*>(ar + (size_t)n * 8 * P.K + k) : make_uint4(0, 0, 0, 0);
+      for (int n = 0; n < NT; ++n) f.a[n] = in && rank0 + n * 8 < t.rank ? *reinterpret_cast<const uint4*>(ar + (size_t)n * 8 * P.K + k) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) xf[m][h] = in && xr[m][h] ? *reinterpret_cast<const uint4*>(xr[m][h] + k) : make_uint4(0, 0, 0, 0);
+        for (int h = 0; h < 2; ++h) f.x[m][h] = in && xr[m][h] ? *reinterpret_cast<const uint4*>(xr[m][h] + k) : make_uint4(0, 0, 0, 0);
+    };
+    auto multiply = [&](const Step& f) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          const uint32_t f0[4] = {xf[m][0].x, xf[m][1].x, xf[m][0].y, xf[m][1].y}, f1[4] = {xf[m][0].z, xf[m][1].z, xf[m][0].w, xf[m][1].w};
-          mma_bf16(acc[m][n], f0, af[n].x, af[n].y);
-          mma_bf16(acc[m][n], f1, af[n].z, af[n].w);
+          const uint32_t f0[4] = {f.x[m][0].x, f.x[m][1].x, f.x[m][0].y, f.x[m][1].y}, f1[4] = {f.x[m][0].z, f.x[m][1].z, f.x[m][0].w, f.x[m][1].w};
+          mma_bf16(acc[m][n], f0, f.a[n].x, f.a[n].y);
+          mma_bf16(acc[m][n], f1, f.a[n].z, f.a[n].w);
         }
+    };
+    if (MT == 1 && NT <= 4) {  // a step's operands are on their way while the one before is worked on
+      Step even, odd;
+      fetch(c0 + wk, even);
+#pragma unroll 1
+      for (int c = c0 + wk; c < c1; c += 2 * WK) {
+        fetch(c + WK, odd);
+        multiply(even);
+        fetch(c + 2 * WK, even);
+        multiply(odd);
+      }
+    } else {
+#pragma unroll 1
+      for (int c = c0 + wk; c < c1; c += WK) {
+        Step f;
+        fetch(c, f);
+        multiply(f);
+      }
     }
+    if (EARLY) fetch_b(u0 + warp, first);  // (B's first part is on its way while the sums meet)
     // ---- the warps' sums, halved until one is left
     auto put = [&](float* to, bool add) {
 #pragma unroll
@@ -227,26 +282,13 @@ __global__ void __launch_bounds__(THREADS) adapters_kernel(const AdapterArgs P) 
   }
 
   // ---- the tile's rows times B^T, over this block's part of the columns, 32 at a time
-  const int units = (P.No + 31) / 32, per = (units + blocks - 1) / blocks, u0 = me * per, u1 = min(u0 + per, units);
-  const int col_g = (g >> 1) * 8 + (g & 1);
+  if (!EARLY || t.e < 0) fetch_b(u0 + warp, first);
 #pragma unroll 1
   for (int u = u0 + warp; u < u1; u += WARPS) {
     const int col = u * 32 + t4 * 8;  // this thread's eight columns
     const bool mine = col < P.No;
-    uint4 bf[STEPS][4];
-    if (t.e >= 0) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = u * 32 + col_g + j * 2;
-        const bf16* br = b + ((size_t)t.e * P.No + n) * P.r;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          const int k = s * 32 + t4 * 8;
-          bf[s][j] = n < P.No && k < t.rank ? *reinterpret_cast<const uint4*>(br + k) : make_uint4(0, 0, 0, 0);
-          if (t.rank & 7) bf[s][j] = first_of(bf[s][j], t.rank - k);
-        }
-      }
-    }
+    const B now = first;
+    if (EARLY) fetch_b(u + WARPS, first);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       Eight<TY> ys[2];
@@ -254,7 +296,8 @@ __global__ void __launch_bounds__(THREADS) adapters_kernel(const AdapterArgs P) 
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         n[h] = mine ? row_s[m * 16 + h * 8 + g] : -1;
-        if (n[h] >= 0) ys[h].load(y + (size_t)n[h] * P.ldy + col);
+        if (EARLY) ys[h] = now.y[h];
+        else if (n[h] >= 0) ys[h].load(y + (size_t)n[h] * P.ldy + col);
       }
       if (t.e < 0) {
 #pragma unroll
@@ -278,8 +321,8 @@ __global__ void __launch_bounds__(THREADS) adapters_kernel(const AdapterArgs P) 
           const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            mma_bf16(d[j], f0, bf[s][j].x, bf[s][j].y);
-            mma_bf16(d[j], f1, bf[s][j].z, bf[s][j].w);
+            mma_bf16(d[j], f0, now.b[s][j].x, now.b[s][j].y);
+            mma_bf16(d[j], f1, now.b[s][j].z, now.b[s][j].w);
           }
         }
       }
@@ -289,6 +332,7 @@ __global__ void __launch_bounds__(THREADS) adapters_kernel(const AdapterArgs P) 
         if (n[h] >= 0) ys[h].add_store(out + (size_t)n[h] * P.ldo + col, f);
       }
     }
+    if (!EARLY) fetch_b(u + WARPS, first);
   }
 }
 
@@ -371,6 +415,7 @@ static int launch_adapters(const AdapterArgs& P, int cluster, cudaStream_t strea
   auto kernel = adapters_kernel<MT, NT, WR, TY>;
   static_assert(smem <= 227 * 1024, "a tile's sums do not fit into shared memory");
   if (smem > 48 * 1024) JLX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (cluster > 8) JLX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   const int subs = (P.tile_rows + ROWS - 1) / ROWS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster, P.n_tiles * subs);
@@ -394,9 +439,9 @@ static int launch_rank(const AdapterArgs& P, int cluster, cudaStream_t stream) {
   if (P.r <= 8) return launch_adapters<MT, 1, 1, TY>(P, cluster, stream);
   if (P.r <= 16) return launch_adapters<MT, 2, 1, TY>(P, cluster, stream);
   if (P.r <= 32) return launch_adapters<MT, 4, 1, TY>(P, cluster, stream);
-  if (P.r <= 64) return launch_adapters<MT, 8, 1, TY>(P, cluster, stream);
-  if (P.r <= 128) return launch_adapters<MT, 8, 2, TY>(P, cluster, stream);
-  return launch_adapters<MT, 8, 4, TY>(P, cluster, stream);
+  if (P.r <= 64) return launch_adapters<MT, 4, 2, TY>(P, cluster, stream);
+  if (P.r <= 128) return launch_adapters<MT, 4, 4, TY>(P, cluster, stream);
+  return launch_adapters<MT == 4 ? 2 : MT, 8, 4, TY>(P, cluster, stream);
 }
 
 static bool rows_on_16(const void* p, long long ld, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0; }
@@ -416,11 +461,12 @@ JLX_API int jlx_adapters(const AdapterArgs* args, int sms, void* stream_) {
   JLX_REQUIRE(P.n_tiles > 0 && (P.tile_rows == 16 || P.tile_rows == 64), "adapters: %d tiles of %d rows", P.n_tiles, P.tile_rows);
   JLX_REQUIRE((long long)P.n_tiles * (P.tile_rows / PLAIN_ROWS) <= 65535, "adapters: too many tiles (%d)", P.n_tiles);
   if (adapters_fast(P)) {
-    const int rows = P.tile_rows == 16 ? 16 : 32, units = P.n_tiles * (P.tile_rows / rows);
+    // one round of blocks
+    const int rows = P.tile_rows == 16 ? 16 : P.r <= 128 ? 64 : 32, units = P.n_tiles * (P.tile_rows / rows);
     int cluster = MAX_CLUSTER;
-    while (cluster > 1 && units * cluster > 4 * sms) cluster /= 2;
-    if (P.out_type == JLX_F32) return P.tile_rows == 16 ? launch_rank<1, float>(P, cluster, stream) : launch_rank<2, float>(P, cluster, stream);
-    return P.tile_rows == 16 ? launch_rank<1, bf16>(P, cluster, stream) : launch_rank<2, bf16>(P, cluster, stream);
+    while (cluster > 1 && units * cluster > 2 * sms) cluster /= 2;
+    if (P.out_type == JLX_F32) return P.tile_rows == 16 ? launch_rank<1, float>(P, cluster, stream) : launch_rank<4, float>(P, cluster, stream);
+    return P.tile_rows == 16 ? launch_rank<1, bf16>(P, cluster, stream) : launch_rank<4, bf16>(P, cluster, stream);
   }
   JLX_REQUIRE(P.low != nullptr, "adapters: scratch is needed");
   const unsigned groups = (unsigned)(P.n_tiles * (P.tile_rows / PLAIN_ROWS));

@@ -4,9 +4,9 @@
 // kv_choose, of a request's L places and n = min(keep, L): the last `recent` ones, then the first `first` ones, as far as n goes, then of the
 // rest those with the largest sums; ties go to the lowest place; NaN counts as the lowest sum, -0 as 0.  Places come in ascending
 // order.  A sum becomes a whole number of 32 bits with the same order; the bits of the smallest kept one are found eight at a time
-// by counting (a digit's count of the places that share the digits before it), and one pass over the places writes what is above it
-// and the first so many that equal it.  A cluster of blocks serves a request and KV head, each with a stretch of the places in
-// shared memory: the sums are read from memory once.
+// by counting (a digit's count of the places that share the digits before it); then the places above it, and the first so many that
+// equal it, are counted and written, a warp going through a stretch of them by votes.  A cluster of blocks serves a request and KV
+// head, each with a stretch of the places in shared memory: the sums are read from memory once.
 //
 // kv_compact moves rows bit for bit.  Into other pages every row is on its own.  In place, row i's new place is at or before its old
 // one: a block takes a column of 32 bytes of one plane's rows through all places in order, some hundreds at a time, all loads of
@@ -21,8 +21,9 @@ namespace cg = cooperative_groups;
 
 #define THREADS 512
 #define WARPS (THREADS / 32)
-#define MAX_CLUSTER 8
-#define HELD (200 * 1024 / 4)  // sums that a block holds in shared memory at most
+#define MAX_CLUSTER 16
+#define COPIES 8  // of the counts: lanes with one digit (of exponents there are few) count in neighbouring banks
+#define HELD (96 * 1024 / 4)  // sums that a block holds in shared memory at most: two blocks a multiprocessor, so that a cluster of 16 has places
 
 struct ChooseArgs {  // _CHOOSE_ARGS in kernels/api.py
   const float* sums;   // [R, H, width]
@@ -68,9 +69,10 @@ template <bool HOLDS>
 __global__ void __launch_bounds__(THREADS) kv_choose_kernel(const ChooseArgs P, int per) {
   JLX_TL(TL_OTHER);
   extern __shared__ uint32_t held[];
-  __shared__ int count[256], warp_sums[WARPS], found[2], mine[2];
+  __shared__ __align__(16) int copies[256][COPIES];
+  __shared__ int count[2][256], warp_sums[WARPS], found[2], warp_kept[2][WARPS], mine[2];
   cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = cluster.num_blocks(), me = cluster.block_rank(), tid = threadIdx.x;
+  const int blocks = cluster.num_blocks(), me = cluster.block_rank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents_if_small();
   pdl_wait();
   const int row = blockIdx.y, r = row / P.H;
@@ -87,83 +89,128 @@ __global__ void __launch_bounds__(THREADS) kv_choose_kernel(const ChooseArgs P, 
   for (int i = n + me * THREADS + tid; i < P.most; i += blocks * THREADS) places[i] = -1;
   // this block's places [p0, p1); of them [q0, q1) are a matter of choice
   const int p0 = min(me * per, L), p1 = min(p0 + per, L), q0 = min(max(p0, first), p1), q1 = max(min(p1, L - recent), q0);
+  const bool all = want >= L - recent - first, some = want > 0 && !all;
   auto key = [&](int p) { return HOLDS ? held[p - p0] : ordered(sums[p]); };
-  if (HOLDS)
+  if (HOLDS && some) {
+#pragma unroll 8
     for (int p = q0 + tid; p < q1; p += THREADS) held[p - p0] = ordered(sums[p]);
-  __syncthreads();
+    __syncthreads();
+  }
   // the smallest sum that is chosen, and how many of the places with just that one
   uint32_t edge = 0u, mask = 0u;
   int left = want;
-  if (want > 0 && want < L - recent - first) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) count[tid] = 0;
+  if (some) {
+    for (int shift = 24, half = 0; shift >= 0; shift -= 8, half ^= 1) {
+      for (int i = tid; i < 256 * COPIES / 4; i += THREADS) reinterpret_cast<int4*>(copies)[i] = make_int4(0, 0, 0, 0);
       __syncthreads();
+#pragma unroll 4
       for (int p = q0 + tid; p < q1; p += THREADS) {
         const uint32_t k = key(p);
-        if ((k & mask) == edge) atomicAdd(&count[k >> shift & 255], 1);
+        if ((k & mask) == edge) atomicAdd(&copies[k >> shift & 255][lane % COPIES], 1);
       }
-      cluster.sync();
+      __syncthreads();
       // digits from the largest: thread i has digit 255 - i
       int c = 0;
-      if (tid < 256)
-        for (int q = 0; q < blocks; ++q) c += *cluster.map_shared_rank(&count[255 - tid], q);
+      if (tid < 256) {
+#pragma unroll
+        for (int i = 0; i < COPIES; i += 4) {
+          const int4 v = *reinterpret_cast<const int4*>(&copies[255 - tid][i]);
+          c += v.x + v.y + v.z + v.w;
+        }
+        count[half][tid] = c;
+      }
+      if (blocks > 1) {
+        cluster.sync();  // (the counts of the digit before last have been read everywhere, too)
+        if (tid < 256) {
+          int t[MAX_CLUSTER];
+#pragma unroll
+          for (int q = 0; q < MAX_CLUSTER; ++q) t[q] = q < blocks ? *cluster.map_shared_rank(&count[half][tid], q) : 0;
+          c = 0;
+#pragma unroll
+          for (int q = 0; q < MAX_CLUSTER; ++q) c += t[q];
+        }
+      }
       const int above = block_scan(c, warp_sums).x;
       if (tid < 256 && above < left && above + c >= left) {
         found[0] = 255 - tid;
         found[1] = left - above;
       }
-      cluster.sync();  // (the counts have been read everywhere)
+      __syncthreads();
       edge |= (uint32_t)found[0] << shift;
       mask |= 255u << shift;
       left = found[1];
     }
   }
-  const bool all = want >= L - recent - first;
-  // ---- how many of this block's places are above the edge, and how many equal it
-  auto above_edge = [&](uint32_t k) { return all || (want > 0 && k > edge); };
-  auto at_edge = [&](uint32_t k) { return !all && want > 0 && k == edge; };
-  int a = 0, e = 0;
-  for (int p = q0 + tid; p < q1; p += THREADS) {
-    const uint32_t k = key(p);
-    a += above_edge(k);
-    e += at_edge(k);
-  }
-  a = block_scan(a, warp_sums).y;
-  e = block_scan(e, warp_sums).y;
-  if (tid == 0) {
-    mine[0] = a;
-    mine[1] = e;
-  }
-  cluster.sync();
-  int equal = 0, at = 0;  // places equal to the edge, and kept places, before this block's
-  for (int q = 0; q < me; ++q) {
-    const int qa = *cluster.map_shared_rank(&mine[0], q), qe = *cluster.map_shared_rank(&mine[1], q);
-    const int forced0 = min(q * per, L), forced1 = min(forced0 + per, L);
-    at += qa + max(min(left, equal + qe) - min(left, equal), 0);
-    at += max(min(forced1, first) - forced0, 0) + max(forced1 - max(forced0, L - recent), 0);
-    equal += qe;
-  }
-  // ---- in order, THREADS at a time
-  for (int base = p0; base < p1; base += THREADS) {
-    const int p = base + tid;
-    bool keep = false, same = false;
-    if (p < p1) {
-      if (p < first || p >= L - recent) {
-        keep = true;
-      } else {
-        const uint32_t k = key(p);
-        keep = above_edge(k);
-        same = at_edge(k);
-      }
+  // ---- a warp's stretch of the block's places: how many are kept for certain, and how many equal the edge
+  const int stretch = (per + 32 * WARPS - 1) / (32 * WARPS) * 32, w0 = min(p0 + warp * stretch, p1), w1 = min(w0 + stretch, p1);
+  auto look = [&](int p, bool& keep, bool& same) {
+    keep = same = false;
+    if (p >= w1) return;
+    if (p < first || p >= L - recent) {
+      keep = true;
+    } else if (!some) {
+      keep = all;
+    } else {
+      const uint32_t k = key(p);
+      keep = k > edge;
+      same = k == edge;
     }
-    const int2 s = block_scan(same, warp_sums);
-    keep |= same && equal + s.x < left;
-    const int2 k = block_scan(keep, warp_sums);
-    if (keep) places[at + k.x] = p;
-    equal += s.y;
-    at += k.y;
+  };
+  int kept = 0, equal = 0;
+#pragma unroll 4
+  for (int base = w0; base < w1; base += 32) {
+    bool k, e;
+    look(base + lane, k, e);
+    kept += __popc(__ballot_sync(0xffffffffu, k));
+    equal += __popc(__ballot_sync(0xffffffffu, e));
   }
-  cluster.sync();  // (a block's shared memory stays until the others have read it)
+  if (lane == 0) {
+    warp_kept[0][warp] = kept;
+    warp_kept[1][warp] = equal;
+  }
+  __syncthreads();
+  int at = 0, before = 0;  // kept places, and places equal to the edge, before the warp's: first of the block
+  if (blocks > 1) {
+    if (tid == 0) {
+      int a = 0, e = 0;
+      for (int w = 0; w < WARPS; ++w) {
+        a += warp_kept[0][w];
+        e += warp_kept[1][w];
+      }
+      mine[0] = a;
+      mine[1] = e;
+    }
+    cluster.sync();
+    int t[2][MAX_CLUSTER];
+#pragma unroll
+    for (int q = 0; q < MAX_CLUSTER; ++q)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) t[i][q] = q < me ? *cluster.map_shared_rank(&mine[i], q) : 0;
+#pragma unroll
+    for (int q = 0; q < MAX_CLUSTER; ++q) {
+      at += t[0][q];
+      before += t[1][q];
+    }
+    cluster.barrier_arrive();  // (a block's shared memory stays until the others have read it)
+  }
+  for (int w = 0; w < warp; ++w) {
+    at += warp_kept[0][w];
+    before += warp_kept[1][w];
+  }
+  at += min(before, left);  // (of those that equal it the first so many are kept)
+  // ---- in order
+  const uint32_t below = (1u << lane) - 1;
+  for (int base = w0; base < w1; base += 32) {
+    bool k, e;
+    look(base + lane, k, e);
+    const uint32_t same = __ballot_sync(0xffffffffu, e);
+    k |= e && before + __popc(same & below) < left;
+    const uint32_t keep = __ballot_sync(0xffffffffu, k);
+    if (k) places[at + __popc(keep & below)] = base + lane;
+    before += __popc(same);
+    at += __popc(keep);
+  }
+  if (blocks > 1) cluster.barrier_wait();
 }
 
 // -------------------------------------------------------------------------------------------- moving
@@ -303,7 +350,8 @@ JLX_API int jlx_kv_choose(const ChooseArgs* args, int cluster, void* stream_) {
   const bool holds = per <= HELD;
   const size_t smem = holds ? (size_t)per * 4 : 0;
   auto kernel = holds ? kv_choose_kernel<true> : kv_choose_kernel<false>;
-  if (smem > 40 * 1024) JLX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (cluster > 8) JLX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (smem > 32 * 1024) JLX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster, P.R * P.H);
   cfg.blockDim = dim3(THREADS);

@@ -1557,7 +1557,7 @@ def kv_choose(sums: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor, pla
     args = _CHOOSE_ARGS.pack(sums.data_ptr(), lengths.data_ptr(), keep.data_ptr(), places.data_ptr(), counts.data_ptr(), status.data_ptr(), R, H, width,
                              places.shape[2], min(first, width), min(recent, width))
     blocks = 1
-    while blocks < 8 and (R * H * blocks < sm_count() and width >= 2048 * blocks or width > 16384 * blocks):
+    while blocks < 16 and (R * H * blocks < sm_count() and width >= 2048 * blocks or width > 16384 * blocks):
         blocks *= 2
     _run("kv_budget", "jlx_kv_choose", args, blocks, _raw_stream(dev))
 
