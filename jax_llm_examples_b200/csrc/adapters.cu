@@ -259,9 +259,16 @@ __global__ void __launch_bounds__(THREADS, WR * NT * 8 > 128 ? 1 : 2) adapters_k
     const int share = (ROWS * RC / 4 + blocks - 1) / blocks;
     for (int i = me * share + tid; i < min((me + 1) * share, ROWS * RC / 4); i += THREADS) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < blocks; ++q) {
-        const float4 w = reinterpret_cast<const float4*>(cluster.map_shared_rank(meet, q))[i];
-        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+#pragma unroll
+      for (int q0 = 0; q0 < MAX_CLUSTER; q0 += 8) {
+        if (q0 >= blocks) break;
+        float4 w[8];  // (asked for together: each takes a trip to another multiprocessor)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) w[q] = q0 + q < blocks ? reinterpret_cast<const float4*>(cluster.map_shared_rank(meet, q0 + q))[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          v.x += w[q].x; v.y += w[q].y; v.z += w[q].z; v.w += w[q].w;
+        }
       }
       float f[4] = {v.x * s, v.y * s, v.z * s, v.w * s};
       const int row = i * 4 / RC, col = i * 4 % RC;
@@ -446,13 +453,12 @@ static int launch_rank(const AdapterArgs& P, int cluster, cudaStream_t stream) {
 
 static bool rows_on_16(const void* p, long long ld, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0; }
 
-// Whether the call takes the one-launch kernel (else the plain ones, which need `low`).
+// Whether the call takes the one-launch kernel (else the plain ones, which need `low`: kernels/api.py has the same rule).
 static bool adapters_fast(const AdapterArgs& a) {
   const int size = a.out_type == JLX_F32 ? 4 : 2;
   return a.type == JLX_BF16 && a.r % 8 == 0 && a.K % 8 == 0 && a.No % 8 == 0 && rows_on_16(a.x, a.ldx, 2) && rows_on_16(a.a, 8, 2) && rows_on_16(a.b, 8, 2) &&
          rows_on_16(a.y, a.ldy, size) && rows_on_16(a.out, a.ldo, size);
 }
-JLX_API int jlx_adapters_fast(const AdapterArgs* a) { return adapters_fast(*a); }
 
 JLX_API int jlx_adapters(const AdapterArgs* args, int sms, void* stream_) {
   const AdapterArgs& P = *args;

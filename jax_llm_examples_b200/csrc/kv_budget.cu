@@ -3,10 +3,11 @@
 //
 // kv_choose, of a request's L places and n = min(keep, L): the last `recent` ones, then the first `first` ones, as far as n goes, then of the
 // rest those with the largest sums; ties go to the lowest place; NaN counts as the lowest sum, -0 as 0.  Places come in ascending
-// order.  A sum becomes a whole number of 32 bits with the same order; the bits of the smallest kept one are found eight at a time
-// by counting (a digit's count of the places that share the digits before it); then the places above it, and the first so many that
-// equal it, are counted and written, a warp going through a stretch of them by votes.  A cluster of blocks serves a request and KV
-// head, each with a stretch of the places in shared memory: the sums are read from memory once.
+// order.  A sum becomes a whole number of 32 bits with the same order, places that are kept in any case the largest one; the bits of the
+// smallest kept one are found eight at a time by counting (a digit's count of the places that share the digits before it), until few enough
+// places share them that each can be compared with all; then the places above it, and the first so many that equal it, are
+// counted and written, a warp going through a stretch of them by votes.  A
+// cluster of blocks serves a request and KV head, each with a stretch of the places in registers: the sums are read once.
 //
 // kv_compact moves rows bit for bit.  Into other pages every row is on its own.  In place, row i's new place is at or before its old
 // one: a block takes a column of 32 bytes of one plane's rows through all places in order, some hundreds at a time, all loads of
@@ -22,8 +23,9 @@ namespace cg = cooperative_groups;
 #define THREADS 512
 #define WARPS (THREADS / 32)
 #define MAX_CLUSTER 16
-#define COPIES 8  // of the counts: lanes with one digit (of exponents there are few) count in neighbouring banks
-#define HELD (96 * 1024 / 4)  // sums that a block holds in shared memory at most: two blocks a multiprocessor, so that a cluster of 16 has places
+#define BINS 256
+#define FEW 64  // places that are compared with each other
+#define MAX_KEYS 16  // sums that a thread keeps at most
 
 struct ChooseArgs {  // _CHOOSE_ARGS in kernels/api.py
   const float* sums;   // [R, H, width]
@@ -35,42 +37,23 @@ struct ChooseArgs {  // _CHOOSE_ARGS in kernels/api.py
   int R, H, width, most, first, recent;
 };
 
-// Larger numbers for larger sums; 0 for NaN (no number has it).
+// Larger numbers for larger sums, from 0x7fffff (-infinity) to 0xff800000 (infinity).
+#define KEY_NONE 0u  // no place
+#define KEY_NAN 1u
+#define KEY_ANY 0xffffffffu  // kept in any case
 __device__ __forceinline__ uint32_t ordered(float x) {
-  if (x != x) return 0u;
+  if (x != x) return KEY_NAN;
   const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// The sum of a number over the threads before this one, and over all of them.
-__device__ __forceinline__ int2 block_scan(int v, int* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    const int s = warp_sums[w];
-    before += w < warp ? s : 0;
-    all += s;
-  }
-  return make_int2(before + x - v, all);
-}
-
-// per: places of a block.  HOLDS: they are kept in shared memory (else read again from memory in every pass).
-template <bool HOLDS>
-__global__ void __launch_bounds__(THREADS) kv_choose_kernel(const ChooseArgs P, int per) {
+// per: places of a block.  KEYS: sums of a thread, its warp's stretch 32 by 32 (0: they are read again from memory in every pass).
+template <int KEYS>
+__global__ void __launch_bounds__(THREADS, 2) kv_choose_kernel(const ChooseArgs P, int per) {
   JLX_TL(TL_OTHER);
-  extern __shared__ uint32_t held[];
-  __shared__ __align__(16) int copies[256][COPIES];
-  __shared__ int count[2][256], warp_sums[WARPS], found[2], warp_kept[2][WARPS], mine[2];
+  __shared__ int bins[2][BINS];  // from the largest digit on
+  __shared__ uint32_t mine_few[FEW], few[FEW], found_edge;
+  __shared__ int warp_sums[WARPS], found[3], n_few, warp_kept[2][WARPS], mine[2];
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), me = cluster.block_rank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents_if_small();
@@ -82,88 +65,128 @@ __global__ void __launch_bounds__(THREADS) kv_choose_kernel(const ChooseArgs P, 
     L = min(max(L, 0), P.width);
   }
   n = min(min(max(n, 0), L), P.most);
-  const int recent = min(P.recent, n), first = min(P.first, n - recent), want = n - recent - first;  // want: chosen by their sums
+  const int recent = min(P.recent, n), first = min(P.first, n - recent);
   if (me == 0 && tid == 0 && row == r * P.H) P.counts[r] = n;
   const float* sums = P.sums + (size_t)row * P.width;
   int* places = P.places + (size_t)row * P.most;
   for (int i = n + me * THREADS + tid; i < P.most; i += blocks * THREADS) places[i] = -1;
-  // this block's places [p0, p1); of them [q0, q1) are a matter of choice
-  const int p0 = min(me * per, L), p1 = min(p0 + per, L), q0 = min(max(p0, first), p1), q1 = max(min(p1, L - recent), q0);
-  const bool all = want >= L - recent - first, some = want > 0 && !all;
-  auto key = [&](int p) { return HOLDS ? held[p - p0] : ordered(sums[p]); };
-  if (HOLDS && some) {
-#pragma unroll 8
-    for (int p = q0 + tid; p < q1; p += THREADS) held[p - p0] = ordered(sums[p]);
-    __syncthreads();
-  }
-  // the smallest sum that is chosen, and how many of the places with just that one
-  uint32_t edge = 0u, mask = 0u;
-  int left = want;
-  if (some) {
-    for (int shift = 24, half = 0; shift >= 0; shift -= 8, half ^= 1) {
-      for (int i = tid; i < 256 * COPIES / 4; i += THREADS) reinterpret_cast<int4*>(copies)[i] = make_int4(0, 0, 0, 0);
+  // this block's places, and of them a warp's
+  const int p1 = min((me + 1) * per, L), stretch = (per + 32 * WARPS - 1) / (32 * WARPS) * 32;
+  const int w0 = min(me * per + warp * stretch, p1), w1 = min(w0 + stretch, p1);
+  auto look = [&](int i) {
+    const int p = w0 + i * 32 + lane;
+    if (p >= w1) return KEY_NONE;
+    return p < first || p >= L - recent ? KEY_ANY : ordered(sums[p]);
+  };
+  uint32_t held[KEYS > 0 ? KEYS : 1];
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) held[i] = look(i);
+  const int steps = KEYS > 0 ? KEYS : stretch / 32;
+  auto key = [&](int i) { return KEYS > 0 ? held[KEYS > 0 ? i : 0] : look(i); };
+  // the smallest one that is kept, and how many of the places with just that one
+  uint32_t edge = KEY_NONE, mask = 0u;
+  int left = 0;
+  if (n > 0 && n < L) {
+    left = n;
+    for (int shift = 24, half = 0;; shift -= 8, half ^= 1) {
+      if (tid < BINS) bins[half][tid] = 0;
+      if (tid == 0) n_few = 0;
       __syncthreads();
-#pragma unroll 4
-      for (int p = q0 + tid; p < q1; p += THREADS) {
-        const uint32_t k = key(p);
-        if ((k & mask) == edge) atomicAdd(&copies[k >> shift & 255][lane % COPIES], 1);
-      }
-      __syncthreads();
-      // digits from the largest: thread i has digit 255 - i
-      int c = 0;
-      if (tid < 256) {
 #pragma unroll
-        for (int i = 0; i < COPIES; i += 4) {
-          const int4 v = *reinterpret_cast<const int4*>(&copies[255 - tid][i]);
-          c += v.x + v.y + v.z + v.w;
+      for (int i = 0; i < steps; ++i) {
+        const uint32_t k = key(i);
+        if (k != KEY_NONE && (k & mask) == edge) atomicAdd(&bins[half][~k >> shift & 255], 1);
+      }
+      if (blocks > 1) cluster.sync();  // (the counts of the digit before last have been read everywhere, too)
+      else __syncthreads();
+      if (tid < BINS) {  // a digit a thread
+        int c = 0;
+        if (blocks > 1) {
+#pragma unroll
+          for (int q0 = 0; q0 < MAX_CLUSTER; q0 += 8) {
+            if (q0 >= blocks) break;
+            int v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = q0 + q < blocks ? *cluster.map_shared_rank(&bins[half][tid], q0 + q) : 0;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) c += v[q];
+          }
+        } else {
+          c = bins[half][tid];
         }
-        count[half][tid] = c;
-      }
-      if (blocks > 1) {
-        cluster.sync();  // (the counts of the digit before last have been read everywhere, too)
-        if (tid < 256) {
-          int t[MAX_CLUSTER];
+        int above = c;
 #pragma unroll
-          for (int q = 0; q < MAX_CLUSTER; ++q) t[q] = q < blocks ? *cluster.map_shared_rank(&count[half][tid], q) : 0;
-          c = 0;
-#pragma unroll
-          for (int q = 0; q < MAX_CLUSTER; ++q) c += t[q];
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, above, o);
+          if (lane >= o) above += y;
         }
-      }
-      const int above = block_scan(c, warp_sums).x;
-      if (tid < 256 && above < left && above + c >= left) {
-        found[0] = 255 - tid;
-        found[1] = left - above;
+        if (lane == 31) warp_sums[warp] = above;
+        asm volatile("bar.sync 1, %0;" ::"n"(BINS) : "memory");
+        above += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0) - c;  // places with a larger digit
+        if (above < left && above + c >= left) {
+          found[0] = 255 - tid;
+          found[1] = left - above;
+          found[2] = c;
+        }
       }
       __syncthreads();
       edge |= (uint32_t)found[0] << shift;
       mask |= 255u << shift;
       left = found[1];
+      const int share = found[2];  // places that share the digits up to here
+      if (shift == 0) break;       // (all digits: they are equal)
+      if (share <= FEW) {
+#pragma unroll
+        for (int i = 0; i < steps; ++i) {
+          const uint32_t k = key(i);
+          if (k != KEY_NONE && (k & mask) == edge) mine_few[atomicAdd(&n_few, 1)] = k;
+        }
+        if (blocks > 1) {
+          cluster.sync();
+          int n_q = lane < blocks ? *cluster.map_shared_rank(&n_few, lane) : 0, at = n_q;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += y;
+          }
+          if (warp < blocks) {  // a warp fetches a block's
+            const int count = __shfl_sync(0xffffffffu, n_q, warp), to = __shfl_sync(0xffffffffu, at, warp) - count;
+            const uint32_t* from = cluster.map_shared_rank(mine_few, warp);
+            for (int i = lane; i < count; i += 32) few[to + i] = from[i];
+          }
+        }
+        __syncthreads();
+        if (tid < share) {
+          const uint32_t* all = blocks > 1 ? few : mine_few;
+          const uint32_t k = all[tid];
+          int more = 0, same = 0;
+          for (int i = 0; i < share; ++i) {
+            more += all[i] > k;
+            same += all[i] == k;
+          }
+          if (more < left && more + same >= left) {  // (whoever has that sum writes the same)
+            found_edge = k;
+            found[0] = left - more;
+          }
+        }
+        __syncthreads();
+        edge = found_edge;
+        left = found[0];
+        break;
+      }
     }
   }
-  // ---- a warp's stretch of the block's places: how many are kept for certain, and how many equal the edge
-  const int stretch = (per + 32 * WARPS - 1) / (32 * WARPS) * 32, w0 = min(p0 + warp * stretch, p1), w1 = min(w0 + stretch, p1);
-  auto look = [&](int p, bool& keep, bool& same) {
-    keep = same = false;
-    if (p >= w1) return;
-    if (p < first || p >= L - recent) {
-      keep = true;
-    } else if (!some) {
-      keep = all;
-    } else {
-      const uint32_t k = key(p);
-      keep = k > edge;
-      same = k == edge;
-    }
-  };
+  // ---- how many of the warp's places are above the edge, and how many equal it.  (Without an edge all places are above it, or none is kept.)
+  if (n == 0) edge = KEY_ANY;
   int kept = 0, equal = 0;
-#pragma unroll 4
-  for (int base = w0; base < w1; base += 32) {
-    bool k, e;
-    look(base + lane, k, e);
-    kept += __popc(__ballot_sync(0xffffffffu, k));
-    equal += __popc(__ballot_sync(0xffffffffu, e));
+#pragma unroll
+  for (int i = 0; i < steps; ++i) {
+    const uint32_t k = key(i);
+    kept += k > edge;
+    equal += k == edge;
   }
+  kept = __reduce_add_sync(0xffffffffu, kept);
+  equal = __reduce_add_sync(0xffffffffu, equal);
   if (lane == 0) {
     warp_kept[0][warp] = kept;
     warp_kept[1][warp] = equal;
@@ -171,43 +194,35 @@ __global__ void __launch_bounds__(THREADS) kv_choose_kernel(const ChooseArgs P, 
   __syncthreads();
   int at = 0, before = 0;  // kept places, and places equal to the edge, before the warp's: first of the block
   if (blocks > 1) {
-    if (tid == 0) {
-      int a = 0, e = 0;
-      for (int w = 0; w < WARPS; ++w) {
-        a += warp_kept[0][w];
-        e += warp_kept[1][w];
+    if (tid < 32) {
+      const int a = __reduce_add_sync(0xffffffffu, lane < WARPS ? warp_kept[0][lane] : 0), e = __reduce_add_sync(0xffffffffu, lane < WARPS ? warp_kept[1][lane] : 0);
+      if (lane == 0) {
+        mine[0] = a;
+        mine[1] = e;
       }
-      mine[0] = a;
-      mine[1] = e;
     }
     cluster.sync();
-    int t[2][MAX_CLUSTER];
-#pragma unroll
-    for (int q = 0; q < MAX_CLUSTER; ++q)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) t[i][q] = q < me ? *cluster.map_shared_rank(&mine[i], q) : 0;
-#pragma unroll
-    for (int q = 0; q < MAX_CLUSTER; ++q) {
-      at += t[0][q];
-      before += t[1][q];
-    }
+    const int a = lane < me ? *cluster.map_shared_rank(&mine[0], lane) : 0, e = lane < me ? *cluster.map_shared_rank(&mine[1], lane) : 0;
+    at = __reduce_add_sync(0xffffffffu, a);
+    before = __reduce_add_sync(0xffffffffu, e);
     cluster.barrier_arrive();  // (a block's shared memory stays until the others have read it)
   }
-  for (int w = 0; w < warp; ++w) {
-    at += warp_kept[0][w];
-    before += warp_kept[1][w];
-  }
+  at += __reduce_add_sync(0xffffffffu, lane < warp ? warp_kept[0][lane] : 0);
+  before += __reduce_add_sync(0xffffffffu, lane < warp ? warp_kept[1][lane] : 0);
   at += min(before, left);  // (of those that equal it the first so many are kept)
   // ---- in order
   const uint32_t below = (1u << lane) - 1;
-  for (int base = w0; base < w1; base += 32) {
-    bool k, e;
-    look(base + lane, k, e);
-    const uint32_t same = __ballot_sync(0xffffffffu, e);
-    k |= e && before + __popc(same & below) < left;
-    const uint32_t keep = __ballot_sync(0xffffffffu, k);
-    if (k) places[at + __popc(keep & below)] = base + lane;
-    before += __popc(same);
+#pragma unroll
+  for (int i = 0; i < steps; ++i) {
+    const uint32_t k = key(i);
+    bool take = k > edge;
+    if (before < left) {  // (the warp's: some that equal it are still to be kept)
+      const uint32_t same = __ballot_sync(0xffffffffu, k == edge);
+      take |= k == edge && before + __popc(same & below) < left;
+      before += __popc(same);
+    }
+    const uint32_t keep = __ballot_sync(0xffffffffu, take);
+    if (take) places[at + __popc(keep & below)] = w0 + i * 32 + lane;
     at += __popc(keep);
   }
   if (blocks > 1) cluster.barrier_wait();
@@ -346,16 +361,13 @@ JLX_API int jlx_kv_choose(const ChooseArgs* args, int cluster, void* stream_) {
   JLX_REQUIRE(P.R > 0 && P.H > 0 && P.width > 0 && P.most >= 0 && P.first >= 0 && P.recent >= 0, "kv_choose: bad sizes");
   JLX_REQUIRE(cluster >= 1 && cluster <= MAX_CLUSTER, "kv_choose: %d blocks a row", cluster);
   JLX_REQUIRE((long long)P.R * P.H <= 65535, "kv_choose: %d requests of %d KV heads are too many for a launch", P.R, P.H);
-  const int per = ((P.width + cluster - 1) / cluster + 3) / 4 * 4;
-  const bool holds = per <= HELD;
-  const size_t smem = holds ? (size_t)per * 4 : 0;
-  auto kernel = holds ? kv_choose_kernel<true> : kv_choose_kernel<false>;
+  const int per = (P.width + cluster - 1) / cluster, keys = (per + THREADS - 1) / THREADS;
+  static_assert(BINS <= THREADS && FEW <= THREADS && MAX_CLUSTER <= WARPS, "a thread has a digit, a warp fetches a block's places");
+  auto kernel = keys <= 2 ? kv_choose_kernel<2> : keys <= 4 ? kv_choose_kernel<4> : keys <= 8 ? kv_choose_kernel<8> : keys <= MAX_KEYS ? kv_choose_kernel<MAX_KEYS> : kv_choose_kernel<0>;
   if (cluster > 8) JLX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  if (smem > 32 * 1024) JLX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster, P.R * P.H);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream_;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

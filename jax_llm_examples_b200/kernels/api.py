@@ -1427,6 +1427,26 @@ def tree_masks(parents) -> "tuple[list[int], list[list[int]]]":
     return depth, [[signed(b >> (32 * w) & 0xFFFFFFFF) for w in range(words)] for b in bits]
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors' rows share bytes.  (Column ranges of the same rows, side by side, do not.)"""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    a1, b1 = (p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else p for t, p in ((a, a0), (b, b0)))
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if a.dim() == b.dim() == 2 and a.shape[0] > 1 and b.shape[0] > 1:
+        wide = a.stride(0) * a.element_size()
+        if wide and wide == b.stride(0) * b.element_size():
+            at, aw, bw = (b0 - a0) % wide, a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+            return not (at >= aw and at + bw <= wide)
+    return True
+
+
+def _same_or_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two whole tensors of one shape and type are one, or share no bytes."""
+    d = a.data_ptr() - b.data_ptr()
+    return d == 0 or abs(d) >= a.numel() * a.element_size()
+
+
 # ------------------------------------------------- a cache kept to a budget: weights, choice, moving the kept rows
 _WEIGHTS_ARGS = struct.Struct("@4P2i")  # WeightsArgs in csrc/attention_weights.cuh
 WEIGHTS_FEW = 16  # query rows of a request and KV head that attention_weights.cu takes
@@ -1485,7 +1505,7 @@ def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.T
     _ints(what, ("cu_q", cu_q, R + 1), ("positions", positions, N), ("status", status, 1))
     if out.dtype is not torch.float32 or out.dim() != 3 or out.shape[:2] != (R, Hkv):
         raise KernelError(f"{what}: out must be float32 [{R}, {Hkv}, places], not {out.dtype} {tuple(out.shape)}")
-    if add is not None and (add.dtype is not torch.float32 or add.shape != out.shape or (add.data_ptr() != out.data_ptr() and _overlap(add, out))):
+    if add is not None and (add.dtype is not torch.float32 or add.shape != out.shape or not _same_or_apart(add, out)):
         raise KernelError(f"{what}: add must be float32 {tuple(out.shape)}, out itself or apart from it")
     if max_kv_len < 1 or max_count < 1:
         raise KernelError(f"{what}: {max_count} tokens of a request over {max_kv_len} keys")
@@ -1557,7 +1577,7 @@ def kv_choose(sums: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor, pla
     args = _CHOOSE_ARGS.pack(sums.data_ptr(), lengths.data_ptr(), keep.data_ptr(), places.data_ptr(), counts.data_ptr(), status.data_ptr(), R, H, width,
                              places.shape[2], min(first, width), min(recent, width))
     blocks = 1
-    while blocks < 16 and (R * H * blocks < sm_count() and width >= 2048 * blocks or width > 16384 * blocks):
+    while blocks < 16 and (R * H * blocks < sm_count() and width >= 2048 * blocks or width > 8192 * blocks):
         blocks *= 2
     _run("kv_budget", "jlx_kv_choose", args, blocks, _raw_stream(dev))
 
@@ -1592,7 +1612,7 @@ def kv_compact(pages: torch.Tensor, block_table: torch.Tensor, places: torch.Ten
     if sums is not None:
         if any(t.dtype is not torch.float32 or t.dim() != 3 or t.shape[:2] != (R, H) for t in (sums, sums_out)):
             raise KernelError(f"{what}: sums must be float32 [{R}, {H}, places]")
-        if _overlap(sums, sums_out) and not (sums.data_ptr() == sums_out.data_ptr() and sums.shape == sums_out.shape):
+        if not _same_or_apart(sums, sums_out) if sums.shape == sums_out.shape else _overlap(sums, sums_out):
             raise KernelError(f"{what}: sums_out must be sums itself or apart from it")
     dev = _placed(what, pages, block_table, places, counts, status, into, scales, sums, sums_out)
     if most == 0 and sums_out is not None:
@@ -1720,21 +1740,6 @@ def _rows_of(what: str, name: str, t: torch.Tensor, n: int, width: int, written:
     return t.stride(0) if n > 1 else width
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors' rows share bytes.  (Column ranges of the same rows, side by side, do not.)"""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else t.data_ptr()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    if a1 <= b0 or b1 <= a0:
-        return False
-    if a.dim() == b.dim() == 2 and a.shape[0] > 1 and b.shape[0] > 1:
-        wide = a.stride(0) * a.element_size()
-        if wide and wide == b.stride(0) * b.element_size():
-            at, aw, bw = (b0 - a0) % wide, a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
-            return not (at >= aw and at + bw <= wide)
-    return True
-
-
 def adapter_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: AdapterPlan, y: torch.Tensor, out: torch.Tensor | None = None,
                 scale: torch.Tensor | None = None, ranks: torch.Tensor | None = None) -> None:
     """out[n] = y[n] + scale[e] (x[n] a[e]^T) b[e]^T for row n's adapter e in ``plan`` (no adapter: out[n] = y[n]): what low-rank
@@ -1746,39 +1751,42 @@ def adapter_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Adapter
     if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
         raise KernelError(f"adapter_add: matrices a {tuple(a.shape)} and b {tuple(b.shape)} are not [E, r, K] and [E, No, r]")
     (E, r, K), No, N = a.shape, b.shape[1], x.shape[0]
-    if x.dtype != a.dtype or x.dtype != b.dtype or y.dtype != out.dtype:
+    type_, out_type = x.dtype, y.dtype
+    if a.dtype is not type_ or b.dtype is not type_ or out.dtype is not out_type:
         raise KernelError("adapter_add: x, a and b must have one type, and so must y and out")
     if plan.rows != N or plan.adapters != E:
         raise KernelError(f"adapter_add: the plan is for {plan.rows} rows and {plan.adapters} adapters, not {N} and {E}")
     if not 0 < r <= ADAPTER_MAX_RANK or K < 1 or No < 1:
         raise KernelError(f"adapter_add: rank {r} (up to {ADAPTER_MAX_RANK}), {K} and {No} entries a row are not supported")
-    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != E):
+    if scale is not None and (scale.dtype is not torch.float32 or scale.numel() != E):
         raise KernelError(f"adapter_add: scale must be float32 [{E}]")
-    if ranks is not None and (ranks.dtype != torch.int32 or ranks.numel() != E):
+    if ranks is not None and (ranks.dtype is not torch.int32 or ranks.numel() != E):
         raise KernelError(f"adapter_add: ranks must be int32 [{E}]")
-    types = code(x.dtype), code(y.dtype)
-    ld = _rows_of("adapter_add", "x", x, N, K), _rows_of("adapter_add", "y", y, N, No), _rows_of("adapter_add", "out", out, N, No, True)
+    type_, out_type = code(type_), code(out_type)
+    ldx, ldy, ldo = _rows_of("adapter_add", "x", x, N, K), _rows_of("adapter_add", "y", y, N, No), _rows_of("adapter_add", "out", out, N, No, True)
     dev = _placed("adapter_add", a, b, plan.order, plan.tiles, scale, ranks)
-    for t in (x, y, out):
-        if t.get_device() != dev:
-            raise KernelError(f"adapter_add: a tensor is on {t.device}, the current device is cuda:{dev}")
-    same = out.data_ptr() == y.data_ptr() and ld[1] == ld[2]
-    if any(_overlap(out, t) for t in (x, a, b)) or not (same or not _overlap(out, y)):
+    if x.get_device() != dev or y.get_device() != dev or out.get_device() != dev:
+        raise KernelError(f"adapter_add: x, y and out are on {x.device}, {y.device} and {out.device}, the current device is cuda:{dev}")
+    x_p, a_p, b_p, y_p, out_p = x.data_ptr(), a.data_ptr(), b.data_ptr(), y.data_ptr(), out.data_ptr()
+    size, out_size = (2 if type_ else 4), (2 if out_type else 4)
+    out_end = out_p + ((N - 1) * ldo + No) * out_size
+    # (first whether anything lies within the rows' span at all)
+    if (out_p < x_p + ((N - 1) * ldx + K) * size and x_p < out_end and _overlap(out, x)) or (out_p < a_p + E * r * K * size and a_p < out_end) or (
+            out_p < b_p + E * r * No * size and b_p < out_end) or (
+            not (out_p == y_p and ldo == ldy) and out_p < y_p + ((N - 1) * ldy + No) * out_size and y_p < out_end and _overlap(out, y)):
         raise KernelError("adapter_add: out shares memory with an operand (only y itself may be written over)")
     if N == 0:
         return
-    args = [x.data_ptr(), a.data_ptr(), b.data_ptr(), y.data_ptr(), out.data_ptr(), plan.order.data_ptr(), plan.tiles.data_ptr(), _address(scale),
-            _address(ranks), 0, *ld, N, N, E, r, K, No, plan.tiles.shape[0], plan.tile_rows, *types]
-    packed = _ADAPTER_ARGS.pack(*args)
-    plain = not library("adapters").jlx_adapters_fast(packed)
+    # the same rule as the launcher's: rows of whole 16 bytes on 16-byte boundaries take one kernel, anything else two
+    plain = not type_ or (r | K | No | ldx) & 7 or (x_p | a_p | b_p | y_p | out_p | ldy * out_size | ldo * out_size) & 15
+    # scratch is made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
+    low = torch.empty(N * r, dtype=torch.float32, device=x.device) if plain else None
+    _run("adapters", "jlx_adapters",
+         _ADAPTER_ARGS.pack(x_p, a_p, b_p, y_p, out_p, plan.order.data_ptr(), plan.tiles.data_ptr(), _address(scale), _address(ranks), _address(low), ldx, ldy, ldo,
+                            N, N, E, r, K, No, plan.tiles.shape[0], plan.tile_rows, type_, out_type), sm_count(), _raw_stream(dev))
     if plain:
-        # made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
-        low = torch.empty(N * r, dtype=torch.float32, device=x.device)
-        args[9] = low.data_ptr()
-        packed = _ADAPTER_ARGS.pack(*args)
-    _run("adapters", "jlx_adapters", packed, sm_count(), _raw_stream(dev))
-    global _launches
-    _launches += plain  # two kernels
+        global _launches
+        _launches += 1  # two kernels
 
 
 # --------------------------------------------------------------------------------------- MoE
