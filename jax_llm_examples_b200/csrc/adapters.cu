@@ -24,6 +24,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "mbarrier.cuh"
 #include "mma_sync.cuh"
 
 namespace cg = cooperative_groups;
@@ -108,6 +109,13 @@ template <> struct Eight<float> {
   }
 };
 
+// Stages of x and A in shared memory.
+template <int MT, int RC, int WK> struct Stage {
+  static constexpr int SUBS = WK > 4 ? WK / 4 : 1, K = 64 * SUBS;
+  static constexpr int X_CHUNKS = SUBS * MT * 16 * 8, A_CHUNKS = SUBS * RC * 8;
+  static constexpr int X_BYTES = X_CHUNKS * 16, BYTES = X_BYTES + A_CHUNKS * 16, STAGES = 4;
+};
+
 // MT: tiles of 16 rows.  NT: tiles of 8 ranks that a warp has; the block's warps are WR groups of them (WR * NT * 8 >= r) times
 // WK cuts of K.  PARTS: bfloat16 numbers that a 32-bit sum between the products becomes.
 template <int MT, int NT, int WR, typename TY>
@@ -116,8 +124,8 @@ __global__ void __launch_bounds__(THREADS, WR * NT * 8 > 128 ? 1 : 2) adapters_k
   constexpr int ROWS = 16 * MT, WK = WARPS / WR, RC = WR * NT * 8, LD = low_stride(RC);
   constexpr int PARTS = sizeof(TY) == 4 ? 3 : 2;
   constexpr int STEPS = (RC + 31) / 32;  // of 32 ranks in the second product (the last one may be short)
-  constexpr bool EARLY = MT == 1 && STEPS <= 2;  // room in registers for what the next 32 columns need
-  extern __shared__ __align__(16) uint8_t smem_raw[];
+  constexpr bool EARLY = MT == 1 && STEPS == 1;  // room in registers for what the next 32 columns need
+  extern __shared__ __align__(128) uint8_t smem_raw[];
   float* meet = reinterpret_cast<float*>(smem_raw);                  // [max(WK / 2, 1)][ROWS][RC]: the warps' sums; then [ROWS][RC] of the block
   bf16* low = reinterpret_cast<bf16*>(meet + (WK > 1 ? WK / 2 : 1) * ROWS * RC);  // [PARTS][ROWS][LD]
   __shared__ int row_s[ROWS];
@@ -153,6 +161,15 @@ __global__ void __launch_bounds__(THREADS, WR * NT * 8 > 128 ? 1 : 2) adapters_k
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
           const int k = s * 32 + t4 * 8;
+          if (P.r & 7) {  // rows of B off 16-byte boundaries: entry by entry
+            const int left = n < P.No ? t.rank - k : 0;
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(br + k);
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (2 * i < left ? e[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)e[2 * i + 1] << 16 : 0u);
+            f.b[s][j] = make_uint4(w[0], w[1], w[2], w[3]);
+            continue;
+          }
           f.b[s][j] = n < P.No && k < t.rank ? *reinterpret_cast<const uint4*>(br + k) : make_uint4(0, 0, 0, 0);
           if (t.rank & 7) f.b[s][j] = first_of(f.b[s][j], t.rank - k);
         }
@@ -219,13 +236,72 @@ __global__ void __launch_bounds__(THREADS, WR * NT * 8 > 128 ? 1 : 2) adapters_k
         fetch(c + 2 * WK, even);
         multiply(odd);
       }
-    } else {
+    } else if (MT == 1) {
 #pragma unroll 1
       for (int c = c0 + wk; c < c1; c += WK) {
         Step f;
         fetch(c, f);
         multiply(f);
       }
+    } else {
+      // Many rows: registers hold the sums, and no second step's operands; so both come through shared memory, STAGES - 1 stages ahead.  A
+      // stage has SUBS times 64 of K, in rows of 128 bytes whose chunks of 16 are swizzled; a warp has every WK-th 16 of K.
+      using S = Stage<MT, RC, WK>;
+      const int k_begin = c0 * 32, k_end = min(c1 * 32, P.K), stages = (k_end - k_begin + S::K - 1) / S::K;
+      const uint32_t ring = smem_u32(smem_raw);
+      auto ask = [&](int st) {
+        const uint32_t to = ring + (st % S::STAGES) * S::BYTES;
+        const int k0 = k_begin + st * S::K;
+#pragma unroll
+        for (int i = 0; i < S::X_CHUNKS / THREADS; ++i) {
+          const int q = i * THREADS + tid, sub = q / (ROWS * 8), row = q / 8 % ROWS, c = q & 7, k = k0 + sub * 64 + c * 8, n = row_s[row];
+          const bool in = n >= 0 && k < k_end;
+          cp_async16(to + (sub * ROWS + row) * 128 + ((c ^ (row & 7)) << 4), in ? x + (size_t)n * P.ldx + k : x, in);
+        }
+#pragma unroll
+        for (int i = 0; i < (S::A_CHUNKS + THREADS - 1) / THREADS; ++i) {
+          const int q = i * THREADS + tid, sub = q / (RC * 8), row = q / 8 % RC, c = q & 7, k = k0 + sub * 64 + c * 8;
+          const bool in = row < t.rank && k < k_end;
+          if (S::A_CHUNKS % THREADS == 0 || q < S::A_CHUNKS)
+            cp_async16(to + S::X_BYTES + (sub * RC + row) * 128 + ((c ^ (row & 7)) << 4), in ? a + ((size_t)t.e * P.r + row) * P.K + k : a, in);
+        }
+      };
+#pragma unroll
+      for (int st = 0; st < S::STAGES - 1; ++st) {
+        if (st < stages) ask(st);
+        cp_async_commit();
+      }
+#pragma unroll 1
+      for (int st = 0; st < stages; ++st) {
+        cp_async_wait<S::STAGES - 2>();
+        __syncthreads();  // (the stage has come, and the one before has been read by all)
+        if (st + S::STAGES - 1 < stages) ask(st + S::STAGES - 1);
+        cp_async_commit();
+        const uint32_t from = ring + (st % S::STAGES) * S::BYTES;
+#pragma unroll
+        for (int z = 0; z < S::K / 16; z += WK) {
+          const int step = z + wk, sub = step >> 2, c = (step & 3) * 2;  // its two chunks of a row
+          uint32_t bf_[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; n += 2) {  // two tiles of 8 ranks (one: the other lanes' addresses are not used)
+            const int row = (wr * NT + n) * 8 + (lane & 7) + (NT > 1 ? (lane >> 4) * 8 : 0), ch = c + (lane >> 3 & 1);
+            uint32_t r0, r1, r2, r3;
+            ldmatrix_x4(from + S::X_BYTES + (sub * RC + row) * 128 + ((ch ^ (row & 7)) << 4), r0, r1, r2, r3);
+            bf_[n][0] = r0; bf_[n][1] = r1;
+            if (NT > 1) { bf_[(n + 1) % NT][0] = r2; bf_[(n + 1) % NT][1] = r3; }
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const int row = m * 16 + (lane & 15), ch = c + (lane >> 4);
+            uint32_t f[4];
+            ldmatrix_x4(from + (sub * ROWS + row) * 128 + ((ch ^ (row & 7)) << 4), f[0], f[1], f[2], f[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(acc[m][n], f, bf_[n][0], bf_[n][1]);
+          }
+        }
+      }
+      cp_async_wait<0>();
+      __syncthreads();  // (the ring's memory is the sums' now)
     }
     if (EARLY) fetch_b(u0 + warp, first);  // (B's first part is on its way while the sums meet)
     // ---- the warps' sums, halved until one is left
@@ -296,15 +372,25 @@ __global__ void __launch_bounds__(THREADS, WR * NT * 8 > 128 ? 1 : 2) adapters_k
     const bool mine = col < P.No;
     const B now = first;
     if (EARLY) fetch_b(u + WARPS, first);
+    constexpr int TOGETHER = sizeof(TY) == 4 && MT > 2 ? 2 : MT;  // tiles of rows whose y is asked for together
+    Eight<TY> yt[TOGETHER][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
+      if (!EARLY && m % TOGETHER == 0) {
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = mine ? row_s[(m + i) * 16 + h * 8 + g] : -1;
+            if (row >= 0) yt[i][h].load(y + (size_t)row * P.ldy + col);
+          }
+      }
       Eight<TY> ys[2];
       int n[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         n[h] = mine ? row_s[m * 16 + h * 8 + g] : -1;
-        if (EARLY) ys[h] = now.y[h];
-        else if (n[h] >= 0) ys[h].load(y + (size_t)n[h] * P.ldy + col);
+        ys[h] = EARLY ? now.y[h] : yt[m % TOGETHER][h];
       }
       if (t.e < 0) {
 #pragma unroll
@@ -418,7 +504,9 @@ __global__ void __launch_bounds__(THREADS) adapters_out_kernel(const AdapterArgs
 template <int MT, int NT, int WR, typename TY>
 static int launch_adapters(const AdapterArgs& P, int cluster, cudaStream_t stream) {
   constexpr int ROWS = 16 * MT, WK = WARPS / WR, RC = WR * NT * 8, PARTS = sizeof(TY) == 4 ? 3 : 2;
-  constexpr size_t smem = (size_t)(WK > 1 ? WK / 2 : 1) * ROWS * RC * 4 + (size_t)PARTS * ROWS * low_stride(RC) * 2;
+  using S = Stage<MT, RC, WK>;
+  constexpr size_t sums = (size_t)(WK > 1 ? WK / 2 : 1) * ROWS * RC * 4 + (size_t)PARTS * ROWS * low_stride(RC) * 2, ring = MT > 1 ? S::STAGES * S::BYTES : 0;
+  constexpr size_t smem = sums > ring ? sums : ring;
   auto kernel = adapters_kernel<MT, NT, WR, TY>;
   static_assert(smem <= 227 * 1024, "a tile's sums do not fit into shared memory");
   if (smem > 48 * 1024) JLX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -456,8 +544,8 @@ static bool rows_on_16(const void* p, long long ld, int size) { return ((uintptr
 // Whether the call takes the one-launch kernel (else the plain ones, which need `low`: kernels/api.py has the same rule).
 static bool adapters_fast(const AdapterArgs& a) {
   const int size = a.out_type == JLX_F32 ? 4 : 2;
-  return a.type == JLX_BF16 && a.r % 8 == 0 && a.K % 8 == 0 && a.No % 8 == 0 && rows_on_16(a.x, a.ldx, 2) && rows_on_16(a.a, 8, 2) && rows_on_16(a.b, 8, 2) &&
-         rows_on_16(a.y, a.ldy, size) && rows_on_16(a.out, a.ldo, size);
+  return a.type == JLX_BF16 && a.K % 8 == 0 && a.No % 8 == 0 && rows_on_16(a.x, a.ldx, 2) && rows_on_16(a.a, 8, 2) && rows_on_16(a.b, 8, 2) && rows_on_16(a.y, a.ldy, size) &&
+         rows_on_16(a.out, a.ldo, size);
 }
 
 JLX_API int jlx_adapters(const AdapterArgs* args, int sms, void* stream_) {

@@ -1778,7 +1778,7 @@ def adapter_add(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Adapter
     if N == 0:
         return
     # the same rule as the launcher's: rows of whole 16 bytes on 16-byte boundaries take one kernel, anything else two
-    plain = not type_ or (r | K | No | ldx) & 7 or (x_p | a_p | b_p | y_p | out_p | ldy * out_size | ldo * out_size) & 15
+    plain = not type_ or (K | No | ldx) & 7 or (x_p | a_p | b_p | y_p | out_p | ldy * out_size | ldo * out_size) & 15
     # scratch is made per call: the caching allocator ties it to this stream, so calls on other streams and captured graphs have their own
     low = torch.empty(N * r, dtype=torch.float32, device=x.device) if plain else None
     _run("adapters", "jlx_adapters",
