@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(THREADS, WR * NT * 8 > 128 ? 1 : 2) adapters_k
   const int blocks = cluster.num_blocks(), me = cluster.block_rank();
   const int subs = (P.tile_rows + ROWS - 1) / ROWS, tile = blockIdx.y / subs;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  pdl_launch_dependents_if_small();
+  if (MT == 1) pdl_launch_dependents_if_small();  // (a successor that waits beside the blocks of many rows costs them half their speed: 50 us for 33)
   pdl_wait();
   AdapterTile t;
   if (!adapter_tile(P, tile, (blockIdx.y - tile * subs) * ROWS, ROWS, t)) return;  // (the whole cluster)
