@@ -8,7 +8,7 @@ from .delta_rule import GatedDeltaRule
 from .feedforward import DenseBiasedMLP, DenseSwiGLU, GroupLimitedGLUExperts, RoutedExperts, RoutedMLPExperts, SoftmaxRoutedMLPExperts, TableRoutedGLUExperts
 from .latent_attention import LatentAttention, rotary_frequencies
 from .linear_attention import GatedLinearAttention, RetentionMixer, TimeMixWKV
-from .linear import grouped_linear, grouped_swiglu_linear, interleave_gate_up, linear, swiglu_linear
+from .linear import Adapters, adapted_linear, grouped_linear, grouped_swiglu_linear, interleave_gate_up, linear, swiglu_linear
 from .parallel import ParallelMixers
 from .norms import GroupRMSNorm, RMSNorm, StreamRMSNorm, add_to_residual
 from .recurrent import HGRN2, InputConvMixer
@@ -26,5 +26,5 @@ __all__ = [
     "Block", "CachePlan", "DecoderModel", "DenseSwiGLU", "FeedForward", "InterleavedRope", "KVNeed", "LayerCache",
     "LayerRun", "Mixer", "NoPositionWithTemperature", "Norm", "PagedAttention", "Part", "PositionEncoding",
     "PreNormBlock", "RMSNorm", "RoutedExperts", "Rows", "RowSum", "Runtime", "Workspace", "as_rows", "grouped_swiglu_linear", "interleave_gate_up", "swiglu_linear", "StateNeed", "StepContext", "StepShape", "plan_attention_tiles", "UnfusedEncoding",
-    "grouped_linear", "known_parts", "linear", "llama3_scaled_frequencies", "make_part", "register_part",
+    "Adapters", "adapted_linear", "grouped_linear", "known_parts", "linear", "llama3_scaled_frequencies", "make_part", "register_part",
 ]

@@ -17,6 +17,8 @@ Which kernel runs:
 
 from __future__ import annotations
 
+import dataclasses
+
 import torch
 
 from ..kernels import api as K
@@ -91,6 +93,27 @@ def linear(ctx: StepContext, a: torch.Tensor, w: torch.Tensor, out_dtype: torch.
         out = torch.empty((M, N), dtype=out_dtype, device=a.device)
         K.gemm_simt(a, w, out)
     return Rows(out, 1) if partials else out
+
+
+@dataclasses.dataclass
+class Adapters:
+    """Low-rank adapters beside one projection: ``a`` [E, r, K] and ``b`` [E, N, r] in the activations' type, ``scale`` float32 [E] and
+    ``ranks`` int32 [E] or None (see ``K.adapter_add``)."""
+
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: torch.Tensor | None = None
+    ranks: torch.Tensor | None = None
+
+
+def adapted_linear(ctx: StepContext, a: torch.Tensor, w: torch.Tensor, adapters: Adapters, plan: K.AdapterPlan, out_dtype: torch.dtype,
+                   partials: bool = False):
+    """:func:`linear` plus what every row's own adapter adds (``plan``: the step's, from ``K.adapter_plan``).  Of split-K partials
+    the first slice takes it, in 32 bits."""
+    out = linear(ctx, a, w, out_dtype, partials)
+    rows = out.data if isinstance(out, Rows) else out
+    K.adapter_add(a, adapters.a, adapters.b, plan, rows[0] if rows.dim() == 3 else rows, scale=adapters.scale, ranks=adapters.ranks)
+    return out
 
 
 def swiglu_linear(ctx: StepContext, a: torch.Tensor, w_gate_up: torch.Tensor, interleaved: bool,

@@ -149,3 +149,24 @@ def test_no_rows_and_counted_launches():
     assert K().launch_count() == before + 1
     Step([0, 1], 2, 8, 63, 64).run()
     assert K().launch_count() == before + 3
+
+
+@pytest.mark.parametrize("rows, dtype, out_dtype, partials", [("few", BF, BF, True), ("shared", BF, F32, False), ("steps beside a portion", BF, F32, True),
+                                                             ("portions", BF, BF, False), ("few", F32, F32, True)])
+def test_beside_a_projection(rows, dtype, out_dtype, partials):
+    """The part that does both: the projection's own kernels for few and for many rows, adapters on its result or its partials."""
+    from jax_llm_examples_b200.parts import Adapters, Runtime, StepContext, Workspace, adapted_linear, linear
+    from jax_llm_examples_b200.parts.base import Rows
+
+    of_row = ROWS[rows] * (3 if rows == "portions" else 1)  # (over 256 rows: the library's product)
+    step = Step(of_row, 6, 16, 1024, 512, dtype, out_dtype, seed=3)
+    w = (torch.randn(512, 1024, generator=torch.Generator().manual_seed(4)) * 1024 ** -0.5).to(dtype).cuda()
+    N, t = len(of_row), torch.zeros(len(of_row), dtype=torch.int32, device="cuda")
+    ctx = StepContext(runtime=Runtime(dtype, torch.device("cuda")), n_tokens=N, n_requests=1, token_ids=t, positions=t, req_of_token=t, cu_q=t[:2], q_start=t[:1],
+                      kv_len=t[:1], slot_ids=t[:1], logit_rows=t[:0], n_logit_rows=0, status=t[:1].clone(), workspace=Workspace(torch.device("cuda")))
+    plain = lambda r: (r.data.float().sum(0) if r.data.dim() == 3 else r.data) if isinstance(r, Rows) else r  # noqa: E731
+    step.y = plain(linear(ctx, step.x, w, out_dtype, partials))  # what the adapters are added to
+    want, off = step.want()
+    got = plain(adapted_linear(ctx, step.x, w, Adapters(step.a, step.b, step.scale), step.plan, out_dtype, partials))
+    # (partials: up to eight slices are added here, each addition off by half a step of the largest)
+    assert bool(((got.double() - want).abs() <= off + 8 * 2.0 ** -24 * (want.abs() + step.y.double().abs() + 8)).all())
