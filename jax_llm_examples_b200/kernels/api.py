@@ -1487,7 +1487,8 @@ def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.T
     gives nothing).  q: bfloat16 [N, Hq, dh], dh 64 or 128; pages: bfloat16, or float8_e4m3fn with ``scales``; out: float32
     [R, Hkv, width], written whole; add: float32 of that shape (out itself, to add to what earlier steps left) or None (zeros).
     ``max_kv_len``, ``max_count``: keys and query tokens of the longest request; a request with more, or with keys beyond ``width``, raises the
-    status and gives nothing.  Keys without a page raise the status and count as zeros.  The order of all sums is fixed."""
+    status and gives nothing.  A call works as if every request brought ``max_count`` tokens: a step's single tokens and its portions are two
+    calls (``cu_q`` with equal neighbours leaves a request out).  Keys without a page raise the status and count as zeros.  The order of all sums is fixed."""
     what = "attention_weights"
     N, Hq, dh = q.shape
     P, two, Hkv, page_size, dh2 = pages.shape
@@ -1587,7 +1588,7 @@ def kv_compact(pages: torch.Tensor, block_table: torch.Tensor, places: torch.Ten
                sums_out: torch.Tensor | None = None) -> None:
     """The kept rows of keys and values move to the front: row i < counts[r] of request r and KV head h comes from place
     places[r, h, i] (:func:`kv_choose`) and goes to place i, in the pages that ``into`` (int32 [R, pages of one]) names; without it in the
-    request's own, where places[r, h, i] >= i is needed (ascending places are).  pages: [P, 2, Hkv, page size, dh] of any type whose
+    request's own, which are no other request's, and where places[r, h, i] >= i is needed (ascending places are).  pages: [P, 2, Hkv, page size, dh] of any type whose
     rows are whole 16 bytes, with ``scales`` in 8 bits; pages of ``into`` are none that the call reads rows from.  ``sums``: float32
     [R, Hkv, width], moved alike into ``sums_out`` [R, Hkv, width of its own] (None: sums itself), whose other entries become 0.
     Rows behind the kept ones stay as they were.  A row whose place or page is missing, or that would move back, is left out and raises
