@@ -170,3 +170,36 @@ def test_beside_a_projection(rows, dtype, out_dtype, partials):
     got = plain(adapted_linear(ctx, step.x, w, Adapters(step.a, step.b, step.scale), step.plan, out_dtype, partials))
     # (partials: up to eight slices are added here, each addition off by half a step of the largest)
     assert bool(((got.double() - want).abs() <= off + 8 * 2.0 ** -24 * (want.abs() + step.y.double().abs() + 8)).all())
+
+
+def test_matrices_beyond_32_bits():
+    """The last of many adapters, whose matrices lie 2^31 entries behind the first one's.  All entries are -1, 0 or 1: every sum is a whole
+    number below 2^24, which 32 bits, and three bfloat16 numbers, hold."""
+    E, r, k, n = 66, 64, 520000, 512
+    a, b = torch.empty((E, r, k), dtype=BF, device="cuda"), torch.zeros((E, n, r), dtype=BF, device="cuda")
+    assert a.numel() > 2 ** 31
+    gen = torch.Generator().manual_seed(1)
+    ones = lambda *s: torch.randint(-1, 2, s, generator=gen)  # noqa: E731
+    a[-1], b[-1] = ones(r, k).to(BF).cuda(), ones(n, r).to(BF).cuda()
+    for of_row in ([65], [65] * 40):
+        x, y = ones(len(of_row), k).to(BF).cuda(), ones(len(of_row), n).float().cuda()
+        out = torch.empty_like(y)
+        K().adapter_add(x, a, b, K().adapter_plan(of_row, E), y, out)
+        low = torch.cat([a[-1, i:i + 8].double() @ x.double().T for i in range(0, r, 8)]).T
+        want = y.double() + low @ b[-1].double().T
+        assert float(want.abs().max()) < 2 ** 24 and torch.equal(out.double(), want)
+
+
+def test_two_calls_at_once():
+    steps = [Step(ROWS["portions"], 4, 16, 520, 264, BF, BF, seed=1), Step(ROWS["few"], 3, 13, 99, 77, BF, F32, seed=2)]  # (one with scratch)
+    want = [s.run() for s in steps]
+    streams, outs = [torch.cuda.Stream() for _ in steps], [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for i, (step, s) in enumerate(zip(steps, streams)):
+            with torch.cuda.stream(s):
+                outs[i].append(step.run())
+    torch.cuda.synchronize()
+    for got, w in zip(outs, want):
+        assert all(torch.equal(g, w) for g in got)

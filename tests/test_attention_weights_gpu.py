@@ -290,3 +290,54 @@ def test_a_few_rows_as_many_rows_gives_them(monkeypatch):
     many = run(c)
     assert_close(few, want, tol)
     assert_close(many, want, tol)
+
+
+# ------------------------------------------------------------------------------------------- far places, calls side by side
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("n", [[1, 1], [40, 3]])
+def test_pages_beyond_32_bits_of_bytes(n, bits8):
+    """The same pages at the far end of a pool of 5 GB (10 GB) and at the near end of a small one."""
+    c = Case(n, [200, 77], 16, 8, 128, 64, bits8=bits8).to_device()
+    want, small = run(c), c.pages
+    P, shift = 40000, 40000 - c.P
+    far = torch.empty((P, *small.shape[1:]), dtype=small.dtype, device="cuda")
+    assert far.numel() * far.element_size() > 2 ** 32
+    far.view(torch.uint8)[shift:] = small.view(torch.uint8)
+    c.pages = far
+    if bits8:
+        scales, c.scales = c.scales, torch.zeros((P, *c.scales.shape[1:]), dtype=torch.uint8, device="cuda")
+        c.scales[shift:] = scales
+    c.table = torch.where(c.table >= 0, c.table + shift, c.table)
+    assert torch.equal(run(c), want)
+    assert int(c.status) == 0
+
+
+def test_two_calls_at_once():
+    """Calls of both kinds on two streams, their scratch apart."""
+    cases = [Case([1] * 6, [900, 3, 77, 2000, 512, 64], 16, 4, 128, 64, bits8=False, seed=1).to_device(), Case([90, 60], [700, 400], 16, 4, 128, 64, bits8=True, seed=2).to_device()]
+    want = [run(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                outs[i].append(run(c))
+    torch.cuda.synchronize()
+    for got, w in zip(outs, want):
+        assert all(torch.equal(g, w) for g in got)
+
+
+def test_a_padded_batch():
+    """Requests behind the last one have no tokens: their rows are what `add` says, and no table entry of theirs is looked at."""
+    c = Case([1, 1, 1, 1], [100, 40, 9, 9], 8, 4, 64, 16, bits8=False)
+    want, tol = received(c, width=120)
+    want[2:], tol[2:] = 0, 0
+    c.table[2:] = 1 << 30
+    c.to_device()
+    for count in (1, 30):  # either kernel
+        c.status.zero_()
+        got = run(c, width=120, cu_q=torch.tensor([0, 1, 2, 2, 2], dtype=torch.int32).cuda(), max_count=count)
+        assert_close(got, want, tol)
+        assert int(c.status) == 0

@@ -310,3 +310,24 @@ def test_the_same_bits_on_another_stream(dtype):
             K().kv_compact(pages, table, places, counts, status, scales=scales, sums=moved)
             got.append((bits(pages), places.cpu(), moved.cpu(), int(status)))
     assert all(torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b == 0 for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_moving_beyond_32_bits_of_bytes(in_place):
+    P, H, page, dh = 33000, 8, 64, 128
+    pages = torch.empty((P, 2, H, page, dh), dtype=torch.bfloat16, device="cuda")
+    assert pages.numel() * 2 > 2 ** 32
+    used = [P - 1, 2, P - 7]
+    for p in used + [P - 3, 5]:
+        pages[p] = torch.randn((2, H, page, dh), device="cuda").to(torch.bfloat16)
+    table = torch.tensor([used], dtype=I32).cuda()
+    into = None if in_place else torch.tensor([[P - 3, 5]], dtype=I32).cuda()
+    gen = torch.Generator().manual_seed(1)
+    places = torch.stack([torch.randperm(3 * page, generator=gen)[:100].sort().values for _ in range(H)])[None].to(I32)
+    rows = pages[used].permute(1, 2, 0, 3, 4).reshape(2, H, 3 * page, dh)
+    want = torch.stack([rows[:, h, places[0, h].long().cuda()] for h in range(H)], 1)
+    status = torch.zeros(1, dtype=I32, device="cuda")
+    K().kv_compact(pages, table, places.cuda(), torch.tensor([100], dtype=I32).cuda(), status, into=into)
+    to = used[:2] if in_place else [P - 3, 5]
+    got = pages[to].permute(1, 2, 0, 3, 4).reshape(2, H, 2 * page, dh)[:, :, :100]
+    assert torch.equal(got, want) and int(status) == 0
