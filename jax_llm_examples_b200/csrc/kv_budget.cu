@@ -283,9 +283,13 @@ __device__ __forceinline__ void compact_sums(const CompactArgs& P, int row) {
   }
 }
 
-// Into other pages: 16 bytes a thread, a row's chunks side by side.  The last grid row moves sums.
-__global__ void __launch_bounds__(THREADS) kv_compact_kernel(const CompactArgs P, int rows_per_block) {
+// Into other pages: a block looks up where its rows come from and go to, then moves 16 bytes of both planes a thread, several rows'
+// loads together.  The last grid column moves sums.
+#define MOVE_ROWS 128  // of a block
+__global__ void __launch_bounds__(THREADS) kv_compact_kernel(const CompactArgs P) {
   JLX_TL(TL_KV_STORE);
+  constexpr int AT_ONCE = 4;
+  __shared__ int2 moves[MOVE_ROWS];
   pdl_launch_dependents_if_small();
   pdl_wait();
   const int row = blockIdx.y, r = row / P.H, h = row - r * P.H;
@@ -293,18 +297,43 @@ __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const CompactArgs P
     if (P.sums) compact_sums(P, row);
     return;
   }
-  const int n = compact_count(P, r), chunks = P.row_bytes / 16;
-  const int i0 = blockIdx.x * rows_per_block, i1 = min(i0 + rows_per_block, n);
-  for (int x = threadIdx.x; x < (i1 - i0) * chunks; x += THREADS) {
-    const int i = i0 + x / chunks, c = x - (i - i0) * chunks;
+  const int i0 = blockIdx.x * MOVE_ROWS, rows = min(compact_count(P, r) - i0, MOVE_ROWS), chunks = P.row_bytes / 16;
+  if (rows <= 0) return;
+  if (threadIdx.x < rows) {
     int src, dst;
-    if (!compact_move(P, r, h, i, false, src, dst)) continue;
+    moves[threadIdx.x] = compact_move(P, r, h, i0 + threadIdx.x, false, src, dst) ? make_int2(src, dst) : make_int2(-1, -1);
+  }
+  __syncthreads();
+  const size_t plane = (size_t)P.H * P.page;  // rows between a key and its value
+  if (P.scales && threadIdx.x < 2 * rows) {
+    const int2 m = moves[threadIdx.x >> 1];
+    const size_t off = (threadIdx.x & 1) * plane;
+    if (m.x >= 0) P.scales[m.y + off] = P.scales[m.x + off];
+  }
+  uint4* pages = reinterpret_cast<uint4*>(P.pages);
+  for (int x0 = threadIdx.x; x0 < rows * chunks; x0 += AT_ONCE * THREADS) {
+    uint4 v[AT_ONCE][2];
+    size_t to[AT_ONCE];
+    bool moved[AT_ONCE];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const size_t s = (size_t)src + w * P.H * P.page, d = (size_t)dst + w * P.H * P.page;
-      reinterpret_cast<uint4*>(P.pages)[d * chunks + c] = reinterpret_cast<const uint4*>(P.pages)[s * chunks + c];
-      if (P.scales && c == 0) P.scales[d] = P.scales[s];
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int x = x0 + u * THREADS, i = x / chunks;
+      moved[u] = false;
+      if (x >= rows * chunks) continue;
+      const int2 m = moves[i];
+      const int c = x - i * chunks;
+      moved[u] = m.x >= 0;
+      to[u] = (size_t)max(m.y, 0) * chunks + c;
+      const size_t from = (size_t)max(m.x, 0) * chunks + c;
+      v[u][0] = pages[from];
+      v[u][1] = pages[from + plane * chunks];
     }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+      if (moved[u]) {
+        pages[to[u]] = v[u][0];
+        pages[to[u] + plane * chunks] = v[u][1];
+      }
   }
 }
 
@@ -395,7 +424,7 @@ JLX_API int jlx_kv_compact(const CompactArgs* args, int in_place, void* stream_)
     JLX_CUDA(jlx_launch_pdl(kv_compact_in_place_kernel, dim3(2 * columns + 3, P.R * P.H), dim3(THREADS), 0, stream, P, columns));
     return 0;
   }
-  const int rows_per_block = 128;
-  JLX_CUDA(jlx_launch_pdl(kv_compact_kernel, dim3((P.most + rows_per_block - 1) / rows_per_block + 1, P.R * P.H), dim3(THREADS), 0, stream, P, rows_per_block));
+  static_assert(2 * MOVE_ROWS <= THREADS, "a thread looks up a row, and moves a scale");
+  JLX_CUDA(jlx_launch_pdl(kv_compact_kernel, dim3((P.most + MOVE_ROWS - 1) / MOVE_ROWS + 1, P.R * P.H), dim3(THREADS), 0, stream, P));
   return 0;
 }
