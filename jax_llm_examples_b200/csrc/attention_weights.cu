@@ -26,6 +26,7 @@ namespace cg = cooperative_groups;
 
 #define THREADS 128
 #define WARPS (THREADS / 32)
+#define EARLY 8  // of a thread's keys, whose places in `add` are asked for before the rows' sums are known
 #define KT 16  // keys of a warp's tile
 
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -285,10 +286,30 @@ __global__ void __launch_bounds__(THREADS, NG == 2 ? 3 : 4) attention_weights_ke
     for (int w = 1; w < WARPS; ++w) v = join(v, part[w][tid]);
     ml[tid] = v;
   }
-  cluster.sync();
+  cluster.barrier_arrive();
+  // while the others come: what no row sees, and what the first of this thread's keys are added to
+  weights_copy(P, row, 0, min(first, P.W.width), everyone, all);
+  weights_copy(P, row, max(end_all, 0), P.W.width, everyone, all);
+  const float* add = P.W.add ? P.W.add + row * P.W.width : nullptr;
+  float* out = P.W.out + row * P.W.width;
+  float early[EARLY];
+#pragma unroll
+  for (int u = 0; u < EARLY; ++u) {
+    const int place = range0 + tid + u * THREADS;
+    early[u] = add && place >= begin && place < end ? add[place] : 0.f;
+  }
+  cluster.barrier_wait();
   if (tid < ROWS) {
-    float2 v = *cluster.map_shared_rank(&ml[tid], 0);
-    for (int q = 1; q < P.splits; ++q) v = join(v, *cluster.map_shared_rank(&ml[tid], q));
+    float2 v = make_float2(ROWS_NEG_BIG, 0.f);
+#pragma unroll
+    for (int q0 = 0; q0 < MAX_SPLITS; q0 += 8) {
+      if (q0 >= P.splits) break;
+      float2 w[8];  // (asked for together: each takes a trip to another multiprocessor)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) w[q] = q0 + q < P.splits ? *cluster.map_shared_rank(&ml[tid], q0 + q) : make_float2(ROWS_NEG_BIG, 0.f);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v = join(v, w[q]);
+    }
     const int qr = min(tid, n_rows - 1), head = hk * G + qr - qr / G * G;
     factor[tid] = make_float2(v.x, rows_inverse(P.R, v.x, v.y, head));
   }
@@ -298,9 +319,22 @@ __global__ void __launch_bounds__(THREADS, NG == 2 ? 3 : 4) attention_weights_ke
   float2 f[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) f[i] = factor[i];
-  const float* add = P.W.add ? P.W.add + row * P.W.width : nullptr;
-  float* out = P.W.out + row * P.W.width;
-  for (int j0 = tid; j0 < tiles * KT; j0 += 4 * THREADS) {
+  auto weigh = [&](int j, float before) {
+    const int place = range0 + j;
+    if (place < begin || place >= end) return;
+    float w = 0.f;
+#pragma unroll
+    for (int i = 0; i < ROWS; i += 2) {
+      if (i >= n_rows) break;
+      const float2 v = *reinterpret_cast<const float2*>(buf + (size_t)j * kept + i);
+      w += rows_exp2(v.x - f[i].x) * f[i].y;
+      if (i + 1 < n_rows) w += rows_exp2(v.y - f[i + 1].x) * f[i + 1].y;
+    }
+    out[place] = before + w;
+  };
+#pragma unroll
+  for (int u = 0; u < EARLY; ++u) weigh(tid + u * THREADS, early[u]);
+  for (int j0 = tid + EARLY * THREADS; j0 < tiles * KT; j0 += 4 * THREADS) {
     float before[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -308,23 +342,8 @@ __global__ void __launch_bounds__(THREADS, NG == 2 ? 3 : 4) attention_weights_ke
       before[u] = add && place >= begin && place < end ? add[place] : 0.f;
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int j = j0 + u * THREADS, place = range0 + j;
-      if (place < begin || place >= end) continue;
-      float w = 0.f;
-#pragma unroll
-      for (int i = 0; i < ROWS; i += 2) {
-        if (i >= n_rows) break;
-        const float2 v = *reinterpret_cast<const float2*>(buf + (size_t)j * kept + i);
-        w += rows_exp2(v.x - f[i].x) * f[i].y;
-        if (i + 1 < n_rows) w += rows_exp2(v.y - f[i + 1].x) * f[i + 1].y;
-      }
-      out[place] = before[u] + w;
-    }
+    for (int u = 0; u < 4; ++u) weigh(j0 + u * THREADS, before[u]);
   }
-  // what no row sees
-  weights_copy(P, row, 0, min(first, P.W.width), everyone, all);
-  weights_copy(P, row, max(end_all, 0), P.W.width, everyone, all);
   cluster.barrier_wait();
 }
 
