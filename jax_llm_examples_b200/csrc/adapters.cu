@@ -22,7 +22,7 @@
 //
 // Everything else (32-bit rows, K or No no multiple of 8, rows off 16-byte boundaries) takes two plain kernels with 32-bit sums.
 //
-// Measured (B200, among others): one row of rank 16, 5120 to 7168, 12.6 us a call, 8.2 on the device, of which the launch is 2 and each
+// Measured (B200, among others): one row of rank 16, 5120 to 7168, 13.1 us a call, 8.2 on the device, of which the launch is 2 and each
 // phase one to two trips to memory; 64 rows of 24 adapters of ranks 16 to 64 21.6 us; 2048 rows of rank 64, 5120 to 5120, 33 us (2 TB/s).
 // A cluster is as large as one round of blocks allows: 2048 rows with four blocks a tile 41 us, with eight 33.
 #include <cooperative_groups.h>
@@ -434,14 +434,14 @@ __global__ void __launch_bounds__(THREADS, WR * NT * 8 > 128 ? 1 : 2) adapters_k
 }
 
 // --------------------------------------------------------------------------- any type and alignment
-#define PLAIN_ROWS 4
+#define PLAIN_ROWS 8
 #define PLAIN_RANKS 4
 
 // low[i, j] = scale x A^T for PLAIN_ROWS rows of a tile and PLAIN_RANKS ranks a block; its threads cut K.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) adapters_low_kernel(const AdapterArgs P) {
   JLX_TL(TL_OTHER);
-  __shared__ float scratch[33];
+  __shared__ float part[WARPS][PLAIN_ROWS * PLAIN_RANKS];
   const int subs = (P.tile_rows + PLAIN_ROWS - 1) / PLAIN_ROWS, tile = blockIdx.y / subs, j0 = blockIdx.x * PLAIN_RANKS;
   AdapterTile t;
   if (!adapter_tile(P, tile, (blockIdx.y - tile * subs) * PLAIN_ROWS, PLAIN_ROWS, t) || t.e < 0) return;
@@ -465,35 +465,49 @@ __global__ void __launch_bounds__(THREADS) adapters_low_kernel(const AdapterArgs
 #pragma unroll
       for (int j = 0; j < PLAIN_RANKS; ++j) acc[i][j] = fmaf(xv[i], av[j], acc[i][j]);
   }
-  const float s = P.scale ? P.scale[t.e] : 1.f;
 #pragma unroll
   for (int i = 0; i < PLAIN_ROWS; ++i)
 #pragma unroll
     for (int j = 0; j < PLAIN_RANKS; ++j) {
-      const float v = block_sum(acc[i][j], scratch);
-      if (threadIdx.x == 0 && i < t.count && j0 + j < P.r) P.low[(size_t)(t.first + i) * P.r + j0 + j] = v * s;
+      const float v = warp_sum(acc[i][j]);
+      if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][i * PLAIN_RANKS + j] = v;
     }
+  __syncthreads();
+  const int i = threadIdx.x / PLAIN_RANKS, j = threadIdx.x % PLAIN_RANKS;
+  if (i < t.count && i < PLAIN_ROWS && j0 + j < P.r) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) v += part[w][threadIdx.x];
+    P.low[(size_t)(t.first + i) * P.r + j0 + j] = v * (P.scale ? P.scale[t.e] : 1.f);
+  }
 }
 
 // out = y + low B^T: a thread per column, PLAIN_ROWS rows.
 template <typename T, typename TY>
 __global__ void __launch_bounds__(THREADS) adapters_out_kernel(const AdapterArgs P) {
   JLX_TL(TL_OTHER);
-  __shared__ float low[PLAIN_ROWS][MAX_RANK];
+  __shared__ __align__(16) float low[MAX_RANK][PLAIN_ROWS];
   const int subs = (P.tile_rows + PLAIN_ROWS - 1) / PLAIN_ROWS, tile = blockIdx.y / subs;
   AdapterTile t;
   if (!adapter_tile(P, tile, (blockIdx.y - tile * subs) * PLAIN_ROWS, PLAIN_ROWS, t)) return;
   if (t.e >= 0)
-    for (int i = threadIdx.x; i < PLAIN_ROWS * t.rank; i += THREADS) low[i / t.rank][i % t.rank] = i / t.rank < t.count ? P.low[(size_t)(t.first + i / t.rank) * P.r + i % t.rank] : 0.f;
+    for (int i = threadIdx.x; i < PLAIN_ROWS * t.rank; i += THREADS) low[i % t.rank][i / t.rank] = i / t.rank < t.count ? P.low[(size_t)(t.first + i / t.rank) * P.r + i % t.rank] : 0.f;
   __syncthreads();
   const int n = blockIdx.x * THREADS + threadIdx.x;
   if (n >= P.No) return;
   float acc[PLAIN_ROWS] = {};
   const T* b = reinterpret_cast<const T*>(P.b) + ((size_t)max(t.e, 0) * P.No + n) * P.r;
+#pragma unroll 4
   for (int j = 0; j < t.rank; ++j) {
     const float w = to_f32<T>(b[j]);
 #pragma unroll
-    for (int i = 0; i < PLAIN_ROWS; ++i) acc[i] = fmaf(low[i][j], w, acc[i]);
+    for (int i = 0; i < PLAIN_ROWS; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(&low[j][i]);
+      acc[i] = fmaf(v.x, w, acc[i]);
+      acc[i + 1] = fmaf(v.y, w, acc[i + 1]);
+      acc[i + 2] = fmaf(v.z, w, acc[i + 2]);
+      acc[i + 3] = fmaf(v.w, w, acc[i + 3]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < PLAIN_ROWS; ++i) {

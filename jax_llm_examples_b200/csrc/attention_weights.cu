@@ -14,8 +14,8 @@
 //
 // It is bound by the keys' bytes, and by the instructions and the latency between a byte and its weight: a warp has 32 registers of
 // keys on their way while it works on as many (without that 64 sessions of up to 8192 keys took 208 us).  Measured (B200, 40 heads on 8 of
-// 128): those sessions 174 us, 4.9 TB/s; 8 of up to 30,000 keys in 8 bits 84 us, 2.5 TB/s; one of 700 keys 12.8 us a call, 7.6 on the
-// device.  Ranges: 64 sessions with 1, 4, 8, 16 of them 194, 198, 176, 237 us.  Tried and slower: two sums a product, to halve its chain
+// 128): those sessions 164 us, 5.2 TB/s; 8 of up to 30,000 keys in 8 bits 79 us, 2.7 TB/s; one of 700 keys 13.4 us a call, 7.5 on the
+// device.  Ranges: 64 sessions with 1, 4, 8, 16 of them 195, 193, 166, 229 us.  Tried and slower: two sums a product, to halve its chain
 // (registers).
 #include <cooperative_groups.h>
 

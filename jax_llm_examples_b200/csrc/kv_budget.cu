@@ -14,8 +14,8 @@
 // which precede all stores; a later row's source lies behind what has been written.
 //
 // Both are bound by bytes, few in the first, so there by the chain of its passes: 100,001 places of one session, 4096 kept, 18.9 us a call;
-// 64 sessions of up to 8192, 2048 kept, 25.4 us (62 with sums in shared memory and a scan of the block for every 512 places; digits of 11
-// bits: 40).  Moving 2048 rows of 8 heads of 128 each of 32 sessions takes 102 us, 5.4 TB/s.
+// 64 sessions of up to 8192, 2048 kept, 25.5 us (62 with sums in shared memory and a scan of the block for every 512 places; digits of 11
+// bits: 40).  Moving 2048 rows of 8 heads of 128 each of 32 sessions takes 94 us, 5.8 TB/s.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
