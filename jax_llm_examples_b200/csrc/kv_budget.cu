@@ -262,6 +262,11 @@ __device__ __forceinline__ bool compact_move(const CompactArgs& P, int r, int h,
   return true;
 }
 __device__ __forceinline__ int compact_count(const CompactArgs& P, int r) { return min(max(P.counts[r], 0), P.most); }
+// A number of rows that `places` does not hold, or that `sums_out` has no room for: cut to it, and the status says so.
+__device__ __forceinline__ void compact_check(const CompactArgs& P, int r) {
+  const int n = P.counts[r];
+  if (n < 0 || n > P.most || (P.sums && n > P.out_width)) atomicOr(P.status, JLX_STATUS_BAD_LENGTH);
+}
 
 // Sums of a request and head: a block, all loads of a stretch before its stores (sums and sums_out may be one).
 __device__ __forceinline__ void compact_sums(const CompactArgs& P, int row) {
@@ -284,7 +289,7 @@ __device__ __forceinline__ void compact_sums(const CompactArgs& P, int row) {
 }
 
 // Into other pages: a block looks up where its rows come from and go to, then moves 16 bytes of both planes a thread, several rows'
-// loads together.  The last grid column moves sums.
+// loads together.  The last grid column looks at the counts and moves sums.
 #define MOVE_ROWS 128  // of a block
 __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const CompactArgs P) {
   JLX_TL(TL_KV_STORE);
@@ -294,6 +299,7 @@ __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const CompactArgs P
   pdl_wait();
   const int row = blockIdx.y, r = row / P.H, h = row - r * P.H;
   if (blockIdx.x == gridDim.x - 1) {
+    if (h == 0 && threadIdx.x == 0) compact_check(P, r);
     if (P.sums) compact_sums(P, row);
     return;
   }
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const CompactArgs P
   }
 }
 
-// In place: a block has a column of 16 or 32 bytes of a plane (grid x: the columns, the scales, the sums).
+// In place: a block has a column of 16 or 32 bytes of a plane (grid x: the columns, the scales, the counts and sums).
 __global__ void __launch_bounds__(THREADS) kv_compact_in_place_kernel(const CompactArgs P, int columns) {
   JLX_TL(TL_KV_STORE);
   constexpr int AT_ONCE = 4;
@@ -345,6 +351,7 @@ __global__ void __launch_bounds__(THREADS) kv_compact_in_place_kernel(const Comp
   pdl_wait();
   const int row = blockIdx.y, r = row / P.H, h = row - r * P.H;
   if (blockIdx.x == 2 * columns + 2) {
+    if (h == 0 && threadIdx.x == 0) compact_check(P, r);
     if (P.sums) compact_sums(P, row);
     return;
   }
@@ -415,7 +422,7 @@ JLX_API int jlx_kv_choose(const ChooseArgs* args, int cluster, void* stream_) {
 JLX_API int jlx_kv_compact(const CompactArgs* args, int in_place, void* stream_) {
   const CompactArgs& P = *args;
   cudaStream_t stream = (cudaStream_t)stream_;
-  JLX_REQUIRE(P.R > 0 && P.H > 0 && P.page > 0 && P.num_pages > 0 && P.row_bytes > 0 && P.row_bytes % 16 == 0 && P.most > 0, "kv_compact: bad sizes");
+  JLX_REQUIRE(P.R > 0 && P.H > 0 && P.page > 0 && P.num_pages > 0 && P.row_bytes > 0 && P.row_bytes % 16 == 0 && P.most >= 0, "kv_compact: bad sizes");
   JLX_REQUIRE(((uintptr_t)P.pages & 15) == 0, "kv_compact: pages must be 16-byte aligned");
   JLX_REQUIRE(((long long)P.num_pages + 1) * 2 * P.H * P.page < (1ll << 31), "kv_compact: cache too large for 32-bit rows");
   JLX_REQUIRE((long long)P.R * P.H <= 65535, "kv_compact: %d requests of %d KV heads are too many for a launch", P.R, P.H);

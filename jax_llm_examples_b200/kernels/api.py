@@ -1592,7 +1592,8 @@ def kv_compact(pages: torch.Tensor, block_table: torch.Tensor, places: torch.Ten
     rows are whole 16 bytes, with ``scales`` in 8 bits; pages of ``into`` are none that the call reads rows from.  ``sums``: float32
     [R, Hkv, width], moved alike into ``sums_out`` [R, Hkv, width of its own] (None: sums itself), whose other entries become 0.
     Rows behind the kept ones stay as they were.  A row whose place or page is missing, or that would move back, is left out and raises
-    the status.  Keys keep the rotation of the position that they were written at; the request's next token lies at place counts[r]."""
+    the status.  A number of rows outside 0 .. the places that ``places`` has room for, or beyond ``sums_out``'s, is cut to it and raises the
+    status.  Keys keep the rotation of the position that they were written at; the request's next token lies at place counts[r]."""
     what = "kv_compact"
     if pages.dim() != 5 or pages.shape[1] != 2 or (scales is None) != (pages.dtype is not FP8):
         raise KernelError(f"{what}: pages must be [pages, 2, KV heads, page size, entries], with scales if and only if they are float8_e4m3fn")
@@ -1616,9 +1617,7 @@ def kv_compact(pages: torch.Tensor, block_table: torch.Tensor, places: torch.Ten
         if not _same_or_apart(sums, sums_out) if sums.shape == sums_out.shape else _overlap(sums, sums_out):
             raise KernelError(f"{what}: sums_out must be sums itself or apart from it")
     dev = _placed(what, pages, block_table, places, counts, status, into, scales, sums, sums_out)
-    if most == 0 and sums_out is not None:
-        sums_out.zero_()
-    if R * H == 0 or P * page_size == 0 or most == 0:
+    if R * H == 0 or P * page_size == 0:
         return
     into_t = block_table if into is None else into
     args = _COMPACT_ARGS.pack(pages.data_ptr(), _address(scales), block_table.data_ptr(), into_t.data_ptr(), places.data_ptr(), counts.data_ptr(), _address(sums),

@@ -331,3 +331,31 @@ def test_moving_beyond_32_bits_of_bytes(in_place):
     to = used[:2] if in_place else [P - 3, 5]
     got = pages[to].permute(1, 2, 0, 3, 4).reshape(2, H, 2 * page, dh)[:, :, :100]
     assert torch.equal(got, want) and int(status) == 0
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("counts, most, out_width, moved, summed", [
+    ([5, 2], 3, 8, [3, 2], [3, 2]),  # more rows than `places` has
+    ([-1, 1], 3, 8, [0, 1], [0, 1]),
+    ([3, 1], 3, 2, [3, 1], [2, 1]),  # more sums than `sums_out` has
+    ([1, 0], 0, 8, [0, 0], [0, 0]),  # no places at all
+])
+def test_counts_that_their_arrays_do_not_hold_raise_the_status(in_place, counts, most, out_width, moved, summed):
+    pages, _ = pool(6, 2, 16, 64, torch.bfloat16)
+    before = bits(pages)
+    table = torch.tensor([[0], [1]], dtype=I32)
+    into = table if in_place else torch.tensor([[4], [5]], dtype=I32)
+    places = torch.tensor([[2, 5, 7], [3, 4, 15]], dtype=I32).expand(2, 2, 3)[:, :, :most].contiguous()  # of each head
+    sums = torch.rand((2, 2, 16), generator=torch.Generator().manual_seed(1)).cuda()
+    out = torch.full((2, 2, out_width), math.nan, device="cuda")
+    status = torch.zeros(1, dtype=I32, device="cuda")
+    K().kv_compact(pages, table.cuda(), places.cuda(), torch.tensor(counts, dtype=I32).cuda(), status, into=None if in_place else into.cuda(), sums=sums, sums_out=out)
+    assert int(status) == 16
+    want, want_sums = before.clone(), torch.zeros((2, 2, out_width))
+    for r in range(2):
+        for h in range(2):
+            for i in range(moved[r]):
+                want[into[r, 0], :, h, i] = before[table[r, 0], :, h, places[r, h, i]]
+            for i in range(summed[r]):
+                want_sums[r, h, i] = sums[r, h, places[r, h, i]].cpu()
+    assert torch.equal(bits(pages), want) and torch.equal(out.cpu(), want_sums)
