@@ -1606,8 +1606,8 @@ def kv_compact(pages: torch.Tensor, block_table: torch.Tensor, places: torch.Ten
     _ints(what, ("block_table", block_table, 0), ("into", into, 0), ("places", places, 0), ("counts", counts, R), ("status", status, 1))
     if any(t is not None and (t.dim() != 2 or t.shape[0] != R) for t in (block_table, into)):
         raise KernelError(f"{what}: block tables must be int32 [{R}, pages of one]")
-    if dh * pages.element_size() % 16 or pages.data_ptr() % 16:
-        raise KernelError(f"{what}: rows of {dh} entries of {pages.dtype} are not whole 16 bytes on 16-byte boundaries")
+    if (R * H and not P * dh * page_size) or dh * pages.element_size() % 16 or pages.data_ptr() % 16:
+        raise KernelError(f"{what}: {P} pages of {page_size} rows of {dh} entries of {pages.dtype} are not rows of whole 16 bytes on 16-byte boundaries")
     if sums is None and sums_out is not None:
         raise KernelError(f"{what}: sums_out without sums")
     sums_out = sums if sums_out is None else sums_out
@@ -1617,7 +1617,7 @@ def kv_compact(pages: torch.Tensor, block_table: torch.Tensor, places: torch.Ten
         if not _same_or_apart(sums, sums_out) if sums.shape == sums_out.shape else _overlap(sums, sums_out):
             raise KernelError(f"{what}: sums_out must be sums itself or apart from it")
     dev = _placed(what, pages, block_table, places, counts, status, into, scales, sums, sums_out)
-    if R * H == 0 or P * page_size == 0:
+    if R * H == 0:
         return
     into_t = block_table if into is None else into
     args = _COMPACT_ARGS.pack(pages.data_ptr(), _address(scales), block_table.data_ptr(), into_t.data_ptr(), places.data_ptr(), counts.data_ptr(), _address(sums),

@@ -120,3 +120,9 @@ def test_sums_move_within_themselves_or_apart(no_launch):
         K.kv_compact(**_compact(sums=one[:54].view(2, 3, 9), sums_out=one[6:60].view(2, 3, 9)))
     with pytest.raises(K.KernelError, match="apart"):
         K.kv_compact(**_compact(sums=one[:54].view(2, 3, 9), sums_out=one[:48].view(2, 3, 8)))
+
+
+@pytest.mark.parametrize("count, page, dh", [(0, 16, 64), (4, 0, 64), (4, 16, 0)])
+def test_moving_refuses_pages_without_rows(no_launch, count, page, dh):
+    with pytest.raises(K.KernelError, match="16 bytes"):
+        K.kv_compact(**_compact(pages=torch.zeros(count, 2, 3, page, dh)))
