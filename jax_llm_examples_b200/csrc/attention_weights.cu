@@ -58,8 +58,9 @@ __global__ void __launch_bounds__(THREADS, NG == 2 ? 3 : 4) attention_weights_ke
   if (!weights_request(P, r, it)) { weights_copy(P, row, 0, P.W.width, everyone, all); return; }
   const int G = P.R.Hq / P.R.Hkv, n_rows = min(it.cnt * G, ROWS);
   const RowsToken tok = rows_token(P.R, it, min(lane, n_rows - 1), hk);
-  const int first = __reduce_min_sync(0xffffffffu, tok.lo), p_max = __reduce_max_sync(0xffffffffu, tok.p);
-  const int end_all = rows_end(P.R, it, p_max), start = first / KT * KT;
+  const int p_max = __reduce_max_sync(0xffffffffu, tok.p), end_all = rows_end(P.R, it, p_max);
+  // (a row that sees nothing has no first key: under a window its 0 would stretch the range over keys that no row sees)
+  const int first = __reduce_min_sync(0xffffffffu, tok.p < 0 ? max(end_all, 0) : tok.lo), start = first / KT * KT;
   // equal ranges of whole tiles
   const int per = max((end_all - start + KT * P.splits - 1) / (KT * P.splits), 0) * KT, range0 = start + split * per;
   const int begin = max(first, range0), end = min(end_all, range0 + per), tiles = end > begin ? (end - range0 + KT - 1) / KT : 0;

@@ -341,3 +341,20 @@ def test_a_padded_batch():
         got = run(c, width=120, cu_q=torch.tensor([0, 1, 2, 2, 2], dtype=torch.int32).cuda(), max_count=count)
         assert_close(got, want, tol)
         assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("few", [True, False])
+@pytest.mark.parametrize("empty", [[0], [1], [0, 1, 2]])
+@pytest.mark.parametrize("mask", [dict(window=64), dict(chunk=64), dict()])
+def test_a_row_that_sees_nothing_beside_rows_that_do(mask, empty, few, bits8, monkeypatch):
+    """Such a row's first key (0) is no key of the request's range, which a window or a chunk keeps short."""
+    c = Case([3, 2], [1400, 700], 8, 2, 64, 16, bits8=bits8)
+    for i in empty:
+        c.positions[i] = -1 - 3 * i
+    want, tol = received(c, **mask)
+    c.to_device()
+    if not few:
+        monkeypatch.setattr(K(), "WEIGHTS_FEW", 0)
+    assert_close(run(c, **mask), want, tol)
+    assert int(c.status) == 0
