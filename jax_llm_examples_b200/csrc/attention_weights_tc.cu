@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) attention_weights_rows_kernel(con
   if (warp >= FIRST_SUM_WARP && warp < FIRST_SUM_WARP + 4) {
     const int row = (warp - FIRST_SUM_WARP) * 32 + lane, p = P.R.positions[it.n0 + (row0 + min(row, n_rows - 1)) / G], lo = rows_first_key(P.R, p);
     const int a = __reduce_min_sync(0xffffffffu, p), b = __reduce_max_sync(0xffffffffu, p);
-    const int c = __reduce_min_sync(0xffffffffu, lo), d = __reduce_max_sync(0xffffffffu, lo);
+    const int c = __reduce_min_sync(0xffffffffu, p < 0 ? 0x7fffffff : lo), d = __reduce_max_sync(0xffffffffu, lo);  // (a row that sees nothing has no first key)
     if (lane == 0) {
       atomicMin(&sh.span[0], a);
       atomicMax(&sh.span[1], b);

@@ -358,3 +358,20 @@ def test_a_row_that_sees_nothing_beside_rows_that_do(mask, empty, few, bits8, mo
         monkeypatch.setattr(K(), "WEIGHTS_FEW", 0)
     assert_close(run(c, **mask), want, tol)
     assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("few", [True, False])
+@pytest.mark.parametrize("empty", [[0], [2], [0, 1, 2]])
+def test_a_row_that_sees_nothing_asks_for_no_page(empty, few, monkeypatch):
+    """Pages that a window has left behind are no business of a row that sees no key at all."""
+    c = Case([3, 2], [500, 300], 8, 4, 64, 16, bits8=False)
+    for i in empty:
+        c.positions[i] = -1
+    want, tol = received(c, window=64)
+    for r in range(2):
+        c.table[r, :(c.held[r] - 64) // 16] = -1
+    c.to_device()
+    if not few:
+        monkeypatch.setattr(K(), "WEIGHTS_FEW", 0)
+    assert_close(run(c, window=64), want, tol)
+    assert int(c.status) == 0
