@@ -79,6 +79,20 @@ __device__ __forceinline__ uint4 first_of(uint4 v, int n) {
 // entries between rows of the shared arrays: rows fall on different banks
 __host__ __device__ constexpr int low_stride(int rank_cols) { return rank_cols + 8; }
 
+// A row of rank r (its parts `apart` entries from each other) times a row of B, in 32 bits.
+template <int PARTS>
+__device__ __forceinline__ float whole_entry(const bf16* l, int apart, const bf16* b, int rank) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int k = 0; k < rank; ++k) {
+    float v = 0.f;
+#pragma unroll
+    for (int p = PARTS - 1; p >= 0; --p) v += __bfloat162float(l[p * apart + k]);
+    sum = fmaf(v, __bfloat162float(b[k]), sum);
+  }
+  return sum;
+}
+
 template <typename TY> struct Eight;
 template <> struct Eight<bf16> {
   uint4 v;
@@ -421,6 +435,25 @@ __global__ void __launch_bounds__(THREADS, WR * NT * 8 > 128 ? 1 : 2) adapters_k
             mma_bf16(d[j], f0, now.b[s][j].x, now.b[s][j].y);
             mma_bf16(d[j], f1, now.b[s][j].z, now.b[s][j].w);
           }
+        }
+      }
+      // Against an infinite entry of B the small part of a number, 0 or of the other sign, makes NaN of an infinity, and so does an
+      // infinite row against the zeros that fill up an adapter's ranks: sums that are not finite are made again of whole numbers, over the
+      // adapter's own ranks.
+      float4 total = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        total.x += d[j][0]; total.y += d[j][1]; total.z += d[j][2]; total.w += d[j][3];
+      }
+      if (!isfinite((total.x + total.y) + (total.z + total.w)) && mine) {
+#pragma unroll 1
+        for (int x = 0; x < 16; ++x) {  // (x = 4 j + i of d[j][i])
+          const float whole = whole_entry<PARTS>(low + (m * 16 + (x >> 1 & 1) * 8 + g) * LD, ROWS * LD, b + ((size_t)t.e * P.No + col + (x >> 2) * 2 + (x & 1)) * P.r, t.rank);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (x == 4 * j + i && !isfinite(d[j][i])) d[j][i] = whole;
         }
       }
 #pragma unroll

@@ -203,3 +203,44 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for got, w in zip(outs, want):
         assert all(torch.equal(g, w) for g in got)
+
+
+@pytest.mark.parametrize("rows", ["few", "tile and one", "portions"])
+@pytest.mark.parametrize("r, k, n, dtype, out_dtype", [(16, 256, 320, BF, BF), (64, 1000, 264, BF, F32), (13, 264, 136, BF, BF), (200, 136, 96, BF, F32), (8, 100, 77, BF, BF),
+                                                       (40, 264, 136, BF, BF), (16, 64, 64, F32, F32)])
+def test_infinite_entries_of_b_give_infinities(rows, r, k, n, dtype, out_dtype):
+    """An entry of a column: the result is infinite, whatever the rows between the products pass as; two of opposite effect: NaN."""
+    step = Step(ROWS[rows], 6, r, k, n, dtype, out_dtype, seed=r)
+    step.x.abs_()
+    step.a.abs_()  # (so no number between the products is near 0)
+    for col, rank, value in ((0, 0, "inf"), (3, r - 1, "-inf"), (n - 1, r // 2, "inf"), (17, 1, "inf"), (17, 2, "-inf"), (20, 4, "nan")):
+        step.b[:, col, rank] = float(value)
+    want, off = step.want()
+    got, sure = step.run(), want.isfinite()
+    assert bool(want[:, 0].isinf().any()) and bool(want[:, 17].isnan().any())
+    assert torch.allclose(got[~sure].double(), want[~sure], rtol=0, atol=0, equal_nan=True)
+    assert bool(((got.double() - want).abs() <= off)[sure].all())
+
+
+@pytest.mark.parametrize("rows", ["few", "tile and one", "portions"])
+@pytest.mark.parametrize("r, k, n, dtype, out_dtype, mixed", [(16, 256, 320, BF, BF, True), (64, 1000, 264, BF, F32, True), (13, 264, 136, BF, BF, False), (200, 136, 96, BF, F32, False),
+                                                              (8, 100, 77, BF, BF, True), (24, 264, 136, BF, BF, True), (24, 264, 136, BF, BF, False), (7, 64, 64, F32, F32, True)])
+def test_infinite_rows_meet_no_rank_that_is_not_there(rows, r, k, n, dtype, out_dtype, mixed):
+    """Ranks behind an adapter's own are not zeros that an infinity is multiplied with: infinite results stay infinite, and an adapter of
+    rank 0 changes nothing."""
+    step = Step(ROWS[rows], 6, r, k, n, dtype, out_dtype, mixed=mixed, seed=r)
+    if mixed:
+        step.ranks[::3] = 0
+        step.ranks[1::3] = 1
+        step.ranks[2::3] = r - 3
+    step.a.abs_()
+    step.b.abs_()
+    step.x[::2, 3] = float("inf")
+    want, off = step.want()
+    got, sure = step.run(), want.isfinite()
+    assert bool(want.isposinf().any()) and not bool(want.isnan().any())
+    assert torch.equal(got[~sure].double(), want[~sure])
+    assert bool(((got.double() - want).abs() <= off)[sure].all())
+    if mixed:
+        none = (step.ranks[torch.tensor(step.of_row).clamp(min=0)] == 0).cuda()
+        assert torch.equal(got[none], step.y[none])
