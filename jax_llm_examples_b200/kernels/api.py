@@ -1447,6 +1447,15 @@ def _same_or_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     return d == 0 or abs(d) >= a.numel() * a.element_size()
 
 
+def _apart(what: str, written: "tuple[tuple[torch.Tensor, int], ...]", read: "tuple[tuple[torch.Tensor, int], ...]") -> None:
+    """(Contiguous tensor, entries of it that a call uses): those that it writes share no bytes with each other, nor with those that it reads."""
+    spans = [(p := t.data_ptr(), p + n * t.element_size()) for t, n in written + read]
+    for i, (begin, end) in enumerate(spans[:len(written)]):
+        for other, other_end in spans[i + 1:]:
+            if (begin if begin > other else other) < (end if end < other_end else other_end):
+                raise KernelError(f"{what}: a tensor that is written and another one share memory")
+
+
 # ------------------------------------------------- a cache kept to a budget: weights, choice, moving the kept rows
 _WEIGHTS_ARGS = struct.Struct("@4P2i")  # WeightsArgs in csrc/attention_weights.cuh
 WEIGHTS_FEW = 16  # query rows of a request and KV head that attention_weights.cu takes
@@ -1559,7 +1568,8 @@ def kv_choose(sums: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor, pla
     places that a request has; keep: int32 [R], how many of them are kept; places: int32 [R, Hkv, most]; counts: int32 [R].
     Of a request's length L, counts[r] = min(keep[r], L) places are kept: the last ``recent``, then the first ``first`` as far as that
     goes, then those with the largest sums (ties: the lowest place; NaN counts as the lowest sum).  They stand in ascending order
-    in places[r, h], followed by -1.  A length outside 0 .. width, or a number to keep that ``places`` has no room for, is cut to it and
+    in places[r, h], followed by -1.  ``places`` and ``counts`` share no memory with each other, nor with what is read (lengths are renewed
+    from ``counts`` after the call).  A length outside 0 .. width, or a number to keep that ``places`` has no room for, is cut to it and
     raises the status."""
     what = "kv_choose"
     if sums.dtype is not torch.float32 or sums.dim() != 3:
@@ -1571,6 +1581,7 @@ def kv_choose(sums: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor, pla
     if first < 0 or recent < 0:
         raise KernelError(f"{what}: the first {first} and the last {recent} places cannot be kept")
     dev = _placed(what, sums, lengths, keep, places, counts, status)
+    _apart(what, ((places, places.numel()), (counts, R)), ((sums, sums.numel()), (lengths, R), (keep, R)))
     if R * H == 0:
         return
     if width == 0:

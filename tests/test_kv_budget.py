@@ -126,3 +126,24 @@ def test_sums_move_within_themselves_or_apart(no_launch):
 def test_moving_refuses_pages_without_rows(no_launch, count, page, dh):
     with pytest.raises(K.KernelError, match="16 bytes"):
         K.kv_compact(**_compact(pages=torch.zeros(count, 2, 3, page, dh)))
+
+
+def test_a_choice_writes_over_nothing_that_it_reads(no_launch, monkeypatch):
+    """Heads of a request read its length and number while another one may have written its count already."""
+    monkeypatch.setattr(K, "_placed", lambda *a: -1)  # as if the tensors were on the device
+    a = _choose()
+    many = torch.zeros(60, dtype=I32)
+    for change in (dict(counts=a["lengths"], lengths=a["lengths"]), dict(counts=a["keep"], keep=a["keep"]), dict(lengths=many[:2], counts=many[1:3]),
+                   dict(places=many[:24].view(2, 3, 4), counts=many[22:24]), dict(places=many[:24].view(2, 3, 4), lengths=many[10:12]),
+                   dict(places=many[:24].view(2, 3, 4), keep=many[23:25]), dict(sums=many.view(torch.float32).view(2, 3, 10), places=many[:24].view(2, 3, 4)),
+                   dict(sums=many.view(torch.float32).view(2, 3, 10), counts=many[58:])):
+        with pytest.raises(K.KernelError, match="share memory"):
+            K.kv_choose(**_choose(**change))
+    # entries behind a request's are not used; places of no size lie nowhere
+    ran = []
+    monkeypatch.setattr(K, "_run", lambda *args: ran.append(args))
+    monkeypatch.setattr(K, "_raw_stream", lambda dev: None)
+    monkeypatch.setattr(K, "sm_count", lambda: 148)
+    K.kv_choose(**_choose(lengths=many, keep=many[2:], counts=many[4:]))
+    K.kv_choose(**_choose(lengths=many, keep=many[2:], counts=many[4:], places=many[:0].view(2, 3, 0)))
+    assert len(ran) == 2
