@@ -1462,6 +1462,9 @@ WEIGHTS_FEW = 16  # query rows of a request and KV head that attention_weights.c
 WEIGHTS_KEYS = 16  # keys of a tile there
 WEIGHTS_TILE = 128  # keys, or query rows, of a tile in attention_weights_tc.cu
 WEIGHTS_HELD = 100 << 10  # bytes of scores that a block keeps in shared memory
+# Bytes of scores in scratch, unless one request has more: the requests of a call take turns in it.  (64 requests of which one has 131,072 keys,
+# one token and three of each: 220 and 321 us with 1.6 and 4.3 GB, 276 and 439 with 512 MB, 306 and 569 with 256.)
+WEIGHTS_SCRATCH = 512 << 20
 
 
 @functools.lru_cache(maxsize=4096)  # (a pure rule on sizes)
@@ -1541,14 +1544,23 @@ def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.T
         scratch = torch.empty(_up4(2 * N * Hq) + 4 * R * q_tiles, dtype=torch.float32, device=q.device)
     else:
         splits, most, fits = attention_weights_plan(keys, R * Hkv, rows, sm_count())
-        scratch = None if fits else torch.empty(R * Hkv * splits * most * -(-rows // 2) * 2, dtype=torch.float32, device=q.device)
+        one = 0 if fits else Hkv * splits * most * -(-rows // 2) * 2  # scores of a request
+        at_once = R if fits else max(1, min(R, WEIGHTS_SCRATCH // (4 * one)))
+        scratch = None if fits else torch.empty(at_once * one, dtype=torch.float32, device=q.device)
+        # (the launches of a call share it: one follows the other)
+        for r in range(0, R, at_once):
+            n = min(at_once, R - r)
+            args = _ROWS_ARGS.pack(q.data_ptr(), pages.data_ptr(), _address(scales), block_table.data_ptr() + 4 * r * width, 0, positions.data_ptr(), 0, 0, 0, 0, 0, 0,
+                                   _address(sink), _address(slopes), 0, 0, status.data_ptr(), width, n, n, max_count, 0, N, Hq, Hkv, dh, page_size, P, chunk, window, 1,
+                                   0, 0, scale, softcap, attn_scale, floor_scale)
+            at = 4 * r * Hkv * out.shape[2]
+            more = _WEIGHTS_ARGS.pack(cu_q.data_ptr() + 4 * r, _address(add) + at if add is not None else 0, out.data_ptr() + at, _address(scratch), out.shape[2], max_kv_len)
+            _run("attention_weights", "jlx_attention_weights", args, more, rows, splits, most, _raw_stream(dev))
+        return
     args = _ROWS_ARGS.pack(q.data_ptr(), pages.data_ptr(), _address(scales), block_table.data_ptr(), 0, positions.data_ptr(), 0, 0, 0, 0, 0, 0, _address(sink),
                            _address(slopes), 0, 0, status.data_ptr(), width, R, R, max_count, 0, N, Hq, Hkv, dh, page_size, P, chunk, window, 1, 0, 0,
                            scale, softcap, attn_scale, floor_scale)
     more = _WEIGHTS_ARGS.pack(cu_q.data_ptr(), _address(add), out.data_ptr(), _address(scratch), out.shape[2], max_kv_len)
-    if rows <= WEIGHTS_FEW:
-        _run("attention_weights", "jlx_attention_weights", args, more, rows, splits, most, _raw_stream(dev))
-        return
     places, k_tiles, passes = 2 * sm_count(), -(-out.shape[2] // WEIGHTS_TILE), -(-rows // WEIGHTS_TILE)
     keys_shares = _weights_shares(R * Hkv * -(-max_kv_len // WEIGHTS_TILE), passes, places)
     key_tiles = max(1, min(8, R * Hkv * k_tiles // (4 * places))) if keys_shares == 1 and passes <= 32 else 1

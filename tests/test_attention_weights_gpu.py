@@ -375,3 +375,36 @@ def test_a_row_that_sees_nothing_asks_for_no_page(empty, few, monkeypatch):
         monkeypatch.setattr(K(), "WEIGHTS_FEW", 0)
     assert_close(run(c, window=64), want, tol)
     assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+def test_requests_in_several_launches_where_their_scratch_would_be_large(monkeypatch, bits8):
+    """The same bits as from one launch, for every number of requests at a time."""
+    c = Case([1, 2, 0, 1, 1], [900, 333, 0, 17, 640], 8, 2, 64, 64, bits8=bits8).to_device()
+    plan = K().attention_weights_plan
+    monkeypatch.setattr(K(), "attention_weights_plan", lambda *a: (*plan(*a)[:2], False))
+    add = torch.rand((5, 2, 901), generator=torch.Generator().manual_seed(1)).cuda()
+    want = run(c, width=901, add=add)
+    assert_close(want, *received(c, width=901, add=add))
+    splits, most, _ = plan(901, 10, 8, 148)
+    one = 2 * splits * most * 8 * 4  # bytes of a request's scores
+    for at_once, launches in ((1, 5), (2, 3), (3, 2), (5, 1), (0, 5)):
+        monkeypatch.setattr(K(), "WEIGHTS_SCRATCH", at_once * one)
+        before = K().launch_count()
+        assert torch.equal(run(c, width=901, add=add), want)
+        assert K().launch_count() == before + launches
+    assert int(c.status) == 0
+
+
+def test_scratch_is_bounded():
+    """64 requests of a call that is sized for 131,072 keys: all of their scores would take 1.6 GB."""
+    assert K().WEIGHTS_SCRATCH <= 512 << 20
+    c = Case([1] * 64, [20 + i for i in range(64)], 40, 8, 128, 16, bits8=False).to_device()
+    want, tol = received(c)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    got = run(c, max_kv=131072)
+    assert torch.cuda.max_memory_allocated() - held <= K().WEIGHTS_SCRATCH + 2 * got.numel() * 4
+    assert_close(got, want, tol)
+    assert int(c.status) == 0
