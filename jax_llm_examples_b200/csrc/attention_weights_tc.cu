@@ -700,6 +700,17 @@ __global__ void __launch_bounds__(NTHREADS, 2) attention_weights_keys_kernel(con
   cluster.sync();
 }
 
+// out = add at the places from `from` on, which no request's keys reach.  (Within the launch above every 128 of them took a block of their
+// own with nothing to do: 128 rows over 4096 keys into 131,072 places 99 us for 23.)
+#define COPY_PLACES 4096
+__global__ void __launch_bounds__(256) attention_weights_behind_kernel(const WeightsParams P, int from) {
+  JLX_TL(TL_ATTN_PREFILL);
+  pdl_launch_dependents_if_small();
+  pdl_wait();
+  const int first = from + blockIdx.y * COPY_PLACES;
+  weights_copy(P, blockIdx.x, first, min(first + COPY_PLACES, P.W.width), threadIdx.x, 256);
+}
+
 // -------------------------------------------------------------------------------------------- host
 template <typename Kernel>
 static int launch_tc(Kernel kernel, int smem, dim3 grid, int splits, const TcParams& T, cudaStream_t stream) {
@@ -723,12 +734,16 @@ static int launch_tc(Kernel kernel, int smem, dim3 grid, int splits, const TcPar
 
 template <int DH, bool F8>
 static int launch_both(TcParams& T, int rows_splits, int keys_splits, cudaStream_t stream) {
-  const int blocks = T.key_tiles * TILE;
+  // tiles of the keys that requests may have; what lies behind them is copied, unless it is there
+  const int block = T.key_tiles * TILE, keys = T.P.W.max_kv < T.P.W.width ? T.P.W.max_kv : T.P.W.width, key_blocks = (keys + block - 1) / block;
+  const int behind = T.P.W.add == T.P.W.out ? 0 : T.P.W.width - key_blocks * block;
   const unsigned pairs = (unsigned)(T.P.R.n_requests * T.P.R.Hkv);
   T.P.splits = rows_splits;
   if (int e = launch_tc(attention_weights_rows_kernel<DH, F8>, TcTile<DH>::SMEM, dim3(pairs * (unsigned)rows_splits, (unsigned)T.q_tiles), rows_splits, T, stream)) return e;
   T.P.splits = keys_splits;
-  return launch_tc(attention_weights_keys_kernel<DH, F8>, TcTile<DH>::SMEM, dim3(pairs * (unsigned)keys_splits, (unsigned)((T.P.W.width + blocks - 1) / blocks)), keys_splits, T, stream);
+  if (int e = launch_tc(attention_weights_keys_kernel<DH, F8>, TcTile<DH>::SMEM, dim3(pairs * (unsigned)keys_splits, (unsigned)key_blocks), keys_splits, T, stream)) return e;
+  if (behind > 0) JLX_CUDA(jlx_launch_pdl(attention_weights_behind_kernel, dim3(pairs, (unsigned)((behind + COPY_PLACES - 1) / COPY_PLACES)), dim3(256), 0, stream, T.P, key_blocks * block));
+  return 0;
 }
 
 // Scratch: float2 [N * Hq], then (on 16 bytes) int4 [R * ceil(max_count * G / 128)].

@@ -1561,13 +1561,15 @@ def attention_weights(q: torch.Tensor, pages: torch.Tensor, block_table: torch.T
                            _address(slopes), 0, 0, status.data_ptr(), width, R, R, max_count, 0, N, Hq, Hkv, dh, page_size, P, chunk, window, 1, 0, 0,
                            scale, softcap, attn_scale, floor_scale)
     more = _WEIGHTS_ARGS.pack(cu_q.data_ptr(), _address(add), out.data_ptr(), _address(scratch), out.shape[2], max_kv_len)
-    places, k_tiles, passes = 2 * sm_count(), -(-out.shape[2] // WEIGHTS_TILE), -(-rows // WEIGHTS_TILE)
+    # (tiles of keys that requests have: what lies behind them, where `out` is wider, is copied by a third launch unless it is there)
+    places, k_tiles, passes = 2 * sm_count(), -(-min(max_kv_len, out.shape[2]) // WEIGHTS_TILE), -(-rows // WEIGHTS_TILE)
     keys_shares = _weights_shares(R * Hkv * -(-max_kv_len // WEIGHTS_TILE), passes, places)
     key_tiles = max(1, min(8, R * Hkv * k_tiles // (4 * places))) if keys_shares == 1 and passes <= 32 else 1
     _run("attention_weights_tc", "jlx_attention_weights_tc", args, more, _weights_shares(R * Hkv * q_tiles, -(-keys // WEIGHTS_TILE), places), keys_shares,
          key_tiles, _raw_stream(dev))
     global _launches
-    _launches += 1  # two kernels
+    behind = out.shape[2] > -(-k_tiles // key_tiles) * key_tiles * WEIGHTS_TILE and (add is None or add.data_ptr() != out.data_ptr())
+    _launches += 1 + behind  # two kernels, or three
 
 
 _CHOOSE_ARGS = struct.Struct("@6P6i")  # ChooseArgs in csrc/kv_budget.cu

@@ -408,3 +408,28 @@ def test_scratch_is_bounded():
     assert torch.cuda.max_memory_allocated() - held <= K().WEIGHTS_SCRATCH + 2 * got.numel() * 4
     assert_close(got, want, tol)
     assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("sms", [1, 148])
+@pytest.mark.parametrize("n", [[1, 1], [40, 3]])
+def test_sums_with_room_for_more_keys_than_requests_have(n, sms, monkeypatch):
+    """Every place is written once, behind the call's longest request, too: from `add`, from itself or with zeros."""
+    c = Case(n, [300, 500], 8, 4, 64, 16, bits8=False).to_device()
+    monkeypatch.setattr(K(), "sm_count", lambda: sms)
+    for width in (501, 1024, 5000, 4096 * 3 + 1):
+        want, tol = received(c, width=max(width, 540))
+        want, tol = want[..., :width], tol[..., :width]
+        add = torch.rand((2, 4, width), generator=torch.Generator().manual_seed(width)).cuda()
+        if width > 540:
+            assert_close(run(c, width=width), want, tol)
+            assert_close(run(c, width=width, add=add), want + add.cpu().double(), tol + 2.0 ** -24 * (want + 1))
+            there, before = add.clone(), K().launch_count()
+            run(c, width=width, add=there, out=there)
+            assert K().launch_count() == before + (1 if n[0] == 1 else 2)  # (and nothing to copy)
+            assert_close(there, want + add.cpu().double(), tol + 2.0 ** -24 * (want + 1))
+            assert torch.equal(there[..., 540:], add[..., 540:])
+            assert int(c.status) == 0
+        else:
+            got = run(c, width=width, add=add, max_kv=600)  # (a request that has more gives nothing, and the status says so)
+            c.status.zero_()
+            assert_close(got[0], (want + add.cpu().double())[0], (tol + 2.0 ** -24 * (want + 1))[0])

@@ -147,3 +147,18 @@ def test_a_choice_writes_over_nothing_that_it_reads(no_launch, monkeypatch):
     K.kv_choose(**_choose(lengths=many, keep=many[2:], counts=many[4:]))
     K.kv_choose(**_choose(lengths=many, keep=many[2:], counts=many[4:], places=many[:0].view(2, 3, 0)))
     assert len(ran) == 2
+
+
+def test_the_width_of_the_sums_does_not_change_the_blocks_of_a_call(no_launch, monkeypatch):
+    """Tiles of keys that a block has one after the other go by the keys that requests have, not by the places that `out` has room for."""
+    ran = []
+    monkeypatch.setattr(K, "_placed", lambda *a: 0)  # as if the tensors were on the device, and a launch a note of its arguments
+    monkeypatch.setattr(K, "_raw_stream", lambda dev: None)
+    monkeypatch.setattr(K, "sm_count", lambda: 148)
+    monkeypatch.setattr(K, "_run", lambda lib, fn, args, more, *rest: ran.append(rest))
+    for width in (4096, 8192, 600000):
+        K.attention_weights(**_weights(out=torch.zeros(1, 2, width), max_kv_len=4096, max_count=64))
+    assert ran[0] == ran[1] == ran[2] and ran[0][2] == 1
+    # several where the keys themselves make more blocks than the device holds many times over
+    K.attention_weights(**_weights(out=torch.zeros(1, 2, 200000), max_kv_len=200000, max_count=64))
+    assert ran[3][2] > 1
