@@ -74,3 +74,13 @@ def test_out_may_be_y_but_no_part_of_an_operand(no_launch, monkeypatch):
     assert not K._overlap(wide[:, :16], wide[:, 16:48]) and K._overlap(wide[:, :17], wide[:, 16:48])
     assert not K._overlap(wide[:2], wide[2:]) and K._overlap(wide[:3], wide[2:])
     assert not K._overlap(wide[:, 48:], wide[:, :48]) and K._overlap(wide[1:, 40:], wide[:, 41:])
+
+
+def test_rows_without_an_adapter_do_not_make_the_tiles_larger():
+    """A tile's size goes by the adapters' rows: decoding sessions keep tiles of 16 though many of them have none."""
+    assert K.adapter_plan([-1] * 17 + list(range(24)), 24, device="cpu").tile_rows == 16
+    assert K.adapter_plan([-1] * K.ADAPTER_BARE + [0], 24, device="cpu").tile_rows == 16
+    assert K.adapter_plan([-1] * (K.ADAPTER_BARE + 1) + [0], 24, device="cpu").tile_rows == 64  # (a portion's)
+    assert K.adapter_plan([-1] * 17 + [3] * 17, 24, device="cpu").tile_rows == 64
+    plan = K.adapter_plan([-1] * 40 + [0, 1, 1], 2, device="cpu")
+    assert plan.tiles.tolist() == [[-1, 0, 16], [-1, 16, 16], [-1, 32, 8], [0, 40, 1], [1, 41, 2]]

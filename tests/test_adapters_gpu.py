@@ -244,3 +244,14 @@ def test_infinite_rows_meet_no_rank_that_is_not_there(rows, r, k, n, dtype, out_
     if mixed:
         none = (step.ranks[torch.tensor(step.of_row).clamp(min=0)] == 0).cuda()
         assert torch.equal(got[none], step.y[none])
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+def test_many_rows_without_an_adapter_beside_single_ones(out_dtype, in_place):
+    step = Step([-1] * 77 + list(range(24)) + [-1] * 3, 24, 32, 264, 136, BF, out_dtype)
+    assert step.plan.tile_rows == 16
+    want, off = step.want()
+    got = step.y.clone() if in_place else torch.full_like(step.y, float("nan"))
+    K().adapter_add(step.x, step.a, step.b, step.plan, got if in_place else step.y, got, scale=step.scale)
+    step.check(got)
