@@ -433,3 +433,48 @@ def test_sums_with_room_for_more_keys_than_requests_have(n, sms, monkeypatch):
             got = run(c, width=width, add=add, max_kv=600)  # (a request that has more gives nothing, and the status says so)
             c.status.zero_()
             assert_close(got[0], (want + add.cpu().double())[0], (tol + 2.0 ** -24 * (want + 1))[0])
+
+
+# ------------------------------------------------------------------------------------ what only large steps reach, at small sizes
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("mask", [dict(), dict(window=64), dict(cap=5.0)])
+def test_several_tiles_of_keys_a_block(monkeypatch, mask, bits8):
+    """As on a device that holds two blocks: up to eight tiles of keys one after the other, some of which (window) no row sees."""
+    c = Case([30, 40], [0, 900], 8, 4, 64, 16, seed=7, bits8=bits8)
+    n = torch.arange(70)
+    c.positions = torch.where(n % 2 == 0, c.positions, c.positions % 30).to(torch.int32)  # near the request's end and near its beginning
+    want, tol = received(c, **mask)
+    if mask.get("window"):
+        assert float(want[1, :, 256:640].abs().max()) == 0
+    c.to_device()
+    monkeypatch.setattr(K(), "sm_count", lambda: 1)
+    assert K()._weights_shares(2 * 4 * 8, 1, 2) == 1  # (and 2 * 4 * 8 tiles of keys on two places: eight a block)
+    add = torch.rand(want.shape, generator=torch.Generator().manual_seed(1)).cuda()
+    assert_close(run(c, **mask), want, tol)
+    want, tol = received(c, add=add, **mask)
+    assert_close(run(c, add=add, **mask), want, tol)
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("sms", [1, 148])
+def test_more_than_32_tiles_of_rows_a_block(monkeypatch, sms):
+    """16 heads on one: 38 tiles of rows, by one block or (several) shared by eight."""
+    c = Case([300, 7], [0, 100], 16, 1, 64, 16, bits8=False, seed=3).to_device()
+    monkeypatch.setattr(K(), "sm_count", lambda: sms)
+    assert (K()._weights_shares(2 * 1 * 3, 38, 2 * sms) == 1) == (sms == 1)
+    want, tol = received(c)
+    assert_close(run(c), want, tol)
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("heads", [(8, 2), (16, 2), (32, 2)])
+def test_ranges_of_more_keys_than_are_added_up_ahead(monkeypatch, bits8, heads):
+    """One range of 2,500 keys a request: a thread adds up 20 of them."""
+    monkeypatch.setattr(K(), "attention_weights_plan", lambda keys, *a: (1, -(-(keys + 16) // 16) * 16, False))
+    c = Case([1, 1], [2500, 1100], *heads, 64, 64, bits8=bits8, seed=1).to_device()
+    add = torch.rand((2, 2, 2501), generator=torch.Generator().manual_seed(1)).cuda()
+    want, tol = received(c, add=add)
+    assert_close(run(c, add=add), want, tol)
+    assert_close(run(c), *received(c))
+    assert int(c.status) == 0

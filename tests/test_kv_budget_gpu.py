@@ -359,3 +359,13 @@ def test_counts_that_their_arrays_do_not_hold_raise_the_status(in_place, counts,
             for i in range(summed[r]):
                 want_sums[r, h, i] = sums[r, h, places[r, h, i]].cpu()
     assert torch.equal(bits(pages), want) and torch.equal(out.cpu(), want_sums)
+
+
+@pytest.mark.parametrize("requests, H, width", [(37, 4, 8192), (1, 1, 100001)])
+def test_choice_of_as_many_places_as_threads_hold(requests, H, width):
+    """13 to 16 sums a thread: a block a row, and sixteen."""
+    gen = torch.Generator().manual_seed(width)
+    sums = torch.exp(1.5 * torch.randn((requests, H, width), generator=gen) - 5)
+    sums[:, ::2] = sums[:, ::2].to(torch.bfloat16).float()
+    sums[0, 0, ::3] = 0.0
+    check(sums, [width - 211 * i for i in range(requests)], [width // 4 + 31 * i for i in range(requests)], 4, 256)
