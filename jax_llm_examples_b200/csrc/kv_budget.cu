@@ -10,12 +10,13 @@
 // a stretch of the places in registers: the sums are read once.
 //
 // kv_compact moves rows bit for bit.  Into other pages every row is on its own.  In place, row i's new place is at or before its old
-// one: a block takes a column of 32 bytes of one plane's rows through all places in order, some hundreds at a time, all loads of
-// which precede all stores; a later row's source lies behind what has been written.
+// one: a block takes a column of 32 bytes of one plane's rows through all places in order, 1024 at a time (2048 where rows are no
+// multiple of 32 bytes and the column has 16), all loads of which precede all stores; a later row's source lies behind what has been written.
 //
 // Both are bound by bytes, few in the first, so there by the chain of its passes: 100,001 places of one session, 4096 kept, 18.9 us a call;
 // 64 sessions of up to 8192, 2048 kept, 25.5 us (62 with sums in shared memory and a scan of the block for every 512 places; digits of 11
-// bits: 40).  Moving 2048 rows of 8 heads of 128 each of 32 sessions takes 94 us, 5.8 TB/s.
+// bits: 40).  Moving 2048 rows of 8 heads of 128 each of 32 sessions takes 94 us, 5.8 TB/s;
+// in place 185: every block of a column looks up each row's place and pages for 32 bytes of it.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
